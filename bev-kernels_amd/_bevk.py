@@ -28,6 +28,7 @@ _DTYPE_CODES = {
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_i64 = ctypes.c_int64
 
 # name -> argument types (after the leading dtype code where present)
 _SIGNATURES = {
@@ -77,6 +78,11 @@ _SIGNATURES = {
     + [_i] * 9 + [_vp, _vp, _vp, _vp, ctypes.c_int64, _vp],
     "bevk_msda_gradients": [_i, _vp, _vp, _vp, _vp, _vp, _vp] + [ctypes.c_int64] * 4
     + [_i] * 9 + [_vp, _vp, _vp, _vp, ctypes.c_int64, _vp],
+    "bevk_group_norm_workspace_bytes": [_i, _i, _i64, _i64, _i, _i],
+    "bevk_group_norm_forward": [_i, _vp, _vp, _vp, _i, _i64, _i64, _i, _i, ctypes.c_double, _i,
+                                _vp, _i64, _vp, _vp, _vp],
+    "bevk_group_norm_backward": [_i] + [_vp] * 4 + [_i, _i64, _i64, _i, _i, _i, _vp, _vp, _i64]
+    + [_vp] * 4,
 }
 
 # entry points that return a value instead of a bevk_status
@@ -88,7 +94,8 @@ _RESTYPES = {"bevk_dcn_packed_weight_bytes": ctypes.c_int64,
              "bevk_dcn_layer_nchw_f32_workspace_bytes": ctypes.c_int64,
              "bevk_dcn_nhwc_workspace_bytes": ctypes.c_int64,
              "bevk_dcn_fused_im2col_nhwc_workspace_bytes": ctypes.c_int64,
-             "bevk_msda_backward_workspace_bytes": ctypes.c_int64}
+             "bevk_msda_backward_workspace_bytes": ctypes.c_int64,
+             "bevk_group_norm_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()
@@ -150,6 +157,17 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().bevk_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"{name} failed with status {rc}")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call() with t's device current and its current stream as the last argument: a launch goes
+    to the current device, which may be another one than the tensors'."""
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -62,6 +62,8 @@ __all__ = [
     "forward",
     "backward",
     "gradients",
+    "group_norm_forward",
+    "group_norm_backward",
 ]
 
 
@@ -947,3 +949,91 @@ def _backward_call(entry, value, spatial_shapes, level_start_index, sampling_loc
             int(im2col_step), 1 if force_generic_col2im else 0, _b.ptr(grad_value),
             _b.ptr(grad_sampling_loc), _b.ptr(grad_attn_weight), _b.ptr(ws), nbytes,
             _b.stream_of(value))
+
+
+# ---------------------------------------------------------------------------------------
+# Group normalization with an activation, channels last (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+GROUP_NORM_ACTS = {None: 0, "relu": 1, "silu": 2}
+
+
+def _group_norm_check(fn, x, num_groups, weight, bias, act):
+    """Checks shared by both directions; returns (images, positions, channels, type of the
+    parameters, code of the activation)."""
+    _b.require_device(fn, x, weight, bias)
+    if x.dim() < 3:
+        raise RuntimeError(f"{fn}: expected x [N, ..., C] with positions between, got "
+                           f"{tuple(x.shape)}")
+    _b.require_contiguous(fn, x=x, weight=weight, bias=bias)
+    if act not in GROUP_NORM_ACTS:
+        raise RuntimeError(f"{fn}: act must be None, 'relu' or 'silu', got {act!r}")
+    channels = x.size(-1)
+    if num_groups <= 0 or channels % num_groups != 0:
+        raise RuntimeError(f"{fn}: channels ({channels}) must be divisible by num_groups "
+                           f"({num_groups})")
+    ptype = None
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if tuple(p.shape) != (channels,):
+            raise RuntimeError(f"{fn}: {name} must be [{channels}], got {tuple(p.shape)}")
+        if p.dtype != x.dtype and p.dtype != torch.float32:
+            raise RuntimeError(f"{fn}: {name} has dtype {p.dtype}, expected {x.dtype} or "
+                               "torch.float32")
+        if ptype is not None and p.dtype != ptype:
+            raise RuntimeError(f"{fn}: weight and bias must have one dtype")
+        ptype = p.dtype
+    images = x.size(0)
+    positions = x.numel() // (images * channels) if x.numel() else 0
+    return (images, positions, channels, _b._DTYPE_CODES[ptype or x.dtype]
+            if x.dtype in _b._DTYPE_CODES else _b.dtype_code(x), GROUP_NORM_ACTS[act])
+
+
+def _group_norm_workspace(fn, x, backward, images, positions, channels, num_groups):
+    nbytes = _b.lib().bevk_group_norm_workspace_bytes(_b.dtype_code(x), backward, images, positions,
+                                                      channels, num_groups)
+    if nbytes < 0:
+        raise RuntimeError(f"{fn}: not implemented for {x.dtype} {tuple(x.shape)}")
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device), nbytes
+
+
+def group_norm_forward(x, num_groups, weight, bias, eps, act):
+    """(y, stats): y = act(group norm of x [N, ..., C]) in x's type; stats [N, groups, 2] float64
+    (mean, 1 / sqrt(var + eps)) for group_norm_backward. weight / bias [C] in x's type or fp32,
+    or None."""
+    fn = "group_norm_forward"
+    images, positions, channels, pcode, acode = _group_norm_check(fn, x, num_groups, weight, bias, act)
+    y = torch.empty_like(x)
+    stats = x.new_empty((images, num_groups, 2), dtype=torch.float64)
+    if positions == 0:
+        return y, stats
+    ws, nbytes = _group_norm_workspace(fn, x, 0, images, positions, channels, num_groups)
+    _b.call_on(x, "bevk_group_norm_forward", _b.dtype_code(x), _b.ptr(x), _b.ptr(weight), _b.ptr(bias),
+               pcode, images, positions, channels, num_groups, float(eps), acode, _b.ptr(ws), nbytes,
+               _b.ptr(y), _b.ptr(stats))
+    return y, stats
+
+
+def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=(True, True, True)):
+    """(grad_x, grad_weight, grad_bias) of group_norm_forward for grad_y; None where `wanted` is
+    false or the parameter is None."""
+    fn = "group_norm_backward"
+    images, positions, channels, pcode, acode = _group_norm_check(fn, x, num_groups, weight, bias, act)
+    _b.require_device(fn, x, grad_y, stats)
+    _b.require_contiguous(fn, grad_y=grad_y, stats=stats)
+    _b.require_dtype(fn, x, grad_y=grad_y)
+    _b.require_numel(fn, "grad_y", grad_y, x.numel())
+    _b.require_numel(fn, "stats", stats, 2 * images * num_groups)
+    if stats.dtype != torch.float64:
+        raise RuntimeError(f"{fn}: stats must be float64, got {stats.dtype}")
+    new = torch.empty_like if positions else torch.zeros_like
+    grads = [new(t) if want and t is not None else None
+             for want, t in zip(wanted, (x, weight, bias))]
+    if positions == 0:
+        return tuple(grads)
+    ws, nbytes = _group_norm_workspace(fn, x, 1, images, positions, channels, num_groups)
+    _b.call_on(x, "bevk_group_norm_backward", _b.dtype_code(x), _b.ptr(grad_y), _b.ptr(x),
+               _b.ptr(weight), _b.ptr(bias), pcode, images, positions, channels, num_groups, acode,
+               _b.ptr(stats), _b.ptr(ws), nbytes, *(_b.ptr(g) for g in grads))
+    return tuple(grads)

@@ -169,6 +169,27 @@ int64_t column_sums_workspace_bytes(int n);
 hipError_t launch_column_sums(int dtype, const void *src, int64_t rows, int ld, int n, void *workspace,
                               int out_dtype, void *out, hipStream_t stream);
 
+// Group normalization with an activation, channels last: x [batch][pixels][channels] -> y (dtype), and
+// stats [batch][groups][2] (mean, 1 / sqrt(var + eps)) for the backward. weight / bias [channels]
+// (param_dtype) or null; channels % groups == 0, no empty sizes. The backward writes grad_x (dtype),
+// grad_w and grad_b (param_dtype), each skipped when null.
+enum GroupNormAct { kActNone = 0, kActRelu = 1, kActSilu = 2 };
+struct GroupNormArgs {
+  const void *x, *weight, *bias;
+  int param_dtype;
+  int64_t batch, pixels;
+  int channels, groups;
+  double eps;
+  int act;
+};
+int64_t group_norm_workspace_bytes(int dtype, bool backward, int64_t batch, int64_t pixels, int channels,
+                                   int groups);
+hipError_t launch_group_norm_forward(int dtype, const GroupNormArgs &a, void *y, double *stats, void *workspace,
+                                     hipStream_t stream);
+hipError_t launch_group_norm_backward(int dtype, const GroupNormArgs &a, const void *grad_y, const double *stats,
+                                      void *workspace, void *grad_x, void *grad_w, void *grad_b,
+                                      hipStream_t stream);
+
 // dst[b][c][r] = src[b][r][c] for 2- or 4-byte elements (NCHW <-> NHWC).
 hipError_t launch_transpose(int elem_bytes, const void *src, void *dst, int batch, int rows,
                             int cols, hipStream_t stream);

@@ -1185,4 +1185,73 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
                            workspace, workspace_bytes, stream);
 }
 
+static int check_group_norm(const char *fn, int dtype, int param_dtype, int64_t batch, int64_t pixels,
+                            int channels, int groups, int act) {
+  for (int d : {dtype, param_dtype})
+    if (d != BEVK_F32 && d != BEVK_F16 && d != BEVK_BF16)
+      return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(d));
+  if (param_dtype != dtype && param_dtype != BEVK_F32)
+    return fail(BEVK_ERR_INVALID, "%s: weight and bias must have the input's type or be fp32", fn);
+  if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0)
+    return fail(BEVK_ERR_INVALID, "%s: sizes must be positive", fn);
+  if (channels % groups != 0)
+    return fail(BEVK_ERR_INVALID, "%s: channels (%d) must be divisible by groups (%d)", fn, channels, groups);
+  if (batch > (1LL << 40) / channels || pixels > (1LL << 40) / channels / batch)
+    return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
+  if (act < 0 || act > 2) return fail(BEVK_ERR_INVALID, "%s: unknown activation %d", fn, act);
+  return 0;
+}
+
+static bevk::GroupNormArgs group_norm_args(const void *x, const void *weight, const void *bias, int param_dtype,
+                                           int64_t batch, int64_t pixels, int channels, int groups, double eps,
+                                           int act) {
+  bevk::GroupNormArgs a;
+  a.x = x; a.weight = weight; a.bias = bias; a.param_dtype = param_dtype;
+  a.batch = batch; a.pixels = pixels; a.channels = channels; a.groups = groups;
+  a.eps = eps; a.act = act;
+  return a;
+}
+
+int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels, int channels,
+                                        int groups) {
+  if (check_group_norm("group_norm", dtype, dtype, batch, pixels, channels, groups, 0)) return -1;
+  return bevk::group_norm_workspace_bytes(dtype, backward != 0, batch, pixels, channels, groups);
+}
+
+int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const void *bias, int param_dtype,
+                            int64_t batch, int64_t pixels, int channels, int groups, double eps, int act,
+                            void *workspace, int64_t workspace_bytes, void *y, double *stats, void *stream) {
+  const char *fn = "group_norm_forward";
+  g_last_error.clear();
+  if (int rc = check_group_norm(fn, dtype, param_dtype, batch, pixels, channels, groups, act)) return rc;
+  if (!(eps >= 0.0)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
+  const int64_t need = bevk::group_norm_workspace_bytes(dtype, false, batch, pixels, channels, groups);
+  if (!x || !y || !stats || (need > 0 && !workspace))
+    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  return hip_status(
+      bevk::launch_group_norm_forward(
+          dtype, group_norm_args(x, weight, bias, param_dtype, batch, pixels, channels, groups, eps, act), y,
+          stats, workspace, (hipStream_t)stream),
+      fn);
+}
+
+int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const void *weight, const void *bias,
+                             int param_dtype, int64_t batch, int64_t pixels, int channels, int groups, int act,
+                             const double *stats, void *workspace, int64_t workspace_bytes, void *grad_x,
+                             void *grad_weight, void *grad_bias, void *stream) {
+  const char *fn = "group_norm_backward";
+  g_last_error.clear();
+  if (int rc = check_group_norm(fn, dtype, param_dtype, batch, pixels, channels, groups, act)) return rc;
+  const int64_t need = bevk::group_norm_workspace_bytes(dtype, true, batch, pixels, channels, groups);
+  if (!grad_y || !x || !stats || !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (!grad_x && !grad_weight && !grad_bias) return ok();
+  return hip_status(
+      bevk::launch_group_norm_backward(
+          dtype, group_norm_args(x, weight, bias, param_dtype, batch, pixels, channels, groups, 0.0, act),
+          grad_y, stats, workspace, grad_x, grad_weight, grad_bias, (hipStream_t)stream),
+      fn);
+}
+
 }  // extern "C"

@@ -10,3 +10,8 @@ from .modulated_deform_conv import (  # noqa: F401
     ext_modulated_deformable_col2im_smem,
     ext_modulated_deformable_col2im_coord_opt,
 )
+from .group_norm import (  # noqa: F401
+    GroupNormAct2d,
+    GroupNormActNHWCFunction,
+    group_norm_act_nhwc,
+)

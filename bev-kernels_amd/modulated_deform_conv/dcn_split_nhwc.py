@@ -21,6 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from ._packing import pack_weight, weight_grad
+from .group_norm import group_norm_act_nhwc
 
 
 def out_size(H, pad, dil, k, stride):
@@ -312,6 +313,15 @@ def dcn_split_nhwc(x_nhwc, w_off, b_off, weight, bias=None, stride=1, padding=1,
     """NHWC DCNv2 forward with the offset conv inside; optional FrozenBN(+ReLU) epilogue."""
     return DCNSplitNHWCFunction.apply(x_nhwc, w_off, b_off, weight, bias, stride, padding,
                                       dilation, bn_scale, bn_shift, act_relu)
+
+
+def dcn_split_gn_nhwc(x_nhwc, w_off, b_off, weight, bias, num_groups, gn_weight=None, gn_bias=None,
+                      eps=1e-5, act="relu", stride=1, padding=1, dilation=1):
+    """dcn_split_nhwc with a group norm and activation behind it where the FrozenBN epilogue of
+    the backbone's layers stands: the layer of a detection head. Two steps, since the norm's
+    statistics need the whole output; gradients flow to every parameter of both."""
+    y = dcn_split_nhwc(x_nhwc, w_off, b_off, weight, bias, stride, padding, dilation)
+    return group_norm_act_nhwc(y, num_groups, gn_weight, gn_bias, eps, act)
 
 
 def _as_int(v):

@@ -458,6 +458,33 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
                         void *grad_value, void *grad_sampling_loc, void *grad_attn_weight,
                         void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Group normalization with an activation, channels last                      */
+/* ------------------------------------------------------------------------- */
+
+/* Group normalization of x [batch, pixels, channels] with an activation behind it (no counterpart
+ * in the reference, whose NHWC layer ends in a FrozenBN + ReLU):
+ *   mean, var    of the pixels * channels / groups values of an image's group (fp64 sums)
+ *   y            act((x - mean) / sqrt(var + eps) * weight + bias), dtype
+ *   weight, bias [channels] param_dtype, or NULL (1 and 0)
+ *   act          0: none, 1: ReLU, 2: SiLU (z / (1 + exp(-z)))
+ *   stats        [batch, groups, 2] fp64, written: mean and 1 / sqrt(var + eps), for the backward
+ * The backward writes grad_x (dtype), grad_weight and grad_bias [channels] (param_dtype), each NULL
+ * where it is not wanted; ReLU's derivative at 0 is 0. The same results on every run. dtype and
+ * param_dtype F32, F16, BF16 (param_dtype: the input's or F32); the workspace holds what
+ * bevk_group_norm_workspace_bytes says (-1 for sizes that are not taken). No size may be 0. */
+int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels,
+                                        int channels, int groups);
+int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const void *bias,
+                            int param_dtype, int64_t batch, int64_t pixels, int channels, int groups,
+                            double eps, int act, void *workspace, int64_t workspace_bytes, void *y,
+                            double *stats, void *stream);
+int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const void *weight,
+                             const void *bias, int param_dtype, int64_t batch, int64_t pixels,
+                             int channels, int groups, int act, const double *stats, void *workspace,
+                             int64_t workspace_bytes, void *grad_x, void *grad_weight,
+                             void *grad_bias, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,97 @@
+"""Refusals of the training-side operators on the CPU, in Python and at the C ABI: nothing here
+reaches a launch (fake device addresses are never followed)."""
+import ctypes
+
+import pytest
+import torch
+
+import _bevk
+import _modulated_deform_conv_ext as ext
+import modulated_deform_conv as mdc
+
+INVALID, UNSUPPORTED = 1, 2
+P = ctypes.c_void_p(0x10000)
+
+
+def _err():
+    return _bevk.lib().bevk_last_error().decode()
+
+
+def _meta(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+@pytest.fixture
+def no_device_check(monkeypatch):
+    monkeypatch.setattr(_bevk, "require_device", lambda fn, *t: 0)
+
+
+def test_group_norm_needs_a_device():
+    with pytest.raises(RuntimeError, match="HIP"):
+        mdc.group_norm_act_nhwc(torch.zeros(1, 4, 4, 8), 2)
+    with pytest.raises(ValueError, match="4D"):
+        mdc.GroupNormAct2d(2, 8)(torch.zeros(1, 4, 8))
+    with pytest.raises(ValueError, match="divisible"):
+        mdc.GroupNormAct2d(3, 8)
+    with pytest.raises(ValueError, match="act"):
+        mdc.GroupNormAct2d(2, 8, act="tanh")
+
+
+def test_group_norm_refusals(no_device_check):
+    x = _meta(2, 4, 4, 8)
+    f = ext.group_norm_forward
+    for bad, match in (((_meta(2, 8), 2, None, None), "positions"),
+                       ((x.permute(0, 3, 1, 2), 2, None, None), "contiguous"),
+                       ((x, 3, None, None), "divisible"), ((x, 0, None, None), "divisible"),
+                       ((x, 2, _meta(4), None), r"weight must be \[8\]"),
+                       ((x, 2, None, _meta(8, dtype=torch.float16)), "bias has dtype"),
+                       ((x.half(), 2, _meta(8), _meta(8, dtype=torch.float16)), "one dtype"),
+                       ((x.double(), 2, None, None), "not implemented"),
+                       ((x.long(), 2, None, None), "not supported")):
+        with pytest.raises(RuntimeError, match=match):
+            f(*bad, 1e-5, None)
+    with pytest.raises(RuntimeError, match="act must be"):
+        f(x, 2, None, None, 1e-5, "gelu")
+    b = ext.group_norm_backward
+    stats = _meta(2, 2, 2, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="grad_y"):
+        b(_meta(2, 4, 4, 4), x, 2, None, None, None, stats)
+    with pytest.raises(RuntimeError, match="grad_y has dtype"):
+        b(x.half(), x, 2, None, None, None, stats)
+    with pytest.raises(RuntimeError, match="stats"):
+        b(x, x, 2, None, None, None, _meta(2, 2, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="stats must be float64"):
+        b(x, x, 2, None, None, None, _meta(2, 2, 2))
+
+
+def test_group_norm_c_abi():
+    lib = _bevk.lib()
+
+    def fwd(dtype=0, x=P, w=None, b=None, pd=0, n=1, p=4, c=8, g=2, eps=1e-5, act=0, ws=P, wb=1 << 30,
+            y=P, st=P):
+        return lib.bevk_group_norm_forward(dtype, x, w, b, pd, n, p, c, g, eps, act, ws, wb, y, st, None)
+
+    assert fwd(dtype=3) == UNSUPPORTED and "Double" in _err()
+    assert fwd(dtype=9) == UNSUPPORTED
+    assert fwd(dtype=1, pd=2) == INVALID and "type" in _err()
+    assert fwd(c=9) == INVALID and "divisible" in _err()
+    for kw in (dict(n=0), dict(p=0), dict(c=0), dict(g=0), dict(n=-1)):
+        assert fwd(**kw) == INVALID and "positive" in _err()
+    assert fwd(n=1 << 30, p=1 << 30) == INVALID and "2^40" in _err()
+    assert fwd(act=3) == INVALID and "activation" in _err()
+    assert fwd(eps=-1.0) == INVALID and "eps" in _err()
+    assert fwd(eps=float("nan")) == INVALID and "eps" in _err()
+    for kw in (dict(x=None), dict(y=None), dict(st=None)):
+        assert fwd(**kw) == INVALID and "null" in _err()
+
+    def bwd(dtype=0, gy=P, x=P, act=0, st=P, ws=P, wb=1 << 30, gx=P):
+        return lib.bevk_group_norm_backward(dtype, gy, x, None, None, dtype, 2, 4, 8, 2, act, st, ws, wb,
+                                            gx, None, None, None)
+
+    assert bwd(dtype=3) == UNSUPPORTED
+    for kw in (dict(gy=None), dict(x=None), dict(st=None), dict(ws=None)):
+        assert bwd(**kw) == INVALID and "null" in _err()
+    assert bwd(wb=0) == INVALID and "workspace" in _err()
+    assert bwd(gx=None) == 0                            # nothing wanted
+    ws = lib.bevk_group_norm_workspace_bytes
+    assert ws(3, 0, 1, 4, 8, 2) == -1 and ws(0, 0, 1, 4, 9, 2) == -1 and ws(0, 1, 1, 4, 8, 2) > 0
