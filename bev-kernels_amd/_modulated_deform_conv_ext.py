@@ -64,6 +64,8 @@ __all__ = [
     "gradients",
     "group_norm_forward",
     "group_norm_backward",
+    "embedding_forward",
+    "embedding_backward",
 ]
 
 
@@ -1037,3 +1039,54 @@ def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=
                _b.ptr(weight), _b.ptr(bias), pcode, images, positions, channels, num_groups, acode,
                _b.ptr(stats), _b.ptr(ws), nbytes, *(_b.ptr(g) for g in grads))
     return tuple(grads)
+
+
+# ---------------------------------------------------------------------------------------
+# Embedding rows by index (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+def _embedding_check(fn, index, table, name):
+    _b.require_device(fn, table, index)
+    _b.require_contiguous(fn, index=index, **{name: table})
+    if index.dtype != torch.int64 and index.dtype != torch.int32:
+        raise RuntimeError(f"{fn}: index must be int64 or int32, got {index.dtype}")
+    if _b.dtype_code(table) == _b.BEVK_F64:
+        raise RuntimeError(f"{fn}: not implemented for {table.dtype}")
+
+
+def embedding_forward(weight, index, scale=1.0):
+    """scale * weight[index] [*index.shape, D] in the type of weight [V, D]; index int64 or int32,
+    rows of zeros where it is outside [0, V)."""
+    fn = "embedding_forward"
+    _embedding_check(fn, index, weight, "weight")
+    if weight.dim() != 2:
+        raise RuntimeError(f"{fn}: weight must be [V, D], got {tuple(weight.shape)}")
+    rows, dim = weight.shape
+    out = weight.new_empty((*index.shape, dim))
+    _b.call_on(weight, "bevk_embedding_forward", _b.dtype_code(weight), _b.ptr(weight), rows, dim,
+               _b.ptr(index), index.dtype == torch.int64, index.numel(), scale, _b.ptr(out))
+    return out
+
+
+def embedding_backward(grad_out, index, num_embeddings, scale=1.0, padding_idx=None):
+    """The gradient [num_embeddings, D] of embedding_forward's weight for grad_out
+    [*index.shape, D]: scale * the fp32 sums of its rows with the same index, added in a fixed
+    order; the row padding_idx gets none."""
+    fn = "embedding_backward"
+    _embedding_check(fn, index, grad_out, "grad_out")
+    if grad_out.dim() != index.dim() + 1 or grad_out.shape[:-1] != index.shape:
+        raise RuntimeError(f"{fn}: grad_out must be [*index.shape, D], got {tuple(grad_out.shape)} "
+                           f"for index {tuple(index.shape)}")
+    if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
+        raise RuntimeError(f"{fn}: padding_idx must be a row of the table, got {padding_idx}")
+    dim, n, code = grad_out.size(-1), index.numel(), _b.dtype_code(grad_out)
+    nbytes = _b.lib().bevk_embedding_backward_workspace_bytes(code, n, num_embeddings, dim)
+    if nbytes < 0:
+        raise RuntimeError(f"{fn}: not implemented for {grad_out.dtype} {tuple(grad_out.shape)}, "
+                           f"{num_embeddings} rows")
+    grad = grad_out.new_empty((num_embeddings, dim))
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=grad_out.device)
+    _b.call_on(grad_out, "bevk_embedding_backward", code, _b.ptr(grad_out), _b.ptr(index),
+               index.dtype == torch.int64, n, num_embeddings, dim, scale,
+               -1 if padding_idx is None else padding_idx, _b.ptr(ws), nbytes, _b.ptr(grad))
+    return grad

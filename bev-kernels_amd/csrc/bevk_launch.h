@@ -190,6 +190,23 @@ hipError_t launch_group_norm_backward(int dtype, const GroupNormArgs &a, const v
                                       void *workspace, void *grad_x, void *grad_w, void *grad_b,
                                       hipStream_t stream);
 
+// Embedding rows by index: index [n] (int32, or int64 with index64), weight [rows][dim] -> out [n][dim]
+// = scale * weight[index] (zeros where the index is outside the table), and grad_w [rows][dim] =
+// scale * the sums of grad_out's rows with that index (zeros for the row `padding`; -1: none).
+// No empty sizes but n == 0 in the backward; n and rows below 2^31.
+struct EmbeddingArgs {
+  const void *index;
+  bool index64;
+  int64_t n, rows;
+  int dim;
+  float scale;
+};
+hipError_t launch_embedding_forward(int dtype, const EmbeddingArgs &a, const void *weight, void *out,
+                                    hipStream_t stream);
+int64_t embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim);
+hipError_t launch_embedding_backward(int dtype, const EmbeddingArgs &a, const void *grad_out, int64_t padding,
+                                     void *workspace, void *grad_w, hipStream_t stream);
+
 // dst[b][c][r] = src[b][r][c] for 2- or 4-byte elements (NCHW <-> NHWC).
 hipError_t launch_transpose(int elem_bytes, const void *src, void *dst, int batch, int rows,
                             int cols, hipStream_t stream);

@@ -1254,4 +1254,48 @@ int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const
       fn);
 }
 
+static int check_embedding(const char *fn, int dtype, int64_t n, int64_t rows, int dim) {
+  if (dtype != BEVK_F32 && dtype != BEVK_F16 && dtype != BEVK_BF16)
+    return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(dtype));
+  if (n < 0 || rows < 0 || dim < 0) return fail(BEVK_ERR_INVALID, "%s: negative size", fn);
+  if (n > (1LL << 31) - 256 || rows > (1LL << 31) - 256)
+    return fail(BEVK_ERR_INVALID, "%s: indices and rows must number less than 2^31 - 256", fn);
+  return 0;
+}
+
+int bevk_embedding_forward(int dtype, const void *weight, int64_t rows, int dim, const void *index, int index64,
+                           int64_t n, float scale, void *out, void *stream) {
+  const char *fn = "embedding_forward";
+  g_last_error.clear();
+  if (int rc = check_embedding(fn, dtype, n, rows, dim)) return rc;
+  if (n == 0 || dim == 0) return ok();
+  if ((!weight && rows > 0) || !index || !out) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  const bevk::EmbeddingArgs a{index, index64 != 0, n, rows, dim, scale};
+  return hip_status(bevk::launch_embedding_forward(dtype, a, weight, out, (hipStream_t)stream), fn);
+}
+
+int64_t bevk_embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim) {
+  if (check_embedding("embedding_backward", dtype, n, rows, dim)) return -1;
+  return bevk::embedding_backward_workspace_bytes(dtype, n, rows, dim);
+}
+
+int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, int index64, int64_t n,
+                            int64_t rows, int dim, float scale, int64_t padding_idx, void *workspace,
+                            int64_t workspace_bytes, void *grad_weight, void *stream) {
+  const char *fn = "embedding_backward";
+  g_last_error.clear();
+  if (int rc = check_embedding(fn, dtype, n, rows, dim)) return rc;
+  if (padding_idx < -1 || (padding_idx >= rows && padding_idx != -1))
+    return fail(BEVK_ERR_INVALID, "%s: padding_idx must be a row of the table, or -1", fn);
+  if (rows == 0 || dim == 0) return ok();
+  const int64_t need = bevk::embedding_backward_workspace_bytes(dtype, n, rows, dim);
+  if ((n > 0 && (!grad_out || !index)) || !grad_weight || (need > 0 && !workspace))
+    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  const bevk::EmbeddingArgs a{index, index64 != 0, n, rows, dim, scale};
+  return hip_status(bevk::launch_embedding_backward(dtype, a, grad_out, padding_idx, workspace, grad_weight,
+                                                    (hipStream_t)stream),
+                    fn);
+}
+
 }  // extern "C"

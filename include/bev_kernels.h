@@ -485,6 +485,27 @@ int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const
                              int64_t workspace_bytes, void *grad_x, void *grad_weight,
                              void *grad_bias, void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Embedding rows by index                                                    */
+/* ------------------------------------------------------------------------- */
+
+/* Rows of a table by index with a scale (no counterpart in the reference): the queries of the
+ * attention, or the cells of a grid that a camera sees.
+ *   index        [n] int32 (index64 == 0) or int64. An index outside [0, rows) stands for no row
+ *   out          [n, dim] = scale * weight[index], fp32 arithmetic rounded once; zeros for no row
+ *   grad_weight  [rows, dim], written: scale * the fp32 sums of the rows of grad_out [n, dim] with
+ *                that index, in a fixed order (the same results on every run); zeros for rows
+ *                without an index, and for the row padding_idx (-1: none)
+ * weight [rows, dim], out and gradients in dtype F32, F16 or BF16; n and rows below 2^31 - 256; the
+ * workspace holds what bevk_embedding_backward_workspace_bytes says (-1 for sizes not taken). */
+int bevk_embedding_forward(int dtype, const void *weight, int64_t rows, int dim, const void *index,
+                           int index64, int64_t n, float scale, void *out, void *stream);
+int64_t bevk_embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim);
+int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, int index64,
+                            int64_t n, int64_t rows, int dim, float scale, int64_t padding_idx,
+                            void *workspace, int64_t workspace_bytes, void *grad_weight,
+                            void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,3 +95,58 @@ def test_group_norm_c_abi():
     assert bwd(gx=None) == 0                            # nothing wanted
     ws = lib.bevk_group_norm_workspace_bytes
     assert ws(3, 0, 1, 4, 8, 2) == -1 and ws(0, 0, 1, 4, 9, 2) == -1 and ws(0, 1, 1, 4, 8, 2) > 0
+
+
+def test_embedding_refusals(no_device_check):
+    import msda_opt2
+    w, i = _meta(10, 8), _meta(3, 4, dtype=torch.int64)
+    for bad, match in (((_meta(10), i), r"weight must be \[V, D\]"), ((w, i.float()), "int64 or int32"),
+                       ((w, i.short()), "int64 or int32"), ((w.t(), i), "contiguous"),
+                       ((w, i.t()), "contiguous"), ((w.long(), i), "not supported"),
+                       ((w.double(), i), "not implemented")):
+        with pytest.raises(RuntimeError, match=match):
+            ext.embedding_forward(*bad)
+    g = _meta(3, 4, 8)
+    for bad, match in (((g, _meta(12, dtype=torch.int64), 10), "grad_out must be"),
+                       ((_meta(3, 8), i, 10), "grad_out must be"),
+                       ((g, i, 10, 1.0, 10), "padding_idx"), ((g, i, 10, 1.0, -1), "padding_idx"),
+                       ((g.double(), i, 10), "not implemented"), ((g, i, -1), "not implemented")):
+        with pytest.raises(RuntimeError, match=match):
+            ext.embedding_backward(*bad)
+    for padding in (-1, 10):
+        with pytest.raises(RuntimeError, match="padding_idx"):
+            msda_opt2.embedding_lookup(w, i, 1.0, padding)
+
+
+def test_embedding_needs_a_device():
+    import msda_opt2
+    with pytest.raises(RuntimeError, match="HIP"):
+        msda_opt2.embedding_lookup(torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64))
+
+
+def test_embedding_c_abi():
+    lib = _bevk.lib()
+
+    def fwd(dtype=0, w=P, rows=10, dim=8, i=P, n=4, out=P):
+        return lib.bevk_embedding_forward(dtype, w, rows, dim, i, 1, n, 1.0, out, None)
+
+    assert fwd(dtype=3) == UNSUPPORTED and "Double" in _err()
+    for kw in (dict(n=-1), dict(rows=-1), dict(dim=-1)):
+        assert fwd(**kw) == INVALID and "negative" in _err()
+    for kw in (dict(n=1 << 31), dict(rows=1 << 31)):
+        assert fwd(**kw) == INVALID and "2^31" in _err()
+    for kw in (dict(w=None), dict(i=None), dict(out=None)):
+        assert fwd(**kw) == INVALID and "null" in _err()
+    assert fwd(n=0) == 0 and fwd(dim=0) == 0
+
+    def bwd(dtype=0, g=P, i=P, n=4, rows=10, dim=8, padding=-1, ws=P, wb=1 << 30, gw=P):
+        return lib.bevk_embedding_backward(dtype, g, i, 1, n, rows, dim, 1.0, padding, ws, wb, gw, None)
+
+    assert bwd(dtype=9) == UNSUPPORTED
+    for padding in (-2, 10):
+        assert bwd(padding=padding) == INVALID and "padding_idx" in _err()
+    for kw in (dict(g=None), dict(i=None), dict(gw=None)):
+        assert bwd(**kw) == INVALID and "null" in _err()
+    assert bwd(rows=0) == 0 and bwd(dim=0) == 0
+    ws = lib.bevk_embedding_backward_workspace_bytes
+    assert ws(3, 4, 10, 8) == -1 and ws(0, -1, 10, 8) == -1 and ws(0, 1 << 31, 10, 8) == -1
