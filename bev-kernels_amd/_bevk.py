@@ -78,6 +78,8 @@ _SIGNATURES = {
     + [_i] * 9 + [_vp, _vp, _vp, _vp, ctypes.c_int64, _vp],
     "bevk_msda_gradients": [_i, _vp, _vp, _vp, _vp, _vp, _vp] + [ctypes.c_int64] * 4
     + [_i] * 9 + [_vp, _vp, _vp, _vp, ctypes.c_int64, _vp],
+    "bevk_clip_gradients_workspace_bytes": [_i, _vp],
+    "bevk_clip_gradients": [_i] + [_vp] * 5 + [ctypes.c_double, _vp, _i64, _vp, _vp],
     "bevk_embedding_forward": [_i, _vp, _i64, _i, _vp, _i, _i64, ctypes.c_float, _vp, _vp],
     "bevk_embedding_backward_workspace_bytes": [_i, _i64, _i64, _i],
     "bevk_embedding_backward": [_i, _vp, _vp, _i, _i64, _i64, _i, ctypes.c_float, _i64, _vp, _i64,
@@ -100,7 +102,8 @@ _RESTYPES = {"bevk_dcn_packed_weight_bytes": ctypes.c_int64,
              "bevk_dcn_fused_im2col_nhwc_workspace_bytes": ctypes.c_int64,
              "bevk_msda_backward_workspace_bytes": ctypes.c_int64,
              "bevk_group_norm_workspace_bytes": ctypes.c_int64,
-             "bevk_embedding_backward_workspace_bytes": ctypes.c_int64}
+             "bevk_embedding_backward_workspace_bytes": ctypes.c_int64,
+             "bevk_clip_gradients_workspace_bytes": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

@@ -18,6 +18,7 @@ added to what the caller passes, everything else is written.
 from __future__ import annotations
 
 import os
+from array import array
 
 import torch
 
@@ -66,6 +67,7 @@ __all__ = [
     "group_norm_backward",
     "embedding_forward",
     "embedding_backward",
+    "clip_gradients",
 ]
 
 
@@ -1090,3 +1092,67 @@ def embedding_backward(grad_out, index, num_embeddings, scale=1.0, padding_idx=N
                index.dtype == torch.int64, n, num_embeddings, dim, scale,
                -1 if padding_idx is None else padding_idx, _b.ptr(ws), nbytes, _b.ptr(grad))
     return grad
+
+
+# ---------------------------------------------------------------------------------------
+# The norm of many gradients, and clipping (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+def _dense(t):
+    """Whether t's values fill one range of memory, in whatever order of its dimensions."""
+    step = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def _grad_arrays(fn, tensors, device):
+    """(pointers, type codes, sizes) as arrays for the library. Plain attribute tests in one loop
+    over what may be hundreds of tensors: the host side of the call."""
+    codes = _b._DTYPE_CODES
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {t.device}")
+        if t.get_device() != device:
+            raise RuntimeError(f"{fn}: tensors are on different devices (cuda:{device}, {t.device})")
+        if t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
+            raise RuntimeError(f"{fn}: gradients must be dense, got {t.layout} with strides "
+                               f"{t.stride() if t.layout is torch.strided else None}")
+        if t.dtype not in codes:
+            _b.dtype_code(t)
+    return (array("Q", [t.data_ptr() for t in tensors]), array("i", [codes[t.dtype] for t in tensors]),
+            array("q", [t.numel() for t in tensors]))
+
+
+def clip_gradients(grads, max_norm=None, out=None):
+    """The fp32 norm (0-dim tensor) of all grads together; with max_norm, out[k] =
+    min(1, max_norm / (norm + 1e-6)) * grads[k]. fp32 / fp16 / bf16 in any mixture, dense in
+    memory; out: tensors of the same shapes and strides (another type if wanted), grads themselves
+    among them."""
+    fn = "clip_gradients"
+    device = grads[0].get_device()
+    ptrs, types, sizes = _grad_arrays(fn, grads, device)
+    optrs = otypes = None
+    if max_norm is not None:
+        out = grads if out is None else out
+        if len(out) != len(grads):
+            raise RuntimeError(f"{fn}: {len(out)} outputs for {len(grads)} gradients")
+        for g, o in zip(grads, out):
+            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (
+                    o.is_contiguous() and g.is_contiguous()))):
+                raise RuntimeError(f"{fn}: an output has shape {tuple(o.shape)} and strides "
+                                   f"{o.stride()}, its gradient {tuple(g.shape)} and {g.stride()}")
+        optrs, otypes = (ptrs, types) if out is grads else _grad_arrays(fn, out, device)[:2]
+    count, at = len(grads), lambda a: a.buffer_info()[0] if a is not None else None
+    nbytes = _b.lib().bevk_clip_gradients_workspace_bytes(count, at(sizes))
+    if nbytes < 0:
+        raise RuntimeError(f"{fn}: more than 2^40 values")
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=grads[0].device)
+    _b.call_on(norm, "bevk_clip_gradients", count, at(ptrs), at(types), at(sizes), at(optrs), at(otypes),
+               0.0 if max_norm is None else max_norm, _b.ptr(ws), nbytes, _b.ptr(norm))
+    if optrs is not None:  # written behind autograd's back
+        torch.autograd.graph.increment_version(out)
+    return norm

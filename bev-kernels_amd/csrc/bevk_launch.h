@@ -207,6 +207,21 @@ int64_t embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, i
 hipError_t launch_embedding_backward(int dtype, const EmbeddingArgs &a, const void *grad_out, int64_t padding,
                                      void *workspace, void *grad_w, hipStream_t stream);
 
+// The norm of `count` gradients together (fp32, device) and, with out, each times
+// min(1, max_norm / (norm + 1e-6)) into out (host arrays; out[k] may be in[k]). Fewer than 2^31
+// chunks of clip_gradients_workspace_bytes / 8.
+struct GradList {
+  int count;
+  const void *const *in;
+  const int *in_type;
+  const int64_t *n;
+  void *const *out;
+  const int *out_type;
+};
+int64_t clip_gradients_workspace_bytes(const GradList &g);
+hipError_t launch_clip_gradients(const GradList &g, double max_norm, void *workspace, float *norm,
+                                 hipStream_t stream);
+
 // dst[b][c][r] = src[b][r][c] for 2- or 4-byte elements (NCHW <-> NHWC).
 hipError_t launch_transpose(int elem_bytes, const void *src, void *dst, int batch, int rows,
                             int cols, hipStream_t stream);

@@ -4,10 +4,13 @@
 // csrc_musa/msda/binding_musa.mu:545-557) with tensors lowered to device pointers.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
+#include <new>
 #include <string>
+#include <vector>
 
 #include "../../include/bev_kernels.h"
 #include "bevk_launch.h"
@@ -1296,6 +1299,84 @@ int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, 
   return hip_status(bevk::launch_embedding_backward(dtype, a, grad_out, padding_idx, workspace, grad_weight,
                                                     (hipStream_t)stream),
                     fn);
+}
+
+static int check_grad_sizes(const char *fn, int count, const int64_t *numels) {
+  if (count < 0) return fail(BEVK_ERR_INVALID, "%s: negative count", fn);
+  if (count > 0 && !numels) return fail(BEVK_ERR_INVALID, "%s: null array", fn);
+  int64_t total = 0;
+  for (int k = 0; k < count; ++k) {
+    if (numels[k] < 0) return fail(BEVK_ERR_INVALID, "%s: negative size", fn);
+    if (numels[k] > (1LL << 40) || (total += numels[k]) > (1LL << 40))
+      return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
+  }
+  return 0;
+}
+
+// Every output apart from the others and from all inputs but its own, which it may stand in for.
+static int check_grad_overlap(const char *fn, const bevk::GradList &g) {
+  struct Range {
+    uintptr_t at, end;
+    int k;
+  };
+  std::vector<Range> w;
+  w.reserve(g.count);
+  for (int k = 0; k < g.count; ++k)
+    if (g.n[k] > 0) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(g.out[k]);
+      w.push_back({at, at + (uintptr_t)g.n[k] * dtype_size(g.out_type[k]), k});
+    }
+  std::sort(w.begin(), w.end(), [](const Range &a, const Range &b) { return a.at < b.at; });
+  for (size_t j = 1; j < w.size(); ++j)
+    if (w[j].at < w[j - 1].end) return fail(BEVK_ERR_INVALID, "%s: two outputs overlap", fn);
+  for (int k = 0; k < g.count; ++k) {
+    if (g.n[k] == 0) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(g.in[k]);
+    const uintptr_t end = at + (uintptr_t)g.n[k] * dtype_size(g.in_type[k]);
+    auto j = std::upper_bound(w.begin(), w.end(), at, [](uintptr_t a, const Range &r) { return a < r.end; });
+    for (; j != w.end() && j->at < end; ++j)
+      if (j->k != k || j->at != at || g.in_type[k] != g.out_type[k])
+        return fail(BEVK_ERR_INVALID, "%s: an output overlaps an input that is not its own", fn);
+  }
+  return 0;
+}
+
+int64_t bevk_clip_gradients_workspace_bytes(int count, const int64_t *numels) {
+  if (check_grad_sizes("clip_gradients", count, numels)) return -1;
+  return bevk::clip_gradients_workspace_bytes({count, nullptr, nullptr, numels, nullptr, nullptr});
+}
+
+int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes, const int64_t *numels,
+                        void *const *out, const int *out_dtypes, double max_norm, void *workspace,
+                        int64_t workspace_bytes, float *norm, void *stream) {
+  const char *fn = "clip_gradients";
+  g_last_error.clear();
+  if (int rc = check_grad_sizes(fn, count, numels)) return rc;
+  if (count > 0 && (!grads || !dtypes || (out && !out_dtypes)))
+    return fail(BEVK_ERR_INVALID, "%s: null array", fn);
+  for (int k = 0; k < count; ++k) {
+    for (int d : {dtypes[k], out ? out_dtypes[k] : (int)BEVK_F32})
+      if (d != BEVK_F32 && d != BEVK_F16 && d != BEVK_BF16)
+        return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(d));
+    const uintptr_t off = reinterpret_cast<uintptr_t>(grads[k]) % dtype_size(dtypes[k]) +
+                          (out ? reinterpret_cast<uintptr_t>(out[k]) % dtype_size(out_dtypes[k]) : 0);
+    if (numels[k] > 0 && (!grads[k] || (out && !out[k])))
+      return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+    if (off != 0) return fail(BEVK_ERR_INVALID, "%s: a tensor is not aligned to its type", fn);
+  }
+  if (out && !(max_norm >= 0.0)) return fail(BEVK_ERR_INVALID, "%s: max_norm must not be negative", fn);
+  if (!norm) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  const bevk::GradList g{count, grads, dtypes, numels, out, out_dtypes};
+  const int64_t need = bevk::clip_gradients_workspace_bytes(g);
+  if (need > 0 && !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  try {
+    if (out)
+      if (int rc = check_grad_overlap(fn, g)) return rc;
+  } catch (const std::bad_alloc &) {
+    return fail(BEVK_ERR_INVALID, "%s: out of host memory", fn);
+  }
+  return hip_status(bevk::launch_clip_gradients(g, max_norm, workspace, norm, (hipStream_t)stream), fn);
 }
 
 }  // extern "C"

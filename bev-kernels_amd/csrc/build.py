@@ -24,7 +24,8 @@ LIB_PATH = os.path.join(PKG, "libbevk.so")
 
 SOURCES = ["binding.cpp", "msda_fwd.hip", "dcn_gather.hip", "dcn_fused.hip", "dcn_fused_h.hip",
            "dcn_bwd.hip", "msda_bwd.hip", "layout.hip", "dcn_f32.hip",
-           "dcn_wgrad.hip", "group_norm.hip", "embedding.hip"]
+           "dcn_wgrad.hip", "group_norm.hip", "embedding.hip",
+           "grad_clip.hip"]
 ARCH = "gfx950"
 
 

@@ -15,3 +15,4 @@ from .group_norm import (  # noqa: F401
     GroupNormActNHWCFunction,
     group_norm_act_nhwc,
 )
+from .grad_clip import clip_grad_norm_, clip_gradients_, grad_norm  # noqa: F401

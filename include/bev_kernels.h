@@ -506,6 +506,27 @@ int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, 
                             void *workspace, int64_t workspace_bytes, void *grad_weight,
                             void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* The norm of many gradients, and clipping                                   */
+/* ------------------------------------------------------------------------- */
+
+/* norm (fp32, one value, device) = sqrt of the sum of squares over `count` tensors (fp64 sums, the
+ * same on every run), and, where out is not NULL, out[k] = min(1, max_norm / (norm + 1e-6)) *
+ * grads[k], rounded once (no counterpart in the reference):
+ *   grads, dtypes, numels   HOST arrays of `count` device pointers, types (F32, F16, BF16), sizes
+ *   out, out_dtypes         HOST arrays, or NULL for the norm alone. out[k] may be grads[k] in the
+ *                           same type; any other overlap of an output with an input or another
+ *                           output is rejected
+ * A norm that is not finite goes on as in plain arithmetic: Inf makes the factor 0, NaN makes it
+ * NaN. Outputs equal to their inputs are not written again where the factor is 1. The host arrays
+ * are read before the call returns. The workspace holds what bevk_clip_gradients_workspace_bytes
+ * says (-1 for sizes not taken). */
+int64_t bevk_clip_gradients_workspace_bytes(int count, const int64_t *numels);
+int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes,
+                        const int64_t *numels, void *const *out, const int *out_dtypes,
+                        double max_norm, void *workspace, int64_t workspace_bytes, float *norm,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -150,3 +150,78 @@ def test_embedding_c_abi():
     assert bwd(rows=0) == 0 and bwd(dim=0) == 0
     ws = lib.bevk_embedding_backward_workspace_bytes
     assert ws(3, 4, 10, 8) == -1 and ws(0, -1, 10, 8) == -1 and ws(0, 1 << 31, 10, 8) == -1
+
+
+def test_clip_refusals(monkeypatch):
+    f = ext.clip_gradients
+    with pytest.raises(RuntimeError, match="HIP"):
+        mdc.clip_gradients_([torch.zeros(3)], 1.0)
+    with pytest.raises(RuntimeError, match="HIP"):
+        mdc.grad_norm(torch.zeros(3))
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(RuntimeError, match="max_norm"):
+            mdc.clip_gradients_([torch.zeros(3)], bad)
+    with pytest.raises(RuntimeError, match="outputs for 0"):
+        mdc.clip_gradients_([], 1.0, out=[torch.zeros(3)])
+
+    class Fake:  # a device tensor's attributes without a device
+        is_cuda, layout, device = True, torch.strided, "cuda:0"
+
+        def __init__(self, t, index=0):
+            self.t, self.index = t, index
+            self.dtype, self.shape = t.dtype, t.shape
+
+        def get_device(self):
+            return self.index
+
+        def data_ptr(self):
+            return 0x10000
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    a = Fake(torch.zeros(4, 6))
+    for bad, match in (([a, Fake(torch.zeros(2), 1)], "different devices"),
+                       ([Fake(torch.zeros(4, 6)[:, :3])], "dense"),
+                       ([Fake(torch.zeros(4, 1).expand(4, 6))], "dense"),
+                       ([Fake(torch.zeros(4).long())], "not supported")):
+        with pytest.raises(RuntimeError, match=match):
+            f(bad, 1.0)
+    for out, match in (([], "0 outputs for 1"), ([Fake(torch.zeros(6, 4))], "an output has shape"),
+                       ([Fake(torch.zeros(6, 4).t())], "an output has shape")):
+        with pytest.raises(RuntimeError, match=match):
+            f([a], 1.0, out)
+
+
+def test_clip_c_abi():
+    lib = _bevk.lib()
+
+    def call(types=(0, 1), sizes=(100, 50), at=(0x10000, 0x20000), out=None, out_types=None, max_norm=1.0,
+             ws=P, wb=1 << 30, norm=P):
+        n = len(sizes)
+        arr = lambda t, v: None if v is None else (t * n)(*v)  # noqa: E731
+        return lib.bevk_clip_gradients(n, arr(ctypes.c_void_p, at), arr(ctypes.c_int, types),
+                                       arr(ctypes.c_int64, sizes), arr(ctypes.c_void_p, out),
+                                       arr(ctypes.c_int, out_types), max_norm, ws, wb, norm, None)
+
+    assert call(types=(0, 3)) == UNSUPPORTED and "Double" in _err()
+    assert call(sizes=(-1, 5)) == INVALID and "negative" in _err()
+    assert call(sizes=(1 << 40, 1)) == INVALID and "2^40" in _err()
+    assert call(at=(0x10000, 0)) == INVALID and "null" in _err()
+    assert call(at=(0x10002, 0x20000)) == INVALID and "aligned" in _err()
+    assert call(norm=None) == INVALID and "null" in _err()
+    assert call(at=None) == INVALID and "null" in _err()
+    assert call(ws=None) == INVALID and "null" in _err()
+    assert call(wb=8) == INVALID and "workspace" in _err()
+    both = dict(out=(0x10000, 0x20000), out_types=(0, 1))
+    for bad in (-1.0, float("nan")):
+        assert call(**both, max_norm=bad) == INVALID and "max_norm" in _err()
+    assert call(out=(0x30000, 0x30000 + 396), out_types=(0, 1)) == INVALID and "two outputs" in _err()
+    assert call(out=(0x10000, 0x10100), out_types=(0, 1)) == INVALID and "overlap" in _err()
+    assert call(out=(0x10004, 0x20000), out_types=(0, 1)) == INVALID and "not its own" in _err()
+    assert call(out=(0x20000, 0x10000), out_types=(0, 1)) == INVALID and "not its own" in _err()
+    assert call(out=(0x10000, 0x20000), out_types=(0, 0)) == INVALID and "not its own" in _err()
+    assert lib.bevk_clip_gradients(-1, None, None, None, None, None, 1.0, P, 8, P, None) == INVALID
+    ws = lib.bevk_clip_gradients_workspace_bytes
+    assert ws(0, None) == 0 and ws(-1, None) == -1 and ws(1, None) == -1
+    assert ws(2, (ctypes.c_int64 * 2)(1, 0)) == 8
