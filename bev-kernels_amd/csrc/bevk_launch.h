@@ -203,7 +203,7 @@ struct EmbeddingArgs {
 };
 hipError_t launch_embedding_forward(int dtype, const EmbeddingArgs &a, const void *weight, void *out,
                                     hipStream_t stream);
-int64_t embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim);
+int64_t embedding_backward_workspace_bytes(int64_t n, int64_t rows, int dim);
 hipError_t launch_embedding_backward(int dtype, const EmbeddingArgs &a, const void *grad_out, int64_t padding,
                                      void *workspace, void *grad_w, hipStream_t stream);
 

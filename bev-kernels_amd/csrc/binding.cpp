@@ -1279,7 +1279,7 @@ int bevk_embedding_forward(int dtype, const void *weight, int64_t rows, int dim,
 
 int64_t bevk_embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim) {
   if (check_embedding("embedding_backward", dtype, n, rows, dim)) return -1;
-  return bevk::embedding_backward_workspace_bytes(dtype, n, rows, dim);
+  return bevk::embedding_backward_workspace_bytes(n, rows, dim);
 }
 
 int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, int index64, int64_t n,
@@ -1291,7 +1291,7 @@ int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, 
   if (padding_idx < -1 || (padding_idx >= rows && padding_idx != -1))
     return fail(BEVK_ERR_INVALID, "%s: padding_idx must be a row of the table, or -1", fn);
   if (rows == 0 || dim == 0) return ok();
-  const int64_t need = bevk::embedding_backward_workspace_bytes(dtype, n, rows, dim);
+  const int64_t need = bevk::embedding_backward_workspace_bytes(n, rows, dim);
   if ((n > 0 && (!grad_out || !index)) || !grad_weight || (need > 0 && !workspace))
     return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);

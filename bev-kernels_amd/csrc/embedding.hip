@@ -1,73 +1,376 @@
 // Embedding rows by index with a scale, and the gradient of the table (gfx950).
 //
 //   out[t] = scale * W[i_t], zeros where i_t is outside [0, rows) (a padded place)
-//   gW[v]  = scale * sum over t with i_t = v of g[t], in the order of t, in fp32
+//   gW[v]  = scale * sum over t with i_t = v of g[t], in fp32 and in an order that does not change
+//
+// Both are bound by memory: a row read for a row written. The gradient's rows come sorted by index:
+//   sort   one launch without a pass between workgroups: workgroup w of R (a power of two) owns the
+//          rows v with v % R = w, so that frequent neighbours spread over workgroups, and reads all
+//          indices, which cost it n * 8 bytes out of L2. It counts its rows' places, knows its part
+//          of the sorted list from how many indices belong to workgroups before it, and writes
+//          that part in the order of t.
+//   sum    a group of lanes for each row of the table adds up its rows of g and writes the sum (or
+//          zeros). Rows with more than kChunk places are left to workgroups for kChunk places of
+//          the sorted list, which write partial sums, so that a row that many places share
+//          does not hang on one group of lanes.
+//   join   adds up the partial sums of those rows in the order of their chunks.
+#include <algorithm>
+
 #include "bevk_launch.h"
 
 namespace bevk {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kSortRows = 512;  // counters of 16 waves: 32 KB
+constexpr int kChunk = 32;
 
-template <typename T, typename I>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(const T *__restrict__ weight, int64_t rows, int dim,
-                                                          const I *__restrict__ index, int64_t total, float scale,
-                                                          T *__restrict__ out) {
-  for (int64_t k = blockIdx.x * (int64_t)kThreads + threadIdx.x; k < total; k += (int64_t)gridDim.x * kThreads) {
-    const int64_t v = (int64_t)index[k / dim];
-    out[k] = v >= 0 && v < rows ? static_cast<T>((float)weight[v * dim + k % dim] * scale) : static_cast<T>(0.f);
+// N elements of T from memory aligned to them all together.
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T *p, float *v) {
+  const Vec<T, N> x = load_vec<T, N>(p);
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = (float)x.v[e];
+}
+
+// ---------------------------------------------------------------------------------------
+// Lookup
+// ---------------------------------------------------------------------------------------
+
+// A workgroup takes kThreads * kUnroll vectors of the output in a row; the indices of a thread's
+// vectors are all loaded before their rows, and those before any store.
+constexpr int kUnroll = 4;
+template <typename T, typename I, int N>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const T *__restrict__ weight, int64_t rows,
+                                                          uint32_t vecs, const I *__restrict__ index,
+                                                          int64_t total, float scale, T *__restrict__ out) {
+  const int64_t base = blockIdx.x * (int64_t)(kThreads * kUnroll);
+  const int64_t t0 = base / vecs;
+  const uint32_t r0 = (uint32_t)(base - t0 * vecs);
+  int64_t row[kUnroll];
+  uint32_t col[kUnroll];
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    const uint32_t o = r0 + j * kThreads + threadIdx.x, t = o / vecs;
+    col[j] = o - t * vecs;
+    row[j] = base + j * kThreads + threadIdx.x < total ? (int64_t)index[t0 + t] : -1;
+  }
+  Vec<T, N> x[kUnroll];
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    if (row[j] >= 0 && row[j] < rows) {
+      x[j] = load_vec<T, N>(weight + (row[j] * vecs + col[j]) * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[j].v[e] = static_cast<T>((float)x[j].v[e] * scale);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[j].v[e] = static_cast<T>(0.f);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    const int64_t k = base + j * kThreads + threadIdx.x;
+    if (k < total) store_vec<T, N>(out + k * N, x[j]);
   }
 }
 
-// One wave for a row of the table and 64 of its channels.
-template <typename T, typename I>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const T *__restrict__ g, const I *__restrict__ index,
-                                                        int64_t n, int64_t rows, int dim, float scale,
-                                                        int64_t padding, T *__restrict__ gw) {
-  const int pieces = (dim + 63) / 64, lane = threadIdx.x % kWave;
-  for (int64_t u = blockIdx.x * (int64_t)(kThreads / kWave) + threadIdx.x / kWave; u < rows * pieces;
-       u += (int64_t)gridDim.x * (kThreads / kWave)) {
-    const int64_t v = u / pieces;
-    const int c = (int)(u % pieces) * 64 + lane;
-    float a = 0.f;
-    for (int64_t t = 0; t < n && v != padding; t += 64) {
-      uint64_t hit = __ballot(t + lane < n && (int64_t)index[t + lane < n ? t + lane : 0] == v);
-      while (hit) {
-        const int k = __builtin_ctzll(hit);
-        hit &= hit - 1;
-        if (c < dim) a += (float)g[(t + k) * dim + c];
+// ---------------------------------------------------------------------------------------
+// Gradient
+// ---------------------------------------------------------------------------------------
+
+// Places of the rows in the sorted list.
+struct Sorted {
+  int2 *span;    // [rows] first place and count
+  int *order;    // [n] t of each place
+  int *row;      // [n] row of each place
+  int *valid;    // places in use
+};
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict__ index, uint32_t n, int64_t rows,
+                                                            int log_r, int per, int64_t padding, Sorted out) {
+  extern __shared__ int count[];  // [wave][per]
+  __shared__ int before[kSortWaves], wave_sum[kSortWaves];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, w = blockIdx.x;
+  const int64_t mask = (1 << log_r) - 1;
+  int *mine = count + wave * per;
+  for (int i = threadIdx.x; i < kSortWaves * per; i += kSortThreads) count[i] = 0;
+  __syncthreads();
+
+  const uint32_t seg = (n + kSortThreads - 1) / kSortThreads * kWave;  // indices of a wave
+  const uint32_t begin = min((uint32_t)wave * seg, n), end = min(begin + seg, n);
+  auto row_at = [&](uint32_t t) __attribute__((always_inline)) {
+    const int64_t v = t < end ? (int64_t)index[t] : -1;
+    return v < rows && v != padding ? v : -1;
+  };
+  int lower = 0;
+  for (uint32_t t = begin; t < end; t += 4 * kWave) {
+    int64_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = row_at(t + j * kWave + lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lower += __popcll(__ballot(v[j] >= 0 && (v[j] & mask) < w));
+      if (v[j] >= 0 && (v[j] & mask) == w) atomicAdd(&mine[v[j] >> log_r], 1);
+    }
+  }
+  if (lane == 0) before[wave] = lower;
+  __syncthreads();
+
+  // First place of every row, and of every wave's part in it.
+  const int i = threadIdx.x;
+  int total = 0;
+  if (i < per)
+    for (int k = 0; k < kSortWaves; ++k) total += count[k * per + i];
+  int sum = total;
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int up = __shfl_up(sum, d, kWave);
+    if (lane >= d) sum += up;
+  }
+  if (lane == kWave - 1) wave_sum[wave] = sum;
+  __syncthreads();
+  int at = sum - total;
+  for (int k = 0; k < kSortWaves; ++k) {
+    at += before[k];
+    if (k < wave) at += wave_sum[k];
+  }
+  if (i < per) {
+    const int64_t v = ((int64_t)i << log_r) | w;
+    if (v < rows) out.span[v] = make_int2(at, total);
+    int run = at;
+    for (int k = 0; k < kSortWaves; ++k) {
+      const int c = count[k * per + i];
+      count[k * per + i] = run;
+      run += c;
+    }
+  }
+  if (w == (int)gridDim.x - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
+  __syncthreads();
+
+  for (uint32_t t = begin; t < end; t += 4 * kWave) {
+    int64_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = row_at(t + j * kWave + lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool own = v[j] >= 0 && (v[j] & mask) == w;
+      const int r = (int)(v[j] >> log_r);
+      uint64_t left = __ballot(own);
+      while (left) {  // one row of this workgroup at a time; its lanes in their order
+        const int lead = __builtin_ctzll(left);
+        const uint64_t same = __ballot(own && r == __builtin_amdgcn_readlane(r, lead));
+        int place = 0;
+        if (lane == lead) place = atomicAdd(&mine[r], __popcll(same));
+        place = __builtin_amdgcn_readlane(place, lead);
+        if (same >> lane & 1) {
+          place += __popcll(same & ((1ull << lane) - 1));
+          out.order[place] = (int)(t + j * kWave + lane);
+          out.row[place] = (int)v[j];
+        }
+        left &= ~same;
       }
     }
-    if (c < dim) gw[v * dim + c] = static_cast<T>(a * scale);
   }
 }
 
-int grid_for(int64_t threads) {
-  const int64_t b = (threads + kThreads - 1) / kThreads;
-  return (int)(b < 16384 ? b : 16384);
+// Sum and join give a group of `lanes` lanes (a power of two) one slice of a row: N channels each.
+struct SumArgs {
+  int64_t rows;
+  int dim, lanes, slices, chunk_blocks;
+  float scale;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void add_row(const T *g, int64_t at, float *a) {
+  float v[N];
+  load_f32<T, N>(g + at, v);
+#pragma unroll
+  for (int e = 0; e < N; ++e) a[e] += v[e];
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void write_row(T *gw, int64_t at, const float *a, float scale) {
+  Vec<T, N> x;
+#pragma unroll
+  for (int e = 0; e < N; ++e) x.v[e] = static_cast<T>(a[e] * scale);
+  store_vec<T, N>(gw + at, x);
+}
+
+// The two rows of more than kChunk places that a chunk of the sorted list can hold: one from the
+// chunks before (places [0, head)) and one that goes on after it (places [tail, kChunk)).
+struct Shared {
+  int head, tail;
+};
+__device__ __forceinline__ Shared shared_rows(const Sorted &s, int chunk, int valid, int2 &span) {
+  const int lane = threadIdx.x % kWave, place = chunk * kChunk + lane;
+  span = make_int2(0, 0);
+  if (lane < kChunk && place < valid) span = s.span[s.row[place]];
+  const bool many = span.y > kChunk;
+  return {(int)__popcll(__ballot(many && span.x < chunk * kChunk)),
+          kChunk - (int)__popcll(__ballot(many && span.x >= chunk * kChunk))};
+}
+
+// a of the workgroup's groups of lanes added up in their order, into the first group's.
+template <int N>
+__device__ __forceinline__ void add_groups(float *a, float *s, int lanes) {
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[threadIdx.x * N + e] = a[e];
+  __syncthreads();
+  if ((int)threadIdx.x < lanes)
+    for (int k = threadIdx.x + lanes; k < kThreads; k += lanes)
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] += s[k * N + e];
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const T *__restrict__ g, Sorted s, SumArgs p,
+                                                       float *__restrict__ part, T *__restrict__ gw) {
+  __shared__ float buf[kThreads * N];
+  const int lane = threadIdx.x % p.lanes, group = threadIdx.x / p.lanes, groups = kThreads / p.lanes;
+  if ((int)blockIdx.x < p.chunk_blocks) {
+    const int chunk = blockIdx.x / p.slices, c = (blockIdx.x % p.slices * p.lanes + lane) * N;
+    int2 span;
+    const Shared sh = shared_rows(s, chunk, *s.valid, span);
+    for (int side = 0; side < 2; ++side) {
+      const int lo = side ? sh.tail : 0, hi = side ? kChunk : sh.head;
+      if (lo >= hi) continue;
+      float a[N] = {};
+      if (c < p.dim)
+#pragma unroll 4
+        for (int k = lo + group; k < hi; k += groups)
+          add_row<T, N>(g, (int64_t)s.order[chunk * kChunk + k] * p.dim + c, a);
+      add_groups<N>(a, buf, p.lanes);
+      if (group == 0 && c < p.dim)
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[((int64_t)chunk * 2 + side) * p.dim + c + e] = a[e];
+    }
+    return;
+  }
+  const int64_t units = p.rows * p.slices;
+  for (int64_t u = (int64_t)(blockIdx.x - p.chunk_blocks) * groups + group; u < units;
+       u += (int64_t)(gridDim.x - p.chunk_blocks) * groups) {
+    const int64_t v = u / p.slices;
+    const int c = ((int)(u - v * p.slices) * p.lanes + lane) * N;
+    const int2 span = s.span != nullptr ? s.span[v] : make_int2(0, 0);
+    if (c >= p.dim || span.y > kChunk) continue;
+    float a[N] = {};
+#pragma unroll 4
+    for (int k = 0; k < span.y; ++k) add_row<T, N>(g, (int64_t)s.order[span.x + k] * p.dim + c, a);
+    write_row<T, N>(gw, v * p.dim + c, a, p.scale);
+  }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) join_kernel(Sorted s, SumArgs p, const float *__restrict__ part,
+                                                        T *__restrict__ gw) {
+  __shared__ float buf[kThreads * N];
+  const int lane = threadIdx.x % p.lanes, group = threadIdx.x / p.lanes, groups = kThreads / p.lanes;
+  const int chunk = blockIdx.x / p.slices, c = (blockIdx.x % p.slices * p.lanes + lane) * N;
+  int2 span;
+  const Shared sh = shared_rows(s, chunk, *s.valid, span);
+  if (sh.tail == kChunk) return;  // no such row begins here
+  span.x = __builtin_amdgcn_readlane(span.x, kChunk - 1);
+  span.y = __builtin_amdgcn_readlane(span.y, kChunk - 1);
+  const int64_t v = s.row[span.x];
+  const int more = (span.x + span.y - 1) / kChunk - chunk, each = (more + groups) / groups;
+  float a[N] = {};
+  if (c < p.dim)
+#pragma unroll 4
+    for (int k = group * each; k < min((group + 1) * each, more + 1); ++k)
+      add_row<float, N>(part, ((int64_t)(chunk + k) * 2 + (k == 0 ? 1 : 0)) * p.dim + c, a);
+  add_groups<N>(a, buf, p.lanes);
+  if (group == 0 && c < p.dim) write_row<T, N>(gw, v * p.dim + c, a, p.scale);
+}
+
+int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+
+// Workspace: span, order, row, valid, then the partial sums.
+struct Layout {
+  int64_t order, row, valid, part, total;
+  Layout(int64_t n, int64_t rows, int dim) {
+    order = align256(rows * 8);
+    row = order + align256(n * 4);
+    valid = row + align256(n * 4);
+    part = valid + 256;
+    total = n == 0 ? 0 : part + (n > kChunk ? (n + kChunk - 1) / kChunk * 2 * dim * 4 : 0);
+  }
+};
+
+// Channels a lane takes: 16 or 8 bytes of them where rows and tensors are aligned to that.
+int lane_bytes(int64_t row_bytes, const void *a, const void *b) {
+  const uintptr_t all = (uintptr_t)row_bytes | reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b);
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : 0;
+}
+
+template <typename T, typename I, int N>
+hipError_t forward_n(const EmbeddingArgs &a, const void *weight, void *out, hipStream_t stream) {
+  const int64_t total = a.n * (a.dim / N), blocks = (total + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((lookup_kernel<T, I, N>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
+                     static_cast<const T *>(weight), a.rows, (uint32_t)(a.dim / N),
+                     static_cast<const I *>(a.index), total, a.scale, static_cast<T *>(out));
+  return hipGetLastError();
 }
 
 template <typename T, typename I>
 hipError_t forward(const EmbeddingArgs &a, const void *weight, void *out, hipStream_t stream) {
-  const int64_t total = a.n * a.dim;
-  hipLaunchKernelGGL((lookup_kernel<T, I>), dim3(grid_for(total)), dim3(kThreads), 0, stream,
-                     static_cast<const T *>(weight), a.rows, a.dim, static_cast<const I *>(a.index), total, a.scale,
-                     static_cast<T *>(out));
+  switch (lane_bytes((int64_t)a.dim * sizeof(T), weight, out)) {
+    case 16: return forward_n<T, I, 16 / sizeof(T)>(a, weight, out, stream);
+    case 8: return forward_n<T, I, 8 / sizeof(T)>(a, weight, out, stream);
+    default: return forward_n<T, I, 1>(a, weight, out, stream);
+  }
+}
+
+template <typename T, int N>
+hipError_t sums(const EmbeddingArgs &a, const void *grad_out, const Sorted &s, float *part, void *grad_w,
+                hipStream_t stream) {
+  SumArgs p;
+  p.rows = a.rows; p.dim = a.dim; p.scale = a.scale;
+  p.lanes = 1;
+  while (p.lanes < kWave && p.lanes * N < a.dim) p.lanes *= 2;
+  p.slices = (a.dim + p.lanes * N - 1) / (p.lanes * N);
+  const int64_t chunks = a.n > kChunk ? (a.n + kChunk - 1) / kChunk * p.slices : 0;
+  const int64_t row_blocks = std::min<int64_t>(1 << 20, (a.rows * p.slices + kThreads / p.lanes - 1) /
+                                                            (kThreads / p.lanes));
+  if (chunks > 1 << 30) return hipErrorInvalidValue;
+  p.chunk_blocks = (int)chunks;
+  hipLaunchKernelGGL((sum_kernel<T, N>), dim3((unsigned)(chunks + row_blocks)), dim3(kThreads), 0, stream,
+                     static_cast<const T *>(grad_out), s, p, part, static_cast<T *>(grad_w));
+  if (chunks > 0)
+    hipLaunchKernelGGL((join_kernel<T, N>), dim3((unsigned)chunks), dim3(kThreads), 0, stream, s, p, part,
+                       static_cast<T *>(grad_w));
   return hipGetLastError();
 }
 
 template <typename T, typename I>
-hipError_t backward(const EmbeddingArgs &a, const void *grad_out, int64_t padding, void *grad_w,
+hipError_t backward(const EmbeddingArgs &a, const void *grad_out, int64_t padding, void *workspace, void *grad_w,
                     hipStream_t stream) {
-  hipLaunchKernelGGL((grad_kernel<T, I>), dim3(grid_for(a.rows * ((a.dim + 63) / 64) * kWave)), dim3(kThreads), 0,
-                     stream, static_cast<const T *>(grad_out), static_cast<const I *>(a.index), a.n, a.rows, a.dim,
-                     a.scale, padding, static_cast<T *>(grad_w));
-  return hipGetLastError();
+  const Layout l(a.n, a.rows, a.dim);
+  char *ws = static_cast<char *>(workspace);
+  Sorted s{};
+  if (a.n > 0) {
+    s = {reinterpret_cast<int2 *>(ws), reinterpret_cast<int *>(ws + l.order), reinterpret_cast<int *>(ws + l.row),
+         reinterpret_cast<int *>(ws + l.valid)};
+    int log_r = 8;  // 256 workgroups, or as many as have at most kSortRows rows each
+    while ((a.rows - 1) >> log_r >= kSortRows) ++log_r;
+    const int per = (int)((a.rows - 1) >> log_r) + 1;
+    hipLaunchKernelGGL((sort_kernel<I>), dim3(1 << log_r), dim3(kSortThreads), kSortWaves * per * 4, stream,
+                       static_cast<const I *>(a.index), (uint32_t)a.n, a.rows, log_r, per, padding, s);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  float *part = reinterpret_cast<float *>(ws + l.part);
+  switch (lane_bytes((int64_t)a.dim * sizeof(T), grad_out, grad_w)) {
+    case 16: return sums<T, 16 / sizeof(T)>(a, grad_out, s, part, grad_w, stream);
+    case 8: return sums<T, 8 / sizeof(T)>(a, grad_out, s, part, grad_w, stream);
+    default: return sums<T, 1>(a, grad_out, s, part, grad_w, stream);
+  }
 }
 
 }  // namespace
 
-int64_t embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim) { return 0; }
+int64_t embedding_backward_workspace_bytes(int64_t n, int64_t rows, int dim) { return Layout(n, rows, dim).total; }
 
 hipError_t launch_embedding_forward(int dtype, const EmbeddingArgs &a, const void *weight, void *out,
                                     hipStream_t stream) {
@@ -84,12 +387,12 @@ hipError_t launch_embedding_forward(int dtype, const EmbeddingArgs &a, const voi
 hipError_t launch_embedding_backward(int dtype, const EmbeddingArgs &a, const void *grad_out, int64_t padding,
                                      void *workspace, void *grad_w, hipStream_t stream) {
   switch (dtype * 2 + (a.index64 ? 1 : 0)) {
-    case 0: return backward<float, int32_t>(a, grad_out, padding, grad_w, stream);
-    case 1: return backward<float, int64_t>(a, grad_out, padding, grad_w, stream);
-    case 2: return backward<f16, int32_t>(a, grad_out, padding, grad_w, stream);
-    case 3: return backward<f16, int64_t>(a, grad_out, padding, grad_w, stream);
-    case 4: return backward<bf16, int32_t>(a, grad_out, padding, grad_w, stream);
-    default: return backward<bf16, int64_t>(a, grad_out, padding, grad_w, stream);
+    case 0: return backward<float, int32_t>(a, grad_out, padding, workspace, grad_w, stream);
+    case 1: return backward<float, int64_t>(a, grad_out, padding, workspace, grad_w, stream);
+    case 2: return backward<f16, int32_t>(a, grad_out, padding, workspace, grad_w, stream);
+    case 3: return backward<f16, int64_t>(a, grad_out, padding, workspace, grad_w, stream);
+    case 4: return backward<bf16, int32_t>(a, grad_out, padding, workspace, grad_w, stream);
+    default: return backward<bf16, int64_t>(a, grad_out, padding, workspace, grad_w, stream);
   }
 }
 
