@@ -87,34 +87,81 @@ struct Sorted {
   int *valid;    // places in use
 };
 
+// The row an index stands for, and the workgroup that owns it: R for an index without a row. An
+// index is compared as unsigned numbers, so that negative ones are past the table too.
+struct Owned {
+  uint32_t row, owner;
+};
+struct SortArgs {
+  uint32_t n, rows, padding;  // padding: ~0 for none
+  int log_r, per;             // rows v with v % R = w are a workgroup's; at most `per` of them
+};
 template <typename I>
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict__ index, uint32_t n, int64_t rows,
-                                                            int log_r, int per, int64_t padding, Sorted out) {
+__device__ __forceinline__ Owned owned(const I *index, uint32_t t, const SortArgs &p) {
+  uint32_t row, high = 0;
+  if constexpr (sizeof(I) == 8) {
+    const uint2 v = reinterpret_cast<const uint2 *>(index)[t];
+    row = v.x;
+    high = v.y;
+  } else {
+    row = (uint32_t)index[t];
+  }
+  const uint32_t count = 1u << p.log_r;
+  return {row, high == 0 && row < p.rows && row != p.padding ? row & (count - 1) : count};
+}
+
+// f(t of the wave's first lane, its 64 indices) over [begin, end), kScan times 64 of them loaded
+// together; lanes past the end have no row.
+constexpr int kScan = 8;
+template <typename I, typename F>
+__device__ __forceinline__ void scan(const I *index, uint32_t begin, uint32_t end, const SortArgs &p, F f) {
+  const int lane = threadIdx.x % kWave;
+  uint32_t t = begin;
+  for (; t + kScan * kWave <= end; t += kScan * kWave) {
+    Owned o[kScan];
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) o[j] = owned(index, t + j * kWave + lane, p);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) f(t + j * kWave, o[j]);
+  }
+  for (; t < end; t += kWave) {
+    Owned o = owned(index, min(t + lane, end - 1), p);
+    if (t + lane >= end) o.owner = 1u << p.log_r;
+    f(t, o);
+  }
+}
+
+// Two passes over the indices' owners, one where no wave finds more than kKept of its workgroup's
+// (n / (16 R) on average): those it keeps.
+constexpr int kKept = 128;
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict__ index, SortArgs p, Sorted out) {
   extern __shared__ int count[];  // [wave][per]
   __shared__ int before[kSortWaves], wave_sum[kSortWaves];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, w = blockIdx.x;
-  const int64_t mask = (1 << log_r) - 1;
+  __shared__ uint2 kept[kSortWaves][kKept];  // (t, row of the workgroup)
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, per = p.per;
+  const uint32_t w = blockIdx.x;
   int *mine = count + wave * per;
   for (int i = threadIdx.x; i < kSortWaves * per; i += kSortThreads) count[i] = 0;
   __syncthreads();
 
-  const uint32_t seg = (n + kSortThreads - 1) / kSortThreads * kWave;  // indices of a wave
-  const uint32_t begin = min((uint32_t)wave * seg, n), end = min(begin + seg, n);
-  auto row_at = [&](uint32_t t) __attribute__((always_inline)) {
-    const int64_t v = t < end ? (int64_t)index[t] : -1;
-    return v < rows && v != padding ? v : -1;
-  };
+  const uint32_t seg = (p.n + kSortThreads - 1) / kSortThreads * kWave;  // indices of a wave
+  const uint32_t begin = min((uint32_t)wave * seg, p.n), end = min(begin + seg, p.n);
+  const uint64_t lanes_before = (1ull << lane) - 1;
   int lower = 0;
-  for (uint32_t t = begin; t < end; t += 4 * kWave) {
-    int64_t v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = row_at(t + j * kWave + lane);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      lower += __popcll(__ballot(v[j] >= 0 && (v[j] & mask) < w));
-      if (v[j] >= 0 && (v[j] & mask) == w) atomicAdd(&mine[v[j] >> log_r], 1);
+  uint32_t found = 0;
+  scan(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
+    lower += __popcll(__ballot(o.owner < w));
+    const uint64_t own = __ballot(o.owner == w);
+    if (own) {
+      if (o.owner == w) {
+        const uint32_t k = found + __popcll(own & lanes_before), r = o.row >> p.log_r;
+        if (k < kKept) kept[wave][k] = make_uint2(t + lane, r);
+        atomicAdd(&mine[r], 1);
+      }
+      found += __popcll(own);
     }
-  }
+  });
   if (lane == 0) before[wave] = lower;
   __syncthreads();
 
@@ -136,8 +183,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
     if (k < wave) at += wave_sum[k];
   }
   if (i < per) {
-    const int64_t v = ((int64_t)i << log_r) | w;
-    if (v < rows) out.span[v] = make_int2(at, total);
+    const uint32_t v = ((uint32_t)i << p.log_r) | w;
+    if (v < p.rows) out.span[v] = make_int2(at, total);
     int run = at;
     for (int k = 0; k < kSortWaves; ++k) {
       const int c = count[k * per + i];
@@ -145,32 +192,35 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
       run += c;
     }
   }
-  if (w == (int)gridDim.x - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
+  if (w == gridDim.x - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
   __syncthreads();
 
-  for (uint32_t t = begin; t < end; t += 4 * kWave) {
-    int64_t v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = row_at(t + j * kWave + lane);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool own = v[j] >= 0 && (v[j] & mask) == w;
-      const int r = (int)(v[j] >> log_r);
-      uint64_t left = __ballot(own);
-      while (left) {  // one row of this workgroup at a time; its lanes in their order
-        const int lead = __builtin_ctzll(left);
-        const uint64_t same = __ballot(own && r == __builtin_amdgcn_readlane(r, lead));
-        int place = 0;
-        if (lane == lead) place = atomicAdd(&mine[r], __popcll(same));
-        place = __builtin_amdgcn_readlane(place, lead);
-        if (same >> lane & 1) {
-          place += __popcll(same & ((1ull << lane) - 1));
-          out.order[place] = (int)(t + j * kWave + lane);
-          out.row[place] = (int)v[j];
-        }
-        left &= ~same;
+  // Places of up to 64 of the wave's indices, in their order: a row at a time.
+  auto place = [&](bool own, uint32_t t, uint32_t r) __attribute__((always_inline)) {
+    uint64_t left = __ballot(own);
+    while (left) {
+      const int lead = __builtin_ctzll(left);
+      const uint64_t same = __ballot(own && r == (uint32_t)__builtin_amdgcn_readlane((int)r, lead));
+      int first = 0;
+      if (lane == lead) first = atomicAdd(&mine[r], __popcll(same));
+      first = __builtin_amdgcn_readlane(first, lead);
+      if (same >> lane & 1) {
+        const int k = first + __popcll(same & lanes_before);
+        out.order[k] = (int)t;
+        out.row[k] = (int)((r << p.log_r) | w);
       }
+      left &= ~same;
     }
+  };
+  if (found <= kKept) {
+    for (uint32_t k = 0; k < found; k += kWave) {
+      const uint2 e = kept[wave][min(k + lane, kKept - 1u)];
+      place(k + lane < found, e.x, e.y);
+    }
+  } else {
+    scan(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
+      place(o.owner == w, t + lane, o.row >> p.log_r);
+    });
   }
 }
 
@@ -353,11 +403,13 @@ hipError_t backward(const EmbeddingArgs &a, const void *grad_out, int64_t paddin
   if (a.n > 0) {
     s = {reinterpret_cast<int2 *>(ws), reinterpret_cast<int *>(ws + l.order), reinterpret_cast<int *>(ws + l.row),
          reinterpret_cast<int *>(ws + l.valid)};
-    int log_r = 8;  // 256 workgroups, or as many as have at most kSortRows rows each
-    while ((a.rows - 1) >> log_r >= kSortRows) ++log_r;
-    const int per = (int)((a.rows - 1) >> log_r) + 1;
-    hipLaunchKernelGGL((sort_kernel<I>), dim3(1 << log_r), dim3(kSortThreads), kSortWaves * per * 4, stream,
-                       static_cast<const I *>(a.index), (uint32_t)a.n, a.rows, log_r, per, padding, s);
+    SortArgs p;
+    p.n = (uint32_t)a.n; p.rows = (uint32_t)a.rows; p.padding = (uint32_t)padding;
+    p.log_r = 8;  // 256 workgroups, or as many as have at most kSortRows rows each
+    while ((a.rows - 1) >> p.log_r >= kSortRows) ++p.log_r;
+    p.per = (int)((a.rows - 1) >> p.log_r) + 1;
+    hipLaunchKernelGGL((sort_kernel<I>), dim3(1 << p.log_r), dim3(kSortThreads), kSortWaves * p.per * 4, stream,
+                       static_cast<const I *>(a.index), p, s);
     if (hipError_t e = hipGetLastError()) return e;
   }
   float *part = reinterpret_cast<float *>(ws + l.part);
