@@ -13,7 +13,8 @@ import ctypes
 import os
 import threading
 
-import torch  # noqa: F401  (must be imported before the library is loaded)
+import torch  # must be imported before the library is loaded
+from torch.autograd.function import once_differentiable as _once_differentiable
 
 _LIB_NAME = "libbevk.so"
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -167,15 +168,42 @@ def call(name: str, *args) -> None:
         raise RuntimeError(msg or f"{name} failed with status {rc}")
 
 
-def call_on(t: torch.Tensor, name: str, *args) -> None:
-    """call() with t's device current and its current stream as the last argument: a launch goes
-    to the current device, which may be another one than the tensors'."""
-    index = t.get_device()
-    if index == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_entries = {}
+
+
+def entry(name: str):
+    """The library's function `name` (looked up once: a small call is as long as its host side)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    return fn
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """call() with device `index` current and its current stream as the last argument: a launch
+    goes to the current device, which may be another one than the tensors'."""
+    fn = _entries.get(name) or entry(name)
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        msg = lib().bevk_last_error().decode(errors="replace")
+        raise RuntimeError(msg or f"{name} failed with status {rc}")
+
+
+def once_differentiable(backward):
+    """torch's once_differentiable where a graph of the backward is asked for; without one the
+    function itself (the decorator's own bookkeeping takes the autograd thread 5 us and more)."""
+    checked = _once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -17,6 +17,7 @@ added to what the caller passes, everything else is written.
 """
 from __future__ import annotations
 
+import functools
 import os
 from array import array
 
@@ -963,59 +964,76 @@ GROUP_NORM_ACTS = {None: 0, "relu": 1, "silu": 2}
 
 
 def _group_norm_check(fn, x, num_groups, weight, bias, act):
-    """Checks shared by both directions; returns (images, positions, channels, type of the
-    parameters, code of the activation)."""
-    _b.require_device(fn, x, weight, bias)
-    if x.dim() < 3:
-        raise RuntimeError(f"{fn}: expected x [N, ..., C] with positions between, got "
-                           f"{tuple(x.shape)}")
-    _b.require_contiguous(fn, x=x, weight=weight, bias=bias)
+    """Checks shared by both directions. Kept to plain attribute tests, as MSDA's: a small call is
+    as long as its host side."""
+    if not x.is_cuda:
+        _b.require_device(fn, x)
+    index, shape, dtype = x.get_device(), x.shape, x.dtype
+    if len(shape) < 3:
+        raise RuntimeError(f"{fn}: expected x [N, ..., C] with positions between, got {tuple(shape)}")
+    if not x.is_contiguous():
+        raise RuntimeError("x must be contiguous")
     if act not in GROUP_NORM_ACTS:
         raise RuntimeError(f"{fn}: act must be None, 'relu' or 'silu', got {act!r}")
-    channels = x.size(-1)
+    channels = shape[-1]
     if num_groups <= 0 or channels % num_groups != 0:
         raise RuntimeError(f"{fn}: channels ({channels}) must be divisible by num_groups "
                            f"({num_groups})")
-    ptype = None
+    if dtype not in _GROUP_NORM_TYPES:
+        _b.dtype_code(x)
+        raise RuntimeError(f"{fn}: not implemented for {dtype}")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (channels,):
+        if not p.is_cuda or p.get_device() != index:
+            _b.require_device(fn, x, p)
+        if p.shape != (channels,):
             raise RuntimeError(f"{fn}: {name} must be [{channels}], got {tuple(p.shape)}")
-        if p.dtype != x.dtype and p.dtype != torch.float32:
-            raise RuntimeError(f"{fn}: {name} has dtype {p.dtype}, expected {x.dtype} or "
+        if not p.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+        if p.dtype != dtype and p.dtype != torch.float32:
+            raise RuntimeError(f"{fn}: {name} has dtype {p.dtype}, expected {dtype} or "
                                "torch.float32")
-        if ptype is not None and p.dtype != ptype:
-            raise RuntimeError(f"{fn}: weight and bias must have one dtype")
-        ptype = p.dtype
-    images = x.size(0)
-    positions = x.numel() // (images * channels) if x.numel() else 0
-    return (images, positions, channels, _b._DTYPE_CODES[ptype or x.dtype]
-            if x.dtype in _b._DTYPE_CODES else _b.dtype_code(x), GROUP_NORM_ACTS[act])
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError(f"{fn}: weight and bias must have one dtype")
 
 
-def _group_norm_workspace(fn, x, backward, images, positions, channels, num_groups):
-    nbytes = _b.lib().bevk_group_norm_workspace_bytes(_b.dtype_code(x), backward, images, positions,
-                                                      channels, num_groups)
+_GROUP_NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _group_norm_sizes(x, weight, bias):
+    """(device, type code, code of the parameters' type, images, positions, channels)."""
+    codes, shape, total = _b._DTYPE_CODES, x.shape, x.numel()
+    code = codes[x.dtype]
+    pcode = code if weight is None and bias is None else codes[(bias if weight is None else weight).dtype]
+    return (x.get_device(), code, pcode, shape[0],
+            total // (shape[0] * shape[-1]) if total else 0, shape[-1])
+
+
+@functools.lru_cache(maxsize=256)
+def _group_norm_workspace_bytes(code, backward, images, positions, channels, num_groups):
+    nbytes = _b.lib().bevk_group_norm_workspace_bytes(code, backward, images, positions, channels,
+                                                      num_groups)
     if nbytes < 0:
-        raise RuntimeError(f"{fn}: not implemented for {x.dtype} {tuple(x.shape)}")
-    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device), nbytes
+        raise RuntimeError("group_norm: more than 2^40 values")
+    return nbytes
 
 
 def group_norm_forward(x, num_groups, weight, bias, eps, act):
     """(y, stats): y = act(group norm of x [N, ..., C]) in x's type; stats [N, groups, 2] float64
     (mean, 1 / sqrt(var + eps)) for group_norm_backward. weight / bias [C] in x's type or fp32,
     or None."""
-    fn = "group_norm_forward"
-    images, positions, channels, pcode, acode = _group_norm_check(fn, x, num_groups, weight, bias, act)
+    _group_norm_check("group_norm_forward", x, num_groups, weight, bias, act)
+    device, code, pcode, images, positions, channels = _group_norm_sizes(x, weight, bias)
     y = torch.empty_like(x)
     stats = x.new_empty((images, num_groups, 2), dtype=torch.float64)
     if positions == 0:
         return y, stats
-    ws, nbytes = _group_norm_workspace(fn, x, 0, images, positions, channels, num_groups)
-    _b.call_on(x, "bevk_group_norm_forward", _b.dtype_code(x), _b.ptr(x), _b.ptr(weight), _b.ptr(bias),
-               pcode, images, positions, channels, num_groups, float(eps), acode, _b.ptr(ws), nbytes,
-               _b.ptr(y), _b.ptr(stats))
+    nbytes = _group_norm_workspace_bytes(code, 0, images, positions, channels, num_groups)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _b.call_on(device, "bevk_group_norm_forward", code, x.data_ptr(), _b.ptr(weight), _b.ptr(bias), pcode,
+               images, positions, channels, num_groups, eps, GROUP_NORM_ACTS[act], _b.ptr(ws), nbytes,
+               y.data_ptr(), stats.data_ptr())
     return y, stats
 
 
@@ -1023,24 +1041,31 @@ def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=
     """(grad_x, grad_weight, grad_bias) of group_norm_forward for grad_y; None where `wanted` is
     false or the parameter is None."""
     fn = "group_norm_backward"
-    images, positions, channels, pcode, acode = _group_norm_check(fn, x, num_groups, weight, bias, act)
+    _group_norm_check(fn, x, num_groups, weight, bias, act)
     _b.require_device(fn, x, grad_y, stats)
     _b.require_contiguous(fn, grad_y=grad_y, stats=stats)
     _b.require_dtype(fn, x, grad_y=grad_y)
     _b.require_numel(fn, "grad_y", grad_y, x.numel())
-    _b.require_numel(fn, "stats", stats, 2 * images * num_groups)
+    _b.require_numel(fn, "stats", stats, 2 * x.size(0) * num_groups)
     if stats.dtype != torch.float64:
         raise RuntimeError(f"{fn}: stats must be float64, got {stats.dtype}")
+    return _group_norm_gradients(grad_y, x, num_groups, weight, bias, act, stats, wanted)
+
+
+def _group_norm_gradients(grad_y, x, num_groups, weight, bias, act, stats, wanted):
+    """group_norm_backward for tensors that are known to fit (a forward's own)."""
+    device, code, pcode, images, positions, channels = _group_norm_sizes(x, weight, bias)
     new = torch.empty_like if positions else torch.zeros_like
-    grads = [new(t) if want and t is not None else None
-             for want, t in zip(wanted, (x, weight, bias))]
-    if positions == 0:
-        return tuple(grads)
-    ws, nbytes = _group_norm_workspace(fn, x, 1, images, positions, channels, num_groups)
-    _b.call_on(x, "bevk_group_norm_backward", _b.dtype_code(x), _b.ptr(grad_y), _b.ptr(x),
-               _b.ptr(weight), _b.ptr(bias), pcode, images, positions, channels, num_groups, acode,
-               _b.ptr(stats), _b.ptr(ws), nbytes, *(_b.ptr(g) for g in grads))
-    return tuple(grads)
+    grad_x = new(x) if wanted[0] else None
+    grad_w = new(weight) if wanted[1] and weight is not None else None
+    grad_b = new(bias) if wanted[2] and bias is not None else None
+    if positions:
+        nbytes = _group_norm_workspace_bytes(code, 1, images, positions, channels, num_groups)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        _b.call_on(device, "bevk_group_norm_backward", code, grad_y.data_ptr(), x.data_ptr(), _b.ptr(weight),
+                   _b.ptr(bias), pcode, images, positions, channels, num_groups, GROUP_NORM_ACTS[act],
+                   stats.data_ptr(), ws.data_ptr(), nbytes, _b.ptr(grad_x), _b.ptr(grad_w), _b.ptr(grad_b))
+    return grad_x, grad_w, grad_b
 
 
 # ---------------------------------------------------------------------------------------
@@ -1048,8 +1073,12 @@ def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=
 # ---------------------------------------------------------------------------------------
 
 def _embedding_check(fn, index, table, name):
-    _b.require_device(fn, table, index)
-    _b.require_contiguous(fn, index=index, **{name: table})
+    if not table.is_cuda or not index.is_cuda or table.get_device() != index.get_device():
+        _b.require_device(fn, table, index)
+    if not index.is_contiguous():
+        raise RuntimeError("index must be contiguous")
+    if not table.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
     if index.dtype != torch.int64 and index.dtype != torch.int32:
         raise RuntimeError(f"{fn}: index must be int64 or int32, got {index.dtype}")
     if _b.dtype_code(table) == _b.BEVK_F64:
@@ -1065,8 +1094,9 @@ def embedding_forward(weight, index, scale=1.0):
         raise RuntimeError(f"{fn}: weight must be [V, D], got {tuple(weight.shape)}")
     rows, dim = weight.shape
     out = weight.new_empty((*index.shape, dim))
-    _b.call_on(weight, "bevk_embedding_forward", _b.dtype_code(weight), _b.ptr(weight), rows, dim,
-               _b.ptr(index), index.dtype == torch.int64, index.numel(), scale, _b.ptr(out))
+    _b.call_on(weight.get_device(), "bevk_embedding_forward", _b._DTYPE_CODES[weight.dtype],
+               weight.data_ptr(), rows, dim, index.data_ptr(), index.dtype == torch.int64, index.numel(),
+               scale, out.data_ptr())
     return out
 
 
@@ -1079,18 +1109,31 @@ def embedding_backward(grad_out, index, num_embeddings, scale=1.0, padding_idx=N
     if grad_out.dim() != index.dim() + 1 or grad_out.shape[:-1] != index.shape:
         raise RuntimeError(f"{fn}: grad_out must be [*index.shape, D], got {tuple(grad_out.shape)} "
                            f"for index {tuple(index.shape)}")
+    if num_embeddings < 0:
+        raise RuntimeError(f"{fn}: not implemented for {num_embeddings} rows")
     if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
         raise RuntimeError(f"{fn}: padding_idx must be a row of the table, got {padding_idx}")
-    dim, n, code = grad_out.size(-1), index.numel(), _b.dtype_code(grad_out)
-    nbytes = _b.lib().bevk_embedding_backward_workspace_bytes(code, n, num_embeddings, dim)
+    return _embedding_gradient(grad_out, index, num_embeddings, scale,
+                               -1 if padding_idx is None else padding_idx)
+
+
+@functools.lru_cache(maxsize=256)
+def _embedding_workspace_bytes(code, n, rows, dim):
+    nbytes = _b.lib().bevk_embedding_backward_workspace_bytes(code, n, rows, dim)
     if nbytes < 0:
-        raise RuntimeError(f"{fn}: not implemented for {grad_out.dtype} {tuple(grad_out.shape)}, "
-                           f"{num_embeddings} rows")
-    grad = grad_out.new_empty((num_embeddings, dim))
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=grad_out.device)
-    _b.call_on(grad_out, "bevk_embedding_backward", code, _b.ptr(grad_out), _b.ptr(index),
-               index.dtype == torch.int64, n, num_embeddings, dim, scale,
-               -1 if padding_idx is None else padding_idx, _b.ptr(ws), nbytes, _b.ptr(grad))
+        raise RuntimeError(f"embedding_backward: {n} indices of {rows} rows are too many")
+    return nbytes
+
+
+def _embedding_gradient(grad_out, index, rows, scale, padding_idx):
+    """embedding_backward for tensors that are known to fit (a forward's own); padding_idx -1: none."""
+    dim, n, code = grad_out.size(-1), index.numel(), _b._DTYPE_CODES[grad_out.dtype]
+    nbytes = _embedding_workspace_bytes(code, n, rows, dim)
+    grad = grad_out.new_empty((rows, dim))
+    ws = grad_out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _b.call_on(grad_out.get_device(), "bevk_embedding_backward", code, grad_out.data_ptr(), index.data_ptr(),
+               index.dtype == torch.int64, n, rows, dim, scale, padding_idx, _b.ptr(ws), nbytes,
+               grad.data_ptr())
     return grad
 
 
@@ -1151,7 +1194,7 @@ def clip_gradients(grads, max_norm=None, out=None):
         raise RuntimeError(f"{fn}: more than 2^40 values")
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
     ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=grads[0].device)
-    _b.call_on(norm, "bevk_clip_gradients", count, at(ptrs), at(types), at(sizes), at(optrs), at(otypes),
+    _b.call_on(device, "bevk_clip_gradients", count, at(ptrs), at(types), at(sizes), at(optrs), at(otypes),
                0.0 if max_norm is None else max_norm, _b.ptr(ws), nbytes, _b.ptr(norm))
     if optrs is not None:  # written behind autograd's back
         torch.autograd.graph.increment_version(out)

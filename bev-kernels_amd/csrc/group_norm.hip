@@ -10,13 +10,43 @@
 //
 // The sums of x and x^2 are held in fp64: then the squares need no second pass over x for their
 // mean to be taken off first (var loses mean^2 / var * 2^-52), and the position where ReLU's
-// derivative jumps is known to about 2^-50 (see Gate).
+// derivative jumps is known to about 2^-50 (see Gate). At two fp64 instructions a value they
+// stay behind the loads.
+//
+// Both directions are bound by memory and take two launches over the same tiles: sums, then values.
+// A tile is a slab of 128 bytes of channels (whole cache lines) by a share of an image's positions,
+// one workgroup. Between the launches only each tile's sums by group pass through memory, and each
+// workgroup of the second adds up again those of its own slab's groups: a few KB, where a third
+// launch between would cost 4 us and tiles of whole rows would read the sums of every group.
+// The second launch takes the tiles in the opposite order (within the XCD that had them), so that
+// what the first one read last is still in the caches.
+#include <algorithm>
+
 #include "bevk_launch.h"
 
 namespace bevk {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kXcds = 8;
+
+// Lanes across a slab: 8 vectors of 16 bytes, or 64 single channels where rows or tensors are not
+// aligned to vectors.
+template <typename T, int V> struct Tile {
+  static constexpr int kLanes = V > 1 ? 8 : 64;
+  static constexpr int kSlab = kLanes * V;            // channels
+  static constexpr int kRows = kThreads / kLanes;     // positions side by side
+  static constexpr int kUnroll = V > 1 ? 4 : 8;       // positions of a thread in flight
+};
+
+struct Geo {
+  int64_t pixels, each;  // positions of an image, and of a tile
+  int channels, per;
+  int slabs, splits;     // tiles of an image: slabs x splits
+  int local;             // room for the groups of a slab
+  int64_t tiles;
+};
 
 __device__ __forceinline__ float to_f32(const void *p, int dtype, int64_t i, float none) {
   if (p == nullptr) return none;
@@ -34,33 +64,22 @@ __device__ __forceinline__ void from_f32(void *p, int dtype, int64_t i, float v)
   }
 }
 
-// Sum over a workgroup; every thread gets it.
-template <typename A>
-__device__ __forceinline__ A block_sum(A v, A *s) {
-  __syncthreads();
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_down(v, d, kWave);
-  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = v;
-  __syncthreads();
-  A t = s[0];
-  for (int k = 1; k < kThreads / kWave; ++k) t += s[k];
-  return t;
+// 1 / (1 + exp(-z)). The types of 16 bits do with the hardware's exp2 and reciprocal (2^-20 relative
+// for |z| up to 10, where fp32's own functions have 2^-22): the second launch of six 116 x 200 x 256
+// bf16 maps takes 29.6 us with them, 34.8 us with fp32's.
+template <typename T> __device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
+template <> __device__ __forceinline__ float sigmoid<float>(float z) { return 1.f / (1.f + expf(-z)); }
 
-__device__ __forceinline__ float act_of(float z, int act) {
-  if (act == kActRelu) return z <= 0.f ? 0.f : z;  // NaN stays
-  if (act == kActSilu) return z / (1.f + expf(-z));
+template <typename T, int ACT> __device__ __forceinline__ float act_of(float z) {
+  if constexpr (ACT == kActRelu) return z <= 0.f ? 0.f : z;  // NaN stays
+  if constexpr (ACT == kActSilu) return z * sigmoid<T>(z);
   return z;
 }
 
 // x - mean with mean as two floats, so that a mean far from 0 costs no digits of the difference.
-struct Mean2 {
-  float h, l;
-};
-__device__ __forceinline__ Mean2 split_mean(double m) {
-  const float h = (float)m;
-  return {h, (float)(m - (double)h)};
-}
-__device__ __forceinline__ float centred(float x, Mean2 m) { return (x - m.h) - m.l; }
+__device__ __forceinline__ float centred(float x, float high, float low) { return (x - high) - low; }
 
 // Where a channel's z is above 0. z = 0 at x = mean - b / (rstd * w), and rounding z to 32 bits
 // may put an element next to it on the wrong side, which moves its gradient by all of its size.
@@ -77,181 +96,501 @@ __device__ __forceinline__ Gate make_gate(double mean, double rstd, float w, flo
   if ((double)f > t) f = nextafterf(f, -INFINITY);
   return {f, (float)s};
 }
-__device__ __forceinline__ float gated(float gy, float x, Gate g) {
-  return x * g.sign <= g.thr ? 0.f : gy;  // NaN passes, as in ReLU's own derivative
-}
 
-__device__ __forceinline__ float silu_grad(float gy, float z) {
-  const float s = 1.f / (1.f + expf(-z));
-  return gy * (s * (1.f + z * (1.f - s)));
-}
+// What a channel's values are computed from, in LDS.
+struct Channel {
+  float high, low, rstd;  // mean, 1 / deviation of its group
+  float w, b;
+  float thr, sign;        // Gate
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x, int64_t P, int C, int per,
-                                                         double eps, double *__restrict__ stats) {
-  __shared__ double s[kThreads / kWave];
-  const int64_t n = blockIdx.y;
-  const int g = blockIdx.x;
-  double a = 0.0, q = 0.0;
-  for (int64_t i = threadIdx.x; i < P * per; i += kThreads) {
-    const double v = (double)x[(n * P + i / per) * C + (int64_t)g * per + i % per];
-    a += v;
-    q += v * v;
-  }
-  a = block_sum(a, s);
-  q = block_sum(q, s);
-  if (threadIdx.x == 0) {
-    const double m = (double)(P * per), mean = a / m, var = q / m - mean * mean;
-    stats[(n * gridDim.x + g) * 2] = mean;
-    stats[(n * gridDim.x + g) * 2 + 1] = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps);
+// gz and xh of one value.
+template <typename T, int ACT>
+__device__ __forceinline__ void grad_of(float gy, float x, const Channel &c, float &gz, float &xh) {
+  xh = centred(x, c.high, c.low) * c.rstd;
+  gz = gy;
+  if constexpr (ACT == kActRelu) gz = x * c.sign <= c.thr ? 0.f : gy;  // NaN passes, as in ReLU's own derivative
+  if constexpr (ACT == kActSilu) {
+    const float z = xh * c.w + c.b, s = sigmoid<T>(z);
+    gz = gy * (s * (1.f + z * (1.f - s)));
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__ x, int64_t total, int64_t P,
-                                                           int C, int per, const void *w, const void *b,
-                                                           int wd, int act,
-                                                           const double *__restrict__ stats, T *__restrict__ y) {
-  const int G = C / per;
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int c = (int)(i % C);
-    const int64_t n = i / C / P;
-    const double *st = stats + (n * G + c / per) * 2;
-    const float z = centred((float)x[i], split_mean(st[0])) * (float)st[1] * to_f32(w, wd, c, 1.f) +
-                    to_f32(b, wd, c, 0.f);
-    y[i] = static_cast<T>(act_of(z, act));
+// One tile's place. `back`: the tiles in reverse, each on the XCD (workgroup number modulo 8) that
+// has it in the forward order.
+struct Place {
+  int64_t n, p0, p1;
+  int slab, split;
+};
+__device__ __forceinline__ int64_t tile_of(const Geo &g, int64_t block, bool back) {
+  return back ? (g.tiles + kXcds - 1) / kXcds * kXcds - kXcds - block / kXcds * kXcds + block % kXcds : block;
+}
+__device__ __forceinline__ Place place_of(const Geo &g, int64_t tile) {
+  Place p;
+  p.slab = (int)(tile % g.slabs);
+  const int64_t r = tile / g.slabs;
+  p.split = (int)(r % g.splits);
+  p.n = r / g.splits;
+  p.p0 = p.split * g.each;
+  p.p1 = min(p.p0 + g.each, g.pixels);
+  return p;
+}
+
+// Groups with channels in a slab.
+template <int SLAB> __device__ __forceinline__ int first_group(const Geo &g, int slab) { return slab * SLAB / g.per; }
+template <int SLAB> __device__ __forceinline__ int group_count(const Geo &g, int slab) {
+  return (min(g.channels, (slab + 1) * SLAB) - 1) / g.per - first_group<SLAB>(g, slab) + 1;
+}
+template <int SLAB>
+__device__ __forceinline__ int64_t part_at(const Geo &g, int64_t n, int slab, int split, int group) {
+  return ((n * g.slabs + slab) * g.splits + split) * g.local + group - first_group<SLAB>(g, slab);
+}
+
+template <typename A> struct Pair {
+  A a, b;
+};
+
+// The sums of a slab's groups over their tiles, in sums[0 .. group_count), 256 wide.
+template <int SLAB, typename A>
+__device__ __forceinline__ void sum_parts(const Geo &g, int64_t n, int slab, const Pair<A> *part,
+                                          Pair<double> *sums) {
+  const int g0 = first_group<SLAB>(g, slab), count = group_count<SLAB>(g, slab);
+  int wide = 1;
+  while (wide < count) wide *= 2;
+  const int k = threadIdx.x & (wide - 1), j = threadIdx.x / wide, step = kThreads / wide;
+  Pair<double> t{0.0, 0.0};
+  if (k < count) {
+    const int group = g0 + k;
+    for (int s = group * g.per / SLAB; s <= ((group + 1) * g.per - 1) / SLAB; ++s) {
+      const Pair<A> *p = part + part_at<SLAB>(g, n, s, 0, group);
+#pragma unroll 4
+      for (int i = j; i < g.splits; i += step) {
+        const Pair<A> v = p[(int64_t)i * g.local];
+        t.a += (double)v.a;
+        t.b += (double)v.b;
+      }
+    }
+  }
+  sums[threadIdx.x] = t;
+  __syncthreads();
+  for (int d = step / 2; d >= 1; d /= 2) {
+    if (j < d) {
+      sums[threadIdx.x].a += sums[threadIdx.x + d * wide].a;
+      sums[threadIdx.x].b += sums[threadIdx.x + d * wide].b;
+    }
+    __syncthreads();
   }
 }
 
-// gz and xh of one element.
-template <typename T>
-__device__ __forceinline__ void grad_of(const T *gy, const T *x, int64_t i, const double *st, float w, float b,
-                                        int act, float &gz, float &xh) {
-  const float xv = (float)x[i];
-  xh = centred(xv, split_mean(st[0])) * (float)st[1];
-  gz = (float)gy[i];
-  if (act == kActRelu) gz = gated(gz, xv, make_gate(st[0], st[1], w, b));
-  if (act == kActSilu) gz = silu_grad(gz, xh * w + b);
+// f(x vector's elements) for this thread's positions of the tile, kUnroll loads ahead.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void for_tile(const Geo &g, const Place &p, int c, F f) {
+  using TL = Tile<T, V>;
+  for (int64_t q = p.p0 + threadIdx.x / TL::kLanes; q < p.p1; q += TL::kRows * TL::kUnroll) f(q, (p.n * g.pixels + q) * g.channels + c);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_sums_kernel(const T *__restrict__ gy, const T *__restrict__ x,
-                                                              int64_t P, int C, int per, const void *w,
-                                                              const void *b, int wd, int act,
-                                                              const double *__restrict__ stats,
-                                                              double *__restrict__ sums) {
-  __shared__ double s[kThreads / kWave];
-  const int64_t n = blockIdx.y, at = n * gridDim.x + blockIdx.x;
-  double a = 0.0, q = 0.0;
-  for (int64_t k = threadIdx.x; k < P * per; k += kThreads) {
-    const int c = (int)(blockIdx.x * per + k % per);
-    float gz, xh;
-    const float wv = to_f32(w, wd, c, 1.f);
-    grad_of(gy, x, (n * P + k / per) * C + c, stats + at * 2, wv, to_f32(b, wd, c, 0.f), act, gz, xh);
-    a += (double)(gz * wv);
-    q += (double)(gz * wv * xh);
-  }
-  a = block_sum(a, s);
-  q = block_sum(q, s);
-  if (threadIdx.x == 0) {
-    sums[at * 2] = a;
-    sums[at * 2 + 1] = q;
-  }
-}
+// ---------------------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------------------
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ gy, const T *__restrict__ x,
-                                                          int64_t total, int64_t P, int C, int per, const void *w,
-                                                          const void *b, int wd, int act,
-                                                          const double *__restrict__ stats,
-                                                          const double *__restrict__ sums, T *__restrict__ gx) {
-  const int G = C / per;
-  const double m = (double)(P * per);
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int c = (int)(i % C);
-    const int64_t at = i / C / P * G + c / per;
-    float gz, xh;
-    const float wv = to_f32(w, wd, c, 1.f);
-    grad_of(gy, x, i, stats + at * 2, wv, to_f32(b, wd, c, 0.f), act, gz, xh);
-    const float m1 = (float)(sums[at * 2] / m), m2 = (float)(sums[at * 2 + 1] / m);
-    gx[i] = static_cast<T>((float)stats[at * 2 + 1] * (wv * gz - (m1 + xh * m2)));
+// Sums of x and x^2 by group of one tile. WHOLE: a vector's channels are of one group.
+template <typename T, int V, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x, Geo g,
+                                                         Pair<double> *__restrict__ part) {
+  using TL = Tile<T, V>;
+  constexpr int E = WHOLE ? 1 : V;  // sums of a thread
+  __shared__ Pair<double> s[kWaves][TL::kLanes * E];
+  const Place p = place_of(g, blockIdx.x);
+  const int lane = threadIdx.x % TL::kLanes, wave = threadIdx.x / kWave;
+  const int c = (p.slab * TL::kLanes + lane) * V;
+  Pair<double> a[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) a[e] = {0.0, 0.0};
+  if (c < g.channels)
+    for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
+      Vec<T, V> v[TL::kUnroll];
+#pragma unroll
+      for (int u = 0; u < TL::kUnroll; ++u)
+        if (q + u * TL::kRows < p.p1) v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+#pragma unroll
+      for (int u = 0; u < TL::kUnroll; ++u)
+        if (q + u * TL::kRows < p.p1)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const double t = (double)(float)v[u].v[e];
+            a[WHOLE ? 0 : e].a += t;
+            a[WHOLE ? 0 : e].b += t * t;
+          }
+    });
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    for (int d = TL::kLanes; d < kWave; d *= 2) {
+      a[e].a += __shfl_xor(a[e].a, d, kWave);
+      a[e].b += __shfl_xor(a[e].b, d, kWave);
+    }
+    if (threadIdx.x % kWave < TL::kLanes) s[wave][lane * E + e] = a[e];
   }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) grad_params_kernel(const T *__restrict__ gy, const T *__restrict__ x,
-                                                               int64_t N, int64_t P, int C, int per, const void *w,
-                                                               const void *b, int wd, int act,
-                                                               const double *__restrict__ stats, void *gw,
-                                                               void *gb) {
-  __shared__ double s[kThreads / kWave];
-  const int c = blockIdx.x, G = C / per;
-  double a = 0.0, q = 0.0;
-  for (int64_t k = threadIdx.x; k < N * P; k += kThreads) {
-    float gz, xh;
-    grad_of(gy, x, k * C + c, stats + (k / P * G + c / per) * 2, to_f32(w, wd, c, 1.f), to_f32(b, wd, c, 0.f),
-            act, gz, xh);
-    a += (double)gz;
-    q += (double)(gz * xh);
-  }
-  a = block_sum(a, s);
-  q = block_sum(q, s);
-  if (threadIdx.x == 0) {
-    if (gb != nullptr) from_f32(gb, wd, c, (float)a);
-    if (gw != nullptr) from_f32(gw, wd, c, (float)q);
+  __syncthreads();
+  const int k = threadIdx.x;
+  if (k < group_count<TL::kSlab>(g, p.slab)) {
+    const int group = first_group<TL::kSlab>(g, p.slab) + k, c0 = p.slab * TL::kSlab;
+    const int lo = max(group * g.per - c0, 0) / (V / E);
+    const int hi = min(min((group + 1) * g.per, g.channels) - c0, TL::kSlab) / (V / E);
+    Pair<double> t{0.0, 0.0};
+    for (int w = 0; w < kWaves; ++w)
+      for (int i = lo; i < hi; ++i) {
+        t.a += s[w][i].a;
+        t.b += s[w][i].b;
+      }
+    part[part_at<TL::kSlab>(g, p.n, p.slab, p.split, group)] = t;
   }
 }
 
-int grid_for(int64_t total) {
-  const int64_t b = (total + kThreads - 1) / kThreads;
-  return (int)(b < 4096 ? b : 4096);
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__ x, Geo g, GroupNormArgs args,
+                                                           const Pair<double> *__restrict__ part,
+                                                           Pair<double> *__restrict__ stats, T *__restrict__ y) {
+  using TL = Tile<T, V>;
+  __shared__ Pair<double> sums[kThreads];
+  const int64_t tile = tile_of(g, blockIdx.x, true);
+  if (tile >= g.tiles) return;
+  const Place p = place_of(g, tile);
+  sum_parts<TL::kSlab>(g, p.n, p.slab, part, sums);
+  const int g0 = first_group<TL::kSlab>(g, p.slab);
+  if ((int)threadIdx.x < group_count<TL::kSlab>(g, p.slab)) {
+    const double m = (double)g.pixels * g.per, mean = sums[threadIdx.x].a / m;
+    const double var = sums[threadIdx.x].b / m - mean * mean;
+    const Pair<double> st{mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + args.eps)};
+    sums[threadIdx.x] = st;
+    const int group = g0 + threadIdx.x;
+    if (p.split == 0 && group * g.per / TL::kSlab == p.slab) stats[p.n * args.groups + group] = st;
+  }
+  __syncthreads();
+  const int c = (p.slab * TL::kLanes + threadIdx.x % TL::kLanes) * V;
+  if (c >= g.channels) return;
+  float high[V], low[V], a[V], b[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const Pair<double> st = sums[(c + e) / g.per - g0];
+    high[e] = (float)st.a;
+    low[e] = (float)(st.a - (double)high[e]);
+    a[e] = (float)st.b * to_f32(args.weight, args.param_dtype, c + e, 1.f);
+    b[e] = to_f32(args.bias, args.param_dtype, c + e, 0.f);
+  }
+  for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
+    Vec<T, V> v[TL::kUnroll];
+#pragma unroll
+    for (int u = 0; u < TL::kUnroll; ++u)
+      if (q + u * TL::kRows < p.p1) v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+#pragma unroll
+    for (int u = 0; u < TL::kUnroll; ++u)
+      if (q + u * TL::kRows < p.p1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          v[u].v[e] = static_cast<T>(act_of<T, ACT>(centred((float)v[u].v[e], high[e], low[e]) * a[e] + b[e]));
+        store_vec<T, V>(y + at + (int64_t)u * TL::kRows * g.channels, v[u]);
+      }
+  });
 }
 
-template <typename T>
-hipError_t forward(const GroupNormArgs &a, void *y, double *stats, hipStream_t stream) {
-  const int per = a.channels / a.groups;
-  const int64_t total = a.batch * a.pixels * a.channels;
-  hipLaunchKernelGGL((stats_kernel<T>), dim3(a.groups, (unsigned)a.batch), dim3(kThreads), 0, stream,
-                     static_cast<const T *>(a.x), a.pixels, a.channels, per, a.eps, stats);
-  hipLaunchKernelGGL((forward_kernel<T>), dim3(grid_for(total)), dim3(kThreads), 0, stream,
-                     static_cast<const T *>(a.x), total, a.pixels, a.channels, per, a.weight, a.bias,
-                     a.param_dtype, a.act, stats, static_cast<T *>(y));
+// ---------------------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------------------
+
+// The slab's channels from the forward's statistics.
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void load_channels(const Geo &g, const GroupNormArgs &args, const Place &p,
+                                              const Pair<double> *stats, Channel *ch) {
+  using TL = Tile<T, V>;
+  const int c = p.slab * TL::kSlab + threadIdx.x;
+  if ((int)threadIdx.x < TL::kSlab && c < g.channels) {
+    const Pair<double> st = stats[p.n * args.groups + c / g.per];
+    Channel r;
+    r.high = (float)st.a;
+    r.low = (float)(st.a - (double)r.high);
+    r.rstd = (float)st.b;
+    r.w = to_f32(args.weight, args.param_dtype, c, 1.f);
+    r.b = to_f32(args.bias, args.param_dtype, c, 0.f);
+    if constexpr (ACT == kActRelu) {
+      const Gate gate = make_gate(st.a, st.b, r.w, r.b);
+      r.thr = gate.thr;
+      r.sign = gate.sign;
+    }
+    ch[threadIdx.x] = r;
+  }
+  __syncthreads();
+}
+
+// Sums of gz and gz * xh of one tile, by channel for the parameters and, times w, by group for gx.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_sums_kernel(const T *__restrict__ gy, const T *__restrict__ x, Geo g,
+                                                             GroupNormArgs args,
+                                                             const Pair<double> *__restrict__ stats,
+                                                             Pair<float> *__restrict__ by_group,
+                                                             Pair<float> *__restrict__ by_channel) {
+  using TL = Tile<T, V>;
+  __shared__ Channel ch[TL::kSlab];
+  __shared__ Pair<float> s[kWaves][TL::kSlab];
+  const Place p = place_of(g, blockIdx.x);
+  load_channels<T, V, ACT>(g, args, p, stats, ch);
+  const int lane = threadIdx.x % TL::kLanes, wave = threadIdx.x / kWave;
+  const int c = (p.slab * TL::kLanes + lane) * V;
+  Pair<float> a[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) a[e] = {0.f, 0.f};
+  if (c < g.channels) {
+    Channel k[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) k[e] = ch[lane * V + e];
+    for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
+      Vec<T, V> v[TL::kUnroll], d[TL::kUnroll];
+#pragma unroll
+      for (int u = 0; u < TL::kUnroll; ++u)
+        if (q + u * TL::kRows < p.p1) {
+          v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+          d[u] = load_vec<T, V>(gy + at + (int64_t)u * TL::kRows * g.channels);
+        }
+#pragma unroll
+      for (int u = 0; u < TL::kUnroll; ++u)
+        if (q + u * TL::kRows < p.p1)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            float gz, xh;
+            grad_of<T, ACT>((float)d[u].v[e], (float)v[u].v[e], k[e], gz, xh);
+            a[e].a += gz;
+            a[e].b += gz * xh;
+          }
+    });
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    for (int d = TL::kLanes; d < kWave; d *= 2) {
+      a[e].a += __shfl_xor(a[e].a, d, kWave);
+      a[e].b += __shfl_xor(a[e].b, d, kWave);
+    }
+    if (threadIdx.x % kWave < TL::kLanes) s[wave][lane * V + e] = a[e];
+  }
+  __syncthreads();
+  const int k = threadIdx.x, c0 = p.slab * TL::kSlab;
+  if (k < TL::kSlab && c0 + k < g.channels) {
+    Pair<float> t = s[0][k];
+    for (int w = 1; w < kWaves; ++w) {
+      t.a += s[w][k].a;
+      t.b += s[w][k].b;
+    }
+    by_channel[(p.n * g.splits + p.split) * g.channels + c0 + k] = t;
+    s[0][k] = {t.a * ch[k].w, t.b * ch[k].w};
+  }
+  __syncthreads();
+  if (k < group_count<TL::kSlab>(g, p.slab)) {
+    const int group = first_group<TL::kSlab>(g, p.slab) + k;
+    const int lo = max(group * g.per - c0, 0), hi = min(min((group + 1) * g.per, g.channels) - c0, TL::kSlab);
+    Pair<double> t{0.0, 0.0};
+    for (int i = lo; i < hi; ++i) {
+      t.a += (double)s[0][i].a;
+      t.b += (double)s[0][i].b;
+    }
+    by_group[part_at<TL::kSlab>(g, p.n, p.slab, p.split, group)] = {(float)t.a, (float)t.b};
+  }
+}
+
+// gw and gb of 32 channels: all tiles' sums of them.
+constexpr int kParamLanes = 32;
+__device__ __forceinline__ void param_grads(const Geo &g, const GroupNormArgs &args, int block,
+                                            const Pair<float> *by_channel, void *grad_w, void *grad_b,
+                                            Pair<double> *sums) {
+  const int lane = threadIdx.x % kParamLanes, c = block * kParamLanes + lane;
+  const int64_t rows = args.batch * g.splits;
+  Pair<double> t{0.0, 0.0};
+  if (c < g.channels)
+#pragma unroll 4
+    for (int64_t r = threadIdx.x / kParamLanes; r < rows; r += kThreads / kParamLanes) {
+      const Pair<float> v = by_channel[r * g.channels + c];
+      t.a += (double)v.a;
+      t.b += (double)v.b;
+    }
+  sums[threadIdx.x] = t;
+  __syncthreads();
+  if ((int)threadIdx.x < kParamLanes && c < g.channels) {
+    for (int k = lane + kParamLanes; k < kThreads; k += kParamLanes) {
+      t.a += sums[k].a;
+      t.b += sums[k].b;
+    }
+    if (grad_b != nullptr) from_f32(grad_b, args.param_dtype, c, (float)t.a);
+    if (grad_w != nullptr) from_f32(grad_w, args.param_dtype, c, (float)t.b);
+  }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ gy, const T *__restrict__ x, Geo g,
+                                                          GroupNormArgs args, int param_blocks,
+                                                          const Pair<double> *__restrict__ stats,
+                                                          const Pair<float> *__restrict__ by_group,
+                                                          const Pair<float> *__restrict__ by_channel,
+                                                          T *__restrict__ gx, void *grad_w, void *grad_b) {
+  using TL = Tile<T, V>;
+  __shared__ Pair<double> sums[kThreads];
+  __shared__ Channel ch[TL::kSlab];
+  if ((int)blockIdx.x < param_blocks) {
+    param_grads(g, args, blockIdx.x, by_channel, grad_w, grad_b, sums);
+    return;
+  }
+  const int64_t tile = tile_of(g, blockIdx.x - param_blocks, true);
+  if (tile >= g.tiles || gx == nullptr) return;
+  const Place p = place_of(g, tile);
+  sum_parts<TL::kSlab>(g, p.n, p.slab, by_group, sums);
+  load_channels<T, V, ACT>(g, args, p, stats, ch);
+  const int lane = threadIdx.x % TL::kLanes, g0 = first_group<TL::kSlab>(g, p.slab);
+  const int c = (p.slab * TL::kLanes + lane) * V;
+  if (c >= g.channels) return;
+  const double m = (double)g.pixels * g.per;
+  Channel k[V];
+  float m1[V], m2[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    k[e] = ch[lane * V + e];
+    const Pair<double> t = sums[(c + e) / g.per - g0];
+    m1[e] = (float)(t.a / m);
+    m2[e] = (float)(t.b / m);
+  }
+  for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
+    Vec<T, V> v[TL::kUnroll], d[TL::kUnroll];
+#pragma unroll
+    for (int u = 0; u < TL::kUnroll; ++u)
+      if (q + u * TL::kRows < p.p1) {
+        v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+        d[u] = load_vec<T, V>(gy + at + (int64_t)u * TL::kRows * g.channels);
+      }
+#pragma unroll
+    for (int u = 0; u < TL::kUnroll; ++u)
+      if (q + u * TL::kRows < p.p1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float gz, xh;
+          grad_of<T, ACT>((float)d[u].v[e], (float)v[u].v[e], k[e], gz, xh);
+          v[u].v[e] = static_cast<T>(k[e].rstd * (k[e].w * gz - (m1[e] + xh * m2[e])));
+        }
+        store_vec<T, V>(gx + at + (int64_t)u * TL::kRows * g.channels, v[u]);
+      }
+  });
+}
+
+// ---------------------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------------------
+
+constexpr int kTiles = 1024;  // about: four workgroups on each CU
+
+Geo make_geo(int64_t batch, int64_t pixels, int channels, int groups, int slab, int rows) {
+  Geo g;
+  g.pixels = pixels;
+  g.channels = channels;
+  g.per = channels / groups;
+  g.slabs = (channels + slab - 1) / slab;
+  g.local = std::min(groups, (slab - 1) / g.per + 2);
+  const int64_t want = std::max<int64_t>(1, kTiles / std::max<int64_t>(1, batch * g.slabs));
+  const int64_t rounds = (pixels + rows - 1) / rows;  // a tile has whole rounds of its positions side by side
+  g.each = std::max<int64_t>(1, (rounds + want - 1) / want) * rows;
+  g.splits = (int)((pixels + g.each - 1) / g.each);
+  g.tiles = batch * g.slabs * g.splits;
+  return g;
+}
+
+template <typename T, int V> Geo geo_of(const GroupNormArgs &a) {
+  return make_geo(a.batch, a.pixels, a.channels, a.groups, Tile<T, V>::kSlab, Tile<T, V>::kRows);
+}
+
+int64_t by_group_pairs(const Geo &g) { return g.tiles * g.local; }
+int64_t by_channel_pairs(const Geo &g, int64_t batch) { return batch * g.splits * g.channels; }
+
+// Vectors of 16 bytes where each row and tensor begins on them.
+template <typename T> bool vectors(const GroupNormArgs &a, const void *p, const void *q, const void *r) {
+  const uintptr_t all = (uintptr_t)((int64_t)a.channels * sizeof(T)) | reinterpret_cast<uintptr_t>(p) |
+                        reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(r);
+  return all % 16 == 0;
+}
+
+template <typename F> hipError_t with_act(int act, F f) {
+  switch (act) {
+    case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
+    default: f(std::integral_constant<int, kActNone>()); break;
+  }
   return hipGetLastError();
 }
 
-template <typename T>
+unsigned back_grid(const Geo &g) { return (unsigned)((g.tiles + kXcds - 1) / kXcds * kXcds); }
+
+template <typename T, int V>
+hipError_t forward(const GroupNormArgs &a, void *y, double *stats, void *workspace, hipStream_t stream) {
+  const Geo g = geo_of<T, V>(a);
+  if (g.tiles > 1 << 30) return hipErrorInvalidValue;
+  const T *x = static_cast<const T *>(a.x);
+  Pair<double> *part = static_cast<Pair<double> *>(workspace), *st = reinterpret_cast<Pair<double> *>(stats);
+  if (g.per % V == 0)
+    hipLaunchKernelGGL((stats_kernel<T, V, true>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
+  else
+    hipLaunchKernelGGL((stats_kernel<T, V, false>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
+  return with_act(a.act, [&](auto act) {
+    hipLaunchKernelGGL((forward_kernel<T, V, decltype(act)::value>), dim3(back_grid(g)), dim3(kThreads), 0, stream, x,
+                       g, a, part, st, static_cast<T *>(y));
+  });
+}
+
+template <typename T, int V>
 hipError_t backward(const GroupNormArgs &a, const void *grad_y, const double *stats, void *workspace, void *grad_x,
                     void *grad_w, void *grad_b, hipStream_t stream) {
-  const int per = a.channels / a.groups;
-  const int64_t total = a.batch * a.pixels * a.channels;
-  double *sums = static_cast<double *>(workspace);
+  const Geo g = geo_of<T, V>(a);
+  if (g.tiles > 1 << 30) return hipErrorInvalidValue;
   const T *gy = static_cast<const T *>(grad_y), *x = static_cast<const T *>(a.x);
-  if (grad_x != nullptr) {
-    hipLaunchKernelGGL((group_sums_kernel<T>), dim3(a.groups, (unsigned)a.batch), dim3(kThreads), 0, stream, gy, x,
-                       a.pixels, a.channels, per, a.weight, a.bias, a.param_dtype, a.act, stats, sums);
-    hipLaunchKernelGGL((grad_x_kernel<T>), dim3(grid_for(total)), dim3(kThreads), 0, stream, gy, x, total,
-                       a.pixels, a.channels, per, a.weight, a.bias, a.param_dtype, a.act, stats, sums,
-                       static_cast<T *>(grad_x));
+  const Pair<double> *st = reinterpret_cast<const Pair<double> *>(stats);
+  Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(g);
+  const int params = grad_w || grad_b ? (a.channels + kParamLanes - 1) / kParamLanes : 0;
+  return with_act(a.act, [&](auto act) {
+    constexpr int A = decltype(act)::value;
+    hipLaunchKernelGGL((grad_sums_kernel<T, V, A>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, gy, x, g, a, st,
+                       by_group, by_channel);
+    hipLaunchKernelGGL((grad_x_kernel<T, V, A>), dim3(params + (grad_x ? back_grid(g) : 0)), dim3(kThreads), 0, stream,
+                       gy, x, g, a, params, st, by_group, by_channel, static_cast<T *>(grad_x), grad_w, grad_b);
+  });
+}
+
+template <typename T> int64_t workspace_bytes(bool backward, int64_t batch, int64_t pixels, int channels, int groups) {
+  int64_t most = 0;  // of both tilings: which one runs goes by the tensors' alignment too
+  for (int v : {(int)(16 / sizeof(T)), 1}) {
+    const int lanes = v > 1 ? 8 : 64;
+    const Geo g = make_geo(batch, pixels, channels, groups, lanes * v, kThreads / lanes);
+    most = std::max(most, backward ? (by_group_pairs(g) + by_channel_pairs(g, batch)) * 8 : by_group_pairs(g) * 16);
   }
-  if (grad_w != nullptr || grad_b != nullptr)
-    hipLaunchKernelGGL((grad_params_kernel<T>), dim3(a.channels), dim3(kThreads), 0, stream, gy, x, a.batch,
-                       a.pixels, a.channels, per, a.weight, a.bias, a.param_dtype, a.act, stats, grad_w, grad_b);
-  return hipGetLastError();
+  return most;
+}
+
+template <typename T>
+hipError_t forward_t(const GroupNormArgs &a, void *y, double *stats, void *ws, hipStream_t stream) {
+  if (vectors<T>(a, a.x, y, y)) return forward<T, 16 / sizeof(T)>(a, y, stats, ws, stream);
+  return forward<T, 1>(a, y, stats, ws, stream);
+}
+template <typename T>
+hipError_t backward_t(const GroupNormArgs &a, const void *gy, const double *stats, void *ws, void *gx, void *gw,
+                      void *gb, hipStream_t stream) {
+  if (vectors<T>(a, a.x, gy, gx)) return backward<T, 16 / sizeof(T)>(a, gy, stats, ws, gx, gw, gb, stream);
+  return backward<T, 1>(a, gy, stats, ws, gx, gw, gb, stream);
 }
 
 }  // namespace
 
 int64_t group_norm_workspace_bytes(int dtype, bool backward, int64_t batch, int64_t pixels, int channels,
                                    int groups) {
-  return backward ? batch * groups * 16 : 0;
+  return dtype == 0 ? workspace_bytes<float>(backward, batch, pixels, channels, groups)
+                    : workspace_bytes<f16>(backward, batch, pixels, channels, groups);
 }
 
 hipError_t launch_group_norm_forward(int dtype, const GroupNormArgs &a, void *y, double *stats, void *workspace,
                                      hipStream_t stream) {
   switch (dtype) {
-    case 0: return forward<float>(a, y, stats, stream);
-    case 1: return forward<f16>(a, y, stats, stream);
-    default: return forward<bf16>(a, y, stats, stream);
+    case 0: return forward_t<float>(a, y, stats, workspace, stream);
+    case 1: return forward_t<f16>(a, y, stats, workspace, stream);
+    default: return forward_t<bf16>(a, y, stats, workspace, stream);
   }
 }
 
@@ -259,9 +598,9 @@ hipError_t launch_group_norm_backward(int dtype, const GroupNormArgs &a, const v
                                       void *workspace, void *grad_x, void *grad_w, void *grad_b,
                                       hipStream_t stream) {
   switch (dtype) {
-    case 0: return backward<float>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
-    case 1: return backward<f16>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
-    default: return backward<bf16>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
+    case 0: return backward_t<float>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
+    case 1: return backward_t<f16>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
+    default: return backward_t<bf16>(a, grad_y, stats, workspace, grad_x, grad_w, grad_b, stream);
   }
 }
 

@@ -7,12 +7,22 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
+
+import _bevk as _b
+
+_loaded = None
 
 
 def _ext():
-    import _modulated_deform_conv_ext as ext
-    return ext
+    global _loaded
+    if _loaded is None:
+        import _modulated_deform_conv_ext
+        _loaded = _modulated_deform_conv_ext
+    return _loaded
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 class GroupNormActNHWCFunction(torch.autograd.Function):
@@ -20,21 +30,20 @@ class GroupNormActNHWCFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x_nhwc, num_groups, weight, bias, eps, act):
-        x = x_nhwc.contiguous()
-        weight, bias = (p if p is None else p.contiguous() for p in (weight, bias))
+        x, weight, bias = _dense(x_nhwc), _dense(weight), _dense(bias)
         y, stats = _ext().group_norm_forward(x, num_groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.num_groups, ctx.act = num_groups, act
+        ctx.args = num_groups, act
         return y
 
     @staticmethod
-    @once_differentiable
+    @_b.once_differentiable
     def backward(ctx, grad_y):
         x, weight, bias, stats = ctx.saved_tensors
+        num_groups, act = ctx.args
         need = ctx.needs_input_grad
-        grad_x, grad_w, grad_b = _ext().group_norm_backward(
-            grad_y.contiguous(), x, ctx.num_groups, weight, bias, ctx.act, stats,
-            (need[0], need[2], need[3]))
+        grad_x, grad_w, grad_b = _ext()._group_norm_gradients(
+            _dense(grad_y), x, num_groups, weight, bias, act, stats, (need[0], need[2], need[3]))
         return grad_x, None, grad_w, grad_b, None, None
 
 

@@ -5,12 +5,18 @@ looks whole ones up. The reference has no counterpart."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
+
+import _bevk as _b
+
+_loaded = None
 
 
 def _ext():
-    import _modulated_deform_conv_ext
-    return _modulated_deform_conv_ext
+    global _loaded
+    if _loaded is None:
+        import _modulated_deform_conv_ext
+        _loaded = _modulated_deform_conv_ext
+    return _loaded
 
 
 class EmbeddingLookupFunction(torch.autograd.Function):
@@ -18,22 +24,28 @@ class EmbeddingLookupFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weight, index, scale=1.0, padding_idx=None):
-        if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        rows = weight.shape[0]
+        if padding_idx is None:
+            padding_idx = -1
+        elif not 0 <= padding_idx < rows:
             raise RuntimeError("embedding_lookup: padding_idx must be a row of the table, got "
                                f"{padding_idx}")
-        index = index.contiguous()
-        out = _ext().embedding_forward(weight.contiguous(), index, scale)
+        if not index.is_contiguous():
+            index = index.contiguous()
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        out = _ext().embedding_forward(weight, index, scale)
         ctx.save_for_backward(index)
-        ctx.num_embeddings, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
+        ctx.args = rows, scale, padding_idx
         return out
 
     @staticmethod
-    @once_differentiable
+    @_b.once_differentiable
     def backward(ctx, grad_output):
         index, = ctx.saved_tensors
-        grad = _ext().embedding_backward(grad_output.contiguous(), index, ctx.num_embeddings,
-                                         ctx.scale, ctx.padding_idx)
-        return grad, None, None, None
+        if not grad_output.is_contiguous():
+            grad_output = grad_output.contiguous()
+        return _ext()._embedding_gradient(grad_output, index, *ctx.args), None, None, None
 
 
 def embedding_lookup(weight, index, scale=1.0, padding_idx=None):

@@ -313,3 +313,15 @@ def test_deformable_layer_with_group_norm():
     grads = torch.autograd.grad(out, leaves, gy)
     assert all(t.shape == v.shape and torch.isfinite(t).all() and t.any()
                for t, v in zip(grads, leaves))
+
+
+def test_second_derivatives_are_refused():
+    import modulated_deform_conv as mdc
+    import msda_opt2
+    x = torch.randn(1, 4, 4, 8, device=DEV, requires_grad=True)
+    w = torch.randn(6, 8, device=DEV, requires_grad=True)
+    i = torch.tensor([1, 2], device=DEV)
+    for y, leaf in ((mdc.group_norm_act_nhwc(x, 2), x), (msda_opt2.embedding_lookup(w, i), w)):
+        g, = torch.autograd.grad(y, leaf, torch.ones_like(y, requires_grad=True), create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
