@@ -1152,21 +1152,23 @@ def _dense(t):
 
 
 def _grad_arrays(fn, tensors, device):
-    """(pointers, type codes, sizes) as arrays for the library. Plain attribute tests in one loop
-    over what may be hundreds of tensors: the host side of the call."""
-    codes = _b._DTYPE_CODES
+    """(pointers, type codes, sizes) as arrays for the library. One expression for each attribute:
+    over hundreds of tensors this is the host side of the call."""
     for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {t.device}")
-        if t.get_device() != device:
-            raise RuntimeError(f"{fn}: tensors are on different devices (cuda:{device}, {t.device})")
-        if t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
-            raise RuntimeError(f"{fn}: gradients must be dense, got {t.layout} with strides "
-                               f"{t.stride() if t.layout is torch.strided else None}")
-        if t.dtype not in codes:
-            _b.dtype_code(t)
-    return (array("Q", [t.data_ptr() for t in tensors]), array("i", [codes[t.dtype] for t in tensors]),
-            array("q", [t.numel() for t in tensors]))
+        if t.get_device() != device or not t.is_contiguous():  # (-1: not on a HIP device)
+            if not t.is_cuda:
+                raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {t.device}")
+            if t.get_device() != device:
+                raise RuntimeError(f"{fn}: tensors are on different devices (cuda:{device}, {t.device})")
+            if t.layout is not torch.strided or not _dense(t):
+                raise RuntimeError(f"{fn}: gradients must be dense in memory, got strides "
+                                   f"{t.stride() if t.layout is torch.strided else t.layout}")
+    codes = _b._DTYPE_CODES
+    try:
+        types = array("i", [codes[t.dtype] for t in tensors])
+    except KeyError:
+        types = array("i", [_b.dtype_code(t) for t in tensors])  # says which
+    return (array("Q", [t.data_ptr() for t in tensors]), types, array("q", [t.numel() for t in tensors]))
 
 
 def clip_gradients(grads, max_norm=None, out=None):
@@ -1182,12 +1184,15 @@ def clip_gradients(grads, max_norm=None, out=None):
         out = grads if out is None else out
         if len(out) != len(grads):
             raise RuntimeError(f"{fn}: {len(out)} outputs for {len(grads)} gradients")
-        for g, o in zip(grads, out):
-            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (
-                    o.is_contiguous() and g.is_contiguous()))):
-                raise RuntimeError(f"{fn}: an output has shape {tuple(o.shape)} and strides "
-                                   f"{o.stride()}, its gradient {tuple(g.shape)} and {g.stride()}")
-        optrs, otypes = (ptrs, types) if out is grads else _grad_arrays(fn, out, device)[:2]
+        if out is grads:
+            optrs, otypes = ptrs, types
+        else:
+            for g, o in zip(grads, out):
+                if o.shape != g.shape or (not (o.is_contiguous() and g.is_contiguous())
+                                          and o.stride() != g.stride()):
+                    raise RuntimeError(f"{fn}: an output has shape {tuple(o.shape)} and strides "
+                                       f"{o.stride()}, its gradient {tuple(g.shape)} and {g.stride()}")
+            optrs, otypes, _ = _grad_arrays(fn, out, device)
     count, at = len(grads), lambda a: a.buffer_info()[0] if a is not None else None
     nbytes = _b.lib().bevk_clip_gradients_workspace_bytes(count, at(sizes))
     if nbytes < 0:

@@ -8,6 +8,9 @@
 // copied to the device first, and a captured graph holds them itself. A tensor is cut into chunks
 // of `per` values, a workgroup each; each leaves the sum of its squares in the workspace, and each
 // workgroup of the second pass adds them all up again in one order, which saves a launch between.
+// Both passes are bound by memory (squares at two fp64 instructions a value stay behind the loads);
+// the second takes the chunks in the opposite order, since what the first read last may still be
+// in the last-level cache of 256 MB.
 #include <algorithm>
 
 #include "bevk_launch.h"
@@ -16,8 +19,10 @@ namespace bevk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 96;   // 25 bytes each: 2.8 KB of the 4 KB of arguments
-constexpr int kChunks = 1024;  // about that many for a large model
+constexpr int kTensors = 128;  // 30 bytes each: 3.8 KB of the 4 KB of arguments
+constexpr int kChunks = 2048;  // about that many for a large model
+constexpr int kUnroll = 4;     // vectors of a thread in flight
+constexpr int kXcds = 8;
 
 struct Table {
   const void *in[kTensors];
@@ -47,12 +52,43 @@ __device__ __forceinline__ int find_tensor(const Table &t, int chunk) {
   return lo;
 }
 
+// The values [0, n) at p as a few single ones up to a 16-byte boundary, vectors, and the rest.
+template <typename T> struct Span {
+  static constexpr int V = 16 / sizeof(T);
+  int64_t head, vecs, tail;  // tail: first value of the rest
+  __device__ __forceinline__ Span(const T *p, int64_t n) {
+    const int64_t off = reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T);
+    head = min((V - off) % V, n);
+    vecs = (n - head) / V;
+    tail = head + vecs * V;
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ double squares(const T *p, int64_t n) {
+  const Span<T> s(p, n);
   double a = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-    const double v = (double)(float)p[i];
+  auto add = [&](T x) __attribute__((always_inline)) {
+    const double v = (double)(float)x;
     a += v * v;
+  };
+  if ((int64_t)threadIdx.x < s.head) add(p[threadIdx.x]);
+  if (s.tail + threadIdx.x < n) add(p[s.tail + threadIdx.x]);
+  const T *q = p + s.head;
+  int64_t i = threadIdx.x;
+  for (; i + (kUnroll - 1) * kThreads < s.vecs; i += kUnroll * kThreads) {
+    Vec<T, Span<T>::V> v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = load_vec<T, Span<T>::V>(q + (i + u * kThreads) * Span<T>::V);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int e = 0; e < Span<T>::V; ++e) add(v[u].v[e]);
+  }
+  for (; i < s.vecs; i += kThreads) {
+    const Vec<T, Span<T>::V> v = load_vec<T, Span<T>::V>(q + i * Span<T>::V);
+#pragma unroll
+    for (int e = 0; e < Span<T>::V; ++e) add(v.v[e]);
   }
   return a;
 }
@@ -77,9 +113,47 @@ __device__ __forceinline__ double norm_of(const double *part, int parts, double 
   return sqrt(block_sum(a, s));
 }
 
+// N values of O in memory instructions of up to 16 bytes.
+template <typename O, int N>
+__device__ __forceinline__ void store_pieces(O *p, const Vec<O, N> &x) {
+  constexpr int W = sizeof(O) * N > 16 ? 16 / sizeof(O) : N;
+#pragma unroll
+  for (int k = 0; k < N; k += W) {
+    Vec<O, W> y;
+#pragma unroll
+    for (int e = 0; e < W; ++e) y.v[e] = x.v[k + e];
+    store_vec<O, W>(p + k, y);
+  }
+}
+
 template <typename T, typename O>
 __device__ __forceinline__ void scale(const T *p, O *out, int64_t n, float by) {
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) out[i] = static_cast<O>((float)p[i] * by);
+  constexpr int V = Span<T>::V;
+  constexpr uintptr_t align = sizeof(O) * V > 16 ? 16 : sizeof(O) * V;
+  const Span<T> s(p, n);
+  auto one = [&](int64_t i) __attribute__((always_inline)) { out[i] = static_cast<O>((float)p[i] * by); };
+  if (reinterpret_cast<uintptr_t>(out + s.head) % align != 0) {  // out starts elsewhere within a vector
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) one(i);
+    return;
+  }
+  if ((int64_t)threadIdx.x < s.head) one(threadIdx.x);
+  if (s.tail + threadIdx.x < n) one(s.tail + threadIdx.x);
+  const T *q = p + s.head;
+  O *o = out + s.head;
+  for (int64_t i = threadIdx.x; i < s.vecs; i += kUnroll * kThreads) {
+    Vec<T, V> v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i + u * kThreads < s.vecs) v[u] = load_vec<T, V>(q + (i + u * kThreads) * V);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i + u * kThreads < s.vecs) {
+        Vec<O, V> x;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x.v[e] = static_cast<O>((float)v[u].v[e] * by);
+        store_pieces<O, V>(o + (i + u * kThreads) * V, x);
+      }
+  }
 }
 template <typename T>
 __device__ __forceinline__ void scale_to(const T *p, void *out, int type, int64_t at, int64_t n, float by) {
@@ -97,8 +171,12 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const Table t, int64_t 
   if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const double q = max_norm / (norm + 1e-6);
   const float by = q >= 1.0 ? 1.f : (float)q;  // NaN stays
-  const int k = find_tensor(t, blockIdx.x);
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * per, n = min(per, t.n[k] - at);
+  const int chunks = t.first[t.count], up = (chunks + kXcds - 1) / kXcds * kXcds;
+  const int chunk = up - kXcds - (int)blockIdx.x / kXcds * kXcds + (int)blockIdx.x % kXcds;  // on its XCD again
+  if (chunk >= chunks) return;
+  const int k = find_tensor(t, chunk);
+  if (by == 1.f && t.in[k] == t.out[k]) return;  // its own values again
+  const int64_t at = (int64_t)(chunk - t.first[k]) * per, n = min(per, t.n[k] - at);
   switch (t.in_type[k]) {
     case 0: scale_to(static_cast<const float *>(t.in[k]), t.out[k], t.out_type[k], at, n, by); break;
     case 1: scale_to(static_cast<const f16 *>(t.in[k]), t.out[k], t.out_type[k], at, n, by); break;
@@ -125,23 +203,25 @@ int64_t chunks_of(const GradList &g, int64_t per) {
   return c;
 }
 
-// launch(table, chunks, chunks before it) for up to kTensors tensors with values at a time.
+// launch(table, chunks, chunks so far) for up to kTensors tensors with values at a time, from the
+// first tensor on or from the last.
 template <typename F>
-hipError_t for_tables(const GradList &g, int64_t per, F launch) {
+hipError_t for_tables(const GradList &g, int64_t per, bool back, F launch) {
   int k = 0, before = 0;
   while (k < g.count) {
     Table t;
     t.count = 0;
     t.first[0] = 0;
     for (; k < g.count && t.count < kTensors; ++k) {
-      if (g.n[k] == 0) continue;
+      const int i = back ? g.count - 1 - k : k;
+      if (g.n[i] == 0) continue;
       const int c = t.count++;
-      t.in[c] = g.in[k];
-      t.out[c] = g.out ? g.out[k] : nullptr;
-      t.n[c] = g.n[k];
-      t.in_type[c] = (unsigned char)g.in_type[k];
-      t.out_type[c] = g.out ? (unsigned char)g.out_type[k] : 0;
-      t.first[c + 1] = t.first[c] + (int)((g.n[k] + per - 1) / per);
+      t.in[c] = g.in[i];
+      t.out[c] = g.out ? g.out[i] : nullptr;
+      t.n[c] = g.n[i];
+      t.in_type[c] = (unsigned char)g.in_type[i];
+      t.out_type[c] = g.out ? (unsigned char)g.out_type[i] : 0;
+      t.first[c + 1] = t.first[c] + (int)((g.n[i] + per - 1) / per);
     }
     if (t.count == 0) break;
     launch(t, t.first[t.count], before);
@@ -160,7 +240,7 @@ hipError_t launch_clip_gradients(const GradList &g, double max_norm, void *works
   const int64_t per = chunk_of(g);
   const int parts = (int)chunks_of(g, per);
   double *part = static_cast<double *>(workspace);
-  hipError_t e = for_tables(g, per, [&](const Table &t, int chunks, int before) {
+  hipError_t e = for_tables(g, per, false, [&](const Table &t, int chunks, int before) {
     hipLaunchKernelGGL(squares_kernel, dim3(chunks), dim3(kThreads), 0, stream, t, per, part + before);
   });
   if (e != hipSuccess) return e;
@@ -168,8 +248,8 @@ hipError_t launch_clip_gradients(const GradList &g, double max_norm, void *works
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, stream, part, parts, norm);
     return hipGetLastError();
   }
-  return for_tables(g, per, [&](const Table &t, int chunks, int before) {
-    hipLaunchKernelGGL(scale_kernel, dim3(chunks), dim3(kThreads), 0, stream, t, per, part, parts, max_norm,
+  return for_tables(g, per, true, [&](const Table &t, int chunks, int before) {
+    hipLaunchKernelGGL(scale_kernel, dim3((chunks + kXcds - 1) / kXcds * kXcds), dim3(kThreads), 0, stream, t, per, part, parts, max_norm,
                        before == 0 ? norm : nullptr);
   });
 }
