@@ -19,7 +19,9 @@
 // workgroup of the second adds up again those of its own slab's groups: a few KB, where a third
 // launch between would cost 4 us and tiles of whole rows would read the sums of every group.
 // The second launch takes the tiles in the opposite order (within the XCD that had them), so that
-// what the first one read last is still in the caches.
+// what the first one read last is still in the caches. Six 58 x 100 x 256 maps in 16 bits (res4): 5.8
+// and 11.1 us forward, 9.5 and 10.6 us backward; their 36 and 53 MB once take 5.5 and 8.2 us at
+// the rate of a copy of that size.
 #include <algorithm>
 
 #include "bevk_launch.h"
@@ -37,7 +39,11 @@ template <typename T, int V> struct Tile {
   static constexpr int kLanes = V > 1 ? 8 : 64;
   static constexpr int kSlab = kLanes * V;            // channels
   static constexpr int kRows = kThreads / kLanes;     // positions side by side
-  static constexpr int kUnroll = V > 1 ? 4 : 8;       // positions of a thread in flight
+  // Positions of a thread loaded together where sums are taken, and where values are written (res4 in
+  // 16 bits, 2 / 4 / 8 of them: sums 6.0 / 6.4 / 7.8 us forward, 9.4 / 10.6 / 11.8 us backward; values
+  // 11.2 / 10.7 / 12.4 and 11.2 / 10.6 / 12.4).
+  static constexpr int kSums = V > 1 ? 2 : 8;
+  static constexpr int kValues = V > 1 ? 4 : 8;
 };
 
 struct Geo {
@@ -97,24 +103,42 @@ __device__ __forceinline__ Gate make_gate(double mean, double rstd, float w, flo
   return {f, (float)s};
 }
 
-// What a channel's values are computed from, in LDS.
+// What a channel's values are computed from: its group's mean and 1 / deviation, its own weight, and
+// for ReLU its gate (thr, sign), for SiLU its bias.
 struct Channel {
-  float high, low, rstd;  // mean, 1 / deviation of its group
-  float w, b;
-  float thr, sign;        // Gate
+  float high, low, rstd, w, u, v;
 };
 
-// gz and xh of one value.
-template <typename T, int ACT>
-__device__ __forceinline__ void grad_of(float gy, float x, const Channel &c, float &gz, float &xh) {
-  xh = centred(x, c.high, c.low) * c.rstd;
-  gz = gy;
-  if constexpr (ACT == kActRelu) gz = x * c.sign <= c.thr ? 0.f : gy;  // NaN passes, as in ReLU's own derivative
-  if constexpr (ACT == kActSilu) {
-    const float z = xh * c.w + c.b, s = sigmoid<T>(z);
-    gz = gy * (s * (1.f + z * (1.f - s)));
+// The constants of a thread's V channels, of one group (WHOLE) or not.
+template <int V, bool WHOLE> struct Channels {
+  static constexpr int E = WHOLE ? 1 : V;
+  float high[E], low[E], rstd[E], w[V], u[V], v[V];
+  __device__ __forceinline__ void read(const Channel *ch) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (e < E) {
+        high[e] = ch[e].high;
+        low[e] = ch[e].low;
+        rstd[e] = ch[e].rstd;
+      }
+      w[e] = ch[e].w;
+      u[e] = ch[e].u;
+      v[e] = ch[e].v;
+    }
   }
-}
+  // gz and xh of one value of channel e
+  template <typename T, int ACT>
+  __device__ __forceinline__ void grad(int e, float gy, float x, float &gz, float &xh) const {
+    const int k = WHOLE ? 0 : e;
+    xh = centred(x, high[k], low[k]) * rstd[k];
+    gz = gy;
+    if constexpr (ACT == kActRelu) gz = x * v[e] <= u[e] ? 0.f : gy;  // NaN passes, as in ReLU's own derivative
+    if constexpr (ACT == kActSilu) {
+      const float z = xh * w[e] + u[e], s = sigmoid<T>(z);
+      gz = gy * (s * (1.f + z * (1.f - s)));
+    }
+  }
+};
 
 // One tile's place. `back`: the tiles in reverse, each on the XCD (workgroup number modulo 8) that
 // has it in the forward order.
@@ -150,10 +174,12 @@ template <typename A> struct Pair {
   A a, b;
 };
 
-// The sums of a slab's groups over their tiles, in sums[0 .. group_count), 256 wide.
+// The sums of a slab's groups over their tiles: thread k of the first ones returns group k's. 16-byte
+// pairs of fp64, or of fp32 as the backward's first launch leaves them.
 template <int SLAB, typename A>
-__device__ __forceinline__ void sum_parts(const Geo &g, int64_t n, int slab, const Pair<A> *part,
-                                          Pair<double> *sums) {
+__device__ __forceinline__ Pair<double> sum_parts(const Geo &g, int64_t n, int slab, const Pair<A> *part,
+                                                  Pair<double> (*sums)[SLAB]) {
+  static_assert(SLAB <= kWave, "a lane of each wave for every group");
   const int g0 = first_group<SLAB>(g, slab), count = group_count<SLAB>(g, slab);
   int wide = 1;
   while (wide < count) wide *= 2;
@@ -171,23 +197,40 @@ __device__ __forceinline__ void sum_parts(const Geo &g, int64_t n, int slab, con
       }
     }
   }
-  sums[threadIdx.x] = t;
-  __syncthreads();
-  for (int d = step / 2; d >= 1; d /= 2) {
-    if (j < d) {
-      sums[threadIdx.x].a += sums[threadIdx.x + d * wide].a;
-      sums[threadIdx.x].b += sums[threadIdx.x + d * wide].b;
-    }
-    __syncthreads();
+  for (int d = wide; d < kWave; d *= 2) {
+    t.a += __shfl_xor(t.a, d, kWave);
+    t.b += __shfl_xor(t.b, d, kWave);
   }
+  if ((int)threadIdx.x % kWave < count) sums[threadIdx.x / kWave][threadIdx.x % kWave] = t;
+  __syncthreads();
+  if ((int)threadIdx.x < count) {
+    t = sums[0][threadIdx.x];
+    for (int w = 1; w < kWaves; ++w) {
+      t.a += sums[w][threadIdx.x].a;
+      t.b += sums[w][threadIdx.x].b;
+    }
+  }
+  return t;
 }
 
-// f(x vector's elements) for this thread's positions of the tile, kUnroll loads ahead.
-template <typename T, int V, typename F>
-__device__ __forceinline__ void for_tile(const Geo &g, const Place &p, int c, F f) {
-  using TL = Tile<T, V>;
-  for (int64_t q = p.p0 + threadIdx.x / TL::kLanes; q < p.p1; q += TL::kRows * TL::kUnroll) f(q, (p.n * g.pixels + q) * g.channels + c);
-}
+// A thread's vectors of U positions of a tile, from position q on. They are loaded a step ahead of
+// their use, the first ones before the workgroup adds up the sums it needs.
+template <typename T, int V, int U> struct Rows {
+  static constexpr int kRows = Tile<T, V>::kRows, kStep = kRows * U;
+  Vec<T, V> v[U];
+  __device__ __forceinline__ void load(const T *src, const Geo &g, const Place &p, int64_t q, int c) {
+    const T *at = src + (p.n * g.pixels + q) * g.channels + c;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * kRows < p.p1 && c < g.channels) v[u] = load_vec<T, V>(at + (int64_t)u * kRows * g.channels);
+  }
+  __device__ __forceinline__ void store(T *dst, const Geo &g, const Place &p, int64_t q, int c) const {
+    T *at = dst + (p.n * g.pixels + q) * g.channels + c;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (q + u * kRows < p.p1) store_vec<T, V>(at + (int64_t)u * kRows * g.channels, v[u]);
+  }
+};
 
 // ---------------------------------------------------------------------------------------
 // Forward
@@ -198,6 +241,7 @@ template <typename T, int V, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x, Geo g,
                                                          Pair<double> *__restrict__ part) {
   using TL = Tile<T, V>;
+  using R = Rows<T, V, TL::kSums>;
   constexpr int E = WHOLE ? 1 : V;  // sums of a thread
   __shared__ Pair<double> s[kWaves][TL::kLanes * E];
   const Place p = place_of(g, blockIdx.x);
@@ -206,22 +250,22 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x
   Pair<double> a[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) a[e] = {0.0, 0.0};
-  if (c < g.channels)
-    for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
-      Vec<T, V> v[TL::kUnroll];
+  int64_t q = p.p0 + threadIdx.x / TL::kLanes;
+  R next;
+  next.load(x, g, p, q, c);
+  for (; q < p.p1 && c < g.channels; q += R::kStep) {
+    const R v = next;
+    next.load(x, g, p, q + R::kStep, c);
 #pragma unroll
-      for (int u = 0; u < TL::kUnroll; ++u)
-        if (q + u * TL::kRows < p.p1) v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+    for (int u = 0; u < TL::kSums; ++u)
+      if (q + u * TL::kRows < p.p1)
 #pragma unroll
-      for (int u = 0; u < TL::kUnroll; ++u)
-        if (q + u * TL::kRows < p.p1)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const double t = (double)(float)v[u].v[e];
-            a[WHOLE ? 0 : e].a += t;
-            a[WHOLE ? 0 : e].b += t * t;
-          }
-    });
+        for (int e = 0; e < V; ++e) {
+          const double t = (double)(float)v.v[u].v[e];
+          a[WHOLE ? 0 : e].a += t;
+          a[WHOLE ? 0 : e].b += t * t;
+        }
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     for (int d = TL::kLanes; d < kWave; d *= 2) {
@@ -246,51 +290,63 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x
   }
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__ x, Geo g, GroupNormArgs args,
                                                            const Pair<double> *__restrict__ part,
                                                            Pair<double> *__restrict__ stats, T *__restrict__ y) {
   using TL = Tile<T, V>;
-  __shared__ Pair<double> sums[kThreads];
+  using R = Rows<T, V, TL::kValues>;
+  constexpr int E = WHOLE ? 1 : V;  // groups of a thread
+  __shared__ Pair<double> sums[kWaves][TL::kSlab];
+  __shared__ float high_of[TL::kSlab], low_of[TL::kSlab], rstd_of[TL::kSlab];
   const int64_t tile = tile_of(g, blockIdx.x, true);
   if (tile >= g.tiles) return;
   const Place p = place_of(g, tile);
-  sum_parts<TL::kSlab>(g, p.n, p.slab, part, sums);
+  const int c = (p.slab * TL::kLanes + threadIdx.x % TL::kLanes) * V;
+  int64_t q = p.p0 + threadIdx.x / TL::kLanes;
+  R next;
+  next.load(x, g, p, q, c);
+  float a[V], b[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    a[e] = c < g.channels ? to_f32(args.weight, args.param_dtype, c + e, 1.f) : 0.f;
+    b[e] = c < g.channels ? to_f32(args.bias, args.param_dtype, c + e, 0.f) : 0.f;
+  }
+  const Pair<double> t = sum_parts<TL::kSlab>(g, p.n, p.slab, part, sums);
   const int g0 = first_group<TL::kSlab>(g, p.slab);
   if ((int)threadIdx.x < group_count<TL::kSlab>(g, p.slab)) {
-    const double m = (double)g.pixels * g.per, mean = sums[threadIdx.x].a / m;
-    const double var = sums[threadIdx.x].b / m - mean * mean;
+    const double m = (double)g.pixels * g.per, mean = t.a / m, var = t.b / m - mean * mean;
     const Pair<double> st{mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + args.eps)};
-    sums[threadIdx.x] = st;
+    high_of[threadIdx.x] = (float)mean;
+    low_of[threadIdx.x] = (float)(mean - (double)(float)mean);
+    rstd_of[threadIdx.x] = (float)st.b;
     const int group = g0 + threadIdx.x;
     if (p.split == 0 && group * g.per / TL::kSlab == p.slab) stats[p.n * args.groups + group] = st;
   }
   __syncthreads();
-  const int c = (p.slab * TL::kLanes + threadIdx.x % TL::kLanes) * V;
   if (c >= g.channels) return;
-  float high[V], low[V], a[V], b[V];
+  float high[E], low[E];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const Pair<double> st = sums[(c + e) / g.per - g0];
-    high[e] = (float)st.a;
-    low[e] = (float)(st.a - (double)high[e]);
-    a[e] = (float)st.b * to_f32(args.weight, args.param_dtype, c + e, 1.f);
-    b[e] = to_f32(args.bias, args.param_dtype, c + e, 0.f);
+    const int k = (c + e) / g.per - g0;
+    if (e < E) {
+      high[e] = high_of[k];
+      low[e] = low_of[k];
+    }
+    a[e] *= rstd_of[k];
   }
-  for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
-    Vec<T, V> v[TL::kUnroll];
+  for (; q < p.p1; q += R::kStep) {
+    R v = next;
+    next.load(x, g, p, q + R::kStep, c);
 #pragma unroll
-    for (int u = 0; u < TL::kUnroll; ++u)
-      if (q + u * TL::kRows < p.p1) v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
+    for (int u = 0; u < TL::kValues; ++u)
 #pragma unroll
-    for (int u = 0; u < TL::kUnroll; ++u)
-      if (q + u * TL::kRows < p.p1) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          v[u].v[e] = static_cast<T>(act_of<T, ACT>(centred((float)v[u].v[e], high[e], low[e]) * a[e] + b[e]));
-        store_vec<T, V>(y + at + (int64_t)u * TL::kRows * g.channels, v[u]);
+      for (int e = 0; e < V; ++e) {
+        const float d = centred((float)v.v[u].v[e], high[WHOLE ? 0 : e], low[WHOLE ? 0 : e]);
+        v.v[u].v[e] = static_cast<T>(act_of<T, ACT>(d * a[e] + b[e]));
       }
-  });
+    v.store(y, g, p, q, c);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -310,11 +366,12 @@ __device__ __forceinline__ void load_channels(const Geo &g, const GroupNormArgs 
     r.low = (float)(st.a - (double)r.high);
     r.rstd = (float)st.b;
     r.w = to_f32(args.weight, args.param_dtype, c, 1.f);
-    r.b = to_f32(args.bias, args.param_dtype, c, 0.f);
+    r.u = to_f32(args.bias, args.param_dtype, c, 0.f);
+    r.v = 0.f;
     if constexpr (ACT == kActRelu) {
-      const Gate gate = make_gate(st.a, st.b, r.w, r.b);
-      r.thr = gate.thr;
-      r.sign = gate.sign;
+      const Gate gate = make_gate(st.a, st.b, r.w, r.u);
+      r.u = gate.thr;
+      r.v = gate.sign;
     }
     ch[threadIdx.x] = r;
   }
@@ -322,45 +379,45 @@ __device__ __forceinline__ void load_channels(const Geo &g, const GroupNormArgs 
 }
 
 // Sums of gz and gz * xh of one tile, by channel for the parameters and, times w, by group for gx.
-template <typename T, int V, int ACT>
+template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const T *__restrict__ gy, const T *__restrict__ x, Geo g,
                                                              GroupNormArgs args,
                                                              const Pair<double> *__restrict__ stats,
                                                              Pair<float> *__restrict__ by_group,
                                                              Pair<float> *__restrict__ by_channel) {
   using TL = Tile<T, V>;
+  using R = Rows<T, V, TL::kSums>;
   __shared__ Channel ch[TL::kSlab];
   __shared__ Pair<float> s[kWaves][TL::kSlab];
   const Place p = place_of(g, blockIdx.x);
-  load_channels<T, V, ACT>(g, args, p, stats, ch);
   const int lane = threadIdx.x % TL::kLanes, wave = threadIdx.x / kWave;
   const int c = (p.slab * TL::kLanes + lane) * V;
+  int64_t q = p.p0 + threadIdx.x / TL::kLanes;
+  R next_x, next_d;
+  next_x.load(x, g, p, q, c);
+  next_d.load(gy, g, p, q, c);
+  load_channels<T, V, ACT>(g, args, p, stats, ch);
   Pair<float> a[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) a[e] = {0.f, 0.f};
   if (c < g.channels) {
-    Channel k[V];
+    Channels<V, WHOLE> k;
+    k.read(ch + lane * V);
+    for (; q < p.p1; q += R::kStep) {
+      const R v = next_x, d = next_d;
+      next_x.load(x, g, p, q + R::kStep, c);
+      next_d.load(gy, g, p, q + R::kStep, c);
 #pragma unroll
-    for (int e = 0; e < V; ++e) k[e] = ch[lane * V + e];
-    for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
-      Vec<T, V> v[TL::kUnroll], d[TL::kUnroll];
-#pragma unroll
-      for (int u = 0; u < TL::kUnroll; ++u)
-        if (q + u * TL::kRows < p.p1) {
-          v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
-          d[u] = load_vec<T, V>(gy + at + (int64_t)u * TL::kRows * g.channels);
-        }
-#pragma unroll
-      for (int u = 0; u < TL::kUnroll; ++u)
+      for (int u = 0; u < TL::kSums; ++u)
         if (q + u * TL::kRows < p.p1)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             float gz, xh;
-            grad_of<T, ACT>((float)d[u].v[e], (float)v[u].v[e], k[e], gz, xh);
+            k.template grad<T, ACT>(e, (float)d.v[u].v[e], (float)v.v[u].v[e], gz, xh);
             a[e].a += gz;
             a[e].b += gz * xh;
           }
-    });
+    }
   }
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -421,7 +478,7 @@ __device__ __forceinline__ void param_grads(const Geo &g, const GroupNormArgs &a
   }
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ gy, const T *__restrict__ x, Geo g,
                                                           GroupNormArgs args, int param_blocks,
                                                           const Pair<double> *__restrict__ stats,
@@ -429,57 +486,62 @@ __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ 
                                                           const Pair<float> *__restrict__ by_channel,
                                                           T *__restrict__ gx, void *grad_w, void *grad_b) {
   using TL = Tile<T, V>;
-  __shared__ Pair<double> sums[kThreads];
+  using R = Rows<T, V, TL::kValues>;
+  constexpr int E = WHOLE ? 1 : V;
+  __shared__ union {
+    Pair<double> by_group[kWaves][TL::kSlab], by_channel[kThreads];
+  } sums;
+  __shared__ Pair<float> means[TL::kSlab];
   __shared__ Channel ch[TL::kSlab];
   if ((int)blockIdx.x < param_blocks) {
-    param_grads(g, args, blockIdx.x, by_channel, grad_w, grad_b, sums);
+    param_grads(g, args, blockIdx.x, by_channel, grad_w, grad_b, sums.by_channel);
     return;
   }
   const int64_t tile = tile_of(g, blockIdx.x - param_blocks, true);
   if (tile >= g.tiles || gx == nullptr) return;
   const Place p = place_of(g, tile);
-  sum_parts<TL::kSlab>(g, p.n, p.slab, by_group, sums);
-  load_channels<T, V, ACT>(g, args, p, stats, ch);
   const int lane = threadIdx.x % TL::kLanes, g0 = first_group<TL::kSlab>(g, p.slab);
   const int c = (p.slab * TL::kLanes + lane) * V;
-  if (c >= g.channels) return;
-  const double m = (double)g.pixels * g.per;
-  Channel k[V];
-  float m1[V], m2[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    k[e] = ch[lane * V + e];
-    const Pair<double> t = sums[(c + e) / g.per - g0];
-    m1[e] = (float)(t.a / m);
-    m2[e] = (float)(t.b / m);
+  int64_t q = p.p0 + threadIdx.x / TL::kLanes;
+  R next_x, next_d;
+  next_x.load(x, g, p, q, c);
+  next_d.load(gy, g, p, q, c);
+  load_channels<T, V, ACT>(g, args, p, stats, ch);
+  const Pair<double> t = sum_parts<TL::kSlab>(g, p.n, p.slab, by_group, sums.by_group);
+  if ((int)threadIdx.x < group_count<TL::kSlab>(g, p.slab)) {
+    const double m = (double)g.pixels * g.per;
+    means[threadIdx.x] = {(float)(t.a / m), (float)(t.b / m)};
   }
-  for_tile<T, V>(g, p, c, [&](int64_t q, int64_t at) __attribute__((always_inline)) {
-    Vec<T, V> v[TL::kUnroll], d[TL::kUnroll];
+  __syncthreads();
+  if (c >= g.channels) return;
+  Channels<V, WHOLE> k;
+  k.read(ch + lane * V);
+  Pair<float> mean[E];
 #pragma unroll
-    for (int u = 0; u < TL::kUnroll; ++u)
-      if (q + u * TL::kRows < p.p1) {
-        v[u] = load_vec<T, V>(x + at + (int64_t)u * TL::kRows * g.channels);
-        d[u] = load_vec<T, V>(gy + at + (int64_t)u * TL::kRows * g.channels);
+  for (int e = 0; e < E; ++e) mean[e] = means[(c + e) / g.per - g0];
+  for (; q < p.p1; q += R::kStep) {
+    R v = next_x;
+    const R d = next_d;
+    next_x.load(x, g, p, q + R::kStep, c);
+    next_d.load(gy, g, p, q + R::kStep, c);
+#pragma unroll
+    for (int u = 0; u < TL::kValues; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float gz, xh;
+        k.template grad<T, ACT>(e, (float)d.v[u].v[e], (float)v.v[u].v[e], gz, xh);
+        const Pair<float> m = mean[WHOLE ? 0 : e];
+        v.v[u].v[e] = static_cast<T>(k.rstd[WHOLE ? 0 : e] * (k.w[e] * gz - (m.a + xh * m.b)));
       }
-#pragma unroll
-    for (int u = 0; u < TL::kUnroll; ++u)
-      if (q + u * TL::kRows < p.p1) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float gz, xh;
-          grad_of<T, ACT>((float)d[u].v[e], (float)v[u].v[e], k[e], gz, xh);
-          v[u].v[e] = static_cast<T>(k[e].rstd * (k[e].w * gz - (m1[e] + xh * m2[e])));
-        }
-        store_vec<T, V>(gx + at + (int64_t)u * TL::kRows * g.channels, v[u]);
-      }
-  });
+    v.store(gx, g, p, q, c);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------------------
 
-constexpr int kTiles = 1024;  // about: four workgroups on each CU
+constexpr int kTiles = 512;  // about: four workgroups on each CU
 
 Geo make_geo(int64_t batch, int64_t pixels, int channels, int groups, int slab, int rows) {
   Geo g;
@@ -510,11 +572,21 @@ template <typename T> bool vectors(const GroupNormArgs &a, const void *p, const 
   return all % 16 == 0;
 }
 
-template <typename F> hipError_t with_act(int act, F f) {
-  switch (act) {
-    case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
-    case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
-    default: f(std::integral_constant<int, kActNone>()); break;
+// f(whether a vector's channels are of one group, the activation) as constants.
+template <int V, typename F> hipError_t with_kinds(const Geo &g, int act, F f) {
+  auto with_act = [&](auto whole) {
+    switch (act) {
+      case kActRelu: f(whole, std::integral_constant<int, kActRelu>()); break;
+      case kActSilu: f(whole, std::integral_constant<int, kActSilu>()); break;
+      default: f(whole, std::integral_constant<int, kActNone>()); break;
+    }
+  };
+  if constexpr (V == 1) {
+    with_act(std::true_type());
+  } else if (g.per % V == 0) {
+    with_act(std::true_type());
+  } else {
+    with_act(std::false_type());
   }
   return hipGetLastError();
 }
@@ -527,13 +599,11 @@ hipError_t forward(const GroupNormArgs &a, void *y, double *stats, void *workspa
   if (g.tiles > 1 << 30) return hipErrorInvalidValue;
   const T *x = static_cast<const T *>(a.x);
   Pair<double> *part = static_cast<Pair<double> *>(workspace), *st = reinterpret_cast<Pair<double> *>(stats);
-  if (g.per % V == 0)
-    hipLaunchKernelGGL((stats_kernel<T, V, true>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
-  else
-    hipLaunchKernelGGL((stats_kernel<T, V, false>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
-  return with_act(a.act, [&](auto act) {
-    hipLaunchKernelGGL((forward_kernel<T, V, decltype(act)::value>), dim3(back_grid(g)), dim3(kThreads), 0, stream, x,
-                       g, a, part, st, static_cast<T *>(y));
+  return with_kinds<V>(g, a.act, [&](auto whole, auto act) {
+    constexpr bool W = decltype(whole)::value;
+    hipLaunchKernelGGL((stats_kernel<T, V, W>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
+    hipLaunchKernelGGL((forward_kernel<T, V, W, decltype(act)::value>), dim3(back_grid(g)), dim3(kThreads), 0, stream,
+                       x, g, a, part, st, static_cast<T *>(y));
   });
 }
 
@@ -546,11 +616,12 @@ hipError_t backward(const GroupNormArgs &a, const void *grad_y, const double *st
   const Pair<double> *st = reinterpret_cast<const Pair<double> *>(stats);
   Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(g);
   const int params = grad_w || grad_b ? (a.channels + kParamLanes - 1) / kParamLanes : 0;
-  return with_act(a.act, [&](auto act) {
+  return with_kinds<V>(g, a.act, [&](auto whole, auto act) {
+    constexpr bool W = decltype(whole)::value;
     constexpr int A = decltype(act)::value;
-    hipLaunchKernelGGL((grad_sums_kernel<T, V, A>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, gy, x, g, a, st,
+    hipLaunchKernelGGL((grad_sums_kernel<T, V, W, A>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, gy, x, g, a, st,
                        by_group, by_channel);
-    hipLaunchKernelGGL((grad_x_kernel<T, V, A>), dim3(params + (grad_x ? back_grid(g) : 0)), dim3(kThreads), 0, stream,
+    hipLaunchKernelGGL((grad_x_kernel<T, V, W, A>), dim3(params + (grad_x ? back_grid(g) : 0)), dim3(kThreads), 0, stream,
                        gy, x, g, a, params, st, by_group, by_channel, static_cast<T *>(grad_x), grad_w, grad_b);
   });
 }
