@@ -85,7 +85,7 @@ _SIGNATURES = {
     "bevk_embedding_backward_workspace_bytes": [_i, _i64, _i64, _i],
     "bevk_embedding_backward": [_i, _vp, _vp, _i, _i64, _i64, _i, ctypes.c_float, _i64, _vp, _i64,
                                 _vp, _vp],
-    "bevk_group_norm_workspace_bytes": [_i, _i, _i64, _i64, _i, _i],
+    "bevk_group_norm_workspace_bytes": [_i, _i, _i64, _i64, _i, _i, _i],
     "bevk_group_norm_forward": [_i, _vp, _vp, _vp, _i, _i64, _i64, _i, _i, ctypes.c_double, _i,
                                 _vp, _i64, _vp, _vp, _vp],
     "bevk_group_norm_backward": [_i] + [_vp] * 4 + [_i, _i64, _i64, _i, _i, _i, _vp, _vp, _i64]

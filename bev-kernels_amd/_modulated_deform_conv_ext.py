@@ -1001,19 +1001,10 @@ def _group_norm_check(fn, x, num_groups, weight, bias, act):
 _GROUP_NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _group_norm_sizes(x, weight, bias):
-    """(device, type code, code of the parameters' type, images, positions, channels)."""
-    codes, shape, total = _b._DTYPE_CODES, x.shape, x.numel()
-    code = codes[x.dtype]
-    pcode = code if weight is None and bias is None else codes[(bias if weight is None else weight).dtype]
-    return (x.get_device(), code, pcode, shape[0],
-            total // (shape[0] * shape[-1]) if total else 0, shape[-1])
-
-
 @functools.lru_cache(maxsize=256)
-def _group_norm_workspace_bytes(code, backward, images, positions, channels, num_groups):
+def _group_norm_workspace_bytes(code, backward, images, positions, channels, num_groups, aligned):
     nbytes = _b.lib().bevk_group_norm_workspace_bytes(code, backward, images, positions, channels,
-                                                      num_groups)
+                                                      num_groups, aligned)
     if nbytes < 0:
         raise RuntimeError("group_norm: more than 2^40 values")
     return nbytes
@@ -1023,18 +1014,34 @@ def group_norm_forward(x, num_groups, weight, bias, eps, act):
     """(y, stats): y = act(group norm of x [N, ..., C]) in x's type; stats [N, groups, 2] float64
     (mean, 1 / sqrt(var + eps)) for group_norm_backward. weight / bias [C] in x's type or fp32,
     or None."""
+    return _group_norm_run(x, num_groups, weight, bias, eps, act)[:2]
+
+
+def _group_norm_sizes(x, num_groups, weight, bias, act):
+    """The library's arguments about the sizes and types: (type, parameters' type, images,
+    positions, channels, groups, activation)."""
+    codes, shape, total = _b._DTYPE_CODES, x.shape, x.numel()
+    code, images, channels = codes[x.dtype], shape[0], shape[-1]
+    pcode = code if weight is None and bias is None else codes[(bias if weight is None else weight).dtype]
+    return (code, pcode, images, total // (images * channels) if total else 0, channels, num_groups,
+            GROUP_NORM_ACTS[act])
+
+
+def _group_norm_run(x, num_groups, weight, bias, eps, act):
+    """(y, stats, sizes): sizes as _group_norm_sizes gives them."""
     _group_norm_check("group_norm_forward", x, num_groups, weight, bias, act)
-    device, code, pcode, images, positions, channels = _group_norm_sizes(x, weight, bias)
+    sizes = _group_norm_sizes(x, num_groups, weight, bias, act)
+    code, pcode, images, positions, channels, _, acode = sizes
     y = torch.empty_like(x)
     stats = x.new_empty((images, num_groups, 2), dtype=torch.float64)
-    if positions == 0:
-        return y, stats
-    nbytes = _group_norm_workspace_bytes(code, 0, images, positions, channels, num_groups)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _b.call_on(device, "bevk_group_norm_forward", code, x.data_ptr(), _b.ptr(weight), _b.ptr(bias), pcode,
-               images, positions, channels, num_groups, eps, GROUP_NORM_ACTS[act], _b.ptr(ws), nbytes,
-               y.data_ptr(), stats.data_ptr())
-    return y, stats
+    if positions:
+        at = x.data_ptr()
+        nbytes = _group_norm_workspace_bytes(code, 0, images, positions, channels, num_groups, at % 16 == 0)
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _b.call_on(x.get_device(), "bevk_group_norm_forward", code, at, _b.ptr(weight), _b.ptr(bias), pcode,
+                   images, positions, channels, num_groups, eps, acode, _b.ptr(ws), nbytes, y.data_ptr(),
+                   stats.data_ptr())
+    return y, stats, sizes
 
 
 def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=(True, True, True)):
@@ -1049,22 +1056,25 @@ def group_norm_backward(grad_y, x, num_groups, weight, bias, act, stats, wanted=
     _b.require_numel(fn, "stats", stats, 2 * x.size(0) * num_groups)
     if stats.dtype != torch.float64:
         raise RuntimeError(f"{fn}: stats must be float64, got {stats.dtype}")
-    return _group_norm_gradients(grad_y, x, num_groups, weight, bias, act, stats, wanted)
+    return _group_norm_gradients(grad_y, x, weight, bias, stats, wanted,
+                                 _group_norm_sizes(x, num_groups, weight, bias, act))
 
 
-def _group_norm_gradients(grad_y, x, num_groups, weight, bias, act, stats, wanted):
+def _group_norm_gradients(grad_y, x, weight, bias, stats, wanted, sizes):
     """group_norm_backward for tensors that are known to fit (a forward's own)."""
-    device, code, pcode, images, positions, channels = _group_norm_sizes(x, weight, bias)
+    code, pcode, images, positions, channels, num_groups, acode = sizes
     new = torch.empty_like if positions else torch.zeros_like
     grad_x = new(x) if wanted[0] else None
     grad_w = new(weight) if wanted[1] and weight is not None else None
     grad_b = new(bias) if wanted[2] and bias is not None else None
     if positions:
-        nbytes = _group_norm_workspace_bytes(code, 1, images, positions, channels, num_groups)
+        at, at_y = x.data_ptr(), grad_y.data_ptr()
+        nbytes = _group_norm_workspace_bytes(code, 1, images, positions, channels, num_groups,
+                                             (at | at_y) % 16 == 0)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
-        _b.call_on(device, "bevk_group_norm_backward", code, grad_y.data_ptr(), x.data_ptr(), _b.ptr(weight),
-                   _b.ptr(bias), pcode, images, positions, channels, num_groups, GROUP_NORM_ACTS[act],
-                   stats.data_ptr(), ws.data_ptr(), nbytes, _b.ptr(grad_x), _b.ptr(grad_w), _b.ptr(grad_b))
+        _b.call_on(x.get_device(), "bevk_group_norm_backward", code, at_y, at, _b.ptr(weight), _b.ptr(bias),
+                   pcode, images, positions, channels, num_groups, acode, stats.data_ptr(), ws.data_ptr(),
+                   nbytes, _b.ptr(grad_x), _b.ptr(grad_w), _b.ptr(grad_b))
     return grad_x, grad_w, grad_b
 
 

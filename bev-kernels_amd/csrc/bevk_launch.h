@@ -182,8 +182,9 @@ struct GroupNormArgs {
   double eps;
   int act;
 };
+// aligned: x and the tensors of its size begin on 16-byte boundaries
 int64_t group_norm_workspace_bytes(int dtype, bool backward, int64_t batch, int64_t pixels, int channels,
-                                   int groups);
+                                   int groups, bool aligned);
 hipError_t launch_group_norm_forward(int dtype, const GroupNormArgs &a, void *y, double *stats, void *workspace,
                                      hipStream_t stream);
 hipError_t launch_group_norm_backward(int dtype, const GroupNormArgs &a, const void *grad_y, const double *stats,

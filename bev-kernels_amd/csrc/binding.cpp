@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -1215,10 +1216,16 @@ static bevk::GroupNormArgs group_norm_args(const void *x, const void *weight, co
   return a;
 }
 
+static bool on_16_bytes(std::initializer_list<const void *> tensors) {
+  uintptr_t all = 0;
+  for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
+  return all % 16 == 0;
+}
+
 int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels, int channels,
-                                        int groups) {
+                                        int groups, int aligned) {
   if (check_group_norm("group_norm", dtype, dtype, batch, pixels, channels, groups, 0)) return -1;
-  return bevk::group_norm_workspace_bytes(dtype, backward != 0, batch, pixels, channels, groups);
+  return bevk::group_norm_workspace_bytes(dtype, backward != 0, batch, pixels, channels, groups, aligned != 0);
 }
 
 int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const void *bias, int param_dtype,
@@ -1228,7 +1235,8 @@ int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const 
   g_last_error.clear();
   if (int rc = check_group_norm(fn, dtype, param_dtype, batch, pixels, channels, groups, act)) return rc;
   if (!(eps >= 0.0)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
-  const int64_t need = bevk::group_norm_workspace_bytes(dtype, false, batch, pixels, channels, groups);
+  const int64_t need = bevk::group_norm_workspace_bytes(dtype, false, batch, pixels, channels, groups,
+                                                        on_16_bytes({x, y}));
   if (!x || !y || !stats || (need > 0 && !workspace))
     return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
@@ -1246,7 +1254,8 @@ int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const
   const char *fn = "group_norm_backward";
   g_last_error.clear();
   if (int rc = check_group_norm(fn, dtype, param_dtype, batch, pixels, channels, groups, act)) return rc;
-  const int64_t need = bevk::group_norm_workspace_bytes(dtype, true, batch, pixels, channels, groups);
+  const int64_t need = bevk::group_norm_workspace_bytes(dtype, true, batch, pixels, channels, groups,
+                                                        on_16_bytes({grad_y, x, grad_x}));
   if (!grad_y || !x || !stats || !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
   if (!grad_x && !grad_weight && !grad_bias) return ok();

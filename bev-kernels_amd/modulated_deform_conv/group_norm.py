@@ -31,19 +31,17 @@ class GroupNormActNHWCFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_nhwc, num_groups, weight, bias, eps, act):
         x, weight, bias = _dense(x_nhwc), _dense(weight), _dense(bias)
-        y, stats = _ext().group_norm_forward(x, num_groups, weight, bias, eps, act)
+        y, stats, ctx.sizes = _ext()._group_norm_run(x, num_groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.args = num_groups, act
         return y
 
     @staticmethod
     @_b.once_differentiable
     def backward(ctx, grad_y):
         x, weight, bias, stats = ctx.saved_tensors
-        num_groups, act = ctx.args
         need = ctx.needs_input_grad
         grad_x, grad_w, grad_b = _ext()._group_norm_gradients(
-            _dense(grad_y), x, num_groups, weight, bias, act, stats, (need[0], need[2], need[3]))
+            _dense(grad_y), x, weight, bias, stats, (need[0], need[2], need[3]), ctx.sizes)
         return grad_x, None, grad_w, grad_b, None, None
 
 

@@ -94,7 +94,9 @@ def test_group_norm_c_abi():
     assert bwd(wb=0) == INVALID and "workspace" in _err()
     assert bwd(gx=None) == 0                            # nothing wanted
     ws = lib.bevk_group_norm_workspace_bytes
-    assert ws(3, 0, 1, 4, 8, 2) == -1 and ws(0, 0, 1, 4, 9, 2) == -1 and ws(0, 1, 1, 4, 8, 2) > 0
+    assert ws(3, 0, 1, 4, 8, 2, 1) == -1 and ws(0, 0, 1, 4, 9, 2, 1) == -1
+    assert ws(0, 1, 1, 4, 8, 2, 1) > 0 and ws(0, 0, 1, 4000, 8, 2, 1) > 0
+    assert ws(0, 0, 1, 4, 8, 2, 1) == 0                # one launch without a workspace
 
 
 def test_embedding_refusals(no_device_check):
