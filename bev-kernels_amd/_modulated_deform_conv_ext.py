@@ -979,6 +979,8 @@ def _group_norm_check(fn, x, num_groups, weight, bias, act):
     if num_groups <= 0 or channels % num_groups != 0:
         raise RuntimeError(f"{fn}: channels ({channels}) must be divisible by num_groups "
                            f"({num_groups})")
+    if channels > _MAX_CHANNELS:
+        raise RuntimeError(f"{fn}: more than 2^30 channels")
     if dtype not in _GROUP_NORM_TYPES:
         _b.dtype_code(x)
         raise RuntimeError(f"{fn}: not implemented for {dtype}")
@@ -998,6 +1000,7 @@ def _group_norm_check(fn, x, num_groups, weight, bias, act):
         raise RuntimeError(f"{fn}: weight and bias must have one dtype")
 
 
+_MAX_CHANNELS = 2 ** 30  # (the library takes an int)
 _GROUP_NORM_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -1093,6 +1096,8 @@ def _embedding_check(fn, index, table, name):
         raise RuntimeError(f"{fn}: index must be int64 or int32, got {index.dtype}")
     if _b.dtype_code(table) == _b.BEVK_F64:
         raise RuntimeError(f"{fn}: not implemented for {table.dtype}")
+    if table.size(-1) > _MAX_CHANNELS:
+        raise RuntimeError(f"{fn}: more than 2^30 channels")
 
 
 def embedding_forward(weight, index, scale=1.0):

@@ -1189,6 +1189,20 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
                            workspace, workspace_bytes, stream);
 }
 
+static bool on_16_bytes(std::initializer_list<const void *> tensors) {
+  uintptr_t all = 0;
+  for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
+  return all % 16 == 0;
+}
+
+static int check_workspace(const char *fn, const void *workspace, int64_t bytes, int64_t need) {
+  if (need > 0 && !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (need > 0 && !on_16_bytes({workspace}))
+    return fail(BEVK_ERR_INVALID, "%s: the workspace must begin on a 16-byte boundary", fn);
+  return 0;
+}
+
 static int check_group_norm(const char *fn, int dtype, int param_dtype, int64_t batch, int64_t pixels,
                             int channels, int groups, int act) {
   for (int d : {dtype, param_dtype})
@@ -1200,6 +1214,7 @@ static int check_group_norm(const char *fn, int dtype, int param_dtype, int64_t 
     return fail(BEVK_ERR_INVALID, "%s: sizes must be positive", fn);
   if (channels % groups != 0)
     return fail(BEVK_ERR_INVALID, "%s: channels (%d) must be divisible by groups (%d)", fn, channels, groups);
+  if (channels > 1 << 30) return fail(BEVK_ERR_INVALID, "%s: more than 2^30 channels", fn);
   if (batch > (1LL << 40) / channels || pixels > (1LL << 40) / channels / batch)
     return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
   if (act < 0 || act > 2) return fail(BEVK_ERR_INVALID, "%s: unknown activation %d", fn, act);
@@ -1214,12 +1229,6 @@ static bevk::GroupNormArgs group_norm_args(const void *x, const void *weight, co
   a.batch = batch; a.pixels = pixels; a.channels = channels; a.groups = groups;
   a.eps = eps; a.act = act;
   return a;
-}
-
-static bool on_16_bytes(std::initializer_list<const void *> tensors) {
-  uintptr_t all = 0;
-  for (const void *p : tensors) all |= reinterpret_cast<uintptr_t>(p);
-  return all % 16 == 0;
 }
 
 int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels, int channels,
@@ -1237,9 +1246,8 @@ int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const 
   if (!(eps >= 0.0)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
   const int64_t need = bevk::group_norm_workspace_bytes(dtype, false, batch, pixels, channels, groups,
                                                         on_16_bytes({x, y}));
-  if (!x || !y || !stats || (need > 0 && !workspace))
-    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
-  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (!x || !y || !stats) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   return hip_status(
       bevk::launch_group_norm_forward(
           dtype, group_norm_args(x, weight, bias, param_dtype, batch, pixels, channels, groups, eps, act), y,
@@ -1256,8 +1264,8 @@ int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const
   if (int rc = check_group_norm(fn, dtype, param_dtype, batch, pixels, channels, groups, act)) return rc;
   const int64_t need = bevk::group_norm_workspace_bytes(dtype, true, batch, pixels, channels, groups,
                                                         on_16_bytes({grad_y, x, grad_x}));
-  if (!grad_y || !x || !stats || !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
-  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (!grad_y || !x || !stats) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   if (!grad_x && !grad_weight && !grad_bias) return ok();
   return hip_status(
       bevk::launch_group_norm_backward(
@@ -1272,6 +1280,7 @@ static int check_embedding(const char *fn, int dtype, int64_t n, int64_t rows, i
   if (n < 0 || rows < 0 || dim < 0) return fail(BEVK_ERR_INVALID, "%s: negative size", fn);
   if (n > (1LL << 31) - 256 || rows > (1LL << 31) - 256)
     return fail(BEVK_ERR_INVALID, "%s: indices and rows must number less than 2^31 - 256", fn);
+  if (dim > 1 << 30) return fail(BEVK_ERR_INVALID, "%s: more than 2^30 channels", fn);
   return 0;
 }
 
@@ -1301,9 +1310,9 @@ int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, 
     return fail(BEVK_ERR_INVALID, "%s: padding_idx must be a row of the table, or -1", fn);
   if (rows == 0 || dim == 0) return ok();
   const int64_t need = bevk::embedding_backward_workspace_bytes(n, rows, dim);
-  if ((n > 0 && (!grad_out || !index)) || !grad_weight || (need > 0 && !workspace))
+  if ((n > 0 && (!grad_out || !index)) || !grad_weight)
     return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
-  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   const bevk::EmbeddingArgs a{index, index64 != 0, n, rows, dim, scale};
   return hip_status(bevk::launch_embedding_backward(dtype, a, grad_out, padding_idx, workspace, grad_weight,
                                                     (hipStream_t)stream),
@@ -1377,8 +1386,7 @@ int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes, 
   if (!norm) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   const bevk::GradList g{count, grads, dtypes, numels, out, out_dtypes};
   const int64_t need = bevk::clip_gradients_workspace_bytes(g);
-  if (need > 0 && !workspace) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
-  if (workspace_bytes < need) return fail(BEVK_ERR_INVALID, "%s: workspace too small", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   try {
     if (out)
       if (int rc = check_grad_overlap(fn, g)) return rc;

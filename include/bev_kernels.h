@@ -471,7 +471,7 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
  *   stats        [batch, groups, 2] fp64, written: mean and 1 / sqrt(var + eps), for the backward
  * The backward writes grad_x (dtype), grad_weight and grad_bias [channels] (param_dtype), each NULL
  * where it is not wanted; ReLU's derivative at 0 is 0. The same results on every run. dtype and
- * param_dtype F32, F16, BF16 (param_dtype: the input's or F32); the workspace holds what
+ * param_dtype F32, F16, BF16 (param_dtype: the input's or F32); the workspace (16-byte aligned) holds what
  * bevk_group_norm_workspace_bytes says (-1 for sizes that are not taken; aligned: x and the tensors
  * of its size all begin on 16-byte boundaries). No size may be 0. */
 int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels,
@@ -520,7 +520,8 @@ int bevk_embedding_backward(int dtype, const void *grad_out, const void *index, 
  *                           output is rejected
  * A norm that is not finite goes on as in plain arithmetic: Inf makes the factor 0, NaN makes it
  * NaN. Outputs equal to their inputs are not written again where the factor is 1. The host arrays
- * are read before the call returns. The workspace holds what bevk_clip_gradients_workspace_bytes
+ * are read before the call returns. The workspace (16-byte
+ * aligned) holds what bevk_clip_gradients_workspace_bytes
  * says (-1 for sizes not taken). */
 int64_t bevk_clip_gradients_workspace_bytes(int count, const int64_t *numels);
 int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes,

@@ -325,3 +325,9 @@ def test_second_derivatives_are_refused():
         g, = torch.autograd.grad(y, leaf, torch.ones_like(y, requires_grad=True), create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+def test_many_tiles():
+    """More slabs than tiles are wanted: shares of an image then go by the longest fp32 sum (64 of a
+    thread), here with single channels, two to an image."""
+    _check(*_inputs(31, (20, 15), 1041, torch.float16, 22), 3, "relu")

@@ -47,6 +47,7 @@ def test_group_norm_refusals(no_device_check):
                        ((x, 2, None, _meta(8, dtype=torch.float16)), "bias has dtype"),
                        ((x.half(), 2, _meta(8), _meta(8, dtype=torch.float16)), "one dtype"),
                        ((x.double(), 2, None, None), "not implemented"),
+                       ((_meta(1, 1, 2 ** 31), 2, None, None), "2\\^30 channels"),
                        ((x.long(), 2, None, None), "not supported")):
         with pytest.raises(RuntimeError, match=match):
             f(*bad, 1e-5, None)
@@ -78,6 +79,7 @@ def test_group_norm_c_abi():
     for kw in (dict(n=0), dict(p=0), dict(c=0), dict(g=0), dict(n=-1)):
         assert fwd(**kw) == INVALID and "positive" in _err()
     assert fwd(n=1 << 30, p=1 << 30) == INVALID and "2^40" in _err()
+    assert fwd(c=(1 << 30) + 2) == INVALID and "2^30" in _err()
     assert fwd(act=3) == INVALID and "activation" in _err()
     assert fwd(eps=-1.0) == INVALID and "eps" in _err()
     assert fwd(eps=float("nan")) == INVALID and "eps" in _err()
@@ -92,6 +94,7 @@ def test_group_norm_c_abi():
     for kw in (dict(gy=None), dict(x=None), dict(st=None), dict(ws=None)):
         assert bwd(**kw) == INVALID and "null" in _err()
     assert bwd(wb=0) == INVALID and "workspace" in _err()
+    assert bwd(ws=ctypes.c_void_p(0x10008)) == INVALID and "16-byte" in _err()
     assert bwd(gx=None) == 0                            # nothing wanted
     ws = lib.bevk_group_norm_workspace_bytes
     assert ws(3, 0, 1, 4, 8, 2, 1) == -1 and ws(0, 0, 1, 4, 9, 2, 1) == -1
@@ -105,7 +108,8 @@ def test_embedding_refusals(no_device_check):
     for bad, match in (((_meta(10), i), r"weight must be \[V, D\]"), ((w, i.float()), "int64 or int32"),
                        ((w, i.short()), "int64 or int32"), ((w.t(), i), "contiguous"),
                        ((w, i.t()), "contiguous"), ((w.long(), i), "not supported"),
-                       ((w.double(), i), "not implemented")):
+                       ((w.double(), i), "not implemented"),
+                       ((_meta(1, 2 ** 32 + 8), i), "2\\^30 channels")):
         with pytest.raises(RuntimeError, match=match):
             ext.embedding_forward(*bad)
     g = _meta(3, 4, 8)
@@ -149,6 +153,9 @@ def test_embedding_c_abi():
         assert bwd(padding=padding) == INVALID and "padding_idx" in _err()
     for kw in (dict(g=None), dict(i=None), dict(gw=None)):
         assert bwd(**kw) == INVALID and "null" in _err()
+    assert bwd(wb=0) == INVALID and "workspace" in _err()
+    assert bwd(ws=ctypes.c_void_p(0x10004)) == INVALID and "16-byte" in _err()
+    assert bwd(dim=(1 << 30) + 1) == INVALID and "2^30" in _err()
     assert bwd(rows=0) == 0 and bwd(dim=0) == 0
     ws = lib.bevk_embedding_backward_workspace_bytes
     assert ws(3, 4, 10, 8) == -1 and ws(0, -1, 10, 8) == -1 and ws(0, 1 << 31, 10, 8) == -1
@@ -227,3 +234,28 @@ def test_clip_c_abi():
     ws = lib.bevk_clip_gradients_workspace_bytes
     assert ws(0, None) == 0 and ws(-1, None) == -1 and ws(1, None) == -1
     assert ws(2, (ctypes.c_int64 * 2)(1, 0)) == 8
+
+
+def test_calls_go_to_the_tensors_device(monkeypatch):
+    """A call for tensors of another device than the current one makes theirs current for the call,
+    and passes that device's stream."""
+    import contextlib
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, current[0] = current[0], index
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(_bevk, "_current_device", lambda: current[0])
+    monkeypatch.setattr(_bevk, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setitem(_bevk._entries, "f", lambda *a: seen.append((current[0], a)) or 0)
+    _bevk.call_on(0, "f", 1)
+    _bevk.call_on(2, "f", 1, 2)
+    assert seen == [(0, (1, 1000)), (2, (1, 2, 1002))] and current == [0]
+    monkeypatch.setitem(_bevk._entries, "f", lambda *a: 1)
+    for index in (0, 1):
+        with pytest.raises(RuntimeError):
+            _bevk.call_on(index, "f")
