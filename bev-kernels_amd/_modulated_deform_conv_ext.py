@@ -18,6 +18,7 @@ added to what the caller passes, everything else is written.
 from __future__ import annotations
 
 import functools
+import operator
 import os
 from array import array
 
@@ -1166,9 +1167,13 @@ def _dense(t):
     return True
 
 
+_shape_of, _dtype_of = operator.attrgetter("shape"), operator.attrgetter("dtype")
+
+
 def _grad_arrays(fn, tensors, device):
-    """(pointers, type codes, sizes) as arrays for the library. One expression for each attribute:
-    over hundreds of tensors this is the host side of the call."""
+    """(pointers, type codes) as arrays for the library, and whether all are contiguous. One
+    expression for each attribute: over hundreds of tensors this is the host side of the call."""
+    contiguous = True
     for t in tensors:
         if t.get_device() != device or not t.is_contiguous():  # (-1: not on a HIP device)
             if not t.is_cuda:
@@ -1178,12 +1183,13 @@ def _grad_arrays(fn, tensors, device):
             if t.layout is not torch.strided or not _dense(t):
                 raise RuntimeError(f"{fn}: gradients must be dense in memory, got strides "
                                    f"{t.stride() if t.layout is torch.strided else t.layout}")
-    codes = _b._DTYPE_CODES
+            contiguous = False
+    types = list(map(_dtype_of, tensors))
     try:
-        types = array("i", [codes[t.dtype] for t in tensors])
+        codes = array("i", map(_b._DTYPE_CODES.__getitem__, types))
     except KeyError:
-        types = array("i", [_b.dtype_code(t) for t in tensors])  # says which
-    return (array("Q", [t.data_ptr() for t in tensors]), types, array("q", [t.numel() for t in tensors]))
+        codes = array("i", map(_b.dtype_code, tensors))  # says which
+    return array("Q", [t.data_ptr() for t in tensors]), codes, contiguous
 
 
 def clip_gradients(grads, max_norm=None, out=None):
@@ -1193,21 +1199,22 @@ def clip_gradients(grads, max_norm=None, out=None):
     among them."""
     fn = "clip_gradients"
     device = grads[0].get_device()
-    ptrs, types, sizes = _grad_arrays(fn, grads, device)
+    ptrs, types, contiguous = _grad_arrays(fn, grads, device)
+    sizes = array("q", [t.numel() for t in grads])
     optrs = otypes = None
-    if max_norm is not None:
-        out = grads if out is None else out
+    if max_norm is not None and (out is None or out is grads):
+        out, optrs, otypes = grads, ptrs, types
+    elif max_norm is not None:
         if len(out) != len(grads):
             raise RuntimeError(f"{fn}: {len(out)} outputs for {len(grads)} gradients")
-        if out is grads:
-            optrs, otypes = ptrs, types
-        else:
+        optrs, otypes, out_contiguous = _grad_arrays(fn, out, device)
+        alike = list(map(_shape_of, grads)) == list(map(_shape_of, out))
+        if not alike or not (contiguous and out_contiguous):
             for g, o in zip(grads, out):
                 if o.shape != g.shape or (not (o.is_contiguous() and g.is_contiguous())
                                           and o.stride() != g.stride()):
                     raise RuntimeError(f"{fn}: an output has shape {tuple(o.shape)} and strides "
                                        f"{o.stride()}, its gradient {tuple(g.shape)} and {g.stride()}")
-            optrs, otypes, _ = _grad_arrays(fn, out, device)
     count, at = len(grads), lambda a: a.buffer_info()[0] if a is not None else None
     nbytes = _b.lib().bevk_clip_gradients_workspace_bytes(count, at(sizes))
     if nbytes < 0:
