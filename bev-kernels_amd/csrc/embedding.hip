@@ -87,54 +87,59 @@ struct Sorted {
   int *valid;    // places in use
 };
 
-// The row an index stands for, and the workgroup that owns it: R for an index without a row. An
-// index is compared as unsigned numbers, so that negative ones are past the table too.
-struct Owned {
-  uint32_t row, owner;
-};
 struct SortArgs {
   uint32_t n, rows, padding;  // padding: ~0 for none
   int log_r, per;             // rows v with v % R = w are a workgroup's; at most `per` of them
 };
-template <typename I>
-__device__ __forceinline__ Owned owned(const I *index, uint32_t t, const SortArgs &p) {
-  uint32_t row, high = 0;
-  if constexpr (sizeof(I) == 8) {
-    const uint2 v = reinterpret_cast<const uint2 *>(index)[t];
-    row = v.x;
-    high = v.y;
-  } else {
-    row = (uint32_t)index[t];
-  }
-  const uint32_t count = 1u << p.log_r;
-  return {row, high == 0 && row < p.rows && row != p.padding ? row & (count - 1) : count};
+
+// Lanes whose index is a row of this workgroup, or of one before it. An index is compared as unsigned
+// numbers, so that negative ones are past the table too.
+struct Owned {
+  uint32_t row;
+  bool mine, before;
+};
+template <bool PADDED, typename I>
+__device__ __forceinline__ Owned owned(I index, const SortArgs &p, uint32_t w) {
+  const uint32_t row = (uint32_t)index;
+  bool there = row < p.rows;
+  if constexpr (sizeof(I) == 8) there = there && (uint64_t)index >> 32 == 0;
+  if constexpr (PADDED) there = there && row != p.padding;
+  const uint32_t owner = row & ((1u << p.log_r) - 1);
+  return {row, there && owner == w, there && owner < w};
 }
 
-// f(t of the wave's first lane, its 64 indices) over [begin, end), kScan times 64 of them loaded
-// together; lanes past the end have no row.
+// f(t of the wave's first lane, what its 64 indices are) over [begin, end), kScan times 64 of them
+// loaded together and the rest by half of that; lanes past the end have no row.
 constexpr int kScan = 8;
-template <typename I, typename F>
+template <bool PADDED, typename I, typename F>
 __device__ __forceinline__ void scan(const I *index, uint32_t begin, uint32_t end, const SortArgs &p, F f) {
-  const int lane = threadIdx.x % kWave;
+  const uint32_t lane = threadIdx.x % kWave, w = blockIdx.x;
   uint32_t t = begin;
-  for (; t + kScan * kWave <= end; t += kScan * kWave) {
-    Owned o[kScan];
+  const I *at = index + begin + lane;
+  for (; t + kScan * kWave <= end; t += kScan * kWave, at += kScan * kWave) {
+    I v[kScan];
 #pragma unroll
-    for (int j = 0; j < kScan; ++j) o[j] = owned(index, t + j * kWave + lane, p);
+    for (int j = 0; j < kScan; ++j) v[j] = at[j * kWave];
 #pragma unroll
-    for (int j = 0; j < kScan; ++j) f(t + j * kWave, o[j]);
+    for (int j = 0; j < kScan; ++j) f(t + j * kWave, owned<PADDED>(v[j], p, w));
   }
-  for (; t < end; t += kWave) {
-    Owned o = owned(index, min(t + lane, end - 1), p);
-    if (t + lane >= end) o.owner = 1u << p.log_r;
-    f(t, o);
+  for (; t < end; t += kScan / 2 * kWave) {
+    I v[kScan / 2];
+#pragma unroll
+    for (int j = 0; j < kScan / 2; ++j) v[j] = index[min(t + j * kWave + lane, end - 1)];
+#pragma unroll
+    for (int j = 0; j < kScan / 2; ++j) {
+      Owned o = owned<PADDED>(v[j], p, w);
+      if (t + j * kWave + lane >= end) o.mine = o.before = false;
+      f(t + j * kWave, o);
+    }
   }
 }
 
 // Two passes over the indices' owners, one where no wave finds more than kKept of its workgroup's
 // (n / (16 R) on average): those it keeps.
 constexpr int kKept = 128;
-template <typename I>
+template <typename I, bool PADDED>
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict__ index, SortArgs p, Sorted out) {
   extern __shared__ int count[];  // [wave][per]
   __shared__ int before[kSortWaves], wave_sum[kSortWaves];
@@ -150,11 +155,11 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
   const uint64_t lanes_before = (1ull << lane) - 1;
   int lower = 0;
   uint32_t found = 0;
-  scan(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
-    lower += __popcll(__ballot(o.owner < w));
-    const uint64_t own = __ballot(o.owner == w);
+  scan<PADDED>(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
+    lower += o.before ? 1 : 0;
+    const uint64_t own = __ballot(o.mine);
     if (own) {
-      if (o.owner == w) {
+      if (o.mine) {
         const uint32_t k = found + __popcll(own & lanes_before), r = o.row >> p.log_r;
         if (k < kKept) kept[wave][k] = make_uint2(t + lane, r);
         atomicAdd(&mine[r], 1);
@@ -162,6 +167,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
       found += __popcll(own);
     }
   });
+  for (int d = kWave / 2; d >= 1; d /= 2) lower += __shfl_xor(lower, d, kWave);
   if (lane == 0) before[wave] = lower;
   __syncthreads();
 
@@ -195,21 +201,21 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
   if (w == gridDim.x - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
   __syncthreads();
 
-  // Places of up to 64 of the wave's indices, in their order: a row at a time.
+  // Places of up to 64 of the wave's indices, in their order: the lanes that have a lane's row are
+  // found from the rows' bits.
+  const int bits = 32 - __builtin_clz(per);
   auto place = [&](bool own, uint32_t t, uint32_t r) __attribute__((always_inline)) {
-    uint64_t left = __ballot(own);
-    while (left) {
-      const int lead = __builtin_ctzll(left);
-      const uint64_t same = __ballot(own && r == (uint32_t)__builtin_amdgcn_readlane((int)r, lead));
-      int first = 0;
-      if (lane == lead) first = atomicAdd(&mine[r], __popcll(same));
-      first = __builtin_amdgcn_readlane(first, lead);
-      if (same >> lane & 1) {
-        const int k = first + __popcll(same & lanes_before);
-        out.order[k] = (int)t;
-        out.row[k] = (int)((r << p.log_r) | w);
-      }
-      left &= ~same;
+    uint64_t same = __ballot(own);
+    for (int k = 0; k < bits; ++k) {
+      const bool bit = r >> k & 1;
+      const uint64_t set = __ballot(bit);
+      same &= bit ? set : ~set;
+    }
+    if (own) {
+      const int rank = __popcll(same & lanes_before), k = mine[r] + rank;
+      out.order[k] = (int)t;
+      out.row[k] = (int)((r << p.log_r) | w);
+      if (rank == 0) atomicAdd(&mine[r], __popcll(same));  // after all lanes have read it
     }
   };
   if (found <= kKept) {
@@ -218,8 +224,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
       place(k + lane < found, e.x, e.y);
     }
   } else {
-    scan(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
-      place(o.owner == w, t + lane, o.row >> p.log_r);
+    scan<PADDED>(index, begin, end, p, [&](uint32_t t, Owned o) __attribute__((always_inline)) {
+      place(o.mine, t + lane, o.row >> p.log_r);
     });
   }
 }
@@ -408,7 +414,8 @@ hipError_t backward(const EmbeddingArgs &a, const void *grad_out, int64_t paddin
     p.log_r = 8;  // 256 workgroups, or as many as have at most kSortRows rows each
     while ((a.rows - 1) >> p.log_r >= kSortRows) ++p.log_r;
     p.per = (int)((a.rows - 1) >> p.log_r) + 1;
-    hipLaunchKernelGGL((sort_kernel<I>), dim3(1 << p.log_r), dim3(kSortThreads), kSortWaves * p.per * 4, stream,
+    const auto sort = padding < 0 ? sort_kernel<I, false> : sort_kernel<I, true>;
+    hipLaunchKernelGGL(sort, dim3(1 << p.log_r), dim3(kSortThreads), kSortWaves * p.per * 4, stream,
                        static_cast<const I *>(a.index), p, s);
     if (hipError_t e = hipGetLastError()) return e;
   }
