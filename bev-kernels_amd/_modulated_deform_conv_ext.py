@@ -1086,6 +1086,9 @@ def _group_norm_gradients(grad_y, x, weight, bias, stats, wanted, sizes):
 # Embedding rows by index (no counterpart in the reference)
 # ---------------------------------------------------------------------------------------
 
+_INDEX_WIDE = {torch.int64: 1, torch.int32: 0}
+
+
 def _embedding_check(fn, index, table, name):
     if not table.is_cuda or not index.is_cuda or table.get_device() != index.get_device():
         _b.require_device(fn, table, index)
@@ -1093,7 +1096,7 @@ def _embedding_check(fn, index, table, name):
         raise RuntimeError("index must be contiguous")
     if not table.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
-    if index.dtype != torch.int64 and index.dtype != torch.int32:
+    if index.dtype not in _INDEX_WIDE:
         raise RuntimeError(f"{fn}: index must be int64 or int32, got {index.dtype}")
     if _b.dtype_code(table) == _b.BEVK_F64:
         raise RuntimeError(f"{fn}: not implemented for {table.dtype}")
@@ -1105,14 +1108,18 @@ def embedding_forward(weight, index, scale=1.0):
     """scale * weight[index] [*index.shape, D] in the type of weight [V, D]; index int64 or int32,
     rows of zeros where it is outside [0, V)."""
     fn = "embedding_forward"
-    _embedding_check(fn, index, weight, "weight")
-    if weight.dim() != 2:
-        raise RuntimeError(f"{fn}: weight must be [V, D], got {tuple(weight.shape)}")
-    rows, dim = weight.shape
+    device, shape, code = weight.get_device(), weight.shape, _b._DTYPE_CODES.get(weight.dtype)
+    wide = _INDEX_WIDE.get(index.dtype)
+    # (one expression where all is well: a decoder's call is as long as its host side)
+    if (device < 0 or index.get_device() != device or wide is None or code is None or code == _b.BEVK_F64
+            or len(shape) != 2 or shape[1] > _MAX_CHANNELS or not index.is_contiguous()
+            or not weight.is_contiguous()):
+        _embedding_check(fn, index, weight, "weight")
+        raise RuntimeError(f"{fn}: weight must be [V, D], got {tuple(shape)}")
+    rows, dim = shape
     out = weight.new_empty((*index.shape, dim))
-    _b.call_on(weight.get_device(), "bevk_embedding_forward", _b._DTYPE_CODES[weight.dtype],
-               weight.data_ptr(), rows, dim, index.data_ptr(), index.dtype == torch.int64, index.numel(),
-               scale, out.data_ptr())
+    _b.call_on(device, "bevk_embedding_forward", code, weight.data_ptr(), rows, dim, index.data_ptr(), wide,
+               index.numel(), scale, out.data_ptr())
     return out
 
 
@@ -1148,7 +1155,7 @@ def _embedding_gradient(grad_out, index, rows, scale, padding_idx):
     grad = grad_out.new_empty((rows, dim))
     ws = grad_out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _b.call_on(grad_out.get_device(), "bevk_embedding_backward", code, grad_out.data_ptr(), index.data_ptr(),
-               index.dtype == torch.int64, n, rows, dim, scale, padding_idx, _b.ptr(ws), nbytes,
+               _INDEX_WIDE[index.dtype], n, rows, dim, scale, padding_idx, _b.ptr(ws), nbytes,
                grad.data_ptr())
     return grad
 
