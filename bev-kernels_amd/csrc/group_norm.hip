@@ -19,9 +19,9 @@
 // workgroup of the second adds up again those of its own slab's groups: a few KB, where a third
 // launch between would cost 4 us and tiles of whole rows would read the sums of every group.
 // The second launch takes the tiles in the opposite order (within the XCD that had them), so that
-// what the first one read last is still in the caches. Six 58 x 100 x 256 maps in 16 bits (res4): 5.8
-// and 11.1 us forward, 9.5 and 10.6 us backward; their 36 and 53 MB once take 5.5 and 8.2 us at
-// the rate of a copy of that size.
+// what the first one read last is still in the caches. Six 58 x 100 x 256 maps in 16 bits (res4): 6.0
+// and 9.0 us forward, 9.9 and 10.5 us backward; their 36 and 53 MB once take 5.5 and 8.2 us at the
+// rate of a copy of that size.
 #include <algorithm>
 
 #include "bevk_launch.h"
@@ -39,11 +39,10 @@ template <typename T, int V> struct Tile {
   static constexpr int kLanes = V > 1 ? 8 : 64;
   static constexpr int kSlab = kLanes * V;            // channels
   static constexpr int kRows = kThreads / kLanes;     // positions side by side
-  // Positions of a thread loaded together where sums are taken, and where values are written (res4 in
-  // 16 bits, 2 / 4 / 8 of them: sums 6.0 / 6.4 / 7.8 us forward, 9.4 / 10.6 / 11.8 us backward; values
-  // 11.2 / 10.7 / 12.4 and 11.2 / 10.6 / 12.4).
-  static constexpr int kSums = V > 1 ? 2 : 8;
-  static constexpr int kValues = V > 1 ? 4 : 8;
+  // Positions of a thread loaded together, one such step ahead (res4 in 16 bits, 2 / 4 / 8 of them:
+  // 6.0 / 6.6 / 8.3 and 9.0 / 9.7 / 10.4 us forward, 9.9 / 10.3 / 11.6 and 10.5 / 10.5 / 12.3
+  // backward).
+  static constexpr int kAhead = V > 1 ? 2 : 8;
 };
 
 struct Geo {
@@ -89,7 +88,7 @@ __device__ __forceinline__ void from_f32(void *p, int dtype, int64_t i, float v)
 
 // 1 / (1 + exp(-z)). The types of 16 bits do with the hardware's exp2 and reciprocal (2^-20 relative
 // for |z| up to 10, where fp32's own functions have 2^-22): the second launch of six 116 x 200 x 256
-// bf16 maps takes 29.6 us with them, 34.8 us with fp32's.
+// bf16 maps took 29.6 us with them and 34.8 us with fp32's (26.5 us now).
 template <typename T> __device__ __forceinline__ float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
@@ -258,7 +257,7 @@ template <typename T, int V, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x, Geo g,
                                                          Pair<double> *__restrict__ part) {
   using TL = Tile<T, V>;
-  using R = Rows<T, V, TL::kSums>;
+  using R = Rows<T, V, TL::kAhead>;
   constexpr int E = WHOLE ? 1 : V;  // sums of a thread
   __shared__ Pair<double> s[kWaves][TL::kLanes * E];
   const Place p = place_of(g, blockIdx.x);
@@ -274,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x
     const R v = next;
     next.load(x, g, p, q + R::kStep, c);
 #pragma unroll
-    for (int u = 0; u < TL::kSums; ++u)
+    for (int u = 0; u < TL::kAhead; ++u)
       if (q + u * TL::kRows < p.p1)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -312,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__
                                                            const Pair<double> *__restrict__ part,
                                                            Pair<double> *__restrict__ stats, T *__restrict__ y) {
   using TL = Tile<T, V>;
-  using R = Rows<T, V, TL::kValues>;
+  using R = Rows<T, V, TL::kAhead>;
   constexpr int E = WHOLE ? 1 : V;  // groups of a thread
   __shared__ Pair<double> sums[kWaves][TL::kSlab];
   __shared__ float high_of[TL::kSlab], low_of[TL::kSlab], rstd_of[TL::kSlab];
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__
     R v = next;
     next.load(x, g, p, q + R::kStep, c);
 #pragma unroll
-    for (int u = 0; u < TL::kValues; ++u)
+    for (int u = 0; u < TL::kAhead; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = centred((float)v.v[u].v[e], high[WHOLE ? 0 : e], low[WHOLE ? 0 : e]);
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const T *__restrict
                                                              Pair<float> *__restrict__ by_group,
                                                              Pair<float> *__restrict__ by_channel) {
   using TL = Tile<T, V>;
-  using R = Rows<T, V, TL::kSums>;
+  using R = Rows<T, V, TL::kAhead>;
   __shared__ Channel ch[TL::kSlab];
   __shared__ Pair<float> s[kWaves][TL::kSlab];
   const Place p = place_of(g, blockIdx.x);
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const T *__restrict
       next_x.load(x, g, p, q + R::kStep, c);
       next_d.load(gy, g, p, q + R::kStep, c);
 #pragma unroll
-      for (int u = 0; u < TL::kSums; ++u)
+      for (int u = 0; u < TL::kAhead; ++u)
         if (q + u * TL::kRows < p.p1)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ 
                                                           const Pair<float> *__restrict__ by_channel,
                                                           T *__restrict__ gx, void *grad_w, void *grad_b) {
   using TL = Tile<T, V>;
-  using R = Rows<T, V, TL::kValues>;
+  using R = Rows<T, V, TL::kAhead>;
   constexpr int E = WHOLE ? 1 : V;
   __shared__ union {
     Pair<double> by_group[kWaves][TL::kSlab], by_channel[kThreads];
@@ -632,7 +631,7 @@ __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ 
     next_x.load(x, g, p, q + R::kStep, c);
     next_d.load(gy, g, p, q + R::kStep, c);
 #pragma unroll
-    for (int u = 0; u < TL::kValues; ++u)
+    for (int u = 0; u < TL::kAhead; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float gz, xh;
