@@ -19,24 +19,26 @@ def _ext():
     return _loaded
 
 
+def _lookup(weight, index, scale, padding_idx):
+    """The rows, and the index as it was read."""
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise RuntimeError("embedding_lookup: padding_idx must be a row of the table, got "
+                           f"{padding_idx}")
+    if not index.is_contiguous():
+        index = index.contiguous()
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    return _ext().embedding_forward(weight, index, scale), index
+
+
 class EmbeddingLookupFunction(torch.autograd.Function):
     """out [*index.shape, D] = scale * weight[index]; the gradient flows to weight [V, D]."""
 
     @staticmethod
     def forward(ctx, weight, index, scale=1.0, padding_idx=None):
-        rows = weight.shape[0]
-        if padding_idx is None:
-            padding_idx = -1
-        elif not 0 <= padding_idx < rows:
-            raise RuntimeError("embedding_lookup: padding_idx must be a row of the table, got "
-                               f"{padding_idx}")
-        if not index.is_contiguous():
-            index = index.contiguous()
-        if not weight.is_contiguous():
-            weight = weight.contiguous()
-        out = _ext().embedding_forward(weight, index, scale)
+        out, index = _lookup(weight, index, scale, padding_idx)
         ctx.save_for_backward(index)
-        ctx.args = rows, scale, padding_idx
+        ctx.args = weight.shape[0], scale, -1 if padding_idx is None else padding_idx
         return out
 
     @staticmethod
@@ -54,4 +56,6 @@ def embedding_lookup(weight, index, scale=1.0, padding_idx=None):
     gets no gradient. The row padding_idx is looked up as any other, and its gradient is zero, as
     in torch.nn.Embedding. The gradient is dense, adds up in fp32 in a fixed order and is the same
     on every run. Differentiable once."""
+    if not torch.is_grad_enabled():  # (without the bookkeeping of a Function, 4 us of a small call)
+        return _lookup(weight, index, scale, padding_idx)[0]
     return EmbeddingLookupFunction.apply(weight, index, scale, padding_idx)

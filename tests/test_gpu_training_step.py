@@ -104,3 +104,21 @@ def test_step_captured():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert (a - b).abs().max().item() <= 4096 * 2.0 ** -24 * b.abs().max().item()
+
+
+def test_without_gradients():
+    """Under no_grad and inference_mode: the same values, nothing recorded; refusals stay."""
+    params, index, _, x, _ = _leaves(torch.bfloat16, 6)
+    grid, gn_w, gn_b = params[0], params[4], params[5]
+    maps = x.repeat(1, 1, 1, 4).permute(0, 2, 1, 3)  # not contiguous
+    want = [msda_opt2.embedding_lookup(grid, index, 2.0, 3), mdc.group_norm_act_nhwc(maps, 32, gn_w, gn_b)]
+    assert all(t.requires_grad for t in want)
+    for mode in (torch.no_grad(), torch.inference_mode()):
+        with mode:
+            got = [msda_opt2.embedding_lookup(grid, index.t().contiguous().t(), 2.0, 3),
+                   mdc.group_norm_act_nhwc(maps, 32, gn_w, gn_b)]
+            assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+            with pytest.raises(RuntimeError, match="padding_idx"):
+                msda_opt2.embedding_lookup(grid, index, 1.0, CELLS)
+            with pytest.raises(RuntimeError, match="act must be"):
+                mdc.group_norm_act_nhwc(maps, 32, gn_w, gn_b, act="gelu")
