@@ -1031,20 +1031,20 @@ def _group_norm_sizes(x, num_groups, weight, bias, act):
             GROUP_NORM_ACTS[act])
 
 
-def _group_norm_run(x, num_groups, weight, bias, eps, act):
-    """(y, stats, sizes): sizes as _group_norm_sizes gives them."""
+def _group_norm_run(x, num_groups, weight, bias, eps, act, with_stats=True):
+    """(y, stats or None, sizes): sizes as _group_norm_sizes gives them."""
     _group_norm_check("group_norm_forward", x, num_groups, weight, bias, act)
     sizes = _group_norm_sizes(x, num_groups, weight, bias, act)
     code, pcode, images, positions, channels, _, acode = sizes
     y = torch.empty_like(x)
-    stats = x.new_empty((images, num_groups, 2), dtype=torch.float64)
+    stats = x.new_empty((images, num_groups, 2), dtype=torch.float64) if with_stats else None
     if positions:
         at = x.data_ptr()
         nbytes = _group_norm_workspace_bytes(code, 0, images, positions, channels, num_groups, at % 16 == 0)
         ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _b.call_on(x.get_device(), "bevk_group_norm_forward", code, at, _b.ptr(weight), _b.ptr(bias), pcode,
                    images, positions, channels, num_groups, eps, acode, _b.ptr(ws), nbytes, y.data_ptr(),
-                   stats.data_ptr())
+                   _b.ptr(stats))
     return y, stats, sizes
 
 

@@ -170,7 +170,7 @@ hipError_t launch_column_sums(int dtype, const void *src, int64_t rows, int ld, 
                               int out_dtype, void *out, hipStream_t stream);
 
 // Group normalization with an activation, channels last: x [batch][pixels][channels] -> y (dtype), and
-// stats [batch][groups][2] (mean, 1 / sqrt(var + eps)) for the backward. weight / bias [channels]
+// stats [batch][groups][2] (mean, 1 / sqrt(var + eps); or null) for the backward. weight / bias [channels]
 // (param_dtype) or null; channels % groups == 0, no empty sizes. The backward writes grad_x (dtype),
 // grad_w and grad_b (param_dtype), each skipped when null.
 enum GroupNormAct { kActNone = 0, kActRelu = 1, kActSilu = 2 };

@@ -1246,7 +1246,7 @@ int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const 
   if (!(eps >= 0.0)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
   const int64_t need = bevk::group_norm_workspace_bytes(dtype, false, batch, pixels, channels, groups,
                                                         on_16_bytes({x, y}));
-  if (!x || !y || !stats) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!x || !y) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   return hip_status(
       bevk::launch_group_norm_forward(

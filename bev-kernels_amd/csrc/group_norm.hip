@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__
     low_of[threadIdx.x] = (float)(mean - (double)(float)mean);
     rstd_of[threadIdx.x] = (float)st.b;
     const int group = g0 + threadIdx.x;
-    if (p.split == 0 && group * g.per / TL::kSlab == p.slab) stats[p.n * args.groups + group] = st;
+    if (stats != nullptr && p.split == 0 && group * g.per / TL::kSlab == p.slab) stats[p.n * args.groups + group] = st;
   }
   __syncthreads();
   if (c >= g.channels) return;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(const T *__restric
       high_of[k] = (float)mean;
       low_of[k] = (float)(mean - (double)(float)mean);
       rstd_of[k] = (float)st.b;
-      stats[n * args.groups + g0 + k] = st;
+      if (stats != nullptr) stats[n * args.groups + g0 + k] = st;
     }
   }
   __syncthreads();

@@ -468,7 +468,7 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
  *   y            act((x - mean) / sqrt(var + eps) * weight + bias), dtype
  *   weight, bias [channels] param_dtype, or NULL (1 and 0)
  *   act          0: none, 1: ReLU, 2: SiLU (z / (1 + exp(-z)))
- *   stats        [batch, groups, 2] fp64, written: mean and 1 / sqrt(var + eps), for the backward
+ *   stats        [batch, groups, 2] fp64, written: mean and 1 / sqrt(var + eps), for the backward; or NULL
  * The backward writes grad_x (dtype), grad_weight and grad_bias [channels] (param_dtype), each NULL
  * where it is not wanted; ReLU's derivative at 0 is 0. The same results on every run. dtype and
  * param_dtype F32, F16, BF16 (param_dtype: the input's or F32); the workspace (16-byte aligned) holds what

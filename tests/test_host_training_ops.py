@@ -83,7 +83,7 @@ def test_group_norm_c_abi():
     assert fwd(act=3) == INVALID and "activation" in _err()
     assert fwd(eps=-1.0) == INVALID and "eps" in _err()
     assert fwd(eps=float("nan")) == INVALID and "eps" in _err()
-    for kw in (dict(x=None), dict(y=None), dict(st=None)):
+    for kw in (dict(x=None), dict(y=None)):
         assert fwd(**kw) == INVALID and "null" in _err()
 
     def bwd(dtype=0, gy=P, x=P, act=0, st=P, ws=P, wb=1 << 30, gx=P):
