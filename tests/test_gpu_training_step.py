@@ -122,3 +122,34 @@ def test_without_gradients():
                 msda_opt2.embedding_lookup(grid, index, 1.0, CELLS)
             with pytest.raises(RuntimeError, match="act must be"):
                 mdc.group_norm_act_nhwc(maps, 32, gn_w, gn_b, act="gelu")
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams without a wait between: each call has its own workspace."""
+    def work(seed):
+        g = torch.Generator().manual_seed(seed)
+        x = torch.randn(6, 40, 50, 256, generator=g).half().to(DEV).requires_grad_()
+        w = torch.rand(256, generator=g).half().to(DEV).requires_grad_()
+        table = torch.randn(3000, 128, generator=g).to(DEV).requires_grad_()
+        index = torch.randint(-1, 3000, (40000,), generator=g).to(DEV)
+        return x, w, table, index, torch.ones(40000, 128, device=DEV)
+
+    def run(x, w, table, index, g):
+        y = mdc.group_norm_act_nhwc(x, 32, w, None, act="relu")
+        grads = list(torch.autograd.grad(y, (x, w), y.detach()))
+        grads += torch.autograd.grad(msda_opt2.embedding_lookup(table, index), table, g)
+        return [y.detach(), mdc.clip_gradients_(grads, 1.0), *grads]
+
+    inputs = [work(1), work(2)]
+    want = [run(*i) for i in inputs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(run(*inputs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for outs in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[k]))
