@@ -1182,7 +1182,7 @@ def _grad_arrays(fn, tensors, device):
     expression for each attribute: over hundreds of tensors this is the host side of the call."""
     contiguous = True
     for t in tensors:
-        if t.get_device() != device or not t.is_contiguous():  # (-1: not on a HIP device)
+        if t.get_device() != device or not t.is_contiguous():
             if not t.is_cuda:
                 raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {t.device}")
             if t.get_device() != device:
@@ -1206,6 +1206,8 @@ def clip_gradients(grads, max_norm=None, out=None):
     among them."""
     fn = "clip_gradients"
     device = grads[0].get_device()
+    if device < 0:  # not on a HIP device: others there too would have the same -1
+        raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {grads[0].device}")
     ptrs, types, contiguous = _grad_arrays(fn, grads, device)
     sizes = array("q", [t.numel() for t in grads])
     optrs = otypes = None
