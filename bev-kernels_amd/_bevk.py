@@ -14,6 +14,7 @@ import os
 import threading
 
 import torch  # must be imported before the library is loaded
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 _LIB_NAME = "libbevk.so"
@@ -193,6 +194,12 @@ def call_on(index: int, name: str, *args) -> None:
     if rc != 0:
         msg = lib().bevk_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"{name} failed with status {rc}")
+
+
+def records_nothing() -> bool:
+    """Whether a call needs no autograd function: neither gradients are recorded nor forward mode is
+    active, which torch.no_grad leaves on and which a Function without a jvp refuses by itself."""
+    return not torch.is_grad_enabled() and _forward_ad._current_level < 0
 
 
 def once_differentiable(backward):

@@ -48,8 +48,8 @@ class GroupNormActNHWCFunction(torch.autograd.Function):
 def group_norm_act_nhwc(x_nhwc, num_groups, weight=None, bias=None, eps=1e-5, act=None):
     """act(group norm of x_nhwc [N, ..., C]) over the positions and the C / num_groups channels of
     each group; weight and bias [C] in the input's type or float32 (or None: 1 and 0); act None,
-    "relu" or "silu". fp32 / fp16 / bf16. Differentiable once."""
-    if not torch.is_grad_enabled():  # (without the bookkeeping of a Function, 4 us of a small call)
+    "relu" or "silu". fp32 / fp16 / bf16. Differentiable once, in reverse mode."""
+    if _b.records_nothing():  # (without the bookkeeping of a Function, 4 us of a small call)
         return _ext()._group_norm_run(_dense(x_nhwc), num_groups, _dense(weight), _dense(bias), eps, act,
                                       False)[0]
     return GroupNormActNHWCFunction.apply(x_nhwc, num_groups, weight, bias, eps, act)

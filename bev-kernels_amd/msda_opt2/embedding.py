@@ -55,7 +55,7 @@ def embedding_lookup(weight, index, scale=1.0, padding_idx=None):
     -> [*index.shape, D]. An index outside [0, V) (-1 in a padded list) gives a row of zeros and
     gets no gradient. The row padding_idx is looked up as any other, and its gradient is zero, as
     in torch.nn.Embedding. The gradient is dense, adds up in fp32 in a fixed order and is the same
-    on every run. Differentiable once."""
-    if not torch.is_grad_enabled():  # (without the bookkeeping of a Function, 4 us of a small call)
+    on every run. Differentiable once, in reverse mode."""
+    if _b.records_nothing():  # (without the bookkeeping of a Function, 4 us of a small call)
         return _lookup(weight, index, scale, padding_idx)[0]
     return EmbeddingLookupFunction.apply(weight, index, scale, padding_idx)
