@@ -6,9 +6,23 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "bevk_common.h"
 
 namespace bevk {
+
+// A launch takes fewer than 2^32 work items: f(first block, blocks) for parts of `blocks` workgroups
+// of `threads`. Parts begin at multiples of 8, so a workgroup of a later one is on the XCD that its
+// number within all of them says.
+template <typename F> hipError_t launch_in_parts(int64_t blocks, int threads, F f) {
+  const int64_t most = (1LL << 31) / threads;
+  for (int64_t first = 0; first < blocks; first += most) {
+    f(first, (unsigned)std::min(most, blocks - first));
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
 
 // Compute units of the current device (cached per device; 0 when the query fails).
 int device_cus();

@@ -51,6 +51,7 @@ struct Geo {
   int slabs, splits;     // tiles of an image: slabs x splits
   int local;             // room for the groups of a slab
   int64_t tiles;
+  int64_t first;         // workgroups in the launches before (launch_in_parts)
 };
 
 __device__ __forceinline__ float to_f32(const void *p, int dtype, int64_t i, float none) {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const T *__restrict__ x
   using R = Rows<T, V, TL::kAhead>;
   constexpr int E = WHOLE ? 1 : V;  // sums of a thread
   __shared__ Pair<double> s[kWaves][TL::kLanes * E];
-  const Place p = place_of(g, blockIdx.x);
+  const Place p = place_of(g, g.first + blockIdx.x);
   const int lane = threadIdx.x % TL::kLanes, wave = threadIdx.x / kWave;
   const int c = (p.slab * TL::kLanes + lane) * V;
   Pair<double> a[E];
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const T *__restrict__
   constexpr int E = WHOLE ? 1 : V;  // groups of a thread
   __shared__ Pair<double> sums[kWaves][TL::kSlab];
   __shared__ float high_of[TL::kSlab], low_of[TL::kSlab], rstd_of[TL::kSlab];
-  const int64_t tile = tile_of(g, blockIdx.x, true);
+  const int64_t tile = tile_of(g, g.first + blockIdx.x, true);
   if (tile >= g.tiles) return;
   const Place p = place_of(g, tile);
   const int c = (p.slab * TL::kLanes + threadIdx.x % TL::kLanes) * V;
@@ -495,7 +496,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const T *__restrict
   using R = Rows<T, V, TL::kAhead>;
   __shared__ Channel ch[TL::kSlab];
   __shared__ Pair<float> s[kWaves][TL::kSlab];
-  const Place p = place_of(g, blockIdx.x);
+  const Place p = place_of(g, g.first + blockIdx.x);
   const int lane = threadIdx.x % TL::kLanes, wave = threadIdx.x / kWave;
   const int c = (p.slab * TL::kLanes + lane) * V;
   int64_t q = p.p0 + threadIdx.x / TL::kLanes;
@@ -599,11 +600,12 @@ __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ 
   } sums;
   __shared__ Pair<float> means[TL::kSlab];
   __shared__ Channel ch[TL::kSlab];
-  if ((int)blockIdx.x < param_blocks) {
-    param_grads(g, args, blockIdx.x, by_channel, grad_w, grad_b, sums.by_channel);
+  const int64_t block = g.first + blockIdx.x;
+  if (block < param_blocks) {
+    param_grads(g, args, (int)block, by_channel, grad_w, grad_b, sums.by_channel);
     return;
   }
-  const int64_t tile = tile_of(g, blockIdx.x - param_blocks, true);
+  const int64_t tile = tile_of(g, block - param_blocks, true);
   if (tile >= g.tiles || gx == nullptr) return;
   const Place p = place_of(g, tile);
   const int lane = threadIdx.x % TL::kLanes, g0 = first_group<TL::kSlab>(g, p.slab);
@@ -662,6 +664,7 @@ Geo make_geo(int64_t batch, int64_t pixels, int channels, int groups, int slab, 
   g.each = std::max<int64_t>(1, (rounds + want - 1) / want) * rows;
   g.splits = (int)((pixels + g.each - 1) / g.each);
   g.tiles = batch * g.slabs * g.splits;
+  g.first = 0;
   return g;
 }
 
@@ -679,68 +682,88 @@ template <typename T> bool vectors(const GroupNormArgs &a, const void *p, const 
   return all % 16 == 0;
 }
 
-// One launch: up to small_pixels() positions, and no group in two slabs.
+// One launch: up to small_pixels() positions, no group in two slabs, and no more workgroups
+// than a launch takes.
 template <typename T, int V> bool small(const GroupNormArgs &a) {
+  constexpr int kSlab = Tile<T, V>::kSlab;
   const int per = a.channels / a.groups;
-  return a.pixels <= small_pixels<T, V>() && (a.channels <= Tile<T, V>::kSlab || Tile<T, V>::kSlab % per == 0);
+  const int64_t workgroups = a.batch * ((a.channels + kSlab - 1) / kSlab);
+  return a.pixels <= small_pixels<T, V>() && (a.channels <= kSlab || kSlab % per == 0) &&
+         workgroups * kSmallThreads < 1LL << 32;
 }
 
 // f(whether a vector's channels are of one group, the activation) as constants.
 template <int V, typename F> hipError_t with_kinds(const Geo &g, int act, F f) {
-  auto with_act = [&](auto whole) {
+  auto with_act = [&](auto whole) -> hipError_t {
     switch (act) {
-      case kActRelu: f(whole, std::integral_constant<int, kActRelu>()); break;
-      case kActSilu: f(whole, std::integral_constant<int, kActSilu>()); break;
-      default: f(whole, std::integral_constant<int, kActNone>()); break;
+      case kActRelu: return f(whole, std::integral_constant<int, kActRelu>());
+      case kActSilu: return f(whole, std::integral_constant<int, kActSilu>());
+      default: return f(whole, std::integral_constant<int, kActNone>());
     }
   };
   if constexpr (V == 1) {
-    with_act(std::true_type());
+    return with_act(std::true_type());
   } else if (g.per % V == 0) {
-    with_act(std::true_type());
+    return with_act(std::true_type());
   } else {
-    with_act(std::false_type());
+    return with_act(std::false_type());
   }
-  return hipGetLastError();
 }
 
-unsigned back_grid(const Geo &g) { return (unsigned)((g.tiles + kXcds - 1) / kXcds * kXcds); }
+int64_t back_grid(const Geo &g) { return (g.tiles + kXcds - 1) / kXcds * kXcds; }
+
+// f(geometry, workgroups) for `blocks` workgroups of kThreads.
+template <typename F> hipError_t in_parts(Geo g, int64_t blocks, F f) {
+  return launch_in_parts(blocks, kThreads, [&](int64_t first, unsigned count) {
+    g.first = first;
+    f(g, count);
+  });
+}
 
 template <typename T, int V>
 hipError_t forward(const GroupNormArgs &a, void *y, double *stats, void *workspace, hipStream_t stream) {
-  const Geo g = geo_of<T, V>(a);
-  if (g.tiles > 1 << 30) return hipErrorInvalidValue;
+  const Geo geo = geo_of<T, V>(a);
   const T *x = static_cast<const T *>(a.x);
   Pair<double> *part = static_cast<Pair<double> *>(workspace), *st = reinterpret_cast<Pair<double> *>(stats);
-  return with_kinds<V>(g, a.act, [&](auto whole, auto act) {
+  return with_kinds<V>(geo, a.act, [&](auto whole, auto act) {
     constexpr bool W = decltype(whole)::value;
+    constexpr int A = decltype(act)::value;
     if (small<T, V>(a)) {
-      hipLaunchKernelGGL((small_kernel<T, V, W, decltype(act)::value>), dim3((unsigned)(a.batch * g.slabs)),
-                         dim3(kSmallThreads), 0, stream, x, g, a, st, static_cast<T *>(y));
-      return;
+      hipLaunchKernelGGL((small_kernel<T, V, W, A>), dim3((unsigned)(a.batch * geo.slabs)), dim3(kSmallThreads), 0,
+                         stream, x, geo, a, st, static_cast<T *>(y));
+      return hipGetLastError();
     }
-    hipLaunchKernelGGL((stats_kernel<T, V, W>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, x, g, part);
-    hipLaunchKernelGGL((forward_kernel<T, V, W, decltype(act)::value>), dim3(back_grid(g)), dim3(kThreads), 0, stream,
-                       x, g, a, part, st, static_cast<T *>(y));
+    const hipError_t e = in_parts(geo, geo.tiles, [&](const Geo &g, unsigned count) {
+      hipLaunchKernelGGL((stats_kernel<T, V, W>), dim3(count), dim3(kThreads), 0, stream, x, g, part);
+    });
+    if (e != hipSuccess) return e;
+    return in_parts(geo, back_grid(geo), [&](const Geo &g, unsigned count) {
+      hipLaunchKernelGGL((forward_kernel<T, V, W, A>), dim3(count), dim3(kThreads), 0, stream, x, g, a, part, st,
+                         static_cast<T *>(y));
+    });
   });
 }
 
 template <typename T, int V>
 hipError_t backward(const GroupNormArgs &a, const void *grad_y, const double *stats, void *workspace, void *grad_x,
                     void *grad_w, void *grad_b, hipStream_t stream) {
-  const Geo g = geo_of<T, V>(a);
-  if (g.tiles > 1 << 30) return hipErrorInvalidValue;
+  const Geo geo = geo_of<T, V>(a);
   const T *gy = static_cast<const T *>(grad_y), *x = static_cast<const T *>(a.x);
   const Pair<double> *st = reinterpret_cast<const Pair<double> *>(stats);
-  Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(g);
+  Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(geo);
   const int params = grad_w || grad_b ? (a.channels + kParamLanes - 1) / kParamLanes : 0;
-  return with_kinds<V>(g, a.act, [&](auto whole, auto act) {
+  return with_kinds<V>(geo, a.act, [&](auto whole, auto act) {
     constexpr bool W = decltype(whole)::value;
     constexpr int A = decltype(act)::value;
-    hipLaunchKernelGGL((grad_sums_kernel<T, V, W, A>), dim3((unsigned)g.tiles), dim3(kThreads), 0, stream, gy, x, g, a, st,
-                       by_group, by_channel);
-    hipLaunchKernelGGL((grad_x_kernel<T, V, W, A>), dim3(params + (grad_x ? back_grid(g) : 0)), dim3(kThreads), 0, stream,
-                       gy, x, g, a, params, st, by_group, by_channel, static_cast<T *>(grad_x), grad_w, grad_b);
+    const hipError_t e = in_parts(geo, geo.tiles, [&](const Geo &g, unsigned count) {
+      hipLaunchKernelGGL((grad_sums_kernel<T, V, W, A>), dim3(count), dim3(kThreads), 0, stream, gy, x, g, a, st,
+                         by_group, by_channel);
+    });
+    if (e != hipSuccess) return e;
+    return in_parts(geo, params + (grad_x ? back_grid(geo) : 0), [&](const Geo &g, unsigned count) {
+      hipLaunchKernelGGL((grad_x_kernel<T, V, W, A>), dim3(count), dim3(kThreads), 0, stream, gy, x, g, a, params, st,
+                         by_group, by_channel, static_cast<T *>(grad_x), grad_w, grad_b);
+    });
   });
 }
 
