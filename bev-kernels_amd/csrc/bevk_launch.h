@@ -208,7 +208,7 @@ hipError_t launch_group_norm_backward(int dtype, const GroupNormArgs &a, const v
 // Embedding rows by index: index [n] (int32, or int64 with index64), weight [rows][dim] -> out [n][dim]
 // = scale * weight[index] (zeros where the index is outside the table), and grad_w [rows][dim] =
 // scale * the sums of grad_out's rows with that index (zeros for the row `padding`; -1: none).
-// No empty sizes but n == 0 in the backward; n and rows below 2^31.
+// No empty sizes but n == 0 in the backward; n and rows below 2^31, times dim at most 2^40.
 struct EmbeddingArgs {
   const void *index;
   bool index64;

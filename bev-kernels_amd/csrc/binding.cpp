@@ -1281,6 +1281,8 @@ static int check_embedding(const char *fn, int dtype, int64_t n, int64_t rows, i
   if (n > (1LL << 31) - 256 || rows > (1LL << 31) - 256)
     return fail(BEVK_ERR_INVALID, "%s: indices and rows must number less than 2^31 - 256", fn);
   if (dim > 1 << 30) return fail(BEVK_ERR_INVALID, "%s: more than 2^30 channels", fn);
+  if (std::max(n, rows) > (1LL << 40) / std::max(dim, 1))
+    return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
   return 0;
 }
 

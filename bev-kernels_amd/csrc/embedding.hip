@@ -48,8 +48,9 @@ constexpr int kUnroll = 4;
 template <typename T, typename I, int N>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const T *__restrict__ weight, int64_t rows,
                                                           uint32_t vecs, const I *__restrict__ index,
-                                                          int64_t total, float scale, T *__restrict__ out) {
-  const int64_t base = blockIdx.x * (int64_t)(kThreads * kUnroll);
+                                                          int64_t total, int64_t first, float scale,
+                                                          T *__restrict__ out) {
+  const int64_t base = (first + blockIdx.x) * (kThreads * kUnroll);
   const int64_t t0 = base / vecs;
   const uint32_t r0 = (uint32_t)(base - t0 * vecs);
   int64_t row[kUnroll];
@@ -94,6 +95,7 @@ struct Sorted {
 struct SortArgs {
   uint32_t n, rows, padding;  // padding: ~0 for none
   int log_r, per;             // rows v with v % R = w are a workgroup's; at most `per` of them
+  uint32_t first;             // workgroups in the launches before (launch_in_parts)
 };
 
 // Lanes whose index is a row of this workgroup, or of one before it. An index is compared as unsigned
@@ -117,7 +119,7 @@ __device__ __forceinline__ Owned owned(I index, const SortArgs &p, uint32_t w) {
 constexpr int kScan = 8;
 template <bool PADDED, typename I, typename F>
 __device__ __forceinline__ void scan(const I *index, uint32_t begin, uint32_t end, const SortArgs &p, F f) {
-  const uint32_t lane = threadIdx.x % kWave, w = blockIdx.x;
+  const uint32_t lane = threadIdx.x % kWave, w = p.first + blockIdx.x;
   uint32_t t = begin;
   const I *at = index + begin + lane;
   for (; t + kScan * kWave <= end; t += kScan * kWave, at += kScan * kWave) {
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
   __shared__ int before[kSortWaves], wave_sum[kSortWaves];
   __shared__ uint2 kept[kSortWaves][kKept];  // (t, row of the workgroup)
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, per = p.per;
-  const uint32_t w = blockIdx.x;
+  const uint32_t w = p.first + blockIdx.x;
   int *mine = count + wave * per;
   for (int i = threadIdx.x; i < kSortWaves * per; i += kSortThreads) count[i] = 0;
   __syncthreads();
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
       run += c;
     }
   }
-  if (w == gridDim.x - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
+  if (w == (1u << p.log_r) - 1 && threadIdx.x == kSortThreads - 1) *out.valid = at + total;
   __syncthreads();
 
   // Places of up to 64 of the wave's indices, in their order: the lanes that have a lane's row are
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const I *__restrict_
 // Sum and join give a group of `lanes` lanes (a power of two) one slice of a row: N channels each.
 struct SumArgs {
   int64_t rows;
-  int dim, lanes, slices, chunk_blocks;
+  int dim, lanes, slices, chunk_blocks, row_blocks;
+  int first;  // workgroups in the launches before (launch_in_parts)
   float scale;
 };
 
@@ -289,8 +292,9 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const T *__restrict__ g, 
                                                        float *__restrict__ part, T *__restrict__ gw) {
   __shared__ float buf[kThreads * N];
   const int lane = threadIdx.x % p.lanes, group = threadIdx.x / p.lanes, groups = kThreads / p.lanes;
-  if ((int)blockIdx.x < p.chunk_blocks) {
-    const int chunk = blockIdx.x / p.slices, c = (blockIdx.x % p.slices * p.lanes + lane) * N;
+  const int block = p.first + (int)blockIdx.x;
+  if (block < p.chunk_blocks) {
+    const int chunk = block / p.slices, c = (block % p.slices * p.lanes + lane) * N;
     int2 span;
     const Shared sh = shared_rows(s, chunk, *s.valid, span);
     for (int side = 0; side < 2; ++side) {
@@ -309,8 +313,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const T *__restrict__ g, 
     return;
   }
   const int64_t units = p.rows * p.slices;
-  for (int64_t u = (int64_t)(blockIdx.x - p.chunk_blocks) * groups + group; u < units;
-       u += (int64_t)(gridDim.x - p.chunk_blocks) * groups) {
+  for (int64_t u = (int64_t)(block - p.chunk_blocks) * groups + group; u < units;
+       u += (int64_t)p.row_blocks * groups) {
     const int64_t v = u / p.slices;
     const int c = ((int)(u - v * p.slices) * p.lanes + lane) * N;
     const int2 span = s.span != nullptr ? s.span[v] : make_int2(0, 0);
@@ -327,7 +331,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Sorted s, SumArgs p, con
                                                         T *__restrict__ gw) {
   __shared__ float buf[kThreads * N];
   const int lane = threadIdx.x % p.lanes, group = threadIdx.x / p.lanes, groups = kThreads / p.lanes;
-  const int chunk = blockIdx.x / p.slices, c = (blockIdx.x % p.slices * p.lanes + lane) * N;
+  const int block = p.first + (int)blockIdx.x;
+  const int chunk = block / p.slices, c = (block % p.slices * p.lanes + lane) * N;
   int2 span;
   const Shared sh = shared_rows(s, chunk, *s.valid, span);
   if (sh.tail == kChunk) return;  // no such row begins here
@@ -367,11 +372,11 @@ int lane_bytes(int64_t row_bytes, const void *a, const void *b) {
 template <typename T, typename I, int N>
 hipError_t forward_n(const EmbeddingArgs &a, const void *weight, void *out, hipStream_t stream) {
   const int64_t total = a.n * (a.dim / N), blocks = (total + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((lookup_kernel<T, I, N>), dim3((unsigned)blocks), dim3(kThreads), 0, stream,
-                     static_cast<const T *>(weight), a.rows, (uint32_t)(a.dim / N),
-                     static_cast<const I *>(a.index), total, a.scale, static_cast<T *>(out));
-  return hipGetLastError();
+  return launch_in_parts(blocks, kThreads, [&](int64_t first, unsigned count) {
+    hipLaunchKernelGGL((lookup_kernel<T, I, N>), dim3(count), dim3(kThreads), 0, stream,
+                       static_cast<const T *>(weight), a.rows, (uint32_t)(a.dim / N),
+                       static_cast<const I *>(a.index), total, first, a.scale, static_cast<T *>(out));
+  });
 }
 
 template <typename T, typename I>
@@ -392,16 +397,20 @@ hipError_t sums(const EmbeddingArgs &a, const void *grad_out, const Sorted &s, f
   while (p.lanes < kWave && p.lanes * N < a.dim) p.lanes *= 2;
   p.slices = (a.dim + p.lanes * N - 1) / (p.lanes * N);
   const int64_t chunks = a.n > kChunk ? (a.n + kChunk - 1) / kChunk * p.slices : 0;
-  const int64_t row_blocks = std::min<int64_t>(1 << 20, (a.rows * p.slices + kThreads / p.lanes - 1) /
-                                                            (kThreads / p.lanes));
-  if (chunks > 1 << 30) return hipErrorInvalidValue;
-  p.chunk_blocks = (int)chunks;
-  hipLaunchKernelGGL((sum_kernel<T, N>), dim3((unsigned)(chunks + row_blocks)), dim3(kThreads), 0, stream,
-                     static_cast<const T *>(grad_out), s, p, part, static_cast<T *>(grad_w));
-  if (chunks > 0)
-    hipLaunchKernelGGL((join_kernel<T, N>), dim3((unsigned)chunks), dim3(kThreads), 0, stream, s, p, part,
+  p.chunk_blocks = (int)chunks;  // below 2^30 with at most 2^40 values of grad_out
+  p.row_blocks = (int)std::min<int64_t>(1 << 20, (a.rows * p.slices + kThreads / p.lanes - 1) /
+                                                     (kThreads / p.lanes));
+  const hipError_t e = launch_in_parts(chunks + p.row_blocks, kThreads, [&](int64_t first, unsigned count) {
+    p.first = (int)first;
+    hipLaunchKernelGGL((sum_kernel<T, N>), dim3(count), dim3(kThreads), 0, stream, static_cast<const T *>(grad_out),
+                       s, p, part, static_cast<T *>(grad_w));
+  });
+  if (e != hipSuccess) return e;
+  return launch_in_parts(chunks, kThreads, [&](int64_t first, unsigned count) {
+    p.first = (int)first;
+    hipLaunchKernelGGL((join_kernel<T, N>), dim3(count), dim3(kThreads), 0, stream, s, p, part,
                        static_cast<T *>(grad_w));
-  return hipGetLastError();
+  });
 }
 
 template <typename T, typename I>
@@ -419,9 +428,12 @@ hipError_t backward(const EmbeddingArgs &a, const void *grad_out, int64_t paddin
     while ((a.rows - 1) >> p.log_r >= kSortRows) ++p.log_r;
     p.per = (int)((a.rows - 1) >> p.log_r) + 1;
     const auto sort = padding < 0 ? sort_kernel<I, false> : sort_kernel<I, true>;
-    hipLaunchKernelGGL(sort, dim3(1 << p.log_r), dim3(kSortThreads), kSortWaves * p.per * 4, stream,
-                       static_cast<const I *>(a.index), p, s);
-    if (hipError_t e = hipGetLastError()) return e;
+    const hipError_t e = launch_in_parts(1 << p.log_r, kSortThreads, [&](int64_t first, unsigned count) {
+      p.first = (uint32_t)first;
+      hipLaunchKernelGGL(sort, dim3(count), dim3(kSortThreads), kSortWaves * p.per * 4, stream,
+                         static_cast<const I *>(a.index), p, s);
+    });
+    if (e != hipSuccess) return e;
   }
   float *part = reinterpret_cast<float *>(ws + l.part);
   switch (lane_bytes((int64_t)a.dim * sizeof(T), grad_out, grad_w)) {

@@ -497,8 +497,9 @@ int bevk_group_norm_backward(int dtype, const void *grad_y, const void *x, const
  *   grad_weight  [rows, dim], written: scale * the fp32 sums of the rows of grad_out [n, dim] with
  *                that index, in a fixed order (the same results on every run); zeros for rows
  *                without an index, and for the row padding_idx (-1: none)
- * weight [rows, dim], out and gradients in dtype F32, F16 or BF16; n and rows below 2^31 - 256; the
- * workspace holds what bevk_embedding_backward_workspace_bytes says (-1 for sizes not taken). */
+ * weight [rows, dim], out and gradients in dtype F32, F16 or BF16; n and rows at most
+ * 2^31 - 256, and times dim at most 2^40; the workspace holds what
+ * bevk_embedding_backward_workspace_bytes says (-1 for sizes not taken). */
 int bevk_embedding_forward(int dtype, const void *weight, int64_t rows, int dim, const void *index,
                            int index64, int64_t n, float scale, void *out, void *stream);
 int64_t bevk_embedding_backward_workspace_bytes(int dtype, int64_t n, int64_t rows, int dim);
