@@ -751,7 +751,8 @@ hipError_t backward(const GroupNormArgs &a, const void *grad_y, const double *st
   const T *gy = static_cast<const T *>(grad_y), *x = static_cast<const T *>(a.x);
   const Pair<double> *st = reinterpret_cast<const Pair<double> *>(stats);
   Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(geo);
-  const int params = grad_w || grad_b ? (a.channels + kParamLanes - 1) / kParamLanes : 0;
+  // a multiple of the XCDs, so that the tiles behind them begin on the first (those past the channels do nothing)
+  const int params = grad_w || grad_b ? (a.channels + kParamLanes * kXcds - 1) / (kParamLanes * kXcds) * kXcds : 0;
   return with_kinds<V>(geo, a.act, [&](auto whole, auto act) {
     constexpr bool W = decltype(whole)::value;
     constexpr int A = decltype(act)::value;
