@@ -14,9 +14,9 @@
 //          the sorted list, which write partial sums, so that a row that many places share
 //          does not hang on one group of lanes.
 //   join   adds up the partial sums of those rows in the order of their chunks.
-// 60,000 places of 40,000 rows of 256 fp16 (six cameras): sort 14 us, 8.5 of them reading the indices,
-// sum 12, join 4; 16,384 tokens of 32,768 rows of 1,024 bf16, frequency as one over the rank: 8,
-// 21 (4.8 TB/s) and 4. The lookup of 16,384 x 2,048 bf16 takes 17.6 us (5.1 TB/s).
+// 60,000 places of 40,000 rows of 256 fp16 (six cameras): sort 14.7 us, 8.5 of them reading the
+// indices, sum 12, join 4; 16,384 tokens of 32,768 rows of 1,024 bf16, frequency as one over the
+// rank: 8.6, 20 (4.9 TB/s) and 4. The lookup of 16,384 x 2,048 bf16 takes 17.6 us (5.1 TB/s).
 #include <algorithm>
 
 #include "bevk_launch.h"

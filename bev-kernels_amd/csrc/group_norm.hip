@@ -19,9 +19,9 @@
 // workgroup of the second adds up again those of its own slab's groups: a few KB, where a third
 // launch between would cost 4 us and tiles of whole rows would read the sums of every group.
 // The second launch takes the tiles in the opposite order (within the XCD that had them), so that
-// what the first one read last is still in the caches. Six 58 x 100 x 256 maps in 16 bits (res4): 6.0
-// and 9.0 us forward, 9.9 and 10.5 us backward; their 36 and 53 MB once take 5.5 and 8.2 us at the
-// rate of a copy of that size.
+// what the first one read last is still in the caches. Six 58 x 100 x 256 maps in 16 bits (res4): 6
+// and 9 us forward, 10 and 11 us backward; their 36 and 53 MB once take 5.5 and 8.2 us at the rate of
+// a copy of that size.
 #include <algorithm>
 
 #include "bevk_launch.h"
@@ -39,9 +39,9 @@ template <typename T, int V> struct Tile {
   static constexpr int kLanes = V > 1 ? 8 : 64;
   static constexpr int kSlab = kLanes * V;            // channels
   static constexpr int kRows = kThreads / kLanes;     // positions side by side
-  // Positions of a thread loaded together, one such step ahead (res4 in 16 bits, 2 / 4 / 8 of them:
-  // 6.0 / 6.6 / 8.3 and 9.0 / 9.7 / 10.4 us forward, 9.9 / 10.3 / 11.6 and 10.5 / 10.5 / 12.3
-  // backward).
+  // Positions of a thread loaded together, one such step ahead (res4 in 16 bits, when it was chosen,
+  // 2 / 4 / 8 of them: 6.0 / 6.6 / 8.3 and 9.0 / 9.7 / 10.4 us forward, 9.9 / 10.3 / 11.6 and
+  // 10.5 / 10.5 / 12.3 backward).
   static constexpr int kAhead = V > 1 ? 2 : 8;
 };
 
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreads) grad_x_kernel(const T *__restrict__ 
 // Launches
 // ---------------------------------------------------------------------------------------
 
-constexpr int kTiles = 512;  // about: four workgroups on each CU
+constexpr int kTiles = 512;  // about: two workgroups on each of 256 CUs
 
 Geo make_geo(int64_t batch, int64_t pixels, int channels, int groups, int slab, int rows) {
   Geo g;
@@ -751,7 +751,8 @@ hipError_t backward(const GroupNormArgs &a, const void *grad_y, const double *st
   const T *gy = static_cast<const T *>(grad_y), *x = static_cast<const T *>(a.x);
   const Pair<double> *st = reinterpret_cast<const Pair<double> *>(stats);
   Pair<float> *by_group = static_cast<Pair<float> *>(workspace), *by_channel = by_group + by_group_pairs(geo);
-  // a multiple of the XCDs, so that the tiles behind them begin on the first (those past the channels do nothing)
+  // a multiple of the XCDs, so that the tiles behind them begin on the first (those past the channels
+  // do nothing)
   const int params = grad_w || grad_b ? (a.channels + kParamLanes * kXcds - 1) / (kParamLanes * kXcds) * kXcds : 0;
   return with_kinds<V>(geo, a.act, [&](auto whole, auto act) {
     constexpr bool W = decltype(whole)::value;

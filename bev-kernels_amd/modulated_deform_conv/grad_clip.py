@@ -17,7 +17,8 @@ def _listed(tensors):
 
 def grad_norm(grads):
     """The 2-norm of all values of the tensors together: a 0-dim float32 tensor on their device
-    (zero on the CPU for no tensors). Squares are summed in 64 bits, in one order."""
+    (zero on the CPU for no tensors). Squares are summed in 64 bits, in one order. The tensors are on
+    a GPU, in fp32 / fp16 / bf16; no gradient flows through the norm."""
     grads = _listed(grads)
     return _ext().clip_gradients(grads) if grads else torch.zeros(())
 

@@ -473,7 +473,8 @@ int bevk_msda_gradients(int dtype, const void *value, const int64_t *spatial_sha
  * where it is not wanted; ReLU's derivative at 0 is 0. The same results on every run. dtype and
  * param_dtype F32, F16, BF16 (param_dtype: the input's or F32); the workspace (16-byte aligned) holds what
  * bevk_group_norm_workspace_bytes says (-1 for sizes that are not taken; aligned: x and the tensors
- * of its size all begin on 16-byte boundaries). No size may be 0. */
+ * of its size all begin on 16-byte boundaries). No size may be 0, channels at most 2^30, and at most
+ * 2^40 values. */
 int64_t bevk_group_norm_workspace_bytes(int dtype, int backward, int64_t batch, int64_t pixels,
                                         int channels, int groups, int aligned);
 int bevk_group_norm_forward(int dtype, const void *x, const void *weight, const void *bias,
