@@ -70,6 +70,8 @@ __all__ = [
     "embedding_forward",
     "embedding_backward",
     "clip_gradients",
+    "adamw_step",
+    "adamw_moments",
 ]
 
 
@@ -1235,3 +1237,117 @@ def clip_gradients(grads, max_norm=None, out=None):
     if optrs is not None:  # written behind autograd's back
         torch.autograd.graph.increment_version(out)
     return norm
+
+
+# ---------------------------------------------------------------------------------------
+# An AdamW step over many tensors (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+ADAMW_BLOCK = 128  # values of an 8-bit moment with one scale; each tensor's part begins at a multiple
+
+
+def adamw_values(tensors):
+    """How many values a moment of these tensors has: each size rounded up to ADAMW_BLOCK."""
+    return sum(-(-t.numel() // ADAMW_BLOCK) * ADAMW_BLOCK for t in tensors)
+
+
+def _adamw_moments_of(fn, state, device):
+    """The state's tensors (exp_avg, exp_avg_sq, their scales or None, step), checked against each
+    other."""
+    try:
+        m, v, step = state["exp_avg"], state["exp_avg_sq"], state["step"]
+        scales = (state["exp_avg_scale"], state["exp_avg_sq_scale"]) if m.dtype == torch.uint8 else (None, None)
+    except KeyError as e:
+        raise RuntimeError(f"{fn}: the state has no {e}") from None
+    if m.dtype not in (torch.uint8, torch.float32) or v.dtype != m.dtype:
+        raise RuntimeError(f"{fn}: exp_avg and exp_avg_sq must both be float32 or uint8, got {m.dtype} "
+                           f"and {v.dtype}")
+    total = m.numel()
+    if total % ADAMW_BLOCK or v.numel() != total:
+        raise RuntimeError(f"{fn}: exp_avg and exp_avg_sq must have one size, a multiple of {ADAMW_BLOCK}, "
+                           f"got {total} and {v.numel()}")
+    for t in scales:
+        if t is not None and (t.dtype != torch.uint8 or t.numel() * ADAMW_BLOCK != total):
+            raise RuntimeError(f"{fn}: a scale must be uint8 [{total // ADAMW_BLOCK}], got {t.dtype} "
+                               f"[{t.numel()}]")
+    if step.dtype != torch.int64 or step.numel() != 1:
+        raise RuntimeError(f"{fn}: step must be one int64, got {step.dtype} [{step.numel()}]")
+    for t in (m, v, *scales, step):
+        if t is None:
+            continue
+        if t.get_device() != device or device < 0:
+            _b.require_device(fn, t)
+            raise RuntimeError(f"{fn}: tensors are on different devices (cuda:{device}, {t.device})")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{fn}: the state's tensors must be contiguous")
+    return m, v, *scales, step
+
+
+def _adamw_scalar(fn, name, t, device):
+    if t.get_device() != device or t.dtype != torch.float32 or t.numel() != 1:
+        raise RuntimeError(f"{fn}: {name} must be one float32 on cuda:{device}, got {t.dtype} "
+                           f"[{t.numel()}] on {t.device}")
+    return t.data_ptr()
+
+
+def _like(fn, name, tensors, others, contiguous):
+    """Whether each of `others` has its tensor's shape and strides; raises where one has not."""
+    if len(others) != len(tensors):
+        raise RuntimeError(f"{fn}: {len(others)} {name} for {len(tensors)} parameters")
+    if not contiguous or list(map(_shape_of, tensors)) != list(map(_shape_of, others)):
+        for t, o in zip(tensors, others):
+            if o.shape != t.shape or (not (o.is_contiguous() and t.is_contiguous())
+                                      and o.stride() != t.stride()):
+                raise RuntimeError(f"{fn}: one of the {name} has shape {tuple(o.shape)} and strides "
+                                   f"{o.stride()}, its parameter {tuple(t.shape)} and {t.stride()}")
+
+
+def adamw_step(params, grads, state, lr, beta1, beta2, eps, weight_decay, norm=None, max_norm=0.0,
+               copies=None):
+    """One AdamW step in place on params (fp32 / fp16 / bf16 in any mixture, dense in memory) and on the
+    state's tensors; copies: tensors that receive the new parameters. lr: a number, or one float32 on
+    the device."""
+    fn = "adamw_step"
+    device = params[0].get_device()
+    if device < 0:  # not on a HIP device: others there too would have the same -1
+        raise RuntimeError(f"{fn}: expected tensors on a HIP (cuda) device, got {params[0].device}")
+    ptrs, types, dense = _grad_arrays(fn, params, device)
+    gptrs, gtypes, gdense = _grad_arrays(fn, grads, device)
+    _like(fn, "gradients", params, grads, dense and gdense)
+    cptrs = ctypes_ = None
+    if copies is not None:
+        cptrs, ctypes_, cdense = _grad_arrays(fn, copies, device)
+        _like(fn, "copies", params, copies, dense and cdense)
+    m, v, ms, vs, step = _adamw_moments_of(fn, state, device)
+    sizes = array("q", [t.numel() for t in params])
+    lr_at = None
+    if isinstance(lr, torch.Tensor):
+        lr, lr_at = 0.0, _adamw_scalar(fn, "lr", lr, device)
+    norm_at = None if norm is None else _adamw_scalar(fn, "norm", norm, device)
+    at = lambda a: a.buffer_info()[0] if a is not None else None  # noqa: E731
+    nbytes = _b.lib().bevk_adamw_workspace_bytes()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=m.device)
+    _b.call_on(device, "bevk_adamw_step", len(params), at(ptrs), at(types), at(gptrs), at(gtypes), at(cptrs),
+               at(ctypes_), at(sizes), 8 if ms is not None else 32, m.data_ptr(), v.data_ptr(), _b.ptr(ms),
+               _b.ptr(vs), m.numel(), step.data_ptr(), state.get("seed", 0), lr, lr_at, beta1, beta2, eps,
+               weight_decay, norm_at, max_norm, ws.data_ptr(), nbytes)
+    # written behind autograd's back
+    torch.autograd.graph.increment_version(params if copies is None else [*params, *copies])
+    torch.autograd.graph.increment_version([t for t in (m, v, ms, vs, step) if t is not None])
+
+
+def adamw_moments(state, dtype=torch.float32):
+    """(exp_avg, exp_avg_sq) of a state as values, flat: its own tensors where they have that type,
+    else new ones. 8-bit moments: float32 or bfloat16, both exact."""
+    fn = "adamw_moments"
+    m, v, ms, vs, _ = _adamw_moments_of(fn, state, state["exp_avg"].get_device())
+    if ms is None:
+        return m.to(dtype), v.to(dtype)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{fn}: 8-bit moments are given as float32 or bfloat16, not {dtype}")
+    out = []
+    for second, (codes, scale) in enumerate(((m, ms), (v, vs))):
+        out.append(codes.new_empty(codes.shape, dtype=dtype))
+        _b.call_on(codes.get_device(), "bevk_adamw_moments", codes.data_ptr(), scale.data_ptr(), second,
+                   codes.numel(), _b._DTYPE_CODES[dtype], out[-1].data_ptr())
+    return tuple(out)

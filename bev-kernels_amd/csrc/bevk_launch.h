@@ -237,6 +237,38 @@ int64_t clip_gradients_workspace_bytes(const GradList &g);
 hipError_t launch_clip_gradients(const GradList &g, double max_norm, void *workspace, float *norm,
                                  hipStream_t stream);
 
+// An AdamW step (host arrays of `count` tensors; copy null for none). The moments of tensor k begin at
+// the sum of the sizes before it, each rounded up to kAdamwBlock; bits 32: fp32; 8: codes, with a
+// scale for each kAdamwBlock. lr_at / norm: device, or null.
+constexpr int kAdamwBlock = 128;
+struct AdamwTensors {
+  int count;
+  void *const *p;
+  const int *p_type;
+  const void *const *g;
+  const int *g_type;
+  void *const *copy;
+  const int *copy_type;
+  const int64_t *n;
+};
+struct AdamwMoments {
+  int bits;
+  void *m, *v;
+  unsigned char *m_scale, *v_scale;
+};
+struct AdamwStep {
+  int64_t *step;
+  uint64_t seed;
+  double lr, beta1, beta2, eps, decay, max_norm;
+  const float *lr_at, *norm;
+};
+int64_t adamw_workspace_bytes();
+hipError_t launch_adamw(const AdamwTensors &a, const AdamwMoments &m, const AdamwStep &s, void *workspace,
+                        hipStream_t stream);
+// The values of n codes (a multiple of kAdamwBlock; second: of a second moment) as fp32 or bf16.
+hipError_t launch_adamw_moments(const unsigned char *codes, const unsigned char *scale, bool second, int64_t n,
+                                int out_dtype, void *out, hipStream_t stream);
+
 // dst[b][c][r] = src[b][r][c] for 2- or 4-byte elements (NCHW <-> NHWC).
 hipError_t launch_transpose(int elem_bytes, const void *src, void *dst, int batch, int rows,
                             int cols, hipStream_t stream);

@@ -1398,4 +1398,116 @@ int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes, 
   return hip_status(bevk::launch_clip_gradients(g, max_norm, workspace, norm, (hipStream_t)stream), fn);
 }
 
+static bool float_type(int d) { return d == BEVK_F32 || d == BEVK_F16 || d == BEVK_BF16; }
+
+// What is written apart from everything else: no two ranges overlap of which one is written.
+static int check_written(const char *fn, std::vector<std::pair<uintptr_t, uintptr_t>> &written,
+                         const std::vector<std::pair<uintptr_t, uintptr_t>> &read) {
+  std::sort(written.begin(), written.end());
+  for (size_t j = 1; j < written.size(); ++j)
+    if (written[j].first < written[j - 1].second)
+      return fail(BEVK_ERR_INVALID, "%s: two tensors that are written overlap", fn);
+  for (const auto &r : read) {
+    const auto j = std::upper_bound(written.begin(), written.end(), r.first,
+                                    [](uintptr_t a, const auto &w) { return a < w.second; });
+    if (j != written.end() && j->first < r.second)
+      return fail(BEVK_ERR_INVALID, "%s: a tensor that is written overlaps one that is read", fn);
+  }
+  return 0;
+}
+
+int64_t bevk_adamw_workspace_bytes(void) { return bevk::adamw_workspace_bytes(); }
+
+int bevk_adamw_step(int count, void *const *params, const int *param_dtypes, const void *const *grads,
+                    const int *grad_dtypes, void *const *copies, const int *copy_dtypes, const int64_t *numels,
+                    int bits, void *exp_avg, void *exp_avg_sq, void *exp_avg_scale, void *exp_avg_sq_scale,
+                    int64_t values, int64_t *step, uint64_t seed, double lr, const float *lr_device, double beta1,
+                    double beta2, double eps, double weight_decay, const float *norm, double max_norm,
+                    void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *fn = "adamw_step";
+  g_last_error.clear();
+  if (int rc = check_grad_sizes(fn, count, numels)) return rc;
+  if (bits != 8 && bits != 32) return fail(BEVK_ERR_INVALID, "%s: moments have 8 or 32 bits, got %d", fn, bits);
+  if (count > 0 && (!params || !param_dtypes || !grads || !grad_dtypes || (copies && !copy_dtypes)))
+    return fail(BEVK_ERR_INVALID, "%s: null array", fn);
+  if (!step || (norm == nullptr && max_norm != 0.0)) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || !(max_norm >= 0.0))
+    return fail(BEVK_ERR_INVALID, "%s: lr, eps, weight_decay and max_norm must not be negative", fn);
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
+    return fail(BEVK_ERR_INVALID, "%s: betas must be in [0, 1)", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::adamw_workspace_bytes())) return rc;
+  int64_t total = 0;
+  try {
+    std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
+    written.reserve((copies ? 2 : 1) * (size_t)count + 6);
+    read.reserve(count + 2);
+    auto range = [](const void *p, int64_t bytes) {
+      return std::make_pair(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes);
+    };
+    for (int k = 0; k < count; ++k) {
+      total += (numels[k] + bevk::kAdamwBlock - 1) / bevk::kAdamwBlock * bevk::kAdamwBlock;
+      for (int d : {param_dtypes[k], grad_dtypes[k], copies ? copy_dtypes[k] : (int)BEVK_F32})
+        if (!float_type(d)) return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(d));
+      if (numels[k] == 0) continue;
+      if (!params[k] || !grads[k] || (copies && !copies[k]))
+        return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+      written.push_back(range(params[k], numels[k] * dtype_size(param_dtypes[k])));
+      read.push_back(range(grads[k], numels[k] * dtype_size(grad_dtypes[k])));
+      bool aligned = written.back().first % dtype_size(param_dtypes[k]) == 0 &&
+                     read.back().first % dtype_size(grad_dtypes[k]) == 0;
+      if (copies) {
+        written.push_back(range(copies[k], numels[k] * dtype_size(copy_dtypes[k])));
+        aligned = aligned && written.back().first % dtype_size(copy_dtypes[k]) == 0;
+      }
+      if (!aligned) return fail(BEVK_ERR_INVALID, "%s: a tensor is not aligned to its type", fn);
+    }
+    if (total != values)
+      return fail(BEVK_ERR_INVALID, "%s: moments of %lld values, the tensors need %lld", fn, (long long)values,
+                  (long long)total);
+    if (total > 0) {
+      if (!exp_avg || !exp_avg_sq || (bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)))
+        return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+      if (!on_16_bytes({exp_avg, exp_avg_sq}))
+        return fail(BEVK_ERR_INVALID, "%s: the moments must begin on 16-byte boundaries", fn);
+      written.push_back(range(exp_avg, total * bits / 8));
+      written.push_back(range(exp_avg_sq, total * bits / 8));
+      if (bits == 8) {
+        written.push_back(range(exp_avg_scale, total / bevk::kAdamwBlock));
+        written.push_back(range(exp_avg_sq_scale, total / bevk::kAdamwBlock));
+      }
+    }
+    written.push_back(range(step, 8));
+    written.push_back(range(workspace, workspace_bytes));
+    if (norm) read.push_back(range(norm, 4));
+    if (lr_device) read.push_back(range(lr_device, 4));
+    if (int rc = check_written(fn, written, read)) return rc;
+  } catch (const std::bad_alloc &) {
+    return fail(BEVK_ERR_INVALID, "%s: out of host memory", fn);
+  }
+  const bevk::AdamwTensors t{count, params, param_dtypes, grads, grad_dtypes, copies, copy_dtypes, numels};
+  const bevk::AdamwMoments m{bits, exp_avg, exp_avg_sq, static_cast<unsigned char *>(exp_avg_scale),
+                             static_cast<unsigned char *>(exp_avg_sq_scale)};
+  const bevk::AdamwStep s{step, seed, lr, beta1, beta2, eps, weight_decay, max_norm, lr_device, norm};
+  return hip_status(bevk::launch_adamw(t, m, s, workspace, (hipStream_t)stream), fn);
+}
+
+int bevk_adamw_moments(const void *codes, const void *scale, int second, int64_t values, int out_dtype, void *out,
+                       void *stream) {
+  const char *fn = "adamw_moments";
+  g_last_error.clear();
+  if (out_dtype != BEVK_F32 && out_dtype != BEVK_BF16)
+    return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(out_dtype));
+  if (values < 0 || values > 1LL << 40 || values % bevk::kAdamwBlock != 0)
+    return fail(BEVK_ERR_INVALID, "%s: the number of values must be a multiple of %d, at most 2^40", fn,
+                bevk::kAdamwBlock);
+  if (values == 0) return ok();
+  if (!codes || !scale || !out) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!on_16_bytes({codes, out}))
+    return fail(BEVK_ERR_INVALID, "%s: codes and values must begin on 16-byte boundaries", fn);
+  return hip_status(bevk::launch_adamw_moments(static_cast<const unsigned char *>(codes),
+                                               static_cast<const unsigned char *>(scale), second != 0, values,
+                                               out_dtype, out, (hipStream_t)stream),
+                    fn);
+}
+
 }  // extern "C"

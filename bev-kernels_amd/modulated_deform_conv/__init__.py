@@ -16,3 +16,4 @@ from .group_norm import (  # noqa: F401
     group_norm_act_nhwc,
 )
 from .grad_clip import clip_grad_norm_, clip_gradients_, grad_norm  # noqa: F401
+from .adamw import adamw_moments, adamw_state, adamw_step_  # noqa: F401

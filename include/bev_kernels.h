@@ -531,6 +531,40 @@ int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes,
                         double max_norm, void *workspace, int64_t workspace_bytes, float *norm,
                         void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* An AdamW step over many tensors                                            */
+/* ------------------------------------------------------------------------- */
+
+/* One step over `count` tensors (no counterpart in the reference): *step += 1, then with t = *step
+ *   g = min(1, max_norm / (norm + 1e-6)) * grad       (the factor where norm is not NULL)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * in fp32, each result rounded once.
+ *   params, grads, copies   HOST arrays of `count` device pointers, with types (F32, F16, BF16) and
+ *                           sizes; copies (NULL for none) receive the new parameters in their type
+ *   exp_avg, exp_avg_sq     m and v of all tensors, `values` in all: tensor k's begin at the sum of the
+ *                           sizes before it, each rounded up to 128. bits 32: fp32. bits 8: codes, with a
+ *                           scale byte for each 128 values (the biased exponent of fp32 of the
+ *                           largest): m = sign bit, 4 exponent and 3 mantissa bits, v = 5 exponent and 3
+ *                           mantissa bits, the largest exponent meaning the scale's, 0 for zero. Rounded
+ *                           at random, by seed, step and place: the same results for the same of them.
+ *   step                    one int64, device: the steps so far
+ *   lr_device               fp32, device, in place of lr; or NULL
+ *   norm                    fp32, device (of bevk_clip_gradients); or NULL with max_norm 0
+ * Nothing that is written may overlap anything else. The host arrays are read before the call
+ * returns. The workspace (16-byte aligned) holds bevk_adamw_workspace_bytes. */
+int64_t bevk_adamw_workspace_bytes(void);
+int bevk_adamw_step(int count, void *const *params, const int *param_dtypes, const void *const *grads,
+                    const int *grad_dtypes, void *const *copies, const int *copy_dtypes,
+                    const int64_t *numels, int bits, void *exp_avg, void *exp_avg_sq,
+                    void *exp_avg_scale, void *exp_avg_sq_scale, int64_t values, int64_t *step,
+                    uint64_t seed, double lr, const float *lr_device, double beta1, double beta2,
+                    double eps, double weight_decay, const float *norm, double max_norm,
+                    void *workspace, int64_t workspace_bytes, void *stream);
+/* The values of 8-bit codes (second: of exp_avg_sq) in F32 or BF16, both exact. */
+int bevk_adamw_moments(const void *codes, const void *scale, int second, int64_t values,
+                       int out_dtype, void *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
