@@ -70,6 +70,8 @@ __all__ = [
     "embedding_forward",
     "embedding_backward",
     "clip_gradients",
+    "residual_norm_forward",
+    "residual_norm_backward",
     "adamw_step",
     "adamw_moments",
 ]
@@ -1351,3 +1353,123 @@ def adamw_moments(state, dtype=torch.float32):
         _b.call_on(codes.get_device(), "bevk_adamw_moments", codes.data_ptr(), scale.data_ptr(), second,
                    codes.numel(), _b._DTYPE_CODES[dtype], out[-1].data_ptr())
     return tuple(out)
+
+
+# ---------------------------------------------------------------------------------------
+# The norms between two blocks (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+NORM_KINDS = {"layer": 0, "rms": 1}
+
+
+def _norm_param(fn, name, p, x, channels):
+    if not p.is_cuda or p.get_device() != x.get_device():
+        _b.require_device(fn, x, p)
+    if p.shape != (channels,):
+        raise RuntimeError(f"{fn}: {name} must be [{channels}], got {tuple(p.shape)}")
+    if not p.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    if p.dtype != x.dtype and p.dtype != torch.float32:
+        raise RuntimeError(f"{fn}: {name} has dtype {p.dtype}, expected {x.dtype} or torch.float32")
+
+
+def _residual_norm_check(fn, x, residual, weight, bias, gate, block, kind):
+    """(type, parameters' type, gate's type, rows, rows of a set or 0, channels, kind, block norm): the
+    library's arguments. Plain attribute tests: a small call is as long as its host side."""
+    if not x.is_cuda:
+        _b.require_device(fn, x)
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 2:
+        raise RuntimeError(f"{fn}: expected x [..., C] of two dimensions or more, got {tuple(shape)}")
+    if dtype not in _GROUP_NORM_TYPES:
+        _b.dtype_code(x)
+        raise RuntimeError(f"{fn}: not implemented for {dtype}")
+    if not x.is_contiguous():
+        raise RuntimeError("x must be contiguous")
+    if kind not in NORM_KINDS:
+        raise RuntimeError(f"{fn}: kind must be 'layer' or 'rms', got {kind!r}")
+    channels = shape[-1]
+    if channels > _MAX_CHANNELS:
+        raise RuntimeError(f"{fn}: more than 2^30 channels")
+    if residual is not None:
+        if not residual.is_cuda or residual.get_device() != x.get_device():
+            _b.require_device(fn, x, residual)
+        if residual.shape != shape or residual.dtype != dtype:
+            raise RuntimeError(f"{fn}: residual must be {tuple(shape)} {dtype}, got {tuple(residual.shape)} "
+                               f"{residual.dtype}")
+        if not residual.is_contiguous():
+            raise RuntimeError("residual must be contiguous")
+    block_weight, block_bias = (None, None) if block is None else block
+    params = None
+    for name, p in (("weight", weight), ("bias", bias), ("block_norm's weight", block_weight),
+                    ("block_norm's bias", block_bias)):
+        if p is not None:
+            _norm_param(fn, name, p, x, channels)
+            if params is not None and p.dtype != params:
+                raise RuntimeError(f"{fn}: weights and biases must have one dtype")
+            params = p.dtype
+    codes, total = _b._DTYPE_CODES, x.numel()
+    code, rows, set_rows = codes[dtype], total // channels if total else 0, 0
+    gcode = code
+    if gate is not None:
+        if not gate.is_cuda or gate.get_device() != x.get_device():
+            _b.require_device(fn, x, gate)
+        if gate.shape != (channels,):
+            if (gate.dim() < 2 or gate.shape[0] != shape[0] or gate.shape[-1] != channels
+                    or gate.numel() != shape[0] * channels):
+                raise RuntimeError(f"{fn}: gate must be [{channels}] or [{shape[0]}, {channels}], got "
+                                   f"{tuple(gate.shape)}")
+            set_rows = rows // shape[0] if rows else 0
+        if not gate.is_contiguous():
+            raise RuntimeError("gate must be contiguous")
+        if gate.dtype != dtype and gate.dtype != torch.float32:
+            raise RuntimeError(f"{fn}: gate has dtype {gate.dtype}, expected {dtype} or torch.float32")
+        gcode = codes[gate.dtype]
+    return (code, code if params is None else codes[params], gcode, rows, set_rows, channels, NORM_KINDS[kind],
+            0 if block is None else 1)
+
+
+def residual_norm_forward(x, residual, weight, bias, gate, scale, block, kind, eps, with_stream=True):
+    """(y, h or None, sizes): h = residual + scale * gate * p with p = x or, with block = (weight, bias),
+    its norm, and y the norm of h; sizes for residual_norm_backward."""
+    fn = "residual_norm_forward"
+    sizes = _residual_norm_check(fn, x, residual, weight, bias, gate, block, kind)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if with_stream else None
+    if sizes[3]:
+        bw, bb = (None, None) if block is None else block
+        ptr = _b.ptr
+        _b.call_on(x.get_device(), "bevk_residual_norm_forward", sizes[0], x.data_ptr(), ptr(residual), ptr(weight),
+                   ptr(bias), ptr(gate), ptr(bw), ptr(bb), *sizes[1:], scale, eps, y.data_ptr(), ptr(h))
+    return y, h, sizes
+
+
+@functools.lru_cache(maxsize=256)
+def _residual_norm_workspace_bytes(code, rows, set_rows, channels):
+    nbytes = _b.lib().bevk_residual_norm_backward_workspace_bytes(code, rows, set_rows, channels)
+    if nbytes < 0:
+        raise RuntimeError("residual_norm: more than 2^40 values")
+    return nbytes
+
+
+def residual_norm_backward(grad_y, grad_stream, stream, x, weight, bias, gate, scale, block, eps, sizes, wanted):
+    """The gradients of residual_norm_forward's x, residual, weight, bias, gate and block's two for grad_y
+    and grad_stream (or None); None where `wanted` is false or there is no such input. The
+    gradients of x and the residual may be one tensor, where they are equal."""
+    code, pcode, gcode, rows, set_rows, channels, kind, block_norm = sizes
+    bw, bb = (None, None) if block is None else block
+    new = torch.empty_like if rows else torch.zeros_like
+    alike = gate is None and block is None and scale == 1.0  # the block's gradient is the stream's
+    grad_r = new(stream) if wanted[1] or (alike and wanted[0]) else None
+    grad_x = grad_r if alike else new(stream) if wanted[0] else None
+    out = [new(p) if want and p is not None else None
+           for want, p in zip(wanted[2:], (weight, bias, gate, bw, bb))]
+    if rows:
+        nbytes = _residual_norm_workspace_bytes(code, rows, set_rows, channels)
+        ws = stream.new_empty(nbytes, dtype=torch.uint8)
+        ptr = _b.ptr
+        _b.call_on(stream.get_device(), "bevk_residual_norm_backward", code, grad_y.data_ptr(), ptr(grad_stream),
+                   stream.data_ptr(), ptr(x), ptr(weight), ptr(gate), ptr(bw), ptr(bb), pcode, gcode, rows,
+                   set_rows, channels, kind, block_norm, scale, eps, ws.data_ptr(), nbytes,
+                   None if alike else ptr(grad_x), ptr(grad_r), *map(ptr, out))
+    return (grad_x if wanted[0] else None, grad_r if wanted[1] else None, *out)

@@ -269,6 +269,31 @@ hipError_t launch_adamw(const AdamwTensors &a, const AdamwMoments &m, const Adam
 hipError_t launch_adamw_moments(const unsigned char *codes, const unsigned char *scale, bool second, int64_t n,
                                 int out_dtype, void *out, hipStream_t stream);
 
+// The norms between two blocks (residual_norm_fwd.hip has the formulas): rows x channels, no empty
+// sizes. Parameters in the input's type or (wide) fp32, null for none; the gate is [channels], or with
+// set_rows > 0 [rows / set_rows][channels] (a row of it for each set of rows).
+struct ResidualNormArgs {
+  const void *x, *residual, *weight, *bias, *gate, *block_weight, *block_bias;
+  bool wide, gate_wide, block, rms;
+  int64_t rows, set_rows;
+  int channels;
+  float scale, eps;
+};
+struct ResidualNormOut {
+  void *y, *h;  // h: or null
+};
+hipError_t launch_residual_norm_forward(int dtype, const ResidualNormArgs &a, const ResidualNormOut &o,
+                                        hipStream_t stream);
+// grad_h may be null (none); outputs are skipped where null; a.x may be null without a block norm where
+// the gate's gradient is not wanted. a.residual and a.bias are not read.
+struct ResidualNormGrads {
+  const void *grad_y, *grad_h, *h;
+  void *grad_x, *grad_residual, *grad_weight, *grad_bias, *grad_gate, *grad_block_weight, *grad_block_bias;
+};
+int64_t residual_norm_backward_workspace_bytes(int dtype, const ResidualNormArgs &a);
+hipError_t launch_residual_norm_backward(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g,
+                                         void *workspace, hipStream_t stream);
+
 // dst[b][c][r] = src[b][r][c] for 2- or 4-byte elements (NCHW <-> NHWC).
 hipError_t launch_transpose(int elem_bytes, const void *src, void *dst, int batch, int rows,
                             int cols, hipStream_t stream);

@@ -1510,4 +1510,87 @@ int bevk_adamw_moments(const void *codes, const void *scale, int second, int64_t
                     fn);
 }
 
+static int check_residual_norm(const char *fn, int dtype, int param_dtype, int gate_dtype, int64_t rows,
+                               int64_t set_rows, int64_t channels, int kind) {
+  for (int d : {dtype, param_dtype, gate_dtype})
+    if (!float_type(d)) return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(d));
+  for (int d : {param_dtype, gate_dtype})
+    if (d != dtype && d != BEVK_F32)
+      return fail(BEVK_ERR_INVALID, "%s: parameters and gate must have the input's type or be fp32", fn);
+  if (rows <= 0 || channels <= 0 || set_rows < 0) return fail(BEVK_ERR_INVALID, "%s: sizes must be positive", fn);
+  if (channels > 1 << 30) return fail(BEVK_ERR_INVALID, "%s: more than 2^30 channels", fn);
+  if (rows > (1LL << 40) / channels) return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
+  if (set_rows > 0 && rows % set_rows != 0)
+    return fail(BEVK_ERR_INVALID, "%s: rows (%lld) must be whole sets of %lld", fn, (long long)rows, (long long)set_rows);
+  if (kind < 0 || kind > 1) return fail(BEVK_ERR_INVALID, "%s: unknown kind %d", fn, kind);
+  return 0;
+}
+
+static bevk::ResidualNormArgs residual_norm_args(const void *x, const void *residual, const void *weight,
+                                                 const void *bias, const void *gate, const void *block_weight,
+                                                 const void *block_bias, int param_dtype, int gate_dtype, int64_t rows,
+                                                 int64_t set_rows, int channels, int kind, int block, float scale,
+                                                 float eps) {
+  bevk::ResidualNormArgs a;
+  a.x = x; a.residual = residual; a.weight = weight; a.bias = bias; a.gate = gate;
+  a.block_weight = block ? block_weight : nullptr;
+  a.block_bias = block ? block_bias : nullptr;
+  a.wide = param_dtype == BEVK_F32; a.gate_wide = gate_dtype == BEVK_F32;
+  a.block = block != 0; a.rms = kind == 1;
+  a.rows = rows; a.set_rows = set_rows; a.channels = channels;
+  a.scale = scale; a.eps = eps;
+  return a;
+}
+
+int bevk_residual_norm_forward(int dtype, const void *x, const void *residual, const void *weight, const void *bias,
+                               const void *gate, const void *block_weight, const void *block_bias, int param_dtype,
+                               int gate_dtype, int64_t rows, int64_t set_rows, int channels, int kind, int block_norm,
+                               float scale, float eps, void *y, void *stream_out, void *stream) {
+  const char *fn = "residual_norm_forward";
+  g_last_error.clear();
+  if (int rc = check_residual_norm(fn, dtype, param_dtype, gate_dtype, rows, set_rows, channels, kind)) return rc;
+  if (!(eps >= 0.f)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
+  if (!x || !y) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  return hip_status(bevk::launch_residual_norm_forward(
+                        dtype, residual_norm_args(x, residual, weight, bias, gate, block_weight, block_bias, param_dtype,
+                                                  gate_dtype, rows, set_rows, channels, kind, block_norm, scale, eps),
+                        {y, stream_out}, (hipStream_t)stream),
+                    fn);
+}
+
+int64_t bevk_residual_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t set_rows, int channels) {
+  if (check_residual_norm("residual_norm", dtype, dtype, dtype, rows, set_rows, channels, 0)) return -1;
+  return bevk::residual_norm_backward_workspace_bytes(
+      dtype, residual_norm_args(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, dtype, dtype, rows,
+                                set_rows, channels, 0, 0, 1.f, 0.f));
+}
+
+int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_stream, const void *stream_out,
+                                const void *x, const void *weight, const void *gate,
+                                const void *block_weight, const void *block_bias, int param_dtype, int gate_dtype,
+                                int64_t rows, int64_t set_rows, int channels, int kind, int block_norm, float scale,
+                                float eps, void *workspace, int64_t workspace_bytes, void *grad_x, void *grad_residual,
+                                void *grad_weight, void *grad_bias, void *grad_gate, void *grad_block_weight,
+                                void *grad_block_bias, void *stream) {
+  const char *fn = "residual_norm_backward";
+  g_last_error.clear();
+  if (int rc = check_residual_norm(fn, dtype, param_dtype, gate_dtype, rows, set_rows, channels, kind)) return rc;
+  if (!(eps >= 0.f)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
+  if (!grad_y || !stream_out || (!x && (block_norm || grad_gate)))
+    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!block_norm && (grad_block_weight || grad_block_bias))
+    return fail(BEVK_ERR_INVALID, "%s: gradients of a block norm that there is not", fn);
+  const bevk::ResidualNormArgs a = residual_norm_args(x, nullptr, weight, nullptr, gate, block_weight, block_bias,
+                                                      param_dtype, gate_dtype, rows, set_rows, channels, kind,
+                                                      block_norm, scale, eps);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::residual_norm_backward_workspace_bytes(dtype, a)))
+    return rc;
+  return hip_status(bevk::launch_residual_norm_backward(
+                        dtype, a,
+                        {grad_y, grad_stream, stream_out, grad_x, grad_residual, grad_weight, grad_bias,
+                         grad_gate, grad_block_weight, grad_block_bias},
+                        workspace, (hipStream_t)stream),
+                    fn);
+}
+
 }  // extern "C"

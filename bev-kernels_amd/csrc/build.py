@@ -25,7 +25,8 @@ LIB_PATH = os.path.join(PKG, "libbevk.so")
 SOURCES = ["binding.cpp", "msda_fwd.hip", "dcn_gather.hip", "dcn_fused.hip", "dcn_fused_h.hip",
            "dcn_bwd.hip", "msda_bwd.hip", "layout.hip", "dcn_f32.hip",
            "dcn_wgrad.hip", "group_norm.hip", "embedding.hip",
-           "grad_clip.hip", "adamw.hip"]
+           "grad_clip.hip", "adamw.hip",
+           "residual_norm_fwd.hip", "residual_norm_bwd.hip"]
 ARCH = "gfx950"
 
 

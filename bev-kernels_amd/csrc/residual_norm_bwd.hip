@@ -1,0 +1,420 @@
+// The gradients of the residual norm (gfx950; residual_norm_fwd.hip has the formulas and names).
+//
+//   hh = (h - mean) rstd, t = gy w
+//   gh = rstd (t - mean(t) - hh mean(t hh)) + gs          (rms: without mean(t)); the residual's too
+//   gw = sum gy hh, gb = sum gy, ggate = scale sum gh p   over the rows (a set's rows)
+//   gp = scale gate gh; without the block's norm the block's gradient gx = gp, else
+//   gbw = sum gp ph, gbb = sum gp, u = gp bw, gx = rstd_x (u - mean(u) - ph mean(u ph))
+//
+// The row in registers as in the forward, and h as the forward wrote it: mean and spread are taken again
+// from that (the unrounded h's would not make hh's mean 0 and its square's 1 where the spread of a row
+// is small next to the rounding of h). A workgroup takes a range of rows and keeps its threads'
+// part of the parameters' sums in registers; at its end (for the gate: at the end of a set) they are
+// added over its rows in LDS and written to the workspace, and join_kernel adds up the workgroups' parts
+// in order: no atomics, the same results on every run.
+#include "residual_norm.h"
+
+namespace bevk {
+namespace {
+using namespace rnorm;
+
+constexpr int kParts = 1024;  // workgroups at most
+
+// Workgroup k: `per` parts of a set (sets split), or whole sets (per == 1).
+struct Split {
+  int64_t sets, set_rows;
+  int per, blocks;
+};
+Split split_of(const ResidualNormArgs &a, int rows_a_block) {
+  Split s;
+  s.set_rows = a.set_rows > 0 ? a.set_rows : a.rows;
+  s.sets = a.rows / s.set_rows;
+  const int64_t most = std::max<int64_t>(1, s.set_rows / (rows_a_block * 2));  // two rows a thread at least
+  s.per = (int)std::max<int64_t>(1, std::min<int64_t>(kParts / std::min<int64_t>(s.sets, kParts), most));
+  s.blocks = (int)(s.per > 1 ? s.sets * s.per : std::min<int64_t>(s.sets, kParts));
+  return s;
+}
+
+// Parts in the workspace: [4][blocks][channels] of weight, bias, block weight, block bias (those that
+// are wanted), then the gate's [sets][per][channels].
+struct Parts {
+  float *sum[4], *gate;
+};
+
+template <typename T, int V, int TPR, int L, bool BLOCK>
+__global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const ResidualNormArgs a, const ResidualNormGrads g,
+                                                                   const Split sp, const Parts parts) {
+  constexpr int THREADS = threads_of(TPR), R = THREADS / TPR, N = BLOCK ? 5 : 3;
+  __shared__ float s[2 * THREADS / 64 * 2];
+  __shared__ float joined[R > 1 ? THREADS * L * V : 1];
+  int turn = 0;
+  const int j = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int64_t set0 = sp.per > 1 ? blockIdx.x / sp.per : sp.sets * blockIdx.x / sp.blocks;
+  const int64_t set1 = sp.per > 1 ? set0 + 1 : sp.sets * (blockIdx.x + 1) / sp.blocks;
+  const int part = sp.per > 1 ? blockIdx.x % sp.per : 0;
+  float sum[N][L][V];  // gate, weight, bias, block weight, block bias
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[n][l][e] = 0.f;
+  // the workgroup's sum of one parameter's parts, in the order of its rows
+  auto write = [&](float (&x)[L][V], float *to) __attribute__((always_inline)) {
+    if constexpr (R > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < V; ++e) joined[(group * L + l) * TPR * V + j * V + e] = x[l][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < L * TPR * V; i += THREADS) {
+        float v = joined[i];
+#pragma unroll
+        for (int k = 1; k < R; ++k) v += joined[k * L * TPR * V + i];
+        if (i < a.channels) to[i] = v;
+      }
+    } else {
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        const int c = (l * TPR + j) * V;
+        if (c < a.channels)
+#pragma unroll
+          for (int e = 0; e < V; ++e) to[c + e] = x[l][e];
+      }
+    }
+  };
+  const float inv = 1.f / (float)a.channels;
+  for (int64_t set = set0; set < set1; ++set) {
+    const int64_t r0 = set * sp.set_rows + sp.set_rows * part / sp.per;
+    const int64_t r1 = set * sp.set_rows + sp.set_rows * (part + 1) / sp.per;
+    for (int64_t r = r0; r < r1; r += R) {
+      const int64_t row = r + group, at = row * a.channels;
+      const bool there = row < r1;
+      float gy[L][V], h[L][V], x[L][V], gs[L][V];
+      bool in[L];
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        const int c = (l * TPR + j) * V;
+        in[l] = there && c < a.channels;
+#pragma unroll
+        for (int e = 0; e < V; ++e) gy[l][e] = h[l][e] = x[l][e] = gs[l][e] = 0.f;
+        if (in[l]) {
+          load_row<T, V>(static_cast<const T *>(g.grad_y) + at + c, gy[l]);
+          load_row<T, V>(static_cast<const T *>(g.h) + at + c, h[l]);
+          if (g.grad_h != nullptr) load_row<T, V>(static_cast<const T *>(g.grad_h) + at + c, gs[l]);
+          if (a.x != nullptr) load_row<T, V>(static_cast<const T *>(a.x) + at + c, x[l]);
+        }
+      }
+      float mean[N == 5 ? 2 : 1], rstd[N == 5 ? 2 : 1], t[2] = {0.f, 0.f};
+      if constexpr (BLOCK) row_moments<TPR, THREADS, 2, L, V>({h, x}, in, a.rms, a.channels, a.eps, mean, rstd, s, turn);
+      else row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, a.channels, a.eps, mean, rstd, s, turn);
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        if (in[l]) {
+          float w[V];
+          load_param<T, V>(a.weight, a.wide, (l * TPR + j) * V, 1.f, w);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float hh = (h[l][e] - mean[0]) * rstd[0];
+            sum[1][l][e] = __builtin_fmaf(gy[l][e], hh, sum[1][l][e]);
+            sum[2][l][e] += gy[l][e];
+            h[l][e] = hh;
+            gy[l][e] *= w[e];
+            t[0] += gy[l][e];
+            t[1] = __builtin_fmaf(gy[l][e], hh, t[1]);
+          }
+        }
+      row_sums<TPR, THREADS, 2>(t, s, turn);
+      const float c1 = a.rms ? 0.f : t[0] * inv, c2 = t[1] * inv;
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          gs[l][e] = __builtin_fmaf(rstd[0], gy[l][e] - c1 - h[l][e] * c2, gs[l][e]);  // gh
+      const int64_t gate_at = a.set_rows > 0 ? set * a.channels : 0;
+      t[0] = t[1] = 0.f;
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+        if (in[l]) {
+          const int c = (l * TPR + j) * V;
+          if (g.grad_residual != nullptr) store_row<T, V>(static_cast<T *>(g.grad_residual) + at + c, gs[l]);
+          float gate[V];
+          load_param<T, V>(a.gate, a.gate_wide, gate_at + c, 1.f, gate);
+          if constexpr (BLOCK) {
+            float w[V], b[V];
+            load_param<T, V>(a.block_weight, a.wide, c, 1.f, w);
+            load_param<T, V>(a.block_bias, a.wide, c, 0.f, b);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float ph = (x[l][e] - mean[1]) * rstd[1], gh = a.scale * gs[l][e], gp = gate[e] * gh;
+              sum[0][l][e] = __builtin_fmaf(gh, __builtin_fmaf(ph, w[e], b[e]), sum[0][l][e]);
+              sum[3][l][e] = __builtin_fmaf(gp, ph, sum[3][l][e]);
+              sum[4][l][e] += gp;
+              x[l][e] = ph;
+              gs[l][e] = gp * w[e];
+              t[0] += gs[l][e];
+              t[1] = __builtin_fmaf(gs[l][e], ph, t[1]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float gh = a.scale * gs[l][e];
+              sum[0][l][e] = __builtin_fmaf(gh, x[l][e], sum[0][l][e]);
+              gs[l][e] = gate[e] * gh;
+            }
+          }
+        }
+      if constexpr (BLOCK) {
+        row_sums<TPR, THREADS, 2>(t, s, turn);
+        const float d1 = a.rms ? 0.f : t[0] * inv, d2 = t[1] * inv;
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+#pragma unroll
+          for (int e = 0; e < V; ++e) gs[l][e] = rstd[1] * (gs[l][e] - d1 - x[l][e] * d2);
+      }
+      if (g.grad_x != nullptr)
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+          if (in[l]) store_row<T, V>(static_cast<T *>(g.grad_x) + at + (l * TPR + j) * V, gs[l]);
+    }
+    if (parts.gate != nullptr) {
+      write(sum[0], parts.gate + (set * sp.per + part) * a.channels);
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[0][l][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int n = 1; n < N; ++n)
+    if (parts.sum[n - 1] != nullptr) write(sum[n], parts.sum[n - 1] + (int64_t)blockIdx.x * a.channels);
+}
+
+// Mean and 1 / spread of a row in memory, by a workgroup of 256.
+template <typename T>
+__device__ __forceinline__ void any_moments(const T *v, const ResidualNormArgs &a, float &mean, float &rstd, float *s,
+                                            int &turn) {
+  float t[1] = {0.f};
+  mean = 0.f;
+  if (!a.rms) {
+    for (int c = threadIdx.x; c < a.channels; c += 256) t[0] += (float)v[c];
+    row_sums<256, 256, 1>(t, s, turn);
+    mean = t[0] / (float)a.channels;
+  }
+  t[0] = 0.f;
+  for (int c = threadIdx.x; c < a.channels; c += 256) {
+    const float d = (float)v[c] - mean;
+    t[0] = __builtin_fmaf(d, d, t[0]);
+  }
+  row_sums<256, 256, 1>(t, s, turn);
+  rstd = 1.f / sqrtf(t[0] / (float)a.channels + a.eps);
+}
+
+// Any row length: a workgroup a row at a time, each sum a pass over it; a thread adds its channels' parts
+// up in the workspace.
+template <typename T, bool BLOCK>
+__global__ void __launch_bounds__(256) any_backward_kernel(const ResidualNormArgs a, const ResidualNormGrads g,
+                                                           const Split sp, const Parts parts) {
+  __shared__ float s[2 * 4 * 2];
+  int turn = 0;
+  const int64_t set0 = sp.per > 1 ? blockIdx.x / sp.per : sp.sets * blockIdx.x / sp.blocks;
+  const int64_t set1 = sp.per > 1 ? set0 + 1 : sp.sets * (blockIdx.x + 1) / sp.blocks;
+  const int part = sp.per > 1 ? blockIdx.x % sp.per : 0;
+  const float inv = 1.f / (float)a.channels;
+  const int64_t mine = (int64_t)blockIdx.x * a.channels;
+  for (int n = 0; n < 4; ++n)
+    if (parts.sum[n] != nullptr)
+      for (int c = threadIdx.x; c < a.channels; c += 256) parts.sum[n][mine + c] = 0.f;
+  for (int64_t set = set0; set < set1; ++set) {
+    const int64_t r0 = set * sp.set_rows + sp.set_rows * part / sp.per;
+    const int64_t r1 = set * sp.set_rows + sp.set_rows * (part + 1) / sp.per;
+    const int64_t gate_at = a.set_rows > 0 ? set * a.channels : 0;
+    float *gate_sum = parts.gate == nullptr ? nullptr : parts.gate + (set * sp.per + part) * a.channels;
+    if (gate_sum != nullptr)
+      for (int c = threadIdx.x; c < a.channels; c += 256) gate_sum[c] = 0.f;
+    for (int64_t row = r0; row < r1; ++row) {
+      const int64_t at = row * a.channels;
+      const T *gy = static_cast<const T *>(g.grad_y) + at, *h = static_cast<const T *>(g.h) + at;
+      const T *x = a.x == nullptr ? nullptr : static_cast<const T *>(a.x) + at;
+      const T *gs = g.grad_h == nullptr ? nullptr : static_cast<const T *>(g.grad_h) + at;
+      float mean, rstd, mean_x = 0.f, rstd_x = 1.f;
+      any_moments<T>(h, a, mean, rstd, s, turn);
+      if (BLOCK) any_moments<T>(x, a, mean_x, rstd_x, s, turn);
+      float t[2] = {0.f, 0.f}, w[1], b[1], gate[1];
+      for (int c = threadIdx.x; c < a.channels; c += 256) {
+        load_param<T, 1>(a.weight, a.wide, c, 1.f, w);
+        const float hh = ((float)h[c] - mean) * rstd, v = (float)gy[c] * w[0];
+        t[0] += v;
+        t[1] = __builtin_fmaf(v, hh, t[1]);
+      }
+      row_sums<256, 256, 2>(t, s, turn);
+      const float c1 = a.rms ? 0.f : t[0] * inv, c2 = t[1] * inv;
+      auto grad_stream = [&](int c, float hh) __attribute__((always_inline)) {
+        load_param<T, 1>(a.weight, a.wide, c, 1.f, w);
+        return __builtin_fmaf(rstd, (float)gy[c] * w[0] - c1 - hh * c2, gs != nullptr ? (float)gs[c] : 0.f);
+      };
+      auto grad_block = [&](int c, float gh) __attribute__((always_inline)) {
+        load_param<T, 1>(a.gate, a.gate_wide, gate_at + c, 1.f, gate);
+        return gate[0] * (a.scale * gh);
+      };
+      t[0] = t[1] = 0.f;
+      if (BLOCK)
+        for (int c = threadIdx.x; c < a.channels; c += 256) {
+          const float hh = ((float)h[c] - mean) * rstd, gp = grad_block(c, grad_stream(c, hh));
+          load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
+          const float ph = ((float)x[c] - mean_x) * rstd_x, u = gp * w[0];
+          t[0] += u;
+          t[1] = __builtin_fmaf(u, ph, t[1]);
+        }
+      if (BLOCK) row_sums<256, 256, 2>(t, s, turn);
+      const float d1 = a.rms ? 0.f : t[0] * inv, d2 = t[1] * inv;
+      for (int c = threadIdx.x; c < a.channels; c += 256) {
+        const float hh = ((float)h[c] - mean) * rstd, dy = (float)gy[c];
+        const float gh = grad_stream(c, hh), gp = grad_block(c, gh);
+        if (parts.sum[0] != nullptr) parts.sum[0][mine + c] += dy * hh;
+        if (parts.sum[1] != nullptr) parts.sum[1][mine + c] += dy;
+        float p = x != nullptr ? (float)x[c] : 0.f, gx = gp;
+        if (BLOCK) {
+          const float ph = (p - mean_x) * rstd_x;
+          load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
+          load_param<T, 1>(a.block_bias, a.wide, c, 0.f, b);
+          p = __builtin_fmaf(ph, w[0], b[0]);
+          if (parts.sum[2] != nullptr) parts.sum[2][mine + c] += gp * ph;
+          if (parts.sum[3] != nullptr) parts.sum[3][mine + c] += gp;
+          gx = rstd_x * (gp * w[0] - d1 - ph * d2);
+        }
+        if (gate_sum != nullptr) gate_sum[c] += a.scale * gh * p;
+        if (g.grad_residual != nullptr) static_cast<T *>(g.grad_residual)[at + c] = static_cast<T>(gh);
+        if (g.grad_x != nullptr) static_cast<T *>(g.grad_x)[at + c] = static_cast<T>(gx);
+      }
+    }
+  }
+}
+
+struct Join {
+  const float *from;
+  void *to;
+  int parts;      // to add up for each output row
+  int64_t rows;   // output rows
+  bool wide;
+};
+struct Joins {
+  Join of[5];
+  int count, channels;
+};
+
+// 16 channels of one output row: 64 threads add up every 64th part each, then in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) join_kernel(const Joins all, int which, int64_t first) {
+  __shared__ float s[64][17];
+  const Join &j = all.of[which + blockIdx.y];
+  const int64_t tiles = (all.channels + 15) / 16, at = first + blockIdx.x;
+  const int64_t row = at / tiles;
+  const int c = (int)(at % tiles) * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
+  float v = 0.f;
+  if (row < j.rows && c < all.channels) {
+    const float *p = j.from + row * j.parts * all.channels + c;
+#pragma unroll 8
+    for (int q = k; q < j.parts; q += 64) v += p[(int64_t)q * all.channels];
+  }
+  s[k][threadIdx.x % 16] = v;
+  __syncthreads();
+  for (int half = 32; half > 0; half /= 2) {
+    if (k < half) s[k][threadIdx.x % 16] += s[k + half][threadIdx.x % 16];
+    __syncthreads();
+  }
+  if (k == 0 && row < j.rows && c < all.channels) {
+    v = s[0][threadIdx.x];
+    if (j.wide) static_cast<float *>(j.to)[row * all.channels + c] = v;
+    else static_cast<T *>(j.to)[row * all.channels + c] = static_cast<T>(v);
+  }
+}
+
+int rows_a_block(int64_t channels, int v) {
+  int rows = 1;
+  for_row((channels + v - 1) / v, [&](auto tpr, auto) {
+    constexpr int TPR = decltype(tpr)::value;
+    rows = threads_of(TPR) / TPR;
+  });
+  return rows;
+}
+
+template <typename T, int V, bool BLOCK>
+hipError_t launch_v(const ResidualNormArgs &a, const ResidualNormGrads &g, const Split &sp, const Parts &parts,
+                    hipStream_t stream) {
+  const bool fits = for_row((a.channels + V - 1) / V, [&](auto tpr, auto l) {
+    constexpr int TPR = decltype(tpr)::value, L = decltype(l)::value;
+    hipLaunchKernelGGL((backward_kernel<T, V, TPR, L, BLOCK>), dim3(sp.blocks), dim3(threads_of(TPR)), 0, stream, a,
+                       g, sp, parts);
+  });
+  if (!fits)
+    hipLaunchKernelGGL((any_backward_kernel<T, BLOCK>), dim3(sp.blocks), dim3(256), 0, stream, a, g, sp, parts);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool whole, void *workspace,
+                    hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const Split sp = split_of(a, rows_a_block(a.channels, whole ? V : 1));
+  float *ws = static_cast<float *>(workspace);
+  Parts parts{};
+  Joins joins{};
+  joins.channels = a.channels;
+  void *to[4] = {g.grad_weight, g.grad_bias, g.grad_block_weight, g.grad_block_bias};
+  for (int n = 0; n < 4; ++n) {
+    if (to[n] == nullptr) continue;
+    parts.sum[n] = ws;
+    joins.of[joins.count++] = Join{ws, to[n], sp.blocks, 1, a.wide};
+    ws += (int64_t)sp.blocks * a.channels;
+  }
+  const int small = joins.count;
+  if (g.grad_gate != nullptr) {
+    parts.gate = ws;
+    joins.of[joins.count++] = Join{ws, g.grad_gate, sp.per, sp.sets, a.gate_wide};
+  }
+  hipError_t e;
+  if (whole) e = a.block ? launch_v<T, V, true>(a, g, sp, parts, stream) : launch_v<T, V, false>(a, g, sp, parts, stream);
+  else e = a.block ? launch_v<T, 1, true>(a, g, sp, parts, stream) : launch_v<T, 1, false>(a, g, sp, parts, stream);
+  if (e != hipSuccess) return e;
+  const int64_t tiles = (a.channels + 15) / 16;
+  const bool one = sp.sets == 1 || parts.gate == nullptr;  // all of them have one output row
+  const int n = one ? joins.count : small;
+  if (n > 0) {
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)tiles, n), dim3(1024), 0, stream, joins, 0, (int64_t)0);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  if (one) return hipSuccess;
+  return launch_in_parts(tiles * sp.sets, 1024, [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL((join_kernel<T>), dim3(blocks, 1), dim3(1024), 0, stream, joins, small, first);
+  });
+}
+
+bool whole_rows(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g) {
+  return a.channels % (dtype == 0 ? 4 : 8) == 0 &&
+         on_16({a.x, a.weight, a.gate, a.block_weight, a.block_bias, g.grad_y, g.grad_h, g.h, g.grad_x, g.grad_residual});
+}
+
+}  // namespace
+
+int64_t residual_norm_backward_workspace_bytes(int dtype, const ResidualNormArgs &a) {
+  int64_t most = 0;  // for either alignment
+  for (int v : {dtype == 0 ? 4 : 8, 1}) {
+    const Split sp = split_of(a, rows_a_block(a.channels, v));
+    most = std::max(most, (4 * (int64_t)sp.blocks + sp.sets * sp.per) * a.channels * 4);
+  }
+  return most;
+}
+
+hipError_t launch_residual_norm_backward(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g,
+                                         void *workspace, hipStream_t stream) {
+  const bool whole = whole_rows(dtype, a, g);
+  switch (dtype) {
+    case 0: return launch_t<float>(a, g, whole, workspace, stream);
+    case 1: return launch_t<f16>(a, g, whole, workspace, stream);
+    default: return launch_t<bf16>(a, g, whole, workspace, stream);
+  }
+}
+
+}  // namespace bevk
