@@ -70,6 +70,8 @@ __all__ = [
     "embedding_forward",
     "embedding_backward",
     "clip_gradients",
+    "linear_forward",
+    "linear_backward",
     "residual_norm_forward",
     "residual_norm_backward",
     "adamw_step",
@@ -1473,3 +1475,99 @@ def residual_norm_backward(grad_y, grad_stream, stream, x, weight, bias, gate, s
                    set_rows, channels, kind, block_norm, scale, eps, ws.data_ptr(), nbytes,
                    None if alike else ptr(grad_x), ptr(grad_r), *map(ptr, out))
     return (grad_x if wanted[0] else None, grad_r if wanted[1] else None, *out)
+
+
+# ---------------------------------------------------------------------------------------
+# Projections with bias, activation and residual (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+LINEAR_ACTS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+_MAX_FEATURES = 2 ** 24
+
+
+def _linear_check(fn, x, weight, bias, act, residual):
+    """(type, rows, in, out, activation, bias' type): the library's arguments. Plain attribute tests: a
+    small call is as long as its host side."""
+    if not x.is_cuda or not weight.is_cuda or weight.get_device() != x.get_device():
+        _b.require_device(fn, x, weight)
+    shape, dtype = x.shape, x.dtype
+    if dtype not in _GROUP_NORM_TYPES:
+        _b.dtype_code(x)
+        raise RuntimeError(f"{fn}: not implemented for {dtype}")
+    if len(weight.shape) != 2 or len(shape) < 1 or weight.shape[1] != shape[-1]:
+        raise RuntimeError(f"{fn}: weight must be [N, K] for x [..., K], got {tuple(weight.shape)} for "
+                           f"{tuple(shape)}")
+    if weight.dtype != dtype:
+        raise RuntimeError(f"{fn}: weight has dtype {weight.dtype}, expected {dtype}")
+    if not x.is_contiguous():
+        raise RuntimeError("x must be contiguous")
+    if not weight.is_contiguous():
+        raise RuntimeError("weight must be contiguous")
+    n, k = weight.shape
+    if not 0 < k <= _MAX_FEATURES or not 0 < n <= _MAX_FEATURES:
+        raise RuntimeError(f"{fn}: features must be from 1 to 2^24, got {k} and {n}")
+    if act not in LINEAR_ACTS:
+        raise RuntimeError(f"{fn}: act must be None, 'relu', 'silu' or 'gelu', got {act!r}")
+    code = bcode = _b._DTYPE_CODES[dtype]
+    if bias is not None:
+        if not bias.is_cuda or bias.get_device() != x.get_device():
+            _b.require_device(fn, x, bias)
+        if bias.shape != (n,):
+            raise RuntimeError(f"{fn}: bias must be [{n}], got {tuple(bias.shape)}")
+        if bias.dtype != dtype and bias.dtype != torch.float32:
+            raise RuntimeError(f"{fn}: bias has dtype {bias.dtype}, expected {dtype} or torch.float32")
+        if not bias.is_contiguous():
+            raise RuntimeError("bias must be contiguous")
+        bcode = _b._DTYPE_CODES[bias.dtype]
+    if residual is not None:
+        if not residual.is_cuda or residual.get_device() != x.get_device():
+            _b.require_device(fn, x, residual)
+        if residual.shape != (*shape[:-1], n) or residual.dtype != dtype:
+            raise RuntimeError(f"{fn}: residual must be {(*shape[:-1], n)} {dtype}, got "
+                               f"{tuple(residual.shape)} {residual.dtype}")
+        if not residual.is_contiguous():
+            raise RuntimeError("residual must be contiguous")
+    return code, x.numel() // k, k, n, LINEAR_ACTS[act], bcode
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_workspace_bytes(code, backward, rows, k, n, act):
+    nbytes = _b.lib().bevk_linear_workspace_bytes(code, backward, rows, k, n, act)
+    if nbytes < 0:
+        raise RuntimeError(f"linear: {_b.lib().bevk_last_error().decode()}")
+    return nbytes
+
+
+def linear_forward(x, weight, bias=None, act=None, residual=None, with_z=False):
+    """(y, z, sizes): y = act(x @ weight.T + bias) + residual for x [..., K], weight [N, K]; z, with with_z,
+    what linear_backward takes for it (None where that needs none, y itself where its sign is enough)."""
+    sizes = _linear_check("linear_forward", x, weight, bias, act, residual)
+    code, rows, k, n, acode, bcode = sizes
+    y = x.new_empty((*x.shape[:-1], n))
+    z = None
+    if with_z and acode:
+        z = y if acode == 1 and residual is None else torch.empty_like(y)
+    if rows:
+        nbytes = _linear_workspace_bytes(code, 0, rows, k, n, acode)
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _b.call_on(x.get_device(), "bevk_linear_forward", code, x.data_ptr(), weight.data_ptr(), _b.ptr(bias), bcode,
+                   _b.ptr(residual), rows, k, n, acode, _b.ptr(ws), nbytes, y.data_ptr(),
+                   None if z is y else _b.ptr(z))
+    return y, z, sizes
+
+
+def linear_backward(grad_y, x, weight, bias, z, sizes, wanted=(True, True, True)):
+    """(grad_x, grad_weight, grad_bias) of linear_forward's y; None where `wanted` is false or there is no
+    bias. The residual's gradient is grad_y."""
+    code, rows, k, n, acode, bcode = sizes
+    new = torch.empty_like if rows else torch.zeros_like
+    grad_x = new(x) if wanted[0] else None
+    grad_w = new(weight) if wanted[1] else None
+    grad_b = new(bias) if wanted[2] and bias is not None else None
+    if rows:
+        nbytes = _linear_workspace_bytes(code, 1, rows, k, n, acode)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        ptr = _b.ptr
+        _b.call_on(x.get_device(), "bevk_linear_backward", code, grad_y.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                   ptr(z), rows, k, n, acode, bcode, ws.data_ptr(), nbytes, ptr(grad_x), ptr(grad_w), ptr(grad_b))
+    return grad_x, grad_w, grad_b

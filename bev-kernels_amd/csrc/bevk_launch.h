@@ -269,6 +269,22 @@ hipError_t launch_adamw(const AdamwTensors &a, const AdamwMoments &m, const Adam
 hipError_t launch_adamw_moments(const unsigned char *codes, const unsigned char *scale, bool second, int64_t n,
                                 int out_dtype, void *out, hipStream_t stream);
 
+// Projections y = act(x W^T + bias) + residual (linear.hip): x [rows][K], weight [N][K], no empty sizes.
+constexpr int kActGelu = 3;  // beside GroupNormAct's
+struct LinearArgs {
+  const void *x, *weight, *bias;  // bias: the input's type or (wide) fp32, or null
+  bool bias_wide;
+  int64_t rows;
+  int K, N, act;
+};
+int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a);
+hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *z,
+                                 void *workspace, hipStream_t stream);
+// z: the forward's (not read where act is none); outputs are skipped where null.
+int64_t linear_backward_workspace_bytes(int dtype, const LinearArgs &a);
+hipError_t launch_linear_backward(int dtype, const LinearArgs &a, const void *grad_y, const void *z, void *workspace,
+                                  void *grad_x, void *grad_w, void *grad_b, hipStream_t stream);
+
 // The norms between two blocks (residual_norm_fwd.hip has the formulas): rows x channels, no empty
 // sizes. Parameters in the input's type or (wide) fp32, null for none; the gate is [channels], or with
 // set_rows > 0 [rows / set_rows][channels] (a row of it for each set of rows).

@@ -1593,4 +1593,64 @@ int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_
                     fn);
 }
 
+static int check_linear(const char *fn, int dtype, int bias_dtype, int64_t rows, int in_features, int out_features,
+                        int act) {
+  for (int d : {dtype, bias_dtype})
+    if (!float_type(d)) return fail(BEVK_ERR_UNSUPPORTED, "\"%s\" not implemented for '%s'", fn, dtype_name(d));
+  if (bias_dtype != dtype && bias_dtype != BEVK_F32)
+    return fail(BEVK_ERR_INVALID, "%s: bias must have the input's type or be fp32", fn);
+  if (rows <= 0 || in_features <= 0 || out_features <= 0)
+    return fail(BEVK_ERR_INVALID, "%s: sizes must be positive", fn);
+  if (in_features > 1 << 24 || out_features > 1 << 24)
+    return fail(BEVK_ERR_INVALID, "%s: more than 2^24 features", fn);
+  if (rows > (1LL << 31) - 256) return fail(BEVK_ERR_INVALID, "%s: rows must number less than 2^31 - 256", fn);
+  if (rows * std::max(in_features, out_features) > 1LL << 40 || (int64_t)in_features * out_features > 1LL << 40)
+    return fail(BEVK_ERR_INVALID, "%s: more than 2^40 values", fn);
+  if (act < 0 || act > 3) return fail(BEVK_ERR_INVALID, "%s: unknown activation %d", fn, act);
+  return 0;
+}
+
+static bevk::LinearArgs linear_args(const void *x, const void *weight, const void *bias, int bias_dtype, int64_t rows,
+                                    int in_features, int out_features, int act) {
+  bevk::LinearArgs a;
+  a.x = x; a.weight = weight; a.bias = bias; a.bias_wide = bias_dtype == BEVK_F32;
+  a.rows = rows; a.K = in_features; a.N = out_features; a.act = act;
+  return a;
+}
+
+int64_t bevk_linear_workspace_bytes(int dtype, int backward, int64_t rows, int in_features, int out_features, int act) {
+  if (check_linear("linear", dtype, dtype, rows, in_features, out_features, act)) return -1;
+  const bevk::LinearArgs a = linear_args(nullptr, nullptr, nullptr, dtype, rows, in_features, out_features, act);
+  return backward ? bevk::linear_backward_workspace_bytes(dtype, a) : bevk::linear_forward_workspace_bytes(dtype, a);
+}
+
+int bevk_linear_forward(int dtype, const void *x, const void *weight, const void *bias, int bias_dtype,
+                        const void *residual, int64_t rows, int in_features, int out_features, int act, void *workspace,
+                        int64_t workspace_bytes, void *y, void *z, void *stream) {
+  const char *fn = "linear_forward";
+  g_last_error.clear();
+  if (int rc = check_linear(fn, dtype, bias_dtype, rows, in_features, out_features, act)) return rc;
+  if (!x || !weight || !y) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  const bevk::LinearArgs a = linear_args(x, weight, bias, bias_dtype, rows, in_features, out_features, act);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::linear_forward_workspace_bytes(dtype, a))) return rc;
+  return hip_status(bevk::launch_linear_forward(dtype, a, residual, y, z, workspace, (hipStream_t)stream), fn);
+}
+
+int bevk_linear_backward(int dtype, const void *grad_y, const void *x, const void *weight, const void *z, int64_t rows,
+                         int in_features, int out_features, int act, int bias_dtype, void *workspace,
+                         int64_t workspace_bytes, void *grad_x, void *grad_weight, void *grad_bias, void *stream) {
+  const char *fn = "linear_backward";
+  g_last_error.clear();
+  if (int rc = check_linear(fn, dtype, bias_dtype, rows, in_features, out_features, act)) return rc;
+  if (!grad_y || (act != 0 && !z) || (grad_x && !weight) || (grad_weight && !x))
+    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  const bevk::LinearArgs a = linear_args(x, weight, nullptr, bias_dtype, rows, in_features, out_features, act);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::linear_backward_workspace_bytes(dtype, a)))
+    return rc;
+  if (!grad_x && !grad_weight && !grad_bias) return ok();
+  return hip_status(bevk::launch_linear_backward(dtype, a, grad_y, z, workspace, grad_x, grad_weight, grad_bias,
+                                                 (hipStream_t)stream),
+                    fn);
+}
+
 }  // extern "C"

@@ -26,7 +26,7 @@ SOURCES = ["binding.cpp", "msda_fwd.hip", "dcn_gather.hip", "dcn_fused.hip", "dc
            "dcn_bwd.hip", "msda_bwd.hip", "layout.hip", "dcn_f32.hip",
            "dcn_wgrad.hip", "group_norm.hip", "embedding.hip",
            "grad_clip.hip", "adamw.hip",
-           "residual_norm_fwd.hip", "residual_norm_bwd.hip"]
+           "residual_norm_fwd.hip", "residual_norm_bwd.hip", "linear.hip"]
 ARCH = "gfx950"
 
 

@@ -1,0 +1,54 @@
+"""Projections with everything behind them: the value, output and feed-forward products around multi-scale
+attention, with bias, activation and residual on the sums before their one rounding. Forward and
+backward run on the kernels of libbevk.so. The reference has no counterpart."""
+from __future__ import annotations
+
+import torch
+
+import _bevk as _b
+
+_loaded = None
+
+
+def _ext():
+    global _loaded
+    if _loaded is None:
+        import _modulated_deform_conv_ext
+        _loaded = _modulated_deform_conv_ext
+    return _loaded
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+class LinearActFunction(torch.autograd.Function):
+    """y = act(x W^T + b) + residual; gradients flow to all tensors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        x, weight, bias = _dense(x), _dense(weight), _dense(bias)
+        y, z, ctx.sizes = _ext().linear_forward(x, weight, bias, act, _dense(residual), True)
+        ctx.save_for_backward(x, weight, bias, z)
+        return y
+
+    @staticmethod
+    @_b.once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, bias, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = (None, None, None)
+        if any(need[:3]):
+            grads = _ext().linear_backward(_dense(grad_y), x, weight, bias, z, ctx.sizes, need[:3])
+        return (*grads, None, grad_y if need[4] else None)
+
+
+def linear_act(x, weight, bias=None, act=None, residual=None):
+    """act(x @ weight.T + bias) + residual: x [..., K], weight [N, K], bias [N] in the input's type or
+    float32 (or None), residual [..., N] (or None) -> [..., N]. fp32 / fp16 / bf16. act None, "relu",
+    "silu" or "gelu" (z times the normal distribution below z, as torch's default). Everything behind the
+    product is in fp32 and rounded once. SiLU and GELU, and ReLU with a residual, keep z in the
+    input's type for the backward. Differentiable once, in reverse mode; the same results on every run."""
+    if _b.records_nothing():  # (without the bookkeeping of a Function)
+        return _ext().linear_forward(_dense(x), _dense(weight), _dense(bias), act, _dense(residual))[0]
+    return LinearActFunction.apply(x, weight, bias, act, residual)
