@@ -140,10 +140,11 @@ hipError_t launch_f32_split_weight(const float *weight, int cout, int C, int T, 
                                    void *packed, hipStream_t stream);
 // out[m, n] = sum_k A[m, k] W[n, k] (+ bias): A the deformable columns of geometry g (dg == 1,
 // <= 9 taps, geo kGeoMask / kGeoY / kGeoYF32; M and K must match it), or with g == nullptr the
-// matrix x [M][K]. K % 32 == 0, x under 2 GiB, 16-byte aligned x.
+// matrix x [M][K] (then also + addend [M][channels_out]). K % 32 == 0, x under 2 GiB, 16-byte aligned x.
 hipError_t launch_f32_split(const DcnGeom *g, int channels_out, int M, int K, const void *x,
                             const void *off, int geo, const void *msk, const void *w_split,
-                            const float *bias, float *out, hipStream_t stream, bool relu);
+                            const float *bias, float *out, hipStream_t stream, bool relu,
+                            const float *addend = nullptr);
 
 // The whole NCHW fp32 layer (groups == 1, any deformable_group): x [B, C, H, W], off [B, dg*2T, Ho,
 // Wo], msk [B, dg*T, Ho, Wo], weight [Cout, C, kh, kw] -> out [B, Cout, Ho, Wo]. C % 32 == 0, at

@@ -63,7 +63,7 @@ struct Params {
   const void *w;              // split weight, then its flags
   const uint32_t *flags;
   const float *bias;
-  const float *addend;        // kTConv: added to the sum before the rounding
+  const float *addend;        // kTConv, kRows: added to the sum before the rounding
   void *out;
   int out_kind;               // 0 fp32, 1 fp16, 2 bf16 (16 bits: kTConv only)
   int plane;                  // > 0: out is [B, Cout, plane] with m = (b, position), fp32
@@ -1012,8 +1012,9 @@ Params make_params(const DcnGeom *g, int channels_out, int M, int K, const void 
 
 hipError_t launch_f32_split(const DcnGeom *g, int channels_out, int M, int K, const void *x,
                             const void *off, int geo, const void *msk, const void *w_split,
-                            const float *bias, float *out, hipStream_t stream, bool relu) {
+                            const float *bias, float *out, hipStream_t stream, bool relu, const float *addend) {
   Params p = make_params(g, channels_out, M, K, x, off, msk, w_split, bias, out, relu);
+  p.addend = addend;
   if (g == nullptr) {
     const Plan pl = make_plan<kRows>(p, false);
     return launch_geo<kRows>(p, pl, false, stream);

@@ -72,6 +72,16 @@ template <typename T> __device__ __forceinline__ float slope(float z, int act) {
   return __builtin_fmaf(z, pdf, cdf);
 }
 
+// f(the activation as a type): a kernel for each, whose code has that one alone.
+template <typename F> void with_act(int act, F f) {
+  switch (act) {
+    case kActNone: f(std::integral_constant<int, kActNone>()); break;
+    case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
+    default: f(std::integral_constant<int, kActGelu>()); break;
+  }
+}
+
 // What is done with a sum. Tensors [M][N].
 struct Epilogue {
   const void *bias, *residual;
@@ -210,6 +220,587 @@ hipError_t launch_any(const T *a, int64_t a_m, int64_t a_k, const T *b, int64_t 
 }
 
 // ---------------------------------------------------------------------------------------
+// 16-bit products of tiles: both operands' rows dense, K a multiple of 8, 16-byte aligned. A workgroup
+// of WM x WN waves takes BM x BN values, 64 terms at a time: rows of 128 bytes go straight from memory
+// into LDS (8 rows an instruction), the next step's while this one multiplies. A row's eight 16-byte
+// pieces lie in the order piece ^ (row / 2 % 8), so that 16 neighbouring rows' reads of one piece
+// meet none of the 64 banks twice; the order is made by the address that a lane loads from, since it always
+// writes where its number says. Rows past the end are the last row's again and are not stored; terms
+// past K are zeros in both operands.
+// ---------------------------------------------------------------------------------------
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+constexpr int kBK = 64;
+constexpr int kRowBytes = kBK * 2;
+
+__device__ __forceinline__ floatx16 mfma32(int4v a, int4v b, floatx16 c, f16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma32(int4v a, int4v b, floatx16 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// 16 bytes from `off` + `k` of the buffer for each lane, to `to` + 16 lane (`to` and k: the wave's).
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char *to, uint32_t off, uint32_t k) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass does not know the builtin, and would leave the kernel out)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)to, 16, off, k, 0, 0);
+#endif
+}
+
+struct TileArgs {
+  const void *a, *b;
+  int64_t M;
+  int K;
+  Epilogue e;
+  int64_t tm;
+  int tn;
+  int64_t per_xcd;
+  bool eights;  // N a multiple of 8, tensors on 16-byte boundaries
+};
+
+// Eight neighbouring values of a row.
+template <typename T, int ACT, bool BIAS = true>
+__device__ __forceinline__ void finish8(const Epilogue &e, int64_t m, int n, float (&v)[8]) {
+  const int64_t at = m * e.N + n;
+  Vec<T, 8> r;
+  if (e.residual != nullptr) r = load_vec<T, 8>(static_cast<const T *>(e.residual) + at);
+  if (BIAS && e.bias != nullptr) {
+    if (e.bias_wide) {
+#pragma unroll
+      for (int h = 0; h < 8; h += 4) {
+        const Vec<float, 4> b = load_vec<float, 4>(static_cast<const float *>(e.bias) + n + h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[h + k] += b.v[k];
+      }
+    } else {
+      const Vec<T, 8> b = load_vec<T, 8>(static_cast<const T *>(e.bias) + n);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += (float)b.v[k];
+    }
+  }
+  Vec<T, 8> y;
+  if (e.z != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y.v[k] = static_cast<T>(v[k]);
+    store_vec<T, 8>(static_cast<T *>(e.z) + at, y);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = activate<T>(v[k], ACT);
+  if (e.residual != nullptr)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += (float)r.v[k];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y.v[k] = static_cast<T>(v[k]);
+  store_vec<T, 8>(static_cast<T *>(e.y) + at, y);
+}
+
+// Tile number L of all: groups of 8 rows of tiles, in a group one column of tiles after another, so that
+// the tiles that run on an XCD at a time share rows of both operands in its L2.
+__device__ __forceinline__ void tile_at(int64_t L, int64_t tm, int tn, int64_t &i, int &j) {
+  const int64_t group = L / (8 * (int64_t)tn), left = L - group * 8 * tn;
+  const int rows = (int)min((int64_t)8, tm - group * 8);
+  j = (int)(left / rows);
+  i = group * 8 + left % rows;
+}
+
+template <typename T, int ACT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, int64_t first) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // 8-row pieces that a wave loads a step
+  static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && TM * 32 * WM == BM && TN * 32 * WN == BN, "tile");
+  __shared__ __attribute__((aligned(1024))) char lds[2][(BM + BN) * kRowBytes];
+  const int64_t block = first + blockIdx.x;
+  const int64_t L = block % 8 * p.per_xcd + block / 8;
+  if (L >= p.tm * p.tn) return;
+  int64_t ti;
+  int tj;
+  tile_at(L, p.tm, p.tn, ti, tj);
+  const int64_t m0 = ti * BM;
+  const int n0 = tj * BN, N = p.e.N, K = p.K;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  // a tile's rows are below 2^31 bytes apart (K at most 2^21)
+  const int ma = (int)min((int64_t)BM, p.M - m0), nb = min(BN, N - n0);
+  const uint32_t ld = (uint32_t)K * 2;
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(static_cast<const char *>(p.a) + m0 * ld, ma * ld);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(static_cast<const char *>(p.b) + (int64_t)n0 * ld, nb * ld);
+  const int piece[2] = {(lane % 8 ^ lane / 16) * 16, (lane % 8 ^ lane / 16 ^ 4) * 16};  // of even and odd groups of 8 rows
+  uint32_t oa[LA], ob[LB];
+#pragma unroll
+  for (int i = 0; i < LA; ++i) oa[i] = min((wave * LA + i) * 8 + lane / 8, ma - 1) * ld + piece[(wave * LA + i) % 2];
+#pragma unroll
+  for (int i = 0; i < LB; ++i) ob[i] = min((wave * LB + i) * 8 + lane / 8, nb - 1) * ld + piece[(wave * LB + i) % 2];
+  const int steps = K / kBK;
+
+  auto load = [&](int step, char *to) __attribute__((always_inline)) {
+    const uint32_t k = (uint32_t)step * kRowBytes;
+    char *da = to + wave * LA * 1024, *db = to + BM * kRowBytes + wave * LB * 1024;
+#pragma unroll
+    for (int i = 0; i < LA; ++i)
+      load_to_lds(ra, da + i * 1024, oa[i], k);
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      load_to_lds(rb, db + i * 1024, ob[i], k);
+  };
+
+  floatx16 acc[TM][TN] = {};
+  const int wm = wave / WN, wn = wave % WN, row = lane % 32, half = lane / 32;
+  auto multiply = [&](const char *from) __attribute__((always_inline)) {
+    const char *fa = from + (wm * TM * 32 + row) * kRowBytes, *fb = from + (BM + wn * TN * 32 + row) * kRowBytes;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = ((k * 2 + half) ^ (row / 2 % 8)) * 16;
+      int4v a[TM], b[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const int4v *>(fa + i * 32 * kRowBytes + at);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const int4v *>(fb + j * 32 * kRowBytes + at);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[j], a[i], acc[i][j], T());
+    }
+  };
+
+  int s = 0;
+  if (steps > 0) load(0, lds[0]);
+  for (; s + 1 < steps; s += 2) {
+    __syncthreads();
+    load(s + 1, lds[1]);
+    multiply(lds[0]);
+    __syncthreads();
+    if (s + 2 < steps) load(s + 2, lds[0]);
+    multiply(lds[1]);
+  }
+  if (s < steps) {
+    __syncthreads();
+    multiply(lds[0]);
+  }
+  if (K % kBK != 0) {  // the rest of the terms, through registers
+    const uint32_t k = (uint32_t)steps * kRowBytes;
+    const bool there[2] = {k + piece[0] < ld, k + piece[1] < ld};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+      const Vec<int, 4> v = buffer_load_vec<int, 4>(ra, there[(wave * LA + i) % 2] ? oa[i] + k : 0xffffffffu);
+      *reinterpret_cast<Vec<int, 4> *>(lds[0] + (wave * LA + i) * 1024 + lane * 16) = v;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      const Vec<int, 4> v = buffer_load_vec<int, 4>(rb, there[(wave * LB + i) % 2] ? ob[i] + k : 0xffffffffu);
+      *reinterpret_cast<Vec<int, 4> *>(lds[0] + BM * kRowBytes + (wave * LB + i) * 1024 + lane * 16) = v;
+    }
+    __syncthreads();
+    multiply(lds[0]);
+  }
+  __syncthreads();
+
+  // A lane holds one row and four times four neighbouring columns of each 32 x 32. Each wave turns 32 rows of
+  // its own at a time in LDS, so that eight lanes store 128 neighbouring bytes of a row.
+  constexpr int P = TN * 32 + 4, C = TN * 4;  // floats of a row, and its pieces of 8
+  float *turn = reinterpret_cast<float *>(lds[0]) + wave * 32 * P;
+  static_assert(WAVES * 32 * P * 4 <= (int)sizeof(lds), "turn");
+  const int wn0 = n0 + wn * TN * 32;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        Vec<float, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v.v[e] = acc[i][j][q * 4 + e];
+        *reinterpret_cast<Vec<float, 4> *>(turn + row * P + j * 32 + q * 8 + half * 4) = v;
+      }
+    const int64_t mi = m0 + wm * TM * 32 + i * 32;
+    if (p.eights) {
+#pragma unroll 2
+      for (int c = lane; c < 32 * C; c += 64) {
+        const int64_t m = mi + c / C;
+        const int n = wn0 + c % C * 8;
+        float v[8];
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          const Vec<float, 4> x = load_vec<float, 4>(turn + c / C * P + c % C * 8 + h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[h + e] = x.v[e];
+        }
+        if (m < p.M && n < N) finish8<T, ACT>(p.e, m, n, v);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = lane; c < 32 * TN * 32; c += 64) {
+        const int64_t m = mi + c / (TN * 32);
+        const int n = wn0 + c % (TN * 32);
+        if (m < p.M && n < N) finish<T>(p.e, m, n, turn[c / (TN * 32) * P + c % (TN * 32)]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// 16-bit products of many rows by a weight of few terms (K 256 or 512): bound by memory, where a tile of
+// few steps waits for its first loads and its stores. A workgroup of eight waves a CU keeps NT
+// columns of the weight in LDS (128 KB) for the whole launch; each wave takes R x 16 rows at a time, whose
+// fragments it loads straight into registers, a whole 256 terms ahead, across the rows' ends.
+// Rows of the weight lie in LDS so that a lane ends up with eight neighbouring columns: row 16 j + 4 g + e
+// is column 32 (j / 2) + 8 g + 4 (j % 2) + e.
+// ---------------------------------------------------------------------------------------
+struct StreamArgs {
+  const void *a, *b;
+  int64_t M, strips;
+  Epilogue e;
+  int parts, shares;  // column parts, workgroups of each
+};
+
+template <typename T, int ACT, int K, int NT, int R>
+__global__ void __launch_bounds__(512) stream_kernel(const StreamArgs p) {
+  constexpr int J = NT / 16, G = J / 4, WAVES = 8;
+  __shared__ __attribute__((aligned(1024))) char w[NT * K * 2];  // [K / 128][NT][128 terms]
+  __shared__ __attribute__((aligned(16))) float bias[NT];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r16 = lane % 16, g = lane / 16, N = p.e.N;
+  constexpr int ld = K * 2, BLOCKS = K / 256;
+  // workgroups of one XCD (their number modulo 8) take the parts of one share of rows after another
+  const int part = (int)(blockIdx.x / 8) % p.parts, share = (int)(blockIdx.x / 8) / p.parts * 8 + (int)blockIdx.x % 8;
+  if (share >= p.shares) return;
+  const int n0 = part * NT;
+  const int64_t step = (int64_t)p.shares * WAVES;
+  int64_t strip = (int64_t)share * WAVES + wave;
+  const char *at[R];
+  auto rows_of = [&](int64_t s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      at[i] = static_cast<const char *>(p.a) + min((s * R + i) * 16 + r16, p.M - 1) * ld + g * 16;
+  };
+  int4v a[4][R][2];  // 64 terms each
+  auto load = [&](int c, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) a[c][i][h] = *reinterpret_cast<const int4v *>(at[i] + k * 512 + c * 128 + h * 64);
+  };
+  if (strip < p.strips) {
+    rows_of(strip);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) load(c, 0);
+  }
+  {
+    // (a row's 16-byte pieces lie in the order piece ^ (row % 16): 16 rows' reads of one meet no bank twice)
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(static_cast<const char *>(p.b) + (int64_t)n0 * ld, min(NT, N - n0) * ld);
+#pragma unroll 4
+    for (int i = wave; i < K / 128 * (NT / 4); i += WAVES) {  // four rows of 256 bytes an instruction
+      const int k = i / (NT / 4), r = i % (NT / 4) * 4 + lane / 16;
+      const int n = r / 32 * 32 + r % 16 / 4 * 8 + r / 16 % 2 * 4 + r % 4;
+      load_to_lds(rb, w + i * 1024, min(n, N - n0 - 1) * ld + (lane ^ r) % 16 * 16, k * 256);
+    }
+  }
+  for (int n = threadIdx.x; n < NT; n += 64 * WAVES) bias[n] = n0 + n < N ? bias_at<T>(p.e, n0 + n) : 0.f;
+  __syncthreads();
+  if (strip >= p.strips) return;
+  const char *from[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) from[h] = w + r16 * 256 + ((h * 4 + g) ^ r16) * 16;
+  // four columns' fragments are read while the four before multiply
+  int4v b[2][4];
+  auto read = [&](int unit, int to) __attribute__((always_inline)) {
+    const int q = unit % G, h = unit / G;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      b[to][j] = *reinterpret_cast<const int4v *>(from[h % 4] + (q * 4 + j) * 16 * 256 + h / 4 * NT * 256);
+  };
+  read(0, 0);
+  for (; strip < p.strips; strip += step) {
+    asm volatile("" ::: "memory");  // (the weight's reads stay in the loop: registers hold no 128 KB)
+    floatx4 acc[R][J];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        acc[i][j] = *reinterpret_cast<const floatx4 *>(bias + j / 2 * 32 + g * 8 + j % 2 * 4);
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) {
+      if (k + 1 == BLOCKS) rows_of(min(strip + step, p.strips - 1));
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < G; ++q) {
+            const int unit = (c * 2 + h) * G + q;
+            read((k * 8 * G + unit + 1) % (BLOCKS * 8 * G), (unit + 1) % 2);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < R; ++i)
+                acc[i][q * 4 + j] = mfma16(b[unit % 2][j], a[c][i][h], acc[i][q * 4 + j], T());
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        load(c, (k + 1) % BLOCKS);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t m = (strip * R + i) * 16 + r16;
+      if (m < p.M)
+#pragma unroll
+        for (int j = 0; j < J; j += 2) {
+          const int n = n0 + j * 16 + g * 8;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = acc[i][j][e];
+            v[4 + e] = acc[i][j + 1][e];
+          }
+          if (n < N) finish8<T, ACT, false>(p.e, m, n, v);
+        }
+    }
+  }
+}
+
+template <typename T, int K, int NT, int R>
+hipError_t launch_stream_of(StreamArgs p, hipStream_t stream) {
+  p.strips = (p.M + R * 16 - 1) / (R * 16);
+  p.parts = (p.e.N + NT - 1) / NT;
+  const int cus = std::max(8, device_cus());
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(cus / p.parts, (p.strips + 7) / 8));
+  with_act(p.e.act, [&](auto act) {
+    hipLaunchKernelGGL((stream_kernel<T, decltype(act)::value, K, NT, R>), dim3((unsigned)((p.shares + 7) / 8 * 8 * p.parts)),
+                       dim3(512), 0, stream, p);
+  });
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows (single tokens, a decoder's queries): the weight's bytes or the latency of a launch are the
+// bound. A workgroup of four waves takes 16 columns of up to MT x 16 rows; the waves take every
+// fourth 64 bytes of the rows, which they load straight into the fragments, eight loads of the weight in
+// flight; their sums meet in LDS. fp32 runs on the fp32 matrix cores.
+// ---------------------------------------------------------------------------------------
+struct FewArgs {
+  const void *a, *b;
+  int64_t M;
+  int K;
+  Epilogue e;
+  int64_t tm;
+};
+
+template <typename T, int MT, int NT, int WAVES, int U>
+__global__ void __launch_bounds__(64 * WAVES) few_kernel(const FewArgs p, int64_t first) {
+  __shared__ __attribute__((aligned(16))) float sum[WAVES][MT * 16][NT * 16 + 4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, g = lane / 16, N = p.e.N, K = p.K;
+  const int64_t tile = first + blockIdx.x, m0 = tile % p.tm * (MT * 16);
+  const int n0 = (int)(tile / p.tm) * (NT * 16);
+  const uint32_t ld = (uint32_t)K * sizeof(T);  // (below 2^23 bytes)
+  const int mt = (int)min((int64_t)MT * 16, p.M - m0), nt = min(NT * 16, N - n0);
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(static_cast<const char *>(p.a) + m0 * ld, mt * ld);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(static_cast<const char *>(p.b) + (int64_t)n0 * ld, nt * ld);
+  uint32_t oa[MT], ob[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) oa[i] = min(i * 16 + r16, mt - 1) * ld;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) ob[j] = min(j * 16 + r16, nt - 1) * ld;
+  floatx4 acc[MT][NT] = {};
+  auto multiply = [&](int4v w, int4v x, floatx4 c) __attribute__((always_inline)) {
+    if constexpr (sizeof(T) == 2) {
+      return mfma16(w, x, c, T());
+    } else {
+      const floatx4 wf = __builtin_bit_cast(floatx4, w), xf = __builtin_bit_cast(floatx4, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[e], xf[e], c, 0, 0, 0);
+      return c;
+    }
+  };
+  for (uint32_t k = wave * 64; k < ld; k += U * WAVES * 64) {  // bytes of a row; past its end a load gives zeros
+    int4v w[U][NT], x[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = k + u * WAVES * 64 + g * 16;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        w[u][j] = __builtin_bit_cast(int4v, buffer_load_vec<int, 4>(rb, at < ld ? ob[j] + at : 0xffffffffu));
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        x[u][i] = __builtin_bit_cast(int4v, buffer_load_vec<int, 4>(ra, at < ld ? oa[i] + at : 0xffffffffu));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = multiply(w[u][j], x[u][i], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *reinterpret_cast<floatx4 *>(&sum[wave][i * 16 + r16][j * 16 + g * 4]) = acc[i][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * NT * 256; i += 64 * WAVES) {
+    const int row = i / (NT * 16), c = i % (NT * 16);
+    float v = sum[0][row][c];
+#pragma unroll
+    for (int q = 1; q < WAVES; ++q) v += sum[q][row][c];
+    if (row < mt && c < nt) finish<T>(p.e, m0 + row, n0 + c, v);
+  }
+}
+
+template <typename T, int MT, int NT, int WAVES, int U>
+hipError_t launch_few_of(FewArgs p, hipStream_t stream) {
+  p.tm = (p.M + MT * 16 - 1) / (MT * 16);
+  return launch_in_parts(p.tm * ((p.e.N + NT * 16 - 1) / (NT * 16)), 64 * WAVES, [&](int64_t first, unsigned n) {
+    hipLaunchKernelGGL((few_kernel<T, MT, NT, WAVES, U>), dim3(n), dim3(64 * WAVES), 0, stream, p, first);
+  });
+}
+
+bool on_16(std::initializer_list<const void *> all) {
+  for (const void *p : all)
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  return true;
+}
+
+bool rows_take(const void *a, const void *b, int64_t K, int size) {
+  return K * size % 16 == 0 && K <= 1 << 21 && on_16({a, b});
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+hipError_t launch_tile_of(TileArgs p, hipStream_t stream) {
+  p.tm = (p.M + BM - 1) / BM;
+  p.tn = (p.e.N + BN - 1) / BN;
+  p.per_xcd = (p.tm * p.tn + 7) / 8;
+  return launch_in_parts(p.per_xcd * 8, 64 * WM * WN, [&](int64_t first, unsigned n) {
+    with_act(p.e.act, [&](auto act) {
+      hipLaunchKernelGGL((tile_kernel<T, decltype(act)::value, BM, BN, WM, WN>), dim3(n), dim3(64 * WM * WN), 0, stream, p, first);
+    });
+  });
+}
+// Which kernel a product of dense rows takes. 16 bits, K 256 or 512 and enough rows for a few strips a
+// wave: the streaming kernel (measured at 40,000 x 256 x 512, 184,950 x 256 x 256, 20,000 x 256 x 4,096
+// and 184,950 x 512 x 256: 20.4, 43, 49 and 72 us, the fastest tile 24.5, 54, 76 and 80; below it
+// loses: 20,000 x 256 x 768 20.0 and 19.6, 40,000 x 512 x 256 22.2 and 20.3). Else the least of these
+// estimates in us, fitted to 40 shapes from 1 x 256 x 256 to 8,192 x 2,048 x 8,192:
+//   tiles   rounds over the CUs, each of K / 64 steps that take the longer of a step's latency and what the
+//           tiles on a CU take at its full rate, and what a round's first loads and stores take
+//   few     a CU's loads at 33 bytes a ns (each touches 16 rows' 64 bytes)
+enum Kind { kFew4, kFew8, kFew22, kFew42, kTile64, kTile64x128, kTile128, kTile256, kStream, kKinds };
+struct Shape {
+  int bm, bn, on_cu;          // rows and columns, workgroups on a CU
+  double first, step, latency;  // tiles: us of a round besides its steps, of a step of one tile at full rate, alone
+};
+constexpr Shape kShapes[kTile256 + 1] = {
+    {16, 16, 0, 2.5, 0, 0},      {16, 16, 0, 2.6, 0, 0},      {32, 32, 0, 3.0, 0, 0},      {64, 32, 0, 3.5, 0, 0},
+    {64, 64, 5, 3.3, 0.2, 0.42}, {64, 128, 3, 4, 0.32, 0.55}, {128, 128, 2, 5, 0.51, 0.7}, {256, 256, 1, 7, 1.8, 1.4}};
+
+Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
+  const int64_t cus = std::max(8, device_cus());
+  if (size == 2 && eights && (K == 256 || K == 512) &&
+      (M + 15) / 16 * ((N + 65536 / K - 1) / (65536 / K)) >= cus * (K == 256 ? 12 : 24))
+    return kStream;
+  Kind best = kFew4;
+  double best_t = 0;
+  for (int k = kFew4; k <= (size == 2 ? kTile256 : kFew42); ++k) {
+    const Shape &s = kShapes[k];
+    const int64_t n = (((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn) + cus - 1) / cus;  // workgroups of a CU
+    double t;
+    if (k <= kFew42) {
+      const double steps = (double)((K * size + 63) / 64);  // (a wave has at least one batch of loads to wait for)
+      t = s.first + (double)n * (s.bm + s.bn) * steps * 64 / 33e3 + (k == kFew4 ? 0.0125 : 0.007) * steps;
+    } else {
+      const int64_t full = n / s.on_cu, rest = n % s.on_cu;
+      const double steps = (double)((K + 63) / 64);
+      t = full * (steps * std::max(s.latency, s.on_cu * s.step) + s.first) +
+          (rest > 0 ? steps * std::max(s.latency, rest * s.step) + s.first : 0);
+    }
+    if (k == kFew4 || t < best_t) {
+      best = (Kind)k;
+      best_t = t;
+    }
+  }
+  return best;
+}
+
+template <typename T>
+hipError_t launch_rows(const T *a, const T *b, int64_t M, int64_t K, const Epilogue &e, hipStream_t stream) {
+  const bool eights = e.N % 8 == 0 && on_16({e.residual, e.y, e.z, e.bias});
+  const Kind kind = plan(sizeof(T), M, e.N, K, eights);
+  const FewArgs few{a, b, M, (int)K, e, 0};
+  switch (kind) {
+    case kFew4: return launch_few_of<T, 1, 1, 4, 8>(few, stream);
+    case kFew8: return launch_few_of<T, 1, 1, 8, 8>(few, stream);
+    case kFew22: return launch_few_of<T, 2, 2, 8, 4>(few, stream);
+    case kFew42: return launch_few_of<T, 4, 2, 8, 4>(few, stream);
+    default: break;
+  }
+  if constexpr (sizeof(T) == 2) {
+    const TileArgs tile{a, b, M, (int)K, e, 0, 0, 0, eights};
+    const StreamArgs rows{a, b, M, 0, e, 0, 0};
+    switch (kind) {
+      case kTile64: return launch_tile_of<T, 64, 64, 2, 2>(tile, stream);
+      case kTile64x128: return launch_tile_of<T, 64, 128, 1, 4>(tile, stream);
+      case kTile128: return launch_tile_of<T, 128, 128, 2, 2>(tile, stream);
+      case kTile256: return launch_tile_of<T, 256, 256, 2, 4>(tile, stream);
+      default: break;
+    }
+    return K == 256 ? launch_stream_of<T, 256, 256, 1>(rows, stream) : launch_stream_of<T, 512, 128, 1>(rows, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+// fp32 products of more than a few rows: the split product of dcn_f32.hip (three bf16 pieces an operand).
+// It adds a residual or applies ReLU itself; other epilogues are a pass behind it.
+bool split_takes(const void *a, const void *b, int64_t N, int64_t K, bool transposed) {
+  return (transposed ? K % 32 == 0 && N % 16 == 0 : K % 32 == 0) && K <= 1 << 20 && on_16({a, b});
+}
+// The split product loses to the kernel for few rows up to this many (measured at K, N of 256 to 2,048).
+bool split_pays(int64_t M, int64_t N, int64_t K) {
+  const int64_t cus = std::max(8, device_cus());
+  const double few = 3.5 + (double)((((M + 63) / 64) * ((N + 31) / 32) + cus - 1) / cus) * 96 * K * 4 / 33e3;
+  return few > 12.0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) act_kernel(const T *z, const T *__restrict__ residual,
+                                                       T *y, int act, int64_t total, bool wide, int64_t first) {  // y: z, or apart
+  constexpr int V = 16 / sizeof(T);
+  const int64_t i = ((first + blockIdx.x) * kThreads + threadIdx.x) * V;
+  if (i >= total) return;
+  auto one = [&](float v, float r) __attribute__((always_inline)) { return static_cast<T>(activate<T>(v, act) + r); };
+  if (wide && i + V <= total) {
+    const Vec<T, V> v = load_vec<T, V>(z + i);
+    Vec<T, V> r{}, o;
+    if (residual != nullptr) r = load_vec<T, V>(residual + i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.v[e] = one((float)v.v[e], (float)r.v[e]);
+    store_vec<T, V>(y + i, o);
+  } else {
+    for (int64_t k = i; k < min(i + V, total); ++k) y[k] = one((float)z[k], residual != nullptr ? (float)residual[k] : 0.f);
+  }
+}
+
+// out = act(x W^T + bias) + residual and z as Epilogue has them; workspace: f32_split_weight_bytes.
+hipError_t launch_split(const float *x, const float *weight, bool transposed, int64_t M, int N, int K, const Epilogue &e,
+                        void *workspace, hipStream_t stream) {
+  hipError_t err = transposed ? launch_f32_split_weight(weight, K, N, 1, true, workspace, stream)
+                              : launch_f32_split_weight(weight, N, K, 1, false, workspace, stream);
+  if (err != hipSuccess) return err;
+  const bool relu = e.act == kActRelu && e.residual == nullptr && e.z == nullptr;
+  const bool pass = e.act != kActNone && !relu;  // act(z) + residual in a pass of its own
+  float *out = static_cast<float *>(pass && e.z != nullptr ? e.z : e.y);
+  const float *addend = pass ? nullptr : static_cast<const float *>(e.residual);
+  const int64_t most = ((1LL << 31) - 4096) / ((int64_t)K * 4) / 16 * 16;  // rows below 2 GiB
+  for (int64_t m = 0; m < M; m += most) {
+    err = launch_f32_split(nullptr, N, (int)std::min(most, M - m), K, x + m * K, nullptr, 0, nullptr, workspace,
+                           static_cast<const float *>(e.bias), out + m * N, stream, relu,
+                           addend == nullptr ? nullptr : addend + m * N);
+    if (err != hipSuccess) return err;
+  }
+  if (!pass) return hipSuccess;
+  const int64_t total = M * N;
+  return launch_in_parts((total + kThreads * 4 - 1) / (kThreads * 4), kThreads, [&](int64_t first, unsigned n) {
+    hipLaunchKernelGGL((act_kernel<float>), dim3(n), dim3(kThreads), 0, stream, out, static_cast<const float *>(e.residual),
+                       static_cast<float *>(e.y), e.act, total, on_16({out, e.residual, e.y}), first);
+  });
+}
+
+// ---------------------------------------------------------------------------------------
 // gz = gy act'(z) and its column sums: a workgroup takes a range of rows of up to 256 vectors of
 // columns; each thread keeps its columns' sums, the workgroup adds up its rows side by side and
 // total_kernel the workgroups, in order.
@@ -280,11 +871,6 @@ hipError_t launch_grad_z_v(const T *gy, const T *z, T *gz, int act, int64_t rows
                      gy, z, gz, act, rows, n, per, part);
   return hipGetLastError();
 }
-bool on_16(std::initializer_list<const void *> all) {
-  for (const void *p : all)
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
-  return true;
-}
 template <typename T>
 hipError_t launch_grad_z(const T *gy, const T *z, T *gz, int act, int64_t rows, int n, float *part, void *grad_bias,
                          bool bias_wide, hipStream_t stream) {
@@ -303,11 +889,38 @@ hipError_t launch_grad_z(const T *gy, const T *z, T *gz, int act, int64_t rows, 
 // ---------------------------------------------------------------------------------------
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// What a product of rows x [M][K] by weight [N][K] (transposed: [K][N]) needs for either alignment.
+int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t K) {
+  int64_t most = any_bytes(M, N, K);
+  if (dtype == 0) most = std::max(most, f32_split_weight_bytes(N, K));
+  if (transposed) most = std::max(most, up(N * K * (dtype == 0 ? 4 : 2)));
+  return most;
+}
+template <typename T>
+hipError_t product(const T *x, const T *weight, bool transposed, int64_t M, int K, const Epilogue &e, void *workspace,
+                   hipStream_t stream) {
+  const int N = e.N;
+  if constexpr (sizeof(T) == 4)
+    if (split_takes(x, weight, N, K, transposed) && split_pays(M, N, K))
+      return launch_split(x, weight, transposed, M, N, K, e, workspace, stream);
+  if (!rows_take(x, weight, K, sizeof(T)))
+    return launch_any<T>(x, K, 1, weight, transposed ? 1 : K, transposed ? N : 1, M, K, e, workspace, stream);
+  if (transposed) {  // the weight is small next to the rows: turned once, its rows are dense
+    if (hipError_t err = launch_transpose(sizeof(T), weight, workspace, 1, K, N, stream)) return err;
+    weight = static_cast<const T *>(workspace);
+  }
+  return launch_rows(x, weight, M, K, e, stream);
+}
+
 template <typename T>
 hipError_t forward(const LinearArgs &a, const void *residual, void *y, void *z, void *workspace, hipStream_t stream) {
   const Epilogue e{a.bias, residual, y, z, a.bias_wide, a.act, a.N};
-  return launch_any(static_cast<const T *>(a.x), a.K, 1, static_cast<const T *>(a.weight), a.K, 1, a.rows, a.K, e,
-                    workspace, stream);
+  return product(static_cast<const T *>(a.x), static_cast<const T *>(a.weight), false, a.rows, a.K, e, workspace, stream);
+}
+
+bool weight_grad_takes(int dtype, const LinearArgs &a) {
+  const int64_t size = dtype == 0 ? 4 : 2, vec = 16 / size;
+  return a.K % vec == 0 && a.N % vec == 0 && a.rows < 1LL << 30 && std::max(a.K, a.N) * size * 64 <= 1LL << 28;
 }
 
 // Workspace of the backward: gz, the bias' parts, then what the products take.
@@ -319,7 +932,9 @@ BackWs back_ws(int dtype, const LinearArgs &a) {
   BackWs w;
   w.part = a.act != kActNone ? up(a.rows * a.N * size) : 0;
   w.product = w.part + up((int64_t)kSumBlocks * a.N * 4);
-  w.total = w.product + up(std::max(any_bytes(a.rows, a.K, a.N), any_bytes(a.N, a.K, a.rows)));
+  int64_t grad_w = any_bytes(a.N, a.K, a.rows);
+  if (weight_grad_takes(dtype, a)) grad_w = std::max(grad_w, weight_grad_workspace_bytes(dtype, a.rows, a.K, 1, a.N));
+  w.total = w.product + up(std::max(product_bytes(dtype, true, a.rows, a.K, a.N), grad_w));
   return w;
 }
 
@@ -328,7 +943,7 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
                     void *grad_w, void *grad_b, hipStream_t stream) {
   const BackWs ws = back_ws(dtype, a);
   char *base = static_cast<char *>(workspace);
-  const T *gy = static_cast<const T *>(grad_y), *gz = gy;
+  const T *gy = static_cast<const T *>(grad_y), *gz = gy, *x = static_cast<const T *>(a.x);
   if (a.act != kActNone) gz = reinterpret_cast<T *>(base);
   if (a.act != kActNone || grad_b != nullptr)
     if (hipError_t e = launch_grad_z<T>(gy, static_cast<const T *>(z), const_cast<T *>(gz), a.act, a.rows, a.N,
@@ -337,20 +952,21 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
       return e;
   if (grad_x != nullptr) {
     const Epilogue e{nullptr, nullptr, grad_x, nullptr, false, kActNone, a.K};
-    if (hipError_t err = launch_any<T>(gz, a.N, 1, static_cast<const T *>(a.weight), 1, a.K, a.rows, a.N, e,
-                                       base + ws.product, stream))
+    if (hipError_t err = product<T>(gz, static_cast<const T *>(a.weight), true, a.rows, a.N, e, base + ws.product, stream))
       return err;
   }
-  if (grad_w != nullptr) {
-    const Epilogue e{nullptr, nullptr, grad_w, nullptr, false, kActNone, a.K};
-    return launch_any<T>(gz, 1, a.N, static_cast<const T *>(a.x), 1, a.K, a.N, a.rows, e, base + ws.product, stream);
-  }
-  return hipSuccess;
+  if (grad_w == nullptr) return hipSuccess;
+  if (weight_grad_takes(dtype, a) && on_16({gz, x}))
+    return launch_weight_grad(dtype, x, gz, a.rows, a.K, 1, a.N, base + ws.product, dtype, grad_w, stream);
+  const Epilogue e{nullptr, nullptr, grad_w, nullptr, false, kActNone, a.K};
+  return launch_any<T>(gz, 1, a.N, x, 1, a.K, a.N, a.rows, e, base + ws.product, stream);
 }
 
 }  // namespace
 
-int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a) { return any_bytes(a.rows, a.N, a.K); }
+int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a) {
+  return product_bytes(dtype, false, a.rows, a.N, a.K);
+}
 
 hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *z, void *workspace,
                                  hipStream_t stream) {
