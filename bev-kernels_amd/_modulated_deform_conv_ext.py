@@ -1538,25 +1538,26 @@ def _linear_workspace_bytes(code, backward, rows, k, n, act):
     return nbytes
 
 
-def linear_forward(x, weight, bias=None, act=None, residual=None, with_z=False):
-    """(y, z, sizes): y = act(x @ weight.T + bias) + residual for x [..., K], weight [N, K]; z, with with_z,
-    what linear_backward takes for it (None where that needs none, y itself where its sign is enough)."""
+def linear_forward(x, weight, bias=None, act=None, residual=None, with_slope=False):
+    """(y, slope, sizes): y = act(x @ weight.T + bias) + residual for x [..., K], weight [N, K]; slope, with
+    with_slope, what linear_backward takes for it (None where that needs none, y itself where its sign
+    is enough)."""
     sizes = _linear_check("linear_forward", x, weight, bias, act, residual)
     code, rows, k, n, acode, bcode = sizes
     y = x.new_empty((*x.shape[:-1], n))
-    z = None
-    if with_z and acode:
-        z = y if acode == 1 and residual is None else torch.empty_like(y)
+    slope = None
+    if with_slope and acode:
+        slope = y if acode == 1 and residual is None else torch.empty_like(y)  # (16 bits: whole numbers)
     if rows:
         nbytes = _linear_workspace_bytes(code, 0, rows, k, n, acode)
         ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _b.call_on(x.get_device(), "bevk_linear_forward", code, x.data_ptr(), weight.data_ptr(), _b.ptr(bias), bcode,
                    _b.ptr(residual), rows, k, n, acode, _b.ptr(ws), nbytes, y.data_ptr(),
-                   None if z is y else _b.ptr(z))
-    return y, z, sizes
+                   None if slope is y else _b.ptr(slope))
+    return y, slope, sizes
 
 
-def linear_backward(grad_y, x, weight, bias, z, sizes, wanted=(True, True, True)):
+def linear_backward(grad_y, x, weight, bias, slope, sizes, wanted=(True, True, True)):
     """(grad_x, grad_weight, grad_bias) of linear_forward's y; None where `wanted` is false or there is no
     bias. The residual's gradient is grad_y."""
     code, rows, k, n, acode, bcode = sizes
@@ -1569,5 +1570,5 @@ def linear_backward(grad_y, x, weight, bias, z, sizes, wanted=(True, True, True)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         ptr = _b.ptr
         _b.call_on(x.get_device(), "bevk_linear_backward", code, grad_y.data_ptr(), x.data_ptr(), weight.data_ptr(),
-                   ptr(z), rows, k, n, acode, bcode, ws.data_ptr(), nbytes, ptr(grad_x), ptr(grad_w), ptr(grad_b))
+                   ptr(slope), rows, k, n, acode, bcode, ws.data_ptr(), nbytes, ptr(grad_x), ptr(grad_w), ptr(grad_b))
     return grad_x, grad_w, grad_b

@@ -279,11 +279,11 @@ struct LinearArgs {
   int K, N, act;
 };
 int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a);
-hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *z,
+hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *slope,
                                  void *workspace, hipStream_t stream);
-// z: the forward's (not read where act is none); outputs are skipped where null.
+// slope: the forward's (not read where act is none); outputs are skipped where null.
 int64_t linear_backward_workspace_bytes(int dtype, const LinearArgs &a);
-hipError_t launch_linear_backward(int dtype, const LinearArgs &a, const void *grad_y, const void *z, void *workspace,
+hipError_t launch_linear_backward(int dtype, const LinearArgs &a, const void *grad_y, const void *slope, void *workspace,
                                   void *grad_x, void *grad_w, void *grad_b, hipStream_t stream);
 
 // The norms between two blocks (residual_norm_fwd.hip has the formulas): rows x channels, no empty

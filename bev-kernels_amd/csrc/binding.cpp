@@ -1626,29 +1626,29 @@ int64_t bevk_linear_workspace_bytes(int dtype, int backward, int64_t rows, int i
 
 int bevk_linear_forward(int dtype, const void *x, const void *weight, const void *bias, int bias_dtype,
                         const void *residual, int64_t rows, int in_features, int out_features, int act, void *workspace,
-                        int64_t workspace_bytes, void *y, void *z, void *stream) {
+                        int64_t workspace_bytes, void *y, void *slope, void *stream) {
   const char *fn = "linear_forward";
   g_last_error.clear();
   if (int rc = check_linear(fn, dtype, bias_dtype, rows, in_features, out_features, act)) return rc;
   if (!x || !weight || !y) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   const bevk::LinearArgs a = linear_args(x, weight, bias, bias_dtype, rows, in_features, out_features, act);
   if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::linear_forward_workspace_bytes(dtype, a))) return rc;
-  return hip_status(bevk::launch_linear_forward(dtype, a, residual, y, z, workspace, (hipStream_t)stream), fn);
+  return hip_status(bevk::launch_linear_forward(dtype, a, residual, y, slope, workspace, (hipStream_t)stream), fn);
 }
 
-int bevk_linear_backward(int dtype, const void *grad_y, const void *x, const void *weight, const void *z, int64_t rows,
+int bevk_linear_backward(int dtype, const void *grad_y, const void *x, const void *weight, const void *slope, int64_t rows,
                          int in_features, int out_features, int act, int bias_dtype, void *workspace,
                          int64_t workspace_bytes, void *grad_x, void *grad_weight, void *grad_bias, void *stream) {
   const char *fn = "linear_backward";
   g_last_error.clear();
   if (int rc = check_linear(fn, dtype, bias_dtype, rows, in_features, out_features, act)) return rc;
-  if (!grad_y || (act != 0 && !z) || (grad_x && !weight) || (grad_weight && !x))
+  if (!grad_y || (act != 0 && !slope) || (grad_x && !weight) || (grad_weight && !x))
     return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   const bevk::LinearArgs a = linear_args(x, weight, nullptr, bias_dtype, rows, in_features, out_features, act);
   if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::linear_backward_workspace_bytes(dtype, a)))
     return rc;
   if (!grad_x && !grad_weight && !grad_bias) return ok();
-  return hip_status(bevk::launch_linear_backward(dtype, a, grad_y, z, workspace, grad_x, grad_weight, grad_bias,
+  return hip_status(bevk::launch_linear_backward(dtype, a, grad_y, slope, workspace, grad_x, grad_weight, grad_bias,
                                                  (hipStream_t)stream),
                     fn);
 }

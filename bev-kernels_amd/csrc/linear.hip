@@ -1,12 +1,13 @@
 // Projections with everything behind them (gfx950): y = act(x W^T + bias) + residual, x [rows][K],
 // W [N][K], and the gradients.
 //
-//   z = x W^T + bias,  y = act(z) + residual
-//   gz = gy act'(z),  gx = gz W,  gW = gz^T x,  gbias = sum gz,  gresidual = gy
+//   z = x W^T + bias,  y = act(z) + residual,  slope = act'(z)
+//   gz = gy slope,  gx = gz W,  gW = gz^T x,  gbias = sum gz,  gresidual = gy
 //
 // Products of 16-bit types on the matrix cores with fp32 sums; bias, activation and residual in fp32 on the
-// sums in registers, one rounding at the end. gz is rounded to the input's type, which is what the
-// matrix cores read.
+// sums in registers, one rounding at the end. The forward keeps the slope, as wide as the input, where the
+// backward needs it, which then has no exp to take (gz of 40,000 x 512 gelu bf16: 46 us from z, 24 from
+// the slope). gz is rounded to the input's type, which is what the matrix cores read.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,25 +52,45 @@ template <typename T> __device__ __forceinline__ void normal(float z, float &cdf
     cdf = z > 0.f ? 1.f - tail : tail;
   }
 }
-template <typename T> __device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActRelu) return z > 0.f || z != z ? z : 0.f;
-  if (act == kActSilu) return z / (1.f + __expf(-z));
+// act(z), and its derivative.
+template <typename T> __device__ __forceinline__ float activate(float z, int act, float &slope) {
+  if (act == kActRelu) {
+    slope = z > 0.f ? 1.f : 0.f;
+    return z > 0.f || z != z ? z : 0.f;
+  }
+  if (act == kActSilu) {
+    const float s = 1.f / (1.f + __expf(-z));
+    slope = s * __builtin_fmaf(z, 1.f - s, 1.f);
+    return z * s;
+  }
   if (act == kActGelu) {
     float cdf, pdf;
     normal<T>(z, cdf, pdf);
+    slope = __builtin_fmaf(z, pdf, cdf);
     return z * cdf;
   }
+  slope = 1.f;
   return z;
 }
-template <typename T> __device__ __forceinline__ float slope(float z, int act) {
-  if (act == kActRelu) return z > 0.f ? 1.f : 0.f;
-  if (act == kActSilu) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return s * __builtin_fmaf(z, 1.f - s, 1.f);
+
+// A slope as the forward keeps it for the backward: fp32 as it is, ReLU's 0 or 1; in 16 bits those of SiLU and
+// GELU, between -0.13 and 1.13, as whole numbers: half a step is 2^-16, where rounding to the type would
+// add an error of the size that gz's own rounding has.
+constexpr uint16_t kSlopeNan = 65535;
+template <typename T, int ACT> __device__ __forceinline__ T keep_slope(float s) {
+  if constexpr (sizeof(T) == 4 || ACT == kActRelu) return static_cast<T>(s);
+  else return __builtin_bit_cast(T, s == s ? (uint16_t)__builtin_rintf(__builtin_fmaf(s, 32768.f, 8192.f)) : kSlopeNan);
+}
+template <typename T> __device__ __forceinline__ float kept_slope(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return v;
+  } else {
+    const uint16_t u = __builtin_bit_cast(uint16_t, v);
+    return u == kSlopeNan ? __builtin_nanf("") : __builtin_fmaf((float)u, 1.f / 32768.f, -0.25f);
   }
-  float cdf, pdf;
-  normal<T>(z, cdf, pdf);
-  return __builtin_fmaf(z, pdf, cdf);
+}
+template <typename T> __device__ __forceinline__ T keep_slope(float s, int act) {
+  return act == kActRelu ? keep_slope<T, kActRelu>(s) : keep_slope<T, kActGelu>(s);
 }
 
 // f(the activation as a type): a kernel for each, whose code has that one alone.
@@ -85,7 +106,7 @@ template <typename F> void with_act(int act, F f) {
 // What is done with a sum. Tensors [M][N].
 struct Epilogue {
   const void *bias, *residual;
-  void *y, *z;  // z: or null
+  void *y, *slope;  // slope: act'(z), or null
   bool bias_wide;
   int act;
   int N;
@@ -97,9 +118,9 @@ template <typename T> __device__ __forceinline__ float bias_at(const Epilogue &e
 }
 template <typename T> __device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, float v) {
   const int64_t at = m * e.N + n;
-  v += bias_at<T>(e, n);
-  if (e.z != nullptr) static_cast<T *>(e.z)[at] = static_cast<T>(v);
-  v = activate<T>(v, e.act);
+  float s;
+  v = activate<T>(v + bias_at<T>(e, n), e.act, s);
+  if (e.act != kActNone && e.slope != nullptr) static_cast<T *>(e.slope)[at] = keep_slope<T>(s, e.act);
   if (e.residual != nullptr) v += (float)static_cast<const T *>(e.residual)[at];
   static_cast<T *>(e.y)[at] = static_cast<T>(v);
 }
@@ -278,13 +299,21 @@ __device__ __forceinline__ void finish8(const Epilogue &e, int64_t m, int n, flo
     }
   }
   Vec<T, 8> y;
-  if (e.z != nullptr) {
+  if (ACT != kActNone && e.slope != nullptr) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y.v[k] = static_cast<T>(v[k]);
-    store_vec<T, 8>(static_cast<T *>(e.z) + at, y);
+    for (int k = 0; k < 8; ++k) {
+      float s;
+      v[k] = activate<T>(v[k], ACT, s);
+      y.v[k] = keep_slope<T, ACT>(s);
+    }
+    store_vec<T, 8>(static_cast<T *>(e.slope) + at, y);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float s;
+      v[k] = activate<T>(v[k], ACT, s);
+    }
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = activate<T>(v[k], ACT);
   if (e.residual != nullptr)
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += (float)r.v[k];
@@ -719,7 +748,7 @@ Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
 
 template <typename T>
 hipError_t launch_rows(const T *a, const T *b, int64_t M, int64_t K, const Epilogue &e, hipStream_t stream) {
-  const bool eights = e.N % 8 == 0 && on_16({e.residual, e.y, e.z, e.bias});
+  const bool eights = e.N % 8 == 0 && on_16({e.residual, e.y, e.slope, e.bias});
   const Kind kind = plan(sizeof(T), M, e.N, K, eights);
   const FewArgs few{a, b, M, (int)K, e, 0};
   switch (kind) {
@@ -756,34 +785,42 @@ bool split_pays(int64_t M, int64_t N, int64_t K) {
   return few > 12.0;
 }
 
+// y = act(y) + residual, and slope (or null).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) act_kernel(const T *z, const T *__restrict__ residual,
-                                                       T *y, int act, int64_t total, bool wide, int64_t first) {  // y: z, or apart
+__global__ void __launch_bounds__(kThreads) act_kernel(T *__restrict__ y, const T *__restrict__ residual,
+                                                       T *__restrict__ slope, int act, int64_t total, bool wide, int64_t first) {
   constexpr int V = 16 / sizeof(T);
   const int64_t i = ((first + blockIdx.x) * kThreads + threadIdx.x) * V;
   if (i >= total) return;
-  auto one = [&](float v, float r) __attribute__((always_inline)) { return static_cast<T>(activate<T>(v, act) + r); };
   if (wide && i + V <= total) {
-    const Vec<T, V> v = load_vec<T, V>(z + i);
-    Vec<T, V> r{}, o;
+    Vec<T, V> v = load_vec<T, V>(y + i), r{}, d;
     if (residual != nullptr) r = load_vec<T, V>(residual + i);
 #pragma unroll
-    for (int e = 0; e < V; ++e) o.v[e] = one((float)v.v[e], (float)r.v[e]);
-    store_vec<T, V>(y + i, o);
+    for (int e = 0; e < V; ++e) {
+      float s;
+      v.v[e] = static_cast<T>(activate<T>((float)v.v[e], act, s) + (float)r.v[e]);
+      d.v[e] = keep_slope<T>(s, act);
+    }
+    store_vec<T, V>(y + i, v);
+    if (slope != nullptr) store_vec<T, V>(slope + i, d);
   } else {
-    for (int64_t k = i; k < min(i + V, total); ++k) y[k] = one((float)z[k], residual != nullptr ? (float)residual[k] : 0.f);
+    for (int64_t k = i; k < min(i + V, total); ++k) {
+      float s;
+      y[k] = static_cast<T>(activate<T>((float)y[k], act, s) + (residual != nullptr ? (float)residual[k] : 0.f));
+      if (slope != nullptr) slope[k] = keep_slope<T>(s, act);
+    }
   }
 }
 
-// out = act(x W^T + bias) + residual and z as Epilogue has them; workspace: f32_split_weight_bytes.
+// act(x W^T + bias) + residual as Epilogue has them; workspace: f32_split_weight_bytes.
 hipError_t launch_split(const float *x, const float *weight, bool transposed, int64_t M, int N, int K, const Epilogue &e,
                         void *workspace, hipStream_t stream) {
   hipError_t err = transposed ? launch_f32_split_weight(weight, K, N, 1, true, workspace, stream)
                               : launch_f32_split_weight(weight, N, K, 1, false, workspace, stream);
   if (err != hipSuccess) return err;
-  const bool relu = e.act == kActRelu && e.residual == nullptr && e.z == nullptr;
+  const bool relu = e.act == kActRelu && e.residual == nullptr && e.slope == nullptr;
   const bool pass = e.act != kActNone && !relu;  // act(z) + residual in a pass of its own
-  float *out = static_cast<float *>(pass && e.z != nullptr ? e.z : e.y);
+  float *out = static_cast<float *>(e.y);
   const float *addend = pass ? nullptr : static_cast<const float *>(e.residual);
   const int64_t most = ((1LL << 31) - 4096) / ((int64_t)K * 4) / 16 * 16;  // rows below 2 GiB
   for (int64_t m = 0; m < M; m += most) {
@@ -796,19 +833,19 @@ hipError_t launch_split(const float *x, const float *weight, bool transposed, in
   const int64_t total = M * N;
   return launch_in_parts((total + kThreads * 4 - 1) / (kThreads * 4), kThreads, [&](int64_t first, unsigned n) {
     hipLaunchKernelGGL((act_kernel<float>), dim3(n), dim3(kThreads), 0, stream, out, static_cast<const float *>(e.residual),
-                       static_cast<float *>(e.y), e.act, total, on_16({out, e.residual, e.y}), first);
+                       static_cast<float *>(e.slope), e.act, total, on_16({out, e.residual, e.slope}), first);
   });
 }
 
 // ---------------------------------------------------------------------------------------
-// gz = gy act'(z) and its column sums: a workgroup takes a range of rows of up to 256 vectors of
-// columns; each thread keeps its columns' sums, the workgroup adds up its rows side by side and
-// total_kernel the workgroups, in order.
+// gz = gy slope and its column sums: a workgroup takes a range of rows of up to 256 vectors of columns;
+// each thread keeps its columns' sums, the workgroup adds up its rows side by side and turn_kernel the
+// workgroups, in order; in the same launch it turns the weight for the gradient of x.
 // ---------------------------------------------------------------------------------------
-constexpr int kSumBlocks = 512;
+constexpr int kSumBlocks = 1024;
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ gy, const T *__restrict__ z,
+__global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ gy, const T *__restrict__ slope,
                                                           T *__restrict__ gz, int act, int64_t rows, int n, int per,
                                                           float *__restrict__ part) {
   __shared__ float s[kThreads][V + 1];
@@ -818,14 +855,17 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
 #pragma unroll
   for (int e = 0; e < V; ++e) a[e] = 0.f;
   if (row < lanes && col < n) {
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t r = r0 + row; r < r1; r += lanes) {
       const int64_t at = r * n + col;
       Vec<T, V> g = load_vec<T, V>(gy + at);
       if (act != kActNone) {
-        const Vec<T, V> x = load_vec<T, V>(z + at);
+        const Vec<T, V> x = load_vec<T, V>(slope + at);
 #pragma unroll
-        for (int e = 0; e < V; ++e) g.v[e] = static_cast<T>((float)g.v[e] * slope<T>((float)x.v[e], act));
+        for (int e = 0; e < V; ++e) {
+          if (act == kActRelu) g.v[e] = (float)x.v[e] > 0.f ? g.v[e] : static_cast<T>(0.f);  // (slope, or y)
+          else g.v[e] = static_cast<T>((float)g.v[e] * kept_slope(x.v[e]));
+        }
         store_vec<T, V>(gz + at, g);
       }
 #pragma unroll
@@ -844,43 +884,75 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
   for (int e = 0; e < V; ++e) part[(int64_t)blockIdx.x * n + col + e] = a[e];
 }
 
-// 16 columns: 64 threads add up every 64th part each, then in order.
-template <typename O>
-__global__ void __launch_bounds__(1024) total_kernel(const float *__restrict__ part, int parts, int n, O *__restrict__ out) {
+// The first `sums` workgroups: 16 columns each, 64 threads add up every 64th part, then in order. The others:
+// 64 x 64 values of weight [rows][cols] into turned [cols][rows].
+struct TurnArgs {
+  const float *part;
+  int parts, n, sums;
+  void *out;
+  const void *weight;
+  void *turned;
+  int rows, cols;
+};
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p) {
   __shared__ float s[64][17];
-  const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
-  float v = 0.f;
-  if (c < n)
+  __shared__ T tile[64][65];
+  if ((int)blockIdx.x < p.sums) {
+    const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
+    float v = 0.f;
+    if (c < p.n)
 #pragma unroll 8
-    for (int q = k; q < parts; q += 64) v += part[(int64_t)q * n + c];
-  s[k][threadIdx.x % 16] = v;
-  __syncthreads();
-  for (int half = 32; half > 0; half /= 2) {
-    if (k < half) s[k][threadIdx.x % 16] += s[k + half][threadIdx.x % 16];
+      for (int q = k; q < p.parts; q += 64) v += p.part[(int64_t)q * p.n + c];
+    s[k][threadIdx.x % 16] = v;
     __syncthreads();
+    for (int half = 32; half > 0; half /= 2) {
+      if (k < half) s[k][threadIdx.x % 16] += s[k + half][threadIdx.x % 16];
+      __syncthreads();
+    }
+    if (k == 0 && c < p.n) {
+      if (WIDE) static_cast<float *>(p.out)[c] = s[0][threadIdx.x];
+      else static_cast<T *>(p.out)[c] = static_cast<T>(s[0][threadIdx.x]);
+    }
+    return;
   }
-  if (k == 0 && c < n) out[c] = static_cast<O>(s[0][threadIdx.x]);
+  const int across = (p.cols + 63) / 64, tile_at = (int)blockIdx.x - p.sums;
+  const int r0 = tile_at / across * 64, c0 = tile_at % across * 64, lane = threadIdx.x % 64;
+  const T *w = static_cast<const T *>(p.weight);
+  T *t = static_cast<T *>(p.turned);
+#pragma unroll
+  for (int i = threadIdx.x / 64; i < 64; i += 16)
+    if (r0 + i < p.rows && c0 + lane < p.cols) tile[i][lane] = w[(int64_t)(r0 + i) * p.cols + c0 + lane];
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x / 64; i < 64; i += 16)
+    if (c0 + i < p.cols && r0 + lane < p.rows) t[(int64_t)(c0 + i) * p.rows + r0 + lane] = tile[lane][i];
 }
 
 int sum_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(kSumBlocks, rows / 16)); }
 
 template <typename T, int V>
-hipError_t launch_grad_z_v(const T *gy, const T *z, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
+hipError_t launch_grad_z_v(const T *gy, const T *slope, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   const int vecs = (n + V - 1) / V, per = std::min(vecs, kThreads);
   hipLaunchKernelGGL((grad_z_kernel<T, V>), dim3(sum_blocks(rows), (vecs + per - 1) / per), dim3(kThreads), 0, stream,
-                     gy, z, gz, act, rows, n, per, part);
+                     gy, slope, gz, act, rows, n, per, part);
   return hipGetLastError();
 }
 template <typename T>
-hipError_t launch_grad_z(const T *gy, const T *z, T *gz, int act, int64_t rows, int n, float *part, void *grad_bias,
-                         bool bias_wide, hipStream_t stream) {
+hipError_t launch_grad_z(const T *gy, const T *slope, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  hipError_t e = n % V == 0 && on_16({gy, z, gz}) ? launch_grad_z_v<T, V>(gy, z, gz, act, rows, n, part, stream)
-                                                  : launch_grad_z_v<T, 1>(gy, z, gz, act, rows, n, part, stream);
-  if (e != hipSuccess || grad_bias == nullptr) return e;
-  const dim3 grid((n + 15) / 16);
-  if (bias_wide) hipLaunchKernelGGL((total_kernel<float>), grid, dim3(1024), 0, stream, part, sum_blocks(rows), n, static_cast<float *>(grad_bias));
-  else hipLaunchKernelGGL((total_kernel<T>), grid, dim3(1024), 0, stream, part, sum_blocks(rows), n, static_cast<T *>(grad_bias));
+  return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<T, V>(gy, slope, gz, act, rows, n, part, stream)
+                                              : launch_grad_z_v<T, 1>(gy, slope, gz, act, rows, n, part, stream);
+}
+// weight null: sums alone; grad_bias null: the weight alone.
+template <typename T>
+hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wide, const LinearArgs &a, bool turn,
+                       void *turned, hipStream_t stream) {
+  const TurnArgs p{part, sum_blocks(rows), a.N, grad_bias != nullptr ? (a.N + 15) / 16 : 0, grad_bias, a.weight, turned, a.N, a.K};
+  const int64_t tiles = turn ? ((a.N + 63) / 64) * (int64_t)((a.K + 63) / 64) : 0, blocks = p.sums + tiles;
+  if (blocks == 0) return hipSuccess;
+  if (wide) hipLaunchKernelGGL((turn_kernel<T, true>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
+  else hipLaunchKernelGGL((turn_kernel<T, false>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -896,25 +968,27 @@ int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t 
   if (transposed) most = std::max(most, up(N * K * (dtype == 0 ? 4 : 2)));
   return most;
 }
+enum Route { kAny, kSplit, kRows };
+template <typename T> Route route(const T *x, const T *weight, bool transposed, int64_t M, int N, int K) {
+  if (sizeof(T) == 4 && split_takes(x, weight, N, K, transposed) && split_pays(M, N, K)) return kSplit;
+  return rows_take(x, transposed ? nullptr : weight, K, sizeof(T)) ? kRows : kAny;
+}
+// transposed: of kRows the workspace holds the weight's transpose already (it is small next to the rows)
 template <typename T>
 hipError_t product(const T *x, const T *weight, bool transposed, int64_t M, int K, const Epilogue &e, void *workspace,
                    hipStream_t stream) {
-  const int N = e.N;
-  if constexpr (sizeof(T) == 4)
-    if (split_takes(x, weight, N, K, transposed) && split_pays(M, N, K))
-      return launch_split(x, weight, transposed, M, N, K, e, workspace, stream);
-  if (!rows_take(x, weight, K, sizeof(T)))
-    return launch_any<T>(x, K, 1, weight, transposed ? 1 : K, transposed ? N : 1, M, K, e, workspace, stream);
-  if (transposed) {  // the weight is small next to the rows: turned once, its rows are dense
-    if (hipError_t err = launch_transpose(sizeof(T), weight, workspace, 1, K, N, stream)) return err;
-    weight = static_cast<const T *>(workspace);
+  switch (route(x, weight, transposed, M, e.N, K)) {
+    case kAny: return launch_any<T>(x, K, 1, weight, transposed ? 1 : K, transposed ? e.N : 1, M, K, e, workspace, stream);
+    case kRows: return launch_rows(x, transposed ? static_cast<const T *>(workspace) : weight, M, K, e, stream);
+    default: break;
   }
-  return launch_rows(x, weight, M, K, e, stream);
+  if constexpr (sizeof(T) == 4) return launch_split(x, weight, transposed, M, e.N, K, e, workspace, stream);
+  return hipErrorInvalidValue;
 }
 
 template <typename T>
-hipError_t forward(const LinearArgs &a, const void *residual, void *y, void *z, void *workspace, hipStream_t stream) {
-  const Epilogue e{a.bias, residual, y, z, a.bias_wide, a.act, a.N};
+hipError_t forward(const LinearArgs &a, const void *residual, void *y, void *slope, void *workspace, hipStream_t stream) {
+  const Epilogue e{a.bias, residual, y, slope, a.bias_wide, a.act, a.N};
   return product(static_cast<const T *>(a.x), static_cast<const T *>(a.weight), false, a.rows, a.K, e, workspace, stream);
 }
 
@@ -939,21 +1013,22 @@ BackWs back_ws(int dtype, const LinearArgs &a) {
 }
 
 template <typename T>
-hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const void *z, void *workspace, void *grad_x,
+hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const void *slope, void *workspace, void *grad_x,
                     void *grad_w, void *grad_b, hipStream_t stream) {
   const BackWs ws = back_ws(dtype, a);
   char *base = static_cast<char *>(workspace);
   const T *gy = static_cast<const T *>(grad_y), *gz = gy, *x = static_cast<const T *>(a.x);
+  const T *weight = static_cast<const T *>(a.weight);
+  float *part = grad_b != nullptr ? reinterpret_cast<float *>(base + ws.part) : nullptr;
   if (a.act != kActNone) gz = reinterpret_cast<T *>(base);
   if (a.act != kActNone || grad_b != nullptr)
-    if (hipError_t e = launch_grad_z<T>(gy, static_cast<const T *>(z), const_cast<T *>(gz), a.act, a.rows, a.N,
-                                        grad_b != nullptr ? reinterpret_cast<float *>(base + ws.part) : nullptr, grad_b,
-                                        a.bias_wide, stream))
+    if (hipError_t e = launch_grad_z<T>(gy, static_cast<const T *>(slope), const_cast<T *>(gz), a.act, a.rows, a.N, part, stream))
       return e;
+  const bool turn = grad_x != nullptr && route(gz, weight, true, a.rows, a.K, a.N) == kRows;
+  if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, turn, base + ws.product, stream)) return e;
   if (grad_x != nullptr) {
     const Epilogue e{nullptr, nullptr, grad_x, nullptr, false, kActNone, a.K};
-    if (hipError_t err = product<T>(gz, static_cast<const T *>(a.weight), true, a.rows, a.N, e, base + ws.product, stream))
-      return err;
+    if (hipError_t err = product<T>(gz, weight, true, a.rows, a.N, e, base + ws.product, stream)) return err;
   }
   if (grad_w == nullptr) return hipSuccess;
   if (weight_grad_takes(dtype, a) && on_16({gz, x}))
@@ -968,23 +1043,23 @@ int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a) {
   return product_bytes(dtype, false, a.rows, a.N, a.K);
 }
 
-hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *z, void *workspace,
+hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *slope, void *workspace,
                                  hipStream_t stream) {
   switch (dtype) {
-    case 0: return forward<float>(a, residual, y, z, workspace, stream);
-    case 1: return forward<f16>(a, residual, y, z, workspace, stream);
-    default: return forward<bf16>(a, residual, y, z, workspace, stream);
+    case 0: return forward<float>(a, residual, y, slope, workspace, stream);
+    case 1: return forward<f16>(a, residual, y, slope, workspace, stream);
+    default: return forward<bf16>(a, residual, y, slope, workspace, stream);
   }
 }
 
 int64_t linear_backward_workspace_bytes(int dtype, const LinearArgs &a) { return back_ws(dtype, a).total; }
 
-hipError_t launch_linear_backward(int dtype, const LinearArgs &a, const void *grad_y, const void *z, void *workspace,
+hipError_t launch_linear_backward(int dtype, const LinearArgs &a, const void *grad_y, const void *slope, void *workspace,
                                   void *grad_x, void *grad_w, void *grad_b, hipStream_t stream) {
   switch (dtype) {
-    case 0: return backward<float>(dtype, a, grad_y, z, workspace, grad_x, grad_w, grad_b, stream);
-    case 1: return backward<f16>(dtype, a, grad_y, z, workspace, grad_x, grad_w, grad_b, stream);
-    default: return backward<bf16>(dtype, a, grad_y, z, workspace, grad_x, grad_w, grad_b, stream);
+    case 0: return backward<float>(dtype, a, grad_y, slope, workspace, grad_x, grad_w, grad_b, stream);
+    case 1: return backward<f16>(dtype, a, grad_y, slope, workspace, grad_x, grad_w, grad_b, stream);
+    default: return backward<bf16>(dtype, a, grad_y, slope, workspace, grad_x, grad_w, grad_b, stream);
   }
 }
 

@@ -28,18 +28,18 @@ class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
         x, weight, bias = _dense(x), _dense(weight), _dense(bias)
-        y, z, ctx.sizes = _ext().linear_forward(x, weight, bias, act, _dense(residual), True)
-        ctx.save_for_backward(x, weight, bias, z)
+        y, slope, ctx.sizes = _ext().linear_forward(x, weight, bias, act, _dense(residual), True)
+        ctx.save_for_backward(x, weight, bias, slope)
         return y
 
     @staticmethod
     @_b.once_differentiable
     def backward(ctx, grad_y):
-        x, weight, bias, z = ctx.saved_tensors
+        x, weight, bias, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         grads = (None, None, None)
         if any(need[:3]):
-            grads = _ext().linear_backward(_dense(grad_y), x, weight, bias, z, ctx.sizes, need[:3])
+            grads = _ext().linear_backward(_dense(grad_y), x, weight, bias, slope, ctx.sizes, need[:3])
         return (*grads, None, grad_y if need[4] else None)
 
 
@@ -47,8 +47,8 @@ def linear_act(x, weight, bias=None, act=None, residual=None):
     """act(x @ weight.T + bias) + residual: x [..., K], weight [N, K], bias [N] in the input's type or
     float32 (or None), residual [..., N] (or None) -> [..., N]. fp32 / fp16 / bf16. act None, "relu",
     "silu" or "gelu" (z times the normal distribution below z, as torch's default). Everything behind the
-    product is in fp32 and rounded once. SiLU and GELU, and ReLU with a residual, keep z in the
-    input's type for the backward. Differentiable once, in reverse mode; the same results on every run."""
+    product is in fp32 and rounded once. SiLU and GELU, and ReLU with a residual, keep their
+    derivative in the input's type for the backward. Differentiable once, in reverse mode; the same results on every run."""
     if _b.records_nothing():  # (without the bookkeeping of a Function)
         return _ext().linear_forward(_dense(x), _dense(weight), _dense(bias), act, _dense(residual))[0]
     return LinearActFunction.apply(x, weight, bias, act, residual)

@@ -611,11 +611,13 @@ int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_
  *   bias         [out_features] bias_dtype (dtype or F32), or NULL
  *   act          0: none, 1: ReLU, 2: SiLU (z / (1 + exp(-z))), 3: GELU (z times the normal
  *                distribution below z)
- *   z            [rows, out_features] z rounded to dtype, for the backward; or NULL
- * Sums, bias, activation and residual in fp32, rounded once. The backward takes z (for ReLU anything
- * of z's sign, such as y where there is no residual; not read for act 0), and writes grad_x, grad_weight
- * (dtype) and grad_bias (bias_dtype), each NULL where it is not wanted; gz = grad_y act'(z) is rounded to
- * dtype, ReLU's derivative at 0 is 0. The residual's gradient is grad_y. The same results on every
+ *   slope        [rows, out_features] act'(z) for the backward, or NULL; as wide as dtype: F32, and for
+ *                ReLU dtype, as it is, else whole numbers u of 16 bits, act'(z) = u / 32768 - 0.25
+ *                (65535: NaN). Not written for act 0
+ * Sums, bias, activation and residual in fp32, rounded once. The backward takes slope (for ReLU anything
+ * that is positive where z is, such as y where there is no residual; not read for act 0), and
+ * writes grad_x, grad_weight (dtype) and grad_bias (bias_dtype), each NULL where it is not wanted;
+ * gz = grad_y slope is rounded to dtype, ReLU's derivative at 0 is 0. The residual's gradient is grad_y. The same results on every
  * run. dtype F32, F16, BF16; features at most 2^24, rows less than 2^31 - 256, no size may be 0 and
  * no tensor have more than 2^40 values. The workspace (16-byte aligned) holds what
  * bevk_linear_workspace_bytes says (-1 for sizes not taken). */
@@ -624,9 +626,9 @@ int64_t bevk_linear_workspace_bytes(int dtype, int backward, int64_t rows, int i
 int bevk_linear_forward(int dtype, const void *x, const void *weight, const void *bias,
                         int bias_dtype, const void *residual, int64_t rows, int in_features,
                         int out_features, int act, void *workspace, int64_t workspace_bytes, void *y,
-                        void *z, void *stream);
+                        void *slope, void *stream);
 int bevk_linear_backward(int dtype, const void *grad_y, const void *x, const void *weight,
-                         const void *z, int64_t rows, int in_features, int out_features, int act,
+                         const void *slope, int64_t rows, int in_features, int out_features, int act,
                          int bias_dtype, void *workspace, int64_t workspace_bytes, void *grad_x,
                          void *grad_weight, void *grad_bias, void *stream);
 

@@ -7,9 +7,9 @@ shallower), with S the sum of the terms' magnitudes:
   z   (D + 4) u S + 2 u |z|
   y   slopes are below 1.13; SiLU and GELU evaluated to (16 + |z|) u |y|, GELU in 16 bits to
       1.5e-7 |z| more (the polynomial's own error is half of that); the residual's sum u; then e |y|
-  gz  the slope at the z that is kept, e |z| + z's error off, with second derivatives below 0.8; evaluated
-      to 32 u (1 + |z|) (16 bits: 3e-7 more); anything where ReLU's z is within its error of 0; then e |gz|
-      where there is an activation
+  gz  the slope is off by z's error times second derivatives below 0.8, evaluated to 32 u (1 + |z|)
+      (16 bits: 3e-7 more) and kept with 2^-16 more in 16 bits; anything where ReLU's z is within its error of 0;
+      then e |gz| where there is an activation
   gx, gW, gbias   sums of gz as above, over N, the rows, the rows; then e"""
 import pytest
 import torch
@@ -47,7 +47,6 @@ class Reference:
         self.z = x @ w.t() + (0 if t["bias"] is None else t["bias"].double())
         z_err = deep(x.shape[1]) * (x.abs() @ w.abs().t()) + 2 * U * self.z.abs()
         z, coarse = self.z, 0 if dtype == torch.float32 else 1.5e-7
-        kept = z_err + half * z.abs()
         if act is None:
             y, s, s_err = z, torch.ones_like(z), torch.zeros_like(z)
         elif act == "relu":
@@ -56,11 +55,13 @@ class Reference:
         elif act == "silu":
             p = 1 / (1 + torch.exp(-z))
             y, s = z * p, p * (1 + z * (1 - p))
-            s_err = 0.8 * kept + 32 * U * (1 + z.abs())
+            s_err = 0.8 * z_err + 32 * U * (1 + z.abs())
         else:
             cdf = torch.special.ndtr(z)
             y, s = z * cdf, cdf + z * torch.exp(-z * z / 2) * (2 * torch.pi) ** -0.5
-            s_err = 0.8 * kept + 32 * U * (1 + z.abs()) + 2 * coarse
+            s_err = 0.8 * z_err + 32 * U * (1 + z.abs()) + 2 * coarse
+        if act in ("silu", "gelu") and dtype != torch.float32:
+            s_err = s_err + 2.0 ** -16
         self.y_err = 1.13 * z_err + (0 if act in (None, "relu") else (16 + z.abs()) * U * y.abs()
                                      + coarse * z.abs())
         if t["residual"] is not None:
