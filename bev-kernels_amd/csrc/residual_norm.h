@@ -50,9 +50,9 @@ __device__ __forceinline__ void row_sums(float (&x)[N], float *s, int &turn) {
 }
 
 // Mean (0 for rms) and 1 / spread over the row of each of N tensors whose values are in registers, in the
-// same sums; the variance about the mean.
+// same sums (inv: 1 / channels); the variance about the mean. Values past the row's end are 0; `full`: there are none.
 template <int TPR, int THREADS, int N, int L, int V>
-__device__ __forceinline__ void row_moments(float (*const (&v)[N])[V], const bool (&in)[L], bool rms, int channels,
+__device__ __forceinline__ void row_moments(float (*const (&v)[N])[V], const bool (&in)[L], bool rms, float inv,
                                             float eps, float (&mean)[N], float (&rstd)[N], float *s, int &turn) {
   float t[N];
 #pragma unroll
@@ -63,25 +63,28 @@ __device__ __forceinline__ void row_moments(float (*const (&v)[N])[V], const boo
 #pragma unroll
       for (int l = 0; l < L; ++l)
 #pragma unroll
-        for (int e = 0; e < V; ++e) t[n] += in[l] ? v[n][l][e] : 0.f;
+        for (int e = 0; e < V; ++e) t[n] += v[n][l][e];
     row_sums<TPR, THREADS, N>(t, s, turn);
 #pragma unroll
-    for (int n = 0; n < N; ++n) mean[n] = t[n] / (float)channels;
+    for (int n = 0; n < N; ++n) mean[n] = t[n] * inv;
   }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     t[n] = 0.f;
 #pragma unroll
-    for (int l = 0; l < L; ++l)
+    for (int l = 0; l < L; ++l) {
+      float q = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float d = in[l] ? v[n][l][e] - mean[n] : 0.f;
-        t[n] = __builtin_fmaf(d, d, t[n]);
+        const float d = v[n][l][e] - mean[n];
+        q = __builtin_fmaf(d, d, q);
       }
+      t[n] += in[l] ? q : 0.f;
+    }
   }
   row_sums<TPR, THREADS, N>(t, s, turn);
 #pragma unroll
-  for (int n = 0; n < N; ++n) rstd[n] = 1.f / sqrtf(t[n] / (float)channels + eps);
+  for (int n = 0; n < N; ++n) rstd[n] = __builtin_amdgcn_rsqf(__builtin_fmaf(t[n], inv, eps));
 }
 
 template <typename T, int V>

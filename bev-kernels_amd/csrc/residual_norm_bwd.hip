@@ -18,20 +18,29 @@ namespace bevk {
 namespace {
 using namespace rnorm;
 
-constexpr int kParts = 1024;  // workgroups at most
+// Workgroups on the chip at a time: what a thread keeps leaves room for two or three waves a SIMD.
+constexpr int parts_at_most(int tpr) { return tpr <= 64 ? 768 : 512 * 256 / threads_of(tpr); }
+
+template <typename T, int V>
+__device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t r, uint32_t off, const Vec<T, V> &y) {
+  typedef int int4v __attribute__((ext_vector_type(4)));
+  if constexpr (sizeof(y) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(int4v, y), r, off, 0, 0);
+  else if constexpr (sizeof(y) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), r, off, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, y), r, off, 0, 0);
+}
 
 // Workgroup k: `per` parts of a set (sets split), or whole sets (per == 1).
 struct Split {
   int64_t sets, set_rows;
   int per, blocks;
 };
-Split split_of(const ResidualNormArgs &a, int rows_a_block) {
+Split split_of(const ResidualNormArgs &a, int rows_a_block, int64_t most_blocks) {
   Split s;
   s.set_rows = a.set_rows > 0 ? a.set_rows : a.rows;
   s.sets = a.rows / s.set_rows;
   const int64_t most = std::max<int64_t>(1, s.set_rows / (rows_a_block * 2));  // two rows a thread at least
-  s.per = (int)std::max<int64_t>(1, std::min<int64_t>(kParts / std::min<int64_t>(s.sets, kParts), most));
-  s.blocks = (int)(s.per > 1 ? s.sets * s.per : std::min<int64_t>(s.sets, kParts));
+  s.per = (int)std::max<int64_t>(1, std::min<int64_t>(most_blocks / std::min(s.sets, most_blocks), most));
+  s.blocks = (int)(s.per > 1 ? s.sets * s.per : std::min(s.sets, most_blocks));
   return s;
 }
 
@@ -59,6 +68,42 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
     for (int l = 0; l < L; ++l)
 #pragma unroll
       for (int e = 0; e < V; ++e) sum[n][l][e] = 0.f;
+  // Rows from r on through a buffer that ends with the part's rows or 2 GiB on, and at nothing where there is no
+  // such tensor: past that a load gives zeros and a store does nothing. So nothing branches around them, and
+  // the next row's loads stay in flight over this row's stores, which count as they do.
+  auto left = [&](int64_t r, int64_t r1) __attribute__((always_inline)) {
+    return (uint32_t)min((r1 - r) * a.channels * (int64_t)sizeof(T), (int64_t)1 << 31);
+  };
+  uint32_t off[L];
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    const int c = (l * TPR + j) * V;
+    off[l] = c < a.channels ? (uint32_t)(group * a.channels + c) * sizeof(T) : 0xffffff00u;
+  }
+  Vec<T, V> next[4][L];
+  auto load = [&](int64_t r, int64_t r1) __attribute__((always_inline)) {
+    const uint32_t bytes = left(r, r1);
+    const void *from[4] = {g.grad_y, g.h, g.grad_h, a.x};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const __amdgpu_buffer_rsrc_t b = make_rsrc(static_cast<const T *>(from[n]) + r * a.channels, from[n] != nullptr ? bytes : 0);
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        if constexpr (V == 1) next[n][l].v[0] = buffer_load_one<T>(b, off[l]);
+        else next[n][l] = buffer_load_vec<T, V>(b, off[l]);
+      }
+    }
+  };
+  auto store = [&](void *to, int64_t r, uint32_t bytes, const float (&v)[L][V]) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t b = make_rsrc(static_cast<T *>(to) + r * a.channels, to != nullptr ? bytes : 0);
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      Vec<T, V> y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) y.v[e] = static_cast<T>(v[l][e]);
+      buffer_store(b, off[l], y);
+    }
+  };
   // the workgroup's sum of one parameter's parts, in the order of its rows
   auto write = [&](float (&x)[L][V], float *to) __attribute__((always_inline)) {
     if constexpr (R > 1) {
@@ -85,42 +130,55 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
     }
   };
   const float inv = 1.f / (float)a.channels;
+  // the parameters stay in registers: read again for each row they came late, in the middle of its sums
+  float w[L][V], gate[L][V], bw[BLOCK ? L : 1][V], bb[BLOCK ? L : 1][V];
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    const int c = (l * TPR + j) * V;
+    if (c >= a.channels) continue;
+    load_param<T, V>(a.weight, a.wide, c, 1.f, w[l]);
+    if constexpr (BLOCK) {
+      load_param<T, V>(a.block_weight, a.wide, c, 1.f, bw[l]);
+      load_param<T, V>(a.block_bias, a.wide, c, 0.f, bb[l]);
+    }
+  }
   for (int64_t set = set0; set < set1; ++set) {
     const int64_t r0 = set * sp.set_rows + sp.set_rows * part / sp.per;
     const int64_t r1 = set * sp.set_rows + sp.set_rows * (part + 1) / sp.per;
+    const int64_t gate_at = a.set_rows > 0 ? set * a.channels : 0;
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+      if ((l * TPR + j) * V < a.channels) load_param<T, V>(a.gate, a.gate_wide, gate_at + (l * TPR + j) * V, 1.f, gate[l]);
+    load(r0, r1);
     for (int64_t r = r0; r < r1; r += R) {
-      const int64_t row = r + group, at = row * a.channels;
-      const bool there = row < r1;
       float gy[L][V], h[L][V], x[L][V], gs[L][V];
       bool in[L];
 #pragma unroll
       for (int l = 0; l < L; ++l) {
-        const int c = (l * TPR + j) * V;
-        in[l] = there && c < a.channels;
+        in[l] = r + group < r1 && (l * TPR + j) * V < a.channels;
 #pragma unroll
-        for (int e = 0; e < V; ++e) gy[l][e] = h[l][e] = x[l][e] = gs[l][e] = 0.f;
-        if (in[l]) {
-          load_row<T, V>(static_cast<const T *>(g.grad_y) + at + c, gy[l]);
-          load_row<T, V>(static_cast<const T *>(g.h) + at + c, h[l]);
-          if (g.grad_h != nullptr) load_row<T, V>(static_cast<const T *>(g.grad_h) + at + c, gs[l]);
-          if (a.x != nullptr) load_row<T, V>(static_cast<const T *>(a.x) + at + c, x[l]);
+        for (int e = 0; e < V; ++e) {
+          gy[l][e] = (float)next[0][l].v[e];
+          h[l][e] = (float)next[1][l].v[e];
+          gs[l][e] = (float)next[2][l].v[e];
+          x[l][e] = (float)next[3][l].v[e];
         }
       }
+      const uint32_t here = left(r, r1);
+      load(min(r + R, r1), r1);
       float mean[N == 5 ? 2 : 1], rstd[N == 5 ? 2 : 1], t[2] = {0.f, 0.f};
-      if constexpr (BLOCK) row_moments<TPR, THREADS, 2, L, V>({h, x}, in, a.rms, a.channels, a.eps, mean, rstd, s, turn);
-      else row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, a.channels, a.eps, mean, rstd, s, turn);
+      if constexpr (BLOCK) row_moments<TPR, THREADS, 2, L, V>({h, x}, in, a.rms, inv, a.eps, mean, rstd, s, turn);
+      else row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, inv, a.eps, mean, rstd, s, turn);
 #pragma unroll
       for (int l = 0; l < L; ++l)
         if (in[l]) {
-          float w[V];
-          load_param<T, V>(a.weight, a.wide, (l * TPR + j) * V, 1.f, w);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float hh = (h[l][e] - mean[0]) * rstd[0];
             sum[1][l][e] = __builtin_fmaf(gy[l][e], hh, sum[1][l][e]);
             sum[2][l][e] += gy[l][e];
             h[l][e] = hh;
-            gy[l][e] *= w[e];
+            gy[l][e] *= w[l][e];
             t[0] += gy[l][e];
             t[1] = __builtin_fmaf(gy[l][e], hh, t[1]);
           }
@@ -132,27 +190,20 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
 #pragma unroll
         for (int e = 0; e < V; ++e)
           gs[l][e] = __builtin_fmaf(rstd[0], gy[l][e] - c1 - h[l][e] * c2, gs[l][e]);  // gh
-      const int64_t gate_at = a.set_rows > 0 ? set * a.channels : 0;
       t[0] = t[1] = 0.f;
+      store(g.grad_residual, r, here, gs);
 #pragma unroll
       for (int l = 0; l < L; ++l)
         if (in[l]) {
-          const int c = (l * TPR + j) * V;
-          if (g.grad_residual != nullptr) store_row<T, V>(static_cast<T *>(g.grad_residual) + at + c, gs[l]);
-          float gate[V];
-          load_param<T, V>(a.gate, a.gate_wide, gate_at + c, 1.f, gate);
           if constexpr (BLOCK) {
-            float w[V], b[V];
-            load_param<T, V>(a.block_weight, a.wide, c, 1.f, w);
-            load_param<T, V>(a.block_bias, a.wide, c, 0.f, b);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float ph = (x[l][e] - mean[1]) * rstd[1], gh = a.scale * gs[l][e], gp = gate[e] * gh;
-              sum[0][l][e] = __builtin_fmaf(gh, __builtin_fmaf(ph, w[e], b[e]), sum[0][l][e]);
+              const float ph = (x[l][e] - mean[1]) * rstd[1], gh = a.scale * gs[l][e], gp = gate[l][e] * gh;
+              sum[0][l][e] = __builtin_fmaf(gh, __builtin_fmaf(ph, bw[l][e], bb[l][e]), sum[0][l][e]);
               sum[3][l][e] = __builtin_fmaf(gp, ph, sum[3][l][e]);
               sum[4][l][e] += gp;
               x[l][e] = ph;
-              gs[l][e] = gp * w[e];
+              gs[l][e] = gp * bw[l][e];
               t[0] += gs[l][e];
               t[1] = __builtin_fmaf(gs[l][e], ph, t[1]);
             }
@@ -161,7 +212,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
             for (int e = 0; e < V; ++e) {
               const float gh = a.scale * gs[l][e];
               sum[0][l][e] = __builtin_fmaf(gh, x[l][e], sum[0][l][e]);
-              gs[l][e] = gate[e] * gh;
+              gs[l][e] = gate[l][e] * gh;
             }
           }
         }
@@ -173,10 +224,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
 #pragma unroll
           for (int e = 0; e < V; ++e) gs[l][e] = rstd[1] * (gs[l][e] - d1 - x[l][e] * d2);
       }
-      if (g.grad_x != nullptr)
-#pragma unroll
-        for (int l = 0; l < L; ++l)
-          if (in[l]) store_row<T, V>(static_cast<T *>(g.grad_x) + at + (l * TPR + j) * V, gs[l]);
+      store(g.grad_x, r, here, gs);
     }
     if (parts.gate != nullptr) {
       write(sum[0], parts.gate + (set * sp.per + part) * a.channels);
@@ -331,13 +379,16 @@ __global__ void __launch_bounds__(1024) join_kernel(const Joins all, int which, 
   }
 }
 
-int rows_a_block(int64_t channels, int v) {
+// The split for rows of vectors of v values.
+Split split_for(const ResidualNormArgs &a, int v) {
   int rows = 1;
-  for_row((channels + v - 1) / v, [&](auto tpr, auto) {
+  int64_t blocks = 1024;
+  for_row((a.channels + v - 1) / v, [&](auto tpr, auto) {
     constexpr int TPR = decltype(tpr)::value;
     rows = threads_of(TPR) / TPR;
+    blocks = parts_at_most(TPR);
   });
-  return rows;
+  return split_of(a, rows, blocks);
 }
 
 template <typename T, int V, bool BLOCK>
@@ -357,7 +408,7 @@ template <typename T>
 hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool whole, void *workspace,
                     hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  const Split sp = split_of(a, rows_a_block(a.channels, whole ? V : 1));
+  const Split sp = split_for(a, whole ? V : 1);
   float *ws = static_cast<float *>(workspace);
   Parts parts{};
   Joins joins{};
@@ -401,7 +452,7 @@ bool whole_rows(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g
 int64_t residual_norm_backward_workspace_bytes(int dtype, const ResidualNormArgs &a) {
   int64_t most = 0;  // for either alignment
   for (int v : {dtype == 0 ? 4 : 8, 1}) {
-    const Split sp = split_of(a, rows_a_block(a.channels, v));
+    const Split sp = split_for(a, v);
     most = std::max(most, (4 * (int64_t)sp.blocks + sp.sets * sp.per) * a.channels * 4);
   }
   return most;

@@ -25,6 +25,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) forward_kernel(const Residual
   __shared__ float s[2 * THREADS / 64 * 2];
   int turn = 0;
   const int j = threadIdx.x % TPR;
+  const float inv = 1.f / (float)a.channels;
   const int64_t row = (first + blockIdx.x) * R + threadIdx.x / TPR;
   const bool there = row < a.rows;
   const int64_t at = row * a.channels;
@@ -44,7 +45,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) forward_kernel(const Residual
   }
   auto moments = [&](float &mean, float &rstd) __attribute__((always_inline)) {
     float m[1], q[1];
-    row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, a.channels, a.eps, m, q, s, turn);
+    row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, inv, a.eps, m, q, s, turn);
     mean = m[0];
     rstd = q[0];
   };
