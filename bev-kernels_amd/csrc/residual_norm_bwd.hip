@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
   // such tensor: past that a load gives zeros and a store does nothing. So nothing branches around them, and
   // the next row's loads stay in flight over this row's stores, which count as they do.
   auto left = [&](int64_t r, int64_t r1) __attribute__((always_inline)) {
-    return (uint32_t)min((r1 - r) * a.channels * (int64_t)sizeof(T), (int64_t)1 << 31);
+    const int64_t bytes = (r1 - r) * a.channels * (int64_t)sizeof(T);
+    return bytes < (int64_t)1 << 31 ? (uint32_t)bytes : 1u << 31;
   };
   uint32_t off[L];
 #pragma unroll
@@ -354,11 +355,12 @@ struct Joins {
 
 // 16 channels of one output row: 64 threads add up every 64th part each, then in order.
 template <typename T>
-__global__ void __launch_bounds__(1024) join_kernel(const Joins all, int which, int64_t first) {
+__global__ void __launch_bounds__(1024) join_kernel(const Joins all, int64_t first) {
   __shared__ float s[64][17];
-  const Join &j = all.of[which + blockIdx.y];
   const int64_t tiles = (all.channels + 15) / 16, at = first + blockIdx.x;
-  const int64_t row = at / tiles;
+  const int which = (int)min(at / tiles, (int64_t)all.count - 1);  // the last one may have several rows
+  const Join &j = all.of[which];
+  const int64_t row = at / tiles - which;
   const int c = (int)(at % tiles) * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
   float v = 0.f;
   if (row < j.rows && c < all.channels) {
@@ -420,25 +422,18 @@ hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool 
     joins.of[joins.count++] = Join{ws, to[n], sp.blocks, 1, a.wide};
     ws += (int64_t)sp.blocks * a.channels;
   }
-  const int small = joins.count;
+  int64_t rows = joins.count;  // output rows of all
   if (g.grad_gate != nullptr) {
     parts.gate = ws;
     joins.of[joins.count++] = Join{ws, g.grad_gate, sp.per, sp.sets, a.gate_wide};
+    rows += sp.sets;
   }
   hipError_t e;
   if (whole) e = a.block ? launch_v<T, V, true>(a, g, sp, parts, stream) : launch_v<T, V, false>(a, g, sp, parts, stream);
   else e = a.block ? launch_v<T, 1, true>(a, g, sp, parts, stream) : launch_v<T, 1, false>(a, g, sp, parts, stream);
   if (e != hipSuccess) return e;
-  const int64_t tiles = (a.channels + 15) / 16;
-  const bool one = sp.sets == 1 || parts.gate == nullptr;  // all of them have one output row
-  const int n = one ? joins.count : small;
-  if (n > 0) {
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)tiles, n), dim3(1024), 0, stream, joins, 0, (int64_t)0);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-  }
-  if (one) return hipSuccess;
-  return launch_in_parts(tiles * sp.sets, 1024, [&](int64_t first, unsigned blocks) {
-    hipLaunchKernelGGL((join_kernel<T>), dim3(blocks, 1), dim3(1024), 0, stream, joins, small, first);
+  return launch_in_parts((a.channels + 15) / 16 * rows, 1024, [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL((join_kernel<T>), dim3(blocks), dim3(1024), 0, stream, joins, first);
   });
 }
 
