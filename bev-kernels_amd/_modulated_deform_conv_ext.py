@@ -1465,7 +1465,7 @@ def residual_norm_backward(grad_y, grad_stream, stream, x, weight, bias, gate, s
     grad_r = new(stream) if wanted[1] or (alike and wanted[0]) else None
     grad_x = grad_r if alike else new(stream) if wanted[0] else None
     out = [new(p) if want and p is not None else None
-           for want, p in zip(wanted[2:], (weight, bias, gate, bw, bb))]
+           for want, p in zip(wanted[2:7], (weight, bias, gate, bw, bb))]
     if rows:
         nbytes = _residual_norm_workspace_bytes(code, rows, set_rows, channels)
         ws = stream.new_empty(nbytes, dtype=torch.uint8)

@@ -27,8 +27,7 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        x, weight, bias = _dense(x), _dense(weight), _dense(bias)
-        y, slope, ctx.sizes = _ext().linear_forward(x, weight, bias, act, _dense(residual), True)
+        y, slope, ctx.sizes = _ext().linear_forward(x, weight, bias, act, residual, True)
         ctx.save_for_backward(x, weight, bias, slope)
         return y
 
@@ -49,6 +48,7 @@ def linear_act(x, weight, bias=None, act=None, residual=None):
     "silu" or "gelu" (z times the normal distribution below z, as torch's default). Everything behind the
     product is in fp32 and rounded once. SiLU and GELU, and ReLU with a residual, keep their
     derivative in the input's type for the backward. Differentiable once, in reverse mode; the same results on every run."""
+    x, weight, bias, residual = _dense(x), _dense(weight), _dense(bias), _dense(residual)
     if _b.records_nothing():  # (without the bookkeeping of a Function)
-        return _ext().linear_forward(_dense(x), _dense(weight), _dense(bias), act, _dense(residual))[0]
+        return _ext().linear_forward(x, weight, bias, act, residual)[0]
     return LinearActFunction.apply(x, weight, bias, act, residual)

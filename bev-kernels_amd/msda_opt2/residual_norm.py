@@ -27,13 +27,11 @@ class ResidualNormFunction(torch.autograd.Function):
     """(y, stream) of residual_norm; gradients flow to all tensors."""
 
     @staticmethod
-    def forward(ctx, x, residual, weight, bias, gate, block_weight, block_bias, scale, block_norm, kind, eps,
-                with_stream):
-        x, residual, weight, bias, gate, block_weight, block_bias = map(
-            _dense, (x, residual, weight, bias, gate, block_weight, block_bias))
-        block = (block_weight, block_bias) if block_norm else None
-        y, h, ctx.sizes = _ext().residual_norm_forward(x, residual, weight, bias, gate, scale, block, kind, eps)
-        ctx.args = scale, block_norm, eps
+    def forward(ctx, x, residual, weight, bias, gate, block_weight, block_bias, options):
+        scale, block_norm, kind, eps, with_stream = options
+        y, h, ctx.sizes = _ext().residual_norm_forward(
+            x, residual, weight, bias, gate, scale, (block_weight, block_bias) if block_norm else None, kind, eps)
+        ctx.options = options
         # (x is read again for its norm and for the gate's gradient alone)
         ctx.save_for_backward(x if block_norm or gate is not None else None, h, weight, bias, gate, block_weight,
                               block_bias)
@@ -44,15 +42,15 @@ class ResidualNormFunction(torch.autograd.Function):
     @_b.once_differentiable
     def backward(ctx, grad_y, grad_stream=None):
         x, h, weight, bias, gate, bw, bb = ctx.saved_tensors
-        scale, block_norm, eps = ctx.args
+        scale, block_norm, _, eps, _ = ctx.options
         if grad_y is None:
             if grad_stream is None:
-                return (None,) * 12
+                return (None,) * 8
             grad_y = torch.zeros_like(h)
         grads = _ext().residual_norm_backward(_dense(grad_y), _dense(grad_stream), h, x, weight, bias, gate, scale,
                                               (bw, bb) if block_norm else None, eps, ctx.sizes,
-                                              ctx.needs_input_grad[:7])
-        return (*grads, None, None, None, None, None)
+                                              ctx.needs_input_grad)
+        return (*grads, None)
 
 
 def residual_norm(x, residual=None, weight=None, bias=None, gate=None, scale=1.0, block_norm=None, kind="layer",
@@ -70,10 +68,13 @@ def residual_norm(x, residual=None, weight=None, bias=None, gate=None, scale=1.0
     Sums are fp32; y is computed from the stream before its rounding, the gradients from the rounded
     one. Differentiable once, in reverse mode; all gradients are the same on every run."""
     block_weight, block_bias = (None, None) if block_norm is None else block_norm
+    x, residual, weight, bias, gate = _dense(x), _dense(residual), _dense(weight), _dense(bias), _dense(gate)
+    if block_norm is not None:
+        block_weight, block_bias = _dense(block_weight), _dense(block_bias)
     if _b.records_nothing():  # (without the bookkeeping of a Function)
-        y, h, _ = _ext().residual_norm_forward(
-            _dense(x), _dense(residual), _dense(weight), _dense(bias), _dense(gate), scale,
-            None if block_norm is None else (_dense(block_weight), _dense(block_bias)), kind, eps, with_stream)
+        y, h, _ = _ext().residual_norm_forward(x, residual, weight, bias, gate, scale,
+                                               None if block_norm is None else (block_weight, block_bias), kind, eps,
+                                               with_stream)
         return (y, h) if with_stream else y
-    return ResidualNormFunction.apply(x, residual, weight, bias, gate, block_weight, block_bias, scale,
-                                      block_norm is not None, kind, eps, with_stream)
+    return ResidualNormFunction.apply(x, residual, weight, bias, gate, block_weight, block_bias,
+                                      (scale, block_norm is not None, kind, eps, with_stream))
