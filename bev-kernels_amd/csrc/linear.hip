@@ -279,12 +279,12 @@ struct TileArgs {
 };
 
 // Eight neighbouring values of a row.
-template <typename T, int ACT, bool BIAS = true>
+template <typename T, int ACT>
 __device__ __forceinline__ void finish8(const Epilogue &e, int64_t m, int n, float (&v)[8]) {
   const int64_t at = m * e.N + n;
   Vec<T, 8> r;
   if (e.residual != nullptr) r = load_vec<T, 8>(static_cast<const T *>(e.residual) + at);
-  if (BIAS && e.bias != nullptr) {
+  if (e.bias != nullptr) {
     if (e.bias_wide) {
 #pragma unroll
       for (int h = 0; h < 8; h += 4) {
@@ -480,7 +480,47 @@ struct StreamArgs {
   int parts, shares;  // column parts, workgroups of each
 };
 
-template <typename T, int ACT, int K, int NT, int R>
+// act(v) + residual of a few rows of the output, eight neighbouring values (16 bits) or four (fp32) at a byte offset
+// that is past `bytes` where there are none. The residual is loaded ahead (RES).
+template <typename T, bool RES> struct Rows {
+  static constexpr int V = 16 / sizeof(T);
+  __amdgpu_buffer_rsrc_t y, slope, residual;
+  bool with_slope;
+  __device__ __forceinline__ Rows(const Epilogue &e, int64_t row, uint32_t bytes) {
+    const int64_t at = row * e.N;
+    y = make_rsrc(static_cast<const T *>(e.y) + at, bytes);
+    slope = make_rsrc(static_cast<const T *>(e.slope) + at, bytes);
+    residual = make_rsrc(static_cast<const T *>(e.residual) + at, bytes);
+    with_slope = e.slope != nullptr;
+  }
+  __device__ __forceinline__ Vec<T, V> ahead(uint32_t at) const { return buffer_load_vec<T, V>(residual, at); }
+  template <int ACT> __device__ __forceinline__ void finish(uint32_t at, const Vec<T, V> &r, float (&v)[V]) const {
+    Vec<T, V> o;
+    if (ACT != kActNone && with_slope) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float s;
+        v[k] = activate<T>(v[k], ACT, s);
+        o.v[k] = keep_slope<T, ACT>(s);
+      }
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(int4v, o), slope, at, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float s;
+        v[k] = activate<T>(v[k], ACT, s);
+      }
+    }
+    if constexpr (RES)
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] += (float)r.v[k];
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = static_cast<T>(v[k]);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(int4v, o), y, at, 0, 0);
+  }
+};
+
+template <typename T, int ACT, bool RES, int K, int NT, int R>
 __global__ void __launch_bounds__(512) stream_kernel(const StreamArgs p) {
   constexpr int J = NT / 16, G = J / 4, WAVES = 8;
   __shared__ __attribute__((aligned(1024))) char w[NT * K * 2];  // [K / 128][NT][128 terms]
@@ -539,6 +579,20 @@ __global__ void __launch_bounds__(512) stream_kernel(const StreamArgs p) {
   read(0, 0);
   for (; strip < p.strips; strip += step) {
     asm volatile("" ::: "memory");  // (the weight's reads stay in the loop: registers hold no 128 KB)
+    // through buffers that end with the rows: nothing branches around the stores, so that the next rows' loads,
+    // which are sent before them, can be waited for without them
+    const int64_t row = strip * R * 16;
+    const Rows<T, RES> out(p.e, row, (uint32_t)min(p.M - row, (int64_t)R * 16) * (uint32_t)N * 2);
+    auto place = [&](int i, int j) __attribute__((always_inline)) {
+      const int n = n0 + j * 16 + g * 8;
+      return n < N ? (uint32_t)((i * 16 + r16) * N + n) * 2 : 0xffffff00u;
+    };
+    Vec<T, 8> ahead[RES ? R : 1][RES ? J / 2 : 1];
+    if constexpr (RES)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < J; j += 2) ahead[i][j / 2] = out.ahead(place(i, j));
     floatx4 acc[R][J];
 #pragma unroll
     for (int j = 0; j < J; ++j)
@@ -568,21 +622,17 @@ __global__ void __launch_bounds__(512) stream_kernel(const StreamArgs p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int64_t m = (strip * R + i) * 16 + r16;
-      if (m < p.M)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < J; j += 2) {
-          const int n = n0 + j * 16 + g * 8;
-          float v[8];
+      for (int j = 0; j < J; j += 2) {
+        float v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = acc[i][j][e];
-            v[4 + e] = acc[i][j + 1][e];
-          }
-          if (n < N) finish8<T, ACT, false>(p.e, m, n, v);
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[i][j][e];
+          v[4 + e] = acc[i][j + 1][e];
         }
-    }
+        out.template finish<ACT>(place(i, j), ahead[RES ? i : 0][RES ? j / 2 : 0], v);
+      }
   }
 }
 
@@ -593,8 +643,9 @@ hipError_t launch_stream_of(StreamArgs p, hipStream_t stream) {
   const int cus = std::max(8, device_cus());
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(cus / p.parts, (p.strips + 7) / 8));
   with_act(p.e.act, [&](auto act) {
-    hipLaunchKernelGGL((stream_kernel<T, decltype(act)::value, K, NT, R>), dim3((unsigned)((p.shares + 7) / 8 * 8 * p.parts)),
-                       dim3(512), 0, stream, p);
+    const auto kernel = p.e.residual != nullptr ? stream_kernel<T, decltype(act)::value, true, K, NT, R>
+                                                : stream_kernel<T, decltype(act)::value, false, K, NT, R>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.shares + 7) / 8 * 8 * p.parts)), dim3(512), 0, stream, p);
   });
   return hipGetLastError();
 }
