@@ -863,12 +863,159 @@ __global__ void __launch_bounds__(kThreads) act_kernel(T *__restrict__ y, const 
   }
 }
 
+// The streaming kernel for fp32: K 256 or 512, N a multiple of 4. NB x 16 columns of the split weight (its three planes
+// in the order of the fragments, 96 KB) stay in LDS, a wave takes 16 rows at a time, eight steps of 32 terms ahead,
+// and cuts its fragments as they come. A strip that meets a value that is not finite (or rounds to Inf as a bf16) is
+// computed again in plain fp32.
+struct SplitStreamArgs {
+  const float *a;
+  const void *w;  // split weight, then its flags
+  int64_t M, strips;
+  Epilogue e;
+  int parts, shares;
+};
+
+template <int ACT, bool RES, int K>
+__global__ void __launch_bounds__(512) split_stream_kernel(const SplitStreamArgs p) {
+  constexpr int S = K / 32, NB = 32 / S, WAVES = 8, BLOCK = S * 3072;  // S steps; bytes of 16 columns
+  __shared__ __attribute__((aligned(1024))) char w[NB * BLOCK];
+  __shared__ __attribute__((aligned(16))) float bias[NB * 16];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r16 = lane % 16, g = lane / 16, N = p.e.N;
+  const int part = (int)(blockIdx.x / 8) % p.parts, share = (int)(blockIdx.x / 8) / p.parts * 8 + (int)blockIdx.x % 8;
+  if (share >= p.shares) return;
+  const int n0 = part * NB * 16, nb_total = (N + 15) / 16, nb = min(NB, nb_total - part * NB);
+  const int64_t step = (int64_t)p.shares * WAVES;
+  int64_t strip = (int64_t)share * WAVES + wave;
+  const float *at;
+  auto rows_of = [&](int64_t s) __attribute__((always_inline)) { at = p.a + min(s * 16 + r16, p.M - 1) * K + g * 8; };
+  floatx4 a[8][2];
+  auto load = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) a[k % 8][h] = *reinterpret_cast<const floatx4 *>(at + k * 32 + h * 4);
+  };
+  if (strip < p.strips) {
+    rows_of(strip);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) load(k);
+  }
+  {
+    const char *from = static_cast<const char *>(p.w) + (int64_t)part * NB * BLOCK;
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(from, nb * BLOCK);
+#pragma unroll 4
+    for (int i = wave; i < NB * BLOCK / 1024; i += WAVES)  // (columns past the last block: the first block's again)
+      load_to_lds(rb, w + i * 1024, (i * 1024 < nb * BLOCK ? i * 1024 : i * 1024 % BLOCK) + lane * 16, 0);
+  }
+  for (int n = threadIdx.x; n < NB * 16; n += 64 * WAVES) bias[n] = n0 + n < N ? bias_at<float>(p.e, n0 + n) : 0.f;
+  const uint32_t *flags = reinterpret_cast<const uint32_t *>(static_cast<const char *>(p.w) + (int64_t)nb_total * BLOCK) + part * NB * S;
+  bool bad_weight = false;
+  for (int i = threadIdx.x; i < nb * S; i += 64 * WAVES) bad_weight |= flags[i] != 0;
+  bad_weight = __syncthreads_or(bad_weight);
+  if (strip >= p.strips) return;
+  // one block's three fragments are read while the block before multiplies
+  int4v b[2][3];
+  auto read = [&](int unit, int to) __attribute__((always_inline)) {
+    const int j = unit % NB, k = unit / NB % S;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      b[to][q] = *reinterpret_cast<const int4v *>(w + j * BLOCK + k * 3072 + q * 1024 + lane * 16);
+  };
+  read(0, 0);
+  for (; strip < p.strips; strip += step) {
+    asm volatile("" ::: "memory");  // (the weight's reads stay in the loop)
+    const int64_t row = strip * 16;
+    const Rows<float, RES> out(p.e, row, (uint32_t)min(p.M - row, (int64_t)16) * (uint32_t)N * 4);
+    auto place = [&](int j) __attribute__((always_inline)) {
+      const int n = n0 + j * 16 + g * 4;
+      return n < N ? (uint32_t)(r16 * N + n) * 4 : 0xffffff00u;
+    };
+    Vec<float, 4> ahead[RES ? NB : 1];
+    if constexpr (RES)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) ahead[j] = out.ahead(place(j));
+    floatx4 hi[NB] = {}, lo[NB] = {};
+    float nf = 0.f;
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      int4v x[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Cut2 c = cut2(a[k % 8][e / 2][e % 2 * 2], a[k % 8][e / 2][e % 2 * 2 + 1]);
+        x[0][e] = c.h; x[1][e] = c.m; x[2][e] = c.l;
+        nf += c.nf;
+      }
+      if (k + 8 == S) rows_of(min(strip + step, p.strips - 1));
+      load((k + 8) % S);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int unit = k * NB + j;
+        read(unit + 1, (unit + 1) % 2);
+        __builtin_amdgcn_sched_barrier(0);
+        const int4v(&f)[3] = b[unit % 2];
+        lo[j] = mfma16(f[0], x[2], lo[j], bf16());
+        hi[j] = mfma16(f[0], x[0], hi[j], bf16());
+        lo[j] = mfma16(f[2], x[0], lo[j], bf16());
+        lo[j] = mfma16(f[1], x[1], lo[j], bf16());
+        lo[j] = mfma16(f[0], x[1], lo[j], bf16());
+        lo[j] = mfma16(f[1], x[0], lo[j], bf16());
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (__any(bad_weight || !(nf == nf))) {
+      const float *xr = p.a + min(row + r16, p.M - 1) * K;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        floatx4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int k = 0; k < K; ++k) {
+          const char *blk = w + j * BLOCK + k / 32 * 3072 + k % 32 / 8 * 256 + k % 8 * 2 + g * 64;  // column 4 g
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float wv = 0.f;
+#pragma unroll
+            for (int q = 2; q >= 0; --q)
+              wv += __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t *>(blk + q * 1024 + e * 16) << 16);
+            v[e] = __builtin_fmaf(xr[k], wv, v[e]);
+          }
+        }
+        hi[j] = v;
+        lo[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const floatx4 c = *reinterpret_cast<const floatx4 *>(bias + j * 16 + g * 4);
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (hi[j][e] + lo[j][e]) + c[e];
+      out.template finish<ACT>(place(j), ahead[RES ? j : 0], v);
+    }
+  }
+}
+
+template <int K> hipError_t launch_split_stream(SplitStreamArgs p, hipStream_t stream) {
+  p.strips = (p.M + 15) / 16;
+  p.parts = (p.e.N + 16384 / K - 1) / (16384 / K);
+  const int cus = std::max(8, device_cus());
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(cus / p.parts, (p.strips + 7) / 8));
+  with_act(p.e.act, [&](auto act) {
+    const auto kernel = p.e.residual != nullptr ? split_stream_kernel<decltype(act)::value, true, K>
+                                                : split_stream_kernel<decltype(act)::value, false, K>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.shares + 7) / 8 * 8 * p.parts)), dim3(512), 0, stream, p);
+  });
+  return hipGetLastError();
+}
+
 // act(x W^T + bias) + residual as Epilogue has them; workspace: f32_split_weight_bytes.
 hipError_t launch_split(const float *x, const float *weight, bool transposed, int64_t M, int N, int K, const Epilogue &e,
                         void *workspace, hipStream_t stream) {
   hipError_t err = transposed ? launch_f32_split_weight(weight, K, N, 1, true, workspace, stream)
                               : launch_f32_split_weight(weight, N, K, 1, false, workspace, stream);
   if (err != hipSuccess) return err;
+  if ((K == 256 || K == 512) && N % 4 == 0 && on_16({e.residual, e.y, e.slope})) {
+    const SplitStreamArgs p{x, workspace, M, 0, e, 0, 0};
+    return K == 256 ? launch_split_stream<256>(p, stream) : launch_split_stream<512>(p, stream);
+  }
   const bool relu = e.act == kActRelu && e.residual == nullptr && e.slope == nullptr;
   const bool pass = e.act != kActNone && !relu;  // act(z) + residual in a pass of its own
   float *out = static_cast<float *>(e.y);
