@@ -90,10 +90,10 @@ _SIGNATURES = {
     "bevk_linear_forward": [_i, _vp, _vp, _vp, _i, _vp, _i64, _i, _i, _i, _vp, _i64, _vp, _vp, _vp],
     "bevk_linear_backward": [_i, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _i64, _vp, _vp, _vp, _vp],
     "bevk_residual_norm_forward": [_i] + [_vp] * 7 + [_i, _i, _i64, _i64, _i, _i, _i, ctypes.c_float,
-                                                      ctypes.c_float] + [_vp] * 3,
+                                                      ctypes.c_float] + [_vp] * 4,
     "bevk_residual_norm_backward_workspace_bytes": [_i, _i64, _i64, _i],
-    "bevk_residual_norm_backward": [_i] + [_vp] * 8 + [_i, _i, _i64, _i64, _i, _i, _i, ctypes.c_float,
-                                                       ctypes.c_float, _vp, _i64] + [_vp] * 8,
+    "bevk_residual_norm_backward": [_i] + [_vp] * 9 + [_i, _i, _i64, _i64, _i, _i, _i, ctypes.c_float, _vp,
+                                                       _i64] + [_vp] * 8,
     "bevk_adamw_moments": [_vp, _vp, _i, _i64, _i, _vp, _vp],
     "bevk_embedding_forward": [_i, _vp, _i64, _i, _vp, _i, _i64, ctypes.c_float, _vp, _vp],
     "bevk_embedding_backward_workspace_bytes": [_i, _i64, _i64, _i],

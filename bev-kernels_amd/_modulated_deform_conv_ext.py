@@ -1431,19 +1431,22 @@ def _residual_norm_check(fn, x, residual, weight, bias, gate, block, kind):
             0 if block is None else 1)
 
 
-def residual_norm_forward(x, residual, weight, bias, gate, scale, block, kind, eps, with_stream=True):
-    """(y, h or None, sizes): h = residual + scale * gate * p with p = x or, with block = (weight, bias),
-    its norm, and y the norm of h; sizes for residual_norm_backward."""
+def residual_norm_forward(x, residual, weight, bias, gate, scale, block, kind, eps, with_stream=True,
+                          with_stats=False):
+    """(y, h or None, stats or None, sizes): h = residual + scale * gate * p with p = x or, with block =
+    (weight, bias), its norm, and y the norm of h. stats [rows, 2 or 4] float32 and sizes for
+    residual_norm_backward."""
     fn = "residual_norm_forward"
     sizes = _residual_norm_check(fn, x, residual, weight, bias, gate, block, kind)
     y = torch.empty_like(x)
     h = torch.empty_like(x) if with_stream else None
+    stats = x.new_empty((sizes[3], 4 if sizes[7] else 2), dtype=torch.float32) if with_stats else None
     if sizes[3]:
         bw, bb = (None, None) if block is None else block
         ptr = _b.ptr
         _b.call_on(x.get_device(), "bevk_residual_norm_forward", sizes[0], x.data_ptr(), ptr(residual), ptr(weight),
-                   ptr(bias), ptr(gate), ptr(bw), ptr(bb), *sizes[1:], scale, eps, y.data_ptr(), ptr(h))
-    return y, h, sizes
+                   ptr(bias), ptr(gate), ptr(bw), ptr(bb), *sizes[1:], scale, eps, y.data_ptr(), ptr(h), ptr(stats))
+    return y, h, stats, sizes
 
 
 @functools.lru_cache(maxsize=256)
@@ -1454,7 +1457,8 @@ def _residual_norm_workspace_bytes(code, rows, set_rows, channels):
     return nbytes
 
 
-def residual_norm_backward(grad_y, grad_stream, stream, x, weight, bias, gate, scale, block, eps, sizes, wanted):
+def residual_norm_backward(grad_y, grad_stream, x, residual, stats, weight, bias, gate, scale, block, sizes,
+                           wanted):
     """The gradients of residual_norm_forward's x, residual, weight, bias, gate and block's two for grad_y
     and grad_stream (or None); None where `wanted` is false or there is no such input. The
     gradients of x and the residual may be one tensor, where they are equal."""
@@ -1462,17 +1466,17 @@ def residual_norm_backward(grad_y, grad_stream, stream, x, weight, bias, gate, s
     bw, bb = (None, None) if block is None else block
     new = torch.empty_like if rows else torch.zeros_like
     alike = gate is None and block is None and scale == 1.0  # the block's gradient is the stream's
-    grad_r = new(stream) if wanted[1] or (alike and wanted[0]) else None
-    grad_x = grad_r if alike else new(stream) if wanted[0] else None
+    grad_r = new(x) if wanted[1] or (alike and wanted[0]) else None
+    grad_x = grad_r if alike else new(x) if wanted[0] else None
     out = [new(p) if want and p is not None else None
            for want, p in zip(wanted[2:7], (weight, bias, gate, bw, bb))]
     if rows:
         nbytes = _residual_norm_workspace_bytes(code, rows, set_rows, channels)
-        ws = stream.new_empty(nbytes, dtype=torch.uint8)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         ptr = _b.ptr
-        _b.call_on(stream.get_device(), "bevk_residual_norm_backward", code, grad_y.data_ptr(), ptr(grad_stream),
-                   stream.data_ptr(), ptr(x), ptr(weight), ptr(gate), ptr(bw), ptr(bb), pcode, gcode, rows,
-                   set_rows, channels, kind, block_norm, scale, eps, ws.data_ptr(), nbytes,
+        _b.call_on(x.get_device(), "bevk_residual_norm_backward", code, grad_y.data_ptr(), ptr(grad_stream),
+                   x.data_ptr(), ptr(residual), stats.data_ptr(), ptr(weight), ptr(gate), ptr(bw), ptr(bb), pcode,
+                   gcode, rows, set_rows, channels, kind, block_norm, scale, ws.data_ptr(), nbytes,
                    None if alike else ptr(grad_x), ptr(grad_r), *map(ptr, out))
     return (grad_x if wanted[0] else None, grad_r if wanted[1] else None, *out)
 

@@ -297,14 +297,15 @@ struct ResidualNormArgs {
   float scale, eps;
 };
 struct ResidualNormOut {
-  void *y, *h;  // h: or null
+  void *y, *h;   // h: or null
+  float *stats;  // [rows][2] mean and 1 / spread of h, with the block's norm [rows][4]: also x's; or null
 };
 hipError_t launch_residual_norm_forward(int dtype, const ResidualNormArgs &a, const ResidualNormOut &o,
                                         hipStream_t stream);
-// grad_h may be null (none); outputs are skipped where null; a.x may be null without a block norm where
-// the gate's gradient is not wanted. a.residual and a.bias are not read.
+// grad_h may be null (none); outputs are skipped where null. a.bias and a.eps are not read.
 struct ResidualNormGrads {
-  const void *grad_y, *grad_h, *h;
+  const void *grad_y, *grad_h;
+  const float *stats;
   void *grad_x, *grad_residual, *grad_weight, *grad_bias, *grad_gate, *grad_block_weight, *grad_block_bias;
 };
 int64_t residual_norm_backward_workspace_bytes(int dtype, const ResidualNormArgs &a);

@@ -1545,7 +1545,7 @@ static bevk::ResidualNormArgs residual_norm_args(const void *x, const void *resi
 int bevk_residual_norm_forward(int dtype, const void *x, const void *residual, const void *weight, const void *bias,
                                const void *gate, const void *block_weight, const void *block_bias, int param_dtype,
                                int gate_dtype, int64_t rows, int64_t set_rows, int channels, int kind, int block_norm,
-                               float scale, float eps, void *y, void *stream_out, void *stream) {
+                               float scale, float eps, void *y, void *stream_out, float *stats, void *stream) {
   const char *fn = "residual_norm_forward";
   g_last_error.clear();
   if (int rc = check_residual_norm(fn, dtype, param_dtype, gate_dtype, rows, set_rows, channels, kind)) return rc;
@@ -1554,7 +1554,7 @@ int bevk_residual_norm_forward(int dtype, const void *x, const void *residual, c
   return hip_status(bevk::launch_residual_norm_forward(
                         dtype, residual_norm_args(x, residual, weight, bias, gate, block_weight, block_bias, param_dtype,
                                                   gate_dtype, rows, set_rows, channels, kind, block_norm, scale, eps),
-                        {y, stream_out}, (hipStream_t)stream),
+                        {y, stream_out, stats}, (hipStream_t)stream),
                     fn);
 }
 
@@ -1565,29 +1565,28 @@ int64_t bevk_residual_norm_backward_workspace_bytes(int dtype, int64_t rows, int
                                 set_rows, channels, 0, 0, 1.f, 0.f));
 }
 
-int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_stream, const void *stream_out,
-                                const void *x, const void *weight, const void *gate,
+int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_stream, const void *x,
+                                const void *residual, const float *stats, const void *weight, const void *gate,
                                 const void *block_weight, const void *block_bias, int param_dtype, int gate_dtype,
                                 int64_t rows, int64_t set_rows, int channels, int kind, int block_norm, float scale,
-                                float eps, void *workspace, int64_t workspace_bytes, void *grad_x, void *grad_residual,
+                                void *workspace, int64_t workspace_bytes, void *grad_x, void *grad_residual,
                                 void *grad_weight, void *grad_bias, void *grad_gate, void *grad_block_weight,
                                 void *grad_block_bias, void *stream) {
   const char *fn = "residual_norm_backward";
   g_last_error.clear();
   if (int rc = check_residual_norm(fn, dtype, param_dtype, gate_dtype, rows, set_rows, channels, kind)) return rc;
-  if (!(eps >= 0.f)) return fail(BEVK_ERR_INVALID, "%s: eps must not be negative", fn);
-  if (!grad_y || !stream_out || (!x && (block_norm || grad_gate)))
-    return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!grad_y || !x || !stats) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
+  if (!on_16_bytes({stats})) return fail(BEVK_ERR_INVALID, "%s: stats must begin on a 16-byte boundary", fn);
   if (!block_norm && (grad_block_weight || grad_block_bias))
     return fail(BEVK_ERR_INVALID, "%s: gradients of a block norm that there is not", fn);
-  const bevk::ResidualNormArgs a = residual_norm_args(x, nullptr, weight, nullptr, gate, block_weight, block_bias,
+  const bevk::ResidualNormArgs a = residual_norm_args(x, residual, weight, nullptr, gate, block_weight, block_bias,
                                                       param_dtype, gate_dtype, rows, set_rows, channels, kind,
-                                                      block_norm, scale, eps);
+                                                      block_norm, scale, 0.f);
   if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::residual_norm_backward_workspace_bytes(dtype, a)))
     return rc;
   return hip_status(bevk::launch_residual_norm_backward(
                         dtype, a,
-                        {grad_y, grad_stream, stream_out, grad_x, grad_residual, grad_weight, grad_bias,
+                        {grad_y, grad_stream, stats, grad_x, grad_residual, grad_weight, grad_bias,
                          grad_gate, grad_block_weight, grad_block_bias},
                         workspace, (hipStream_t)stream),
                     fn);

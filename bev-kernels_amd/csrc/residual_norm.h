@@ -49,42 +49,12 @@ __device__ __forceinline__ void row_sums(float (&x)[N], float *s, int &turn) {
   }
 }
 
-// Mean (0 for rms) and 1 / spread over the row of each of N tensors whose values are in registers, in the
-// same sums (inv: 1 / channels); the variance about the mean. Values past the row's end are 0; `full`: there are none.
-template <int TPR, int THREADS, int N, int L, int V>
-__device__ __forceinline__ void row_moments(float (*const (&v)[N])[V], const bool (&in)[L], bool rms, float inv,
-                                            float eps, float (&mean)[N], float (&rstd)[N], float *s, int &turn) {
-  float t[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) mean[n] = t[n] = 0.f;
-  if (!rms) {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int l = 0; l < L; ++l)
-#pragma unroll
-        for (int e = 0; e < V; ++e) t[n] += v[n][l][e];
-    row_sums<TPR, THREADS, N>(t, s, turn);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mean[n] = t[n] * inv;
-  }
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    t[n] = 0.f;
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      float q = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = v[n][l][e] - mean[n];
-        q = __builtin_fmaf(d, d, q);
-      }
-      t[n] += in[l] ? q : 0.f;
-    }
-  }
-  row_sums<TPR, THREADS, N>(t, s, turn);
-#pragma unroll
-  for (int n = 0; n < N; ++n) rstd[n] = __builtin_amdgcn_rsqf(__builtin_fmaf(t[n], inv, eps));
+// The stream's value, in the forward and again in the backward: the same bits.
+__device__ __forceinline__ float block_value(float x, float mean, float rstd, float w, float b) {
+  return __builtin_fmaf((x - mean) * rstd, w, b);
+}
+__device__ __forceinline__ float stream_value(float p, float scale, float gate, float residual) {
+  return __builtin_fmaf(scale * gate, p, residual);
 }
 
 template <typename T, int V>

@@ -6,9 +6,9 @@
 //   gp = scale gate gh; without the block's norm the block's gradient gx = gp, else
 //   gbw = sum gp ph, gbb = sum gp, u = gp bw, gx = rstd_x (u - mean(u) - ph mean(u ph))
 //
-// The row in registers as in the forward, and h as the forward wrote it: mean and spread are taken again
-// from that (the unrounded h's would not make hh's mean 0 and its square's 1 where the spread of a row
-// is small next to the rounding of h). A workgroup takes a range of rows and keeps its threads'
+// The row in registers as in the forward; h is computed again from x and the residual with the forward's means
+// and spreads, to the same bits (read as it was written, rounded, it would be off by half a step of h where hh is
+// small next to it, for as many bytes in most cases). A workgroup takes a range of rows and keeps its threads'
 // part of the parameters' sums in registers; at its end (for the gate: at the end of a set) they are
 // added over its rows in LDS and written to the workspace, and join_kernel adds up the workgroups' parts
 // in order: no atomics, the same results on every run.
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
   Vec<T, V> next[4][L];
   auto load = [&](int64_t r, int64_t r1) __attribute__((always_inline)) {
     const uint32_t bytes = left(r, r1);
-    const void *from[4] = {g.grad_y, g.h, g.grad_h, a.x};
+    const void *from[4] = {g.grad_y, a.x, g.grad_h, a.residual};
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const __amdgpu_buffer_rsrc_t b = make_rsrc(static_cast<const T *>(from[n]) + r * a.channels, from[n] != nullptr ? bytes : 0);
@@ -94,6 +94,10 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
         else next[n][l] = buffer_load_vec<T, V>(b, off[l]);
       }
     }
+  };
+  Vec<float, BLOCK ? 4 : 2> st_next;
+  auto load_stats = [&](int64_t r) __attribute__((always_inline)) {  // of row r + group or, past the end, the last one
+    st_next = load_vec<float, BLOCK ? 4 : 2>(g.stats + min(r + group, sp.sets * sp.set_rows - 1) * (BLOCK ? 4 : 2));
   };
   auto store = [&](void *to, int64_t r, uint32_t bytes, const float (&v)[L][V]) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t b = make_rsrc(static_cast<T *>(to) + r * a.channels, to != nullptr ? bytes : 0);
@@ -151,6 +155,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
     for (int l = 0; l < L; ++l)
       if ((l * TPR + j) * V < a.channels) load_param<T, V>(a.gate, a.gate_wide, gate_at + (l * TPR + j) * V, 1.f, gate[l]);
     load(r0, r1);
+    load_stats(r0);
     for (int64_t r = r0; r < r1; r += R) {
       float gy[L][V], h[L][V], x[L][V], gs[L][V];
       bool in[L];
@@ -160,22 +165,28 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           gy[l][e] = (float)next[0][l].v[e];
-          h[l][e] = (float)next[1][l].v[e];
+          x[l][e] = (float)next[1][l].v[e];
           gs[l][e] = (float)next[2][l].v[e];
-          x[l][e] = (float)next[3][l].v[e];
+          h[l][e] = (float)next[3][l].v[e];
         }
       }
       const uint32_t here = left(r, r1);
       load(min(r + R, r1), r1);
-      float mean[N == 5 ? 2 : 1], rstd[N == 5 ? 2 : 1], t[2] = {0.f, 0.f};
-      if constexpr (BLOCK) row_moments<TPR, THREADS, 2, L, V>({h, x}, in, a.rms, inv, a.eps, mean, rstd, s, turn);
-      else row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, inv, a.eps, mean, rstd, s, turn);
+      const Vec<float, BLOCK ? 4 : 2> st = st_next;
+      load_stats(min(r + R, r1 - 1));
+      const float mean = st.v[0], rstd = st.v[1];
+      float t[2] = {0.f, 0.f};
 #pragma unroll
       for (int l = 0; l < L; ++l)
         if (in[l]) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float hh = (h[l][e] - mean[0]) * rstd[0];
+            float p = x[l][e];
+            if constexpr (BLOCK) {
+              x[l][e] = (p - st.v[2]) * st.v[3];  // ph
+              p = __builtin_fmaf(x[l][e], bw[l][e], bb[l][e]);
+            }
+            const float hh = (stream_value(p, a.scale, gate[l][e], h[l][e]) - mean) * rstd;
             sum[1][l][e] = __builtin_fmaf(gy[l][e], hh, sum[1][l][e]);
             sum[2][l][e] += gy[l][e];
             h[l][e] = hh;
@@ -190,7 +201,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
       for (int l = 0; l < L; ++l)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          gs[l][e] = __builtin_fmaf(rstd[0], gy[l][e] - c1 - h[l][e] * c2, gs[l][e]);  // gh
+          gs[l][e] = __builtin_fmaf(rstd, gy[l][e] - c1 - h[l][e] * c2, gs[l][e]);  // gh
       t[0] = t[1] = 0.f;
       store(g.grad_residual, r, here, gs);
 #pragma unroll
@@ -199,11 +210,10 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
           if constexpr (BLOCK) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float ph = (x[l][e] - mean[1]) * rstd[1], gh = a.scale * gs[l][e], gp = gate[l][e] * gh;
+              const float ph = x[l][e], gh = a.scale * gs[l][e], gp = gate[l][e] * gh;
               sum[0][l][e] = __builtin_fmaf(gh, __builtin_fmaf(ph, bw[l][e], bb[l][e]), sum[0][l][e]);
               sum[3][l][e] = __builtin_fmaf(gp, ph, sum[3][l][e]);
               sum[4][l][e] += gp;
-              x[l][e] = ph;
               gs[l][e] = gp * bw[l][e];
               t[0] += gs[l][e];
               t[1] = __builtin_fmaf(gs[l][e], ph, t[1]);
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
 #pragma unroll
         for (int l = 0; l < L; ++l)
 #pragma unroll
-          for (int e = 0; e < V; ++e) gs[l][e] = rstd[1] * (gs[l][e] - d1 - x[l][e] * d2);
+          for (int e = 0; e < V; ++e) gs[l][e] = st.v[3] * (gs[l][e] - d1 - x[l][e] * d2);
       }
       store(g.grad_x, r, here, gs);
     }
@@ -238,26 +248,6 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
 #pragma unroll
   for (int n = 1; n < N; ++n)
     if (parts.sum[n - 1] != nullptr) write(sum[n], parts.sum[n - 1] + (int64_t)blockIdx.x * a.channels);
-}
-
-// Mean and 1 / spread of a row in memory, by a workgroup of 256.
-template <typename T>
-__device__ __forceinline__ void any_moments(const T *v, const ResidualNormArgs &a, float &mean, float &rstd, float *s,
-                                            int &turn) {
-  float t[1] = {0.f};
-  mean = 0.f;
-  if (!a.rms) {
-    for (int c = threadIdx.x; c < a.channels; c += 256) t[0] += (float)v[c];
-    row_sums<256, 256, 1>(t, s, turn);
-    mean = t[0] / (float)a.channels;
-  }
-  t[0] = 0.f;
-  for (int c = threadIdx.x; c < a.channels; c += 256) {
-    const float d = (float)v[c] - mean;
-    t[0] = __builtin_fmaf(d, d, t[0]);
-  }
-  row_sums<256, 256, 1>(t, s, turn);
-  rstd = 1.f / sqrtf(t[0] / (float)a.channels + a.eps);
 }
 
 // Any row length: a workgroup a row at a time, each sum a pass over it; a thread adds its channels' parts
@@ -284,16 +274,26 @@ __global__ void __launch_bounds__(256) any_backward_kernel(const ResidualNormArg
       for (int c = threadIdx.x; c < a.channels; c += 256) gate_sum[c] = 0.f;
     for (int64_t row = r0; row < r1; ++row) {
       const int64_t at = row * a.channels;
-      const T *gy = static_cast<const T *>(g.grad_y) + at, *h = static_cast<const T *>(g.h) + at;
-      const T *x = a.x == nullptr ? nullptr : static_cast<const T *>(a.x) + at;
+      const T *gy = static_cast<const T *>(g.grad_y) + at, *x = static_cast<const T *>(a.x) + at;
+      const T *res = a.residual == nullptr ? nullptr : static_cast<const T *>(a.residual) + at;
       const T *gs = g.grad_h == nullptr ? nullptr : static_cast<const T *>(g.grad_h) + at;
-      float mean, rstd, mean_x = 0.f, rstd_x = 1.f;
-      any_moments<T>(h, a, mean, rstd, s, turn);
-      if (BLOCK) any_moments<T>(x, a, mean_x, rstd_x, s, turn);
+      const float *st = g.stats + row * (BLOCK ? 4 : 2);
+      const float mean = st[0], rstd = st[1], mean_x = BLOCK ? st[2] : 0.f, rstd_x = BLOCK ? st[3] : 1.f;
       float t[2] = {0.f, 0.f}, w[1], b[1], gate[1];
+      auto normed = [&](int c) __attribute__((always_inline)) {  // hh
+        float p = (float)x[c];
+        if (BLOCK) {
+          load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
+          load_param<T, 1>(a.block_bias, a.wide, c, 0.f, b);
+          p = block_value(p, mean_x, rstd_x, w[0], b[0]);
+        }
+        load_param<T, 1>(a.gate, a.gate_wide, gate_at + c, 1.f, gate);
+        return (stream_value(p, a.scale, gate[0], res != nullptr ? (float)res[c] : 0.f) - mean) * rstd;
+      };
       for (int c = threadIdx.x; c < a.channels; c += 256) {
+        const float hh = normed(c);
         load_param<T, 1>(a.weight, a.wide, c, 1.f, w);
-        const float hh = ((float)h[c] - mean) * rstd, v = (float)gy[c] * w[0];
+        const float v = (float)gy[c] * w[0];
         t[0] += v;
         t[1] = __builtin_fmaf(v, hh, t[1]);
       }
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(256) any_backward_kernel(const ResidualNormArg
       t[0] = t[1] = 0.f;
       if (BLOCK)
         for (int c = threadIdx.x; c < a.channels; c += 256) {
-          const float hh = ((float)h[c] - mean) * rstd, gp = grad_block(c, grad_stream(c, hh));
+          const float hh = normed(c), gp = grad_block(c, grad_stream(c, hh));
           load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
           const float ph = ((float)x[c] - mean_x) * rstd_x, u = gp * w[0];
           t[0] += u;
@@ -319,11 +319,11 @@ __global__ void __launch_bounds__(256) any_backward_kernel(const ResidualNormArg
       if (BLOCK) row_sums<256, 256, 2>(t, s, turn);
       const float d1 = a.rms ? 0.f : t[0] * inv, d2 = t[1] * inv;
       for (int c = threadIdx.x; c < a.channels; c += 256) {
-        const float hh = ((float)h[c] - mean) * rstd, dy = (float)gy[c];
+        const float hh = normed(c), dy = (float)gy[c];
         const float gh = grad_stream(c, hh), gp = grad_block(c, gh);
         if (parts.sum[0] != nullptr) parts.sum[0][mine + c] += dy * hh;
         if (parts.sum[1] != nullptr) parts.sum[1][mine + c] += dy;
-        float p = x != nullptr ? (float)x[c] : 0.f, gx = gp;
+        float p = (float)x[c], gx = gp;
         if (BLOCK) {
           const float ph = (p - mean_x) * rstd_x;
           load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
@@ -439,7 +439,7 @@ hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool 
 
 bool whole_rows(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g) {
   return a.channels % (dtype == 0 ? 4 : 8) == 0 &&
-         on_16({a.x, a.weight, a.gate, a.block_weight, a.block_bias, g.grad_y, g.grad_h, g.h, g.grad_x, g.grad_residual});
+         on_16({a.x, a.residual, a.weight, a.gate, a.block_weight, a.block_bias, g.grad_y, g.grad_h, g.grad_x, g.grad_residual});
 }
 
 }  // namespace

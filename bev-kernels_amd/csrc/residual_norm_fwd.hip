@@ -43,15 +43,39 @@ __global__ void __launch_bounds__(threads_of(TPR)) forward_kernel(const Residual
       if (a.residual != nullptr) load_row<T, V>(res + c, r[l]);
     }
   }
-  auto moments = [&](float &mean, float &rstd) __attribute__((always_inline)) {
-    float m[1], q[1];
-    row_moments<TPR, THREADS, 1, L, V>({h}, in, a.rms, inv, a.eps, m, q, s, turn);
-    mean = m[0];
-    rstd = q[0];
+  float *stats = o.stats == nullptr ? nullptr : o.stats + row * (a.block ? 4 : 2);
+  // mean (0 for rms) and 1 / spread of h over the row; what is past its end is 0 and stays out of the variance
+  auto moments = [&](float &mean, float &rstd, float *keep) __attribute__((always_inline)) {
+    float t[1] = {0.f};
+    if (!a.rms) {
+#pragma unroll
+      for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[0] += h[l][e];
+      row_sums<TPR, THREADS, 1>(t, s, turn);
+    }
+    mean = t[0] * inv;
+    t[0] = 0.f;
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      float q = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = h[l][e] - mean;
+        q = __builtin_fmaf(d, d, q);
+      }
+      t[0] += in[l] ? q : 0.f;
+    }
+    row_sums<TPR, THREADS, 1>(t, s, turn);
+    rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(t[0], inv, a.eps));
+    if (keep != nullptr && there && j == 0) {
+      keep[0] = mean;
+      keep[1] = rstd;
+    }
   };
   float mean, rstd;
   if (a.block) {
-    moments(mean, rstd);
+    moments(mean, rstd, stats == nullptr ? nullptr : stats + 2);
 #pragma unroll
     for (int l = 0; l < L; ++l)
       if (in[l]) {
@@ -60,7 +84,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) forward_kernel(const Residual
         load_param<T, V>(a.block_weight, a.wide, c, 1.f, w);
         load_param<T, V>(a.block_bias, a.wide, c, 0.f, b);
 #pragma unroll
-        for (int e = 0; e < V; ++e) h[l][e] = __builtin_fmaf((h[l][e] - mean) * rstd, w[e], b[e]);
+        for (int e = 0; e < V; ++e) h[l][e] = block_value(h[l][e], mean, rstd, w[e], b[e]);
       }
   }
   const int64_t gate_at = a.set_rows > 0 ? row / a.set_rows * a.channels : 0;
@@ -71,10 +95,10 @@ __global__ void __launch_bounds__(threads_of(TPR)) forward_kernel(const Residual
       float g[V];
       load_param<T, V>(a.gate, a.gate_wide, gate_at + c, 1.f, g);
 #pragma unroll
-      for (int e = 0; e < V; ++e) h[l][e] = __builtin_fmaf(a.scale * g[e], h[l][e], r[l][e]);
+      for (int e = 0; e < V; ++e) h[l][e] = stream_value(h[l][e], a.scale, g[e], r[l][e]);
       if (o.h != nullptr) store_row<T, V>(static_cast<T *>(o.h) + at + c, h[l]);
     }
-  moments(mean, rstd);
+  moments(mean, rstd, stats);
 #pragma unroll
   for (int l = 0; l < L; ++l)
     if (in[l]) {
@@ -104,10 +128,10 @@ __global__ void __launch_bounds__(256) any_forward_kernel(const ResidualNormArgs
     if (a.block) {
       load_param<T, 1>(a.block_weight, a.wide, c, 1.f, w);
       load_param<T, 1>(a.block_bias, a.wide, c, 0.f, b);
-      p = __builtin_fmaf((p - mean_x) * rstd_x, w[0], b[0]);
+      p = block_value(p, mean_x, rstd_x, w[0], b[0]);
     }
     load_param<T, 1>(a.gate, a.gate_wide, gate_at + c, 1.f, g);
-    return __builtin_fmaf(a.scale * g[0], p, a.residual != nullptr ? (float)res[c] : 0.f);
+    return stream_value(p, a.scale, g[0], a.residual != nullptr ? (float)res[c] : 0.f);
   };
   auto moments = [&](auto value, float &mean_of, float &rstd_of) __attribute__((always_inline)) {
     float m = 0.f;
@@ -128,6 +152,15 @@ __global__ void __launch_bounds__(256) any_forward_kernel(const ResidualNormArgs
   };
   if (a.block) moments([&](int c) { return (float)x[c]; }, mean_x, rstd_x);
   moments(stream_at, mean, rstd);
+  if (o.stats != nullptr && threadIdx.x == 0) {
+    float *d = o.stats + row * (a.block ? 4 : 2);
+    d[0] = mean;
+    d[1] = rstd;
+    if (a.block) {
+      d[2] = mean_x;
+      d[3] = rstd_x;
+    }
+  }
   for (int c = threadIdx.x; c < a.channels; c += 256) {
     const float h = stream_at(c);
     if (o.h != nullptr) static_cast<T *>(o.h)[at + c] = static_cast<T>(h);

@@ -29,26 +29,25 @@ class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, gate, block_weight, block_bias, options):
         scale, block_norm, kind, eps, with_stream = options
-        y, h, ctx.sizes = _ext().residual_norm_forward(
-            x, residual, weight, bias, gate, scale, (block_weight, block_bias) if block_norm else None, kind, eps)
+        y, h, stats, ctx.sizes = _ext().residual_norm_forward(
+            x, residual, weight, bias, gate, scale, (block_weight, block_bias) if block_norm else None, kind, eps,
+            with_stream, True)
         ctx.options = options
-        # (x is read again for its norm and for the gate's gradient alone)
-        ctx.save_for_backward(x if block_norm or gate is not None else None, h, weight, bias, gate, block_weight,
-                              block_bias)
+        ctx.save_for_backward(x, residual, stats, weight, bias, gate, block_weight, block_bias)
         ctx.set_materialize_grads(False)
         return (y, h) if with_stream else y
 
     @staticmethod
     @_b.once_differentiable
     def backward(ctx, grad_y, grad_stream=None):
-        x, h, weight, bias, gate, bw, bb = ctx.saved_tensors
-        scale, block_norm, _, eps, _ = ctx.options
+        x, residual, stats, weight, bias, gate, bw, bb = ctx.saved_tensors
+        scale, block_norm, *_ = ctx.options
         if grad_y is None:
             if grad_stream is None:
                 return (None,) * 8
-            grad_y = torch.zeros_like(h)
-        grads = _ext().residual_norm_backward(_dense(grad_y), _dense(grad_stream), h, x, weight, bias, gate, scale,
-                                              (bw, bb) if block_norm else None, eps, ctx.sizes,
+            grad_y = torch.zeros_like(x)
+        grads = _ext().residual_norm_backward(_dense(grad_y), _dense(grad_stream), x, residual, stats, weight, bias,
+                                              gate, scale, (bw, bb) if block_norm else None, ctx.sizes,
                                               ctx.needs_input_grad)
         return (*grads, None)
 
@@ -65,16 +64,17 @@ def residual_norm(x, residual=None, weight=None, bias=None, gate=None, scale=1.0
     bias or "rms" v / sqrt(mean of squares + eps) * weight + bias. A weight or bias of None is 1 or 0,
     a residual of None 0. gate: [C], or one for each first index of x ([B, C], or with ones between).
     fp32 / fp16 / bf16; weights and biases in the input's type or fp32 (all of one), the gate too.
-    Sums are fp32; y is computed from the stream before its rounding, the gradients from the rounded
-    one. Differentiable once, in reverse mode; all gradients are the same on every run."""
+    Sums are fp32; y and the gradients are those of the stream before its rounding. x and residual are
+    kept for the backward, the stream is not. Differentiable once, in reverse mode; all gradients are
+    the same on every run."""
     block_weight, block_bias = (None, None) if block_norm is None else block_norm
     x, residual, weight, bias, gate = _dense(x), _dense(residual), _dense(weight), _dense(bias), _dense(gate)
     if block_norm is not None:
         block_weight, block_bias = _dense(block_weight), _dense(block_bias)
     if _b.records_nothing():  # (without the bookkeeping of a Function)
-        y, h, _ = _ext().residual_norm_forward(x, residual, weight, bias, gate, scale,
-                                               None if block_norm is None else (block_weight, block_bias), kind, eps,
-                                               with_stream)
+        y, h, _, _ = _ext().residual_norm_forward(
+            x, residual, weight, bias, gate, scale, None if block_norm is None else (block_weight, block_bias), kind,
+            eps, with_stream)
         return (y, h) if with_stream else y
     return ResidualNormFunction.apply(x, residual, weight, bias, gate, block_weight, block_bias,
                                       (scale, block_norm is not None, kind, eps, with_stream))

@@ -578,9 +578,10 @@ int bevk_adamw_moments(const void *codes, const void *scale, int second, int64_t
  *   weight, bias, block_weight, block_bias [channels]   param_dtype, NULL for 1 and 0
  *   gate         gate_dtype, NULL for 1; [channels], or with set_rows > 0 [rows / set_rows, channels]
  *   stream_out   [rows, channels] h rounded to dtype, or NULL (y is computed from the unrounded h)
- * The backward takes stream_out (the gradients are those there) and writes those gradients that are not NULL (x's and the
- * residual's in dtype, the others in their parameter's type); grad_stream may be NULL (0), x may be
- * without block_norm where grad_gate is. Sums fp32 in one order: the same results on every run.
+ *   stats        fp32 for the backward, or NULL: [rows, 2] mean (0 for kind 1) and 1 / spread of h;
+ *                with block_norm [rows, 4], then x's. 16-byte aligned
+ * The backward takes the forward's inputs and stats and writes those gradients that are not NULL (x's and the
+ * residual's in dtype, the others in their parameter's type); grad_stream may be NULL (0). Sums fp32 in one order: the same results on every run.
  * dtype F32, F16, BF16; param_dtype and gate_dtype the same or F32. No size may be 0, channels at
  * most 2^30, and at most 2^40 values. The workspace (16-byte aligned) holds what
  * bevk_residual_norm_backward_workspace_bytes says (-1 for sizes not taken). */
@@ -588,14 +589,15 @@ int bevk_residual_norm_forward(int dtype, const void *x, const void *residual, c
                                const void *bias, const void *gate, const void *block_weight,
                                const void *block_bias, int param_dtype, int gate_dtype, int64_t rows,
                                int64_t set_rows, int channels, int kind, int block_norm, float scale,
-                               float eps, void *y, void *stream_out, void *stream);
+                               float eps, void *y, void *stream_out, float *stats,
+                               void *stream);
 int64_t bevk_residual_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t set_rows,
                                                     int channels);
 int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_stream,
-                                const void *stream_out, const void *x, const void *weight, const void *gate, const void *block_weight,
+                                const void *x, const void *residual, const float *stats, const void *weight, const void *gate, const void *block_weight,
                                 const void *block_bias, int param_dtype, int gate_dtype, int64_t rows,
                                 int64_t set_rows, int channels, int kind, int block_norm, float scale,
-                                float eps, void *workspace, int64_t workspace_bytes, void *grad_x,
+                                void *workspace, int64_t workspace_bytes, void *grad_x,
                                 void *grad_residual, void *grad_weight, void *grad_bias,
                                 void *grad_gate, void *grad_block_weight, void *grad_block_bias,
                                 void *stream);

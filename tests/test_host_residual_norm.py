@@ -35,11 +35,11 @@ def test_refusals(kw, code, match):
 
     def forward(dtype=0, pd=0, gd=0, rows=4, sr=0, c=8, kind=0):
         return lib.bevk_residual_norm_forward(dtype, P, P, None, None, None, None, None, pd, gd, rows, sr, c, kind, 0,
-                                              1.0, 1e-5, P, P, None)
+                                              1.0, 1e-5, P, P, P, None)
 
     def backward(dtype=0, pd=0, gd=0, rows=4, sr=0, c=8, kind=0):
-        return lib.bevk_residual_norm_backward(dtype, P, None, P, P, None, None, None, None, pd, gd, rows, sr, c,
-                                               kind, 0, 1.0, 1e-5, P, 1 << 40, P, P, None, None, None, None, None, None)
+        return lib.bevk_residual_norm_backward(dtype, P, None, P, P, P, None, None, None, None, pd, gd, rows, sr, c,
+                                               kind, 0, 1.0, P, 1 << 40, P, P, None, None, None, None, None, None)
     for f in (forward, backward):
         assert f(**kw) == code and re.search(match, _err()), _err()
 
@@ -51,19 +51,18 @@ def test_pointers_and_workspace():
 
     def forward(x=P, y=P, eps=1e-5):
         return lib.bevk_residual_norm_forward(0, x, None, None, None, None, None, None, 0, 0, 4, 0, 8, 0, 0, 1.0, eps,
-                                              y, None, None)
+                                              y, None, None, None)
 
     assert forward(x=None) == INVALID and "null" in _err()
     assert forward(y=None) == INVALID and "null" in _err()
     assert forward(eps=-1.0) == INVALID and "eps" in _err()
     assert forward(eps=float("nan")) == INVALID and "eps" in _err()
 
-    def backward(gy=P, h=P, x=P, eps=1e-5, block=0, ws=P, wb=1 << 20, gg=None, gbw=None):
-        return lib.bevk_residual_norm_backward(0, gy, None, h, x, None, None, None, None, 0, 0, 4, 0, 8, 0, block,
-                                               1.0, eps, ws, wb, P, P, None, None, gg, gbw, None, None)
-    for kw in (dict(gy=None), dict(h=None), dict(x=None, block=1), dict(x=None, gg=P), dict(ws=None)):
+    def backward(gy=P, x=P, st=P, block=0, ws=P, wb=1 << 20, gg=None, gbw=None):
+        return lib.bevk_residual_norm_backward(0, gy, None, x, None, st, None, None, None, None, 0, 0, 4, 0, 8, 0, block,
+                                               1.0, ws, wb, P, P, None, None, gg, gbw, None, None)
+    for kw in (dict(gy=None), dict(st=None), dict(x=None), dict(x=None, block=1), dict(ws=None)):
         assert backward(**kw) == INVALID and "null" in _err()
-    assert backward(eps=-1.0) == INVALID and "eps" in _err()
     assert backward(wb=16) == INVALID and "too small" in _err()
     assert backward(ws=P + 8) == INVALID and "16-byte" in _err()
     assert backward(gbw=P) == INVALID and "block norm" in _err()
