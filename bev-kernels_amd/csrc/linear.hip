@@ -249,16 +249,8 @@ hipError_t launch_any(const T *a, int64_t a_m, int64_t a_k, const T *b, int64_t 
 // writes where its number says. Rows past the end are the last row's again and are not stored; terms
 // past K are zeros in both operands.
 // ---------------------------------------------------------------------------------------
-typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kBK = 64;
 constexpr int kRowBytes = kBK * 2;
-
-__device__ __forceinline__ floatx16 mfma32(int4v a, int4v b, floatx16 c, f16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ floatx16 mfma32(int4v a, int4v b, floatx16 c, bf16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 
 // 16 bytes from `off` + `k` of the buffer for each lane, to `to` + 16 lane (`to` and k: the wave's).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char *to, uint32_t off, uint32_t k) {
@@ -370,22 +362,33 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
       load_to_lds(rb, db + i * 1024, ob[i], k);
   };
 
-  floatx16 acc[TM][TN] = {};
-  const int wm = wave / WN, wn = wave % WN, row = lane % 32, half = lane / 32;
+  floatx4 acc[TM * 2][TN * 2] = {};
+  const int wm = wave / WN, wn = wave % WN, row = lane % 16, half = lane / 16;
   auto multiply = [&](const char *from) __attribute__((always_inline)) {
     const char *fa = from + (wm * TM * 32 + row) * kRowBytes, *fb = from + (BM + wn * TN * 32 + row) * kRowBytes;
+    int4v a[2][TM * 2], b[2][TN * 2];
+    auto read = [&](int k) __attribute__((always_inline)) {
+      const int at = ((k * 4 + half) ^ (row / 2 % 8)) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int at = ((k * 2 + half) ^ (row / 2 % 8)) * 16;
-      int4v a[TM], b[TN];
+      for (int j = 0; j < TN * 2; ++j) b[k][j] = *reinterpret_cast<const int4v *>(fb + j * 16 * kRowBytes + at);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const int4v *>(fa + i * 32 * kRowBytes + at);
+      for (int i = 0; i < TM * 2; ++i) a[k][i] = *reinterpret_cast<const int4v *>(fa + i * 16 * kRowBytes + at);
+    };
+    constexpr bool kAhead = TM * TN <= 4;  // both steps' fragments fit beside the sums
+    if constexpr (kAhead) {
+      read(0);
+      read(1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const int4v *>(fb + j * 32 * kRowBytes + at);
+    for (int k = 0; k < 2; ++k) {
+      if constexpr (!kAhead) read(k);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM * 2; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[j], a[i], acc[i][j], T());
+        for (int j = 0; j < TN * 2; ++j) acc[i][j] = mfma16(b[k][j], a[k][i], acc[i][j], T());
+      __builtin_amdgcn_s_setprio(0);
     }
   };
 
@@ -431,14 +434,10 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        Vec<float, 4> v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v.v[e] = acc[i][j][q * 4 + e];
-        *reinterpret_cast<Vec<float, 4> *>(turn + row * P + j * 32 + q * 8 + half * 4) = v;
-      }
+      for (int j = 0; j < TN * 2; ++j)
+        *reinterpret_cast<floatx4 *>(turn + (ii * 16 + row) * P + j * 16 + half * 4) = acc[i * 2 + ii][j];
     const int64_t mi = m0 + wm * TM * 32 + i * 32;
     if (p.eights) {
 #pragma unroll 2
@@ -756,18 +755,18 @@ hipError_t launch_tile_of(TileArgs p, hipStream_t stream) {
 // wave: the streaming kernel (measured at 40,000 x 256 x 512, 184,950 x 256 x 256, 20,000 x 256 x 4,096
 // and 184,950 x 512 x 256: 20.4, 43, 49 and 72 us, the fastest tile 24.5, 54, 76 and 80; below it
 // loses: 20,000 x 256 x 768 20.0 and 19.6, 40,000 x 512 x 256 22.2 and 20.3). Else the least of these
-// estimates in us, fitted to 40 shapes from 1 x 256 x 256 to 8,192 x 2,048 x 8,192:
+// estimates in us, fitted to some 200 shapes from 1 x 256 x 256 to 40,000 x 4,096 x 1,024:
 //   tiles   rounds over the CUs, each of K / 64 steps that take the longer of a step's latency and what the
 //           tiles on a CU take at its full rate, and what a round's first loads and stores take
 //   few     a CU's loads at 33 bytes a ns (each touches 16 rows' 64 bytes)
-enum Kind { kFew4, kFew8, kFew22, kFew42, kTile64, kTile64x128, kTile128, kTile256, kStream, kKinds };
+enum Kind { kFew4, kFew8, kFew22, kFew42, kTile64, kTile64x128, kTile128, kTile256, kStream };
 struct Shape {
   int bm, bn, on_cu;          // rows and columns, workgroups on a CU
   double first, step, latency;  // tiles: us of a round besides its steps, of a step of one tile at full rate, alone
 };
 constexpr Shape kShapes[kTile256 + 1] = {
     {16, 16, 0, 2.5, 0, 0},      {16, 16, 0, 2.6, 0, 0},      {32, 32, 0, 3.0, 0, 0},      {64, 32, 0, 3.5, 0, 0},
-    {64, 64, 5, 3.3, 0.2, 0.42}, {64, 128, 3, 4, 0.32, 0.55}, {128, 128, 2, 5, 0.51, 0.7}, {256, 256, 1, 7, 1.8, 1.4}};
+    {64, 64, 5, 3, 0.21, 0.49}, {64, 128, 3, 3.4, 0.32, 0.56}, {128, 128, 2, 5.9, 0.46, 0.62}, {256, 256, 1, 8, 1.51, 1.51}};
 
 Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
   const int64_t cus = std::max(8, device_cus());
