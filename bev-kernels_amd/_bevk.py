@@ -86,7 +86,7 @@ _SIGNATURES = {
     "bevk_adamw_step": [_i] + [_vp] * 7 + [_i] + [_vp] * 4 + [_i64, _vp, ctypes.c_uint64, ctypes.c_double,
                                                            _vp] + [ctypes.c_double] * 4
     + [_vp, ctypes.c_double, _vp, _i64, _vp],
-    "bevk_linear_workspace_bytes": [_i, _i, _i64, _i, _i, _i],
+    "bevk_linear_workspace_bytes": [_i, _i, _i, _i64, _i, _i, _i],
     "bevk_linear_forward": [_i, _vp, _vp, _vp, _i, _vp, _i64, _i, _i, _i, _vp, _i64, _vp, _vp, _vp],
     "bevk_linear_backward": [_i, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _i64, _vp, _vp, _vp, _vp],
     "bevk_residual_norm_forward": [_i] + [_vp] * 7 + [_i, _i, _i64, _i64, _i, _i, _i, ctypes.c_float,

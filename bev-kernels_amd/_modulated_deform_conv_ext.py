@@ -1318,6 +1318,9 @@ def adamw_step(params, grads, state, lr, beta1, beta2, eps, weight_decay, norm=N
     ptrs, types, dense = _grad_arrays(fn, params, device)
     gptrs, gtypes, gdense = _grad_arrays(fn, grads, device)
     _like(fn, "gradients", params, grads, dense and gdense)
+    seed = state.get("seed", 0)
+    if not isinstance(seed, int) or not 0 <= seed < 2 ** 64:
+        raise RuntimeError(f"{fn}: the state's seed must be a whole number in [0, 2^64), got {seed!r}")
     cptrs = ctypes_ = None
     if copies is not None:
         cptrs, ctypes_, cdense = _grad_arrays(fn, copies, device)
@@ -1333,7 +1336,7 @@ def adamw_step(params, grads, state, lr, beta1, beta2, eps, weight_decay, norm=N
     ws = torch.empty(nbytes, dtype=torch.uint8, device=m.device)
     _b.call_on(device, "bevk_adamw_step", len(params), at(ptrs), at(types), at(gptrs), at(gtypes), at(cptrs),
                at(ctypes_), at(sizes), 8 if ms is not None else 32, m.data_ptr(), v.data_ptr(), _b.ptr(ms),
-               _b.ptr(vs), m.numel(), step.data_ptr(), state.get("seed", 0), lr, lr_at, beta1, beta2, eps,
+               _b.ptr(vs), m.numel(), step.data_ptr(), seed, lr, lr_at, beta1, beta2, eps,
                weight_decay, norm_at, max_norm, ws.data_ptr(), nbytes)
     # written behind autograd's back
     torch.autograd.graph.increment_version(params if copies is None else [*params, *copies])
@@ -1535,8 +1538,8 @@ def _linear_check(fn, x, weight, bias, act, residual):
 
 
 @functools.lru_cache(maxsize=256)
-def _linear_workspace_bytes(code, backward, rows, k, n, act):
-    nbytes = _b.lib().bevk_linear_workspace_bytes(code, backward, rows, k, n, act)
+def _linear_workspace_bytes(code, backward, aligned, rows, k, n, act):
+    nbytes = _b.lib().bevk_linear_workspace_bytes(code, backward, aligned, rows, k, n, act)
     if nbytes < 0:
         raise RuntimeError(f"linear: {_b.lib().bevk_last_error().decode()}")
     return nbytes
@@ -1553,9 +1556,10 @@ def linear_forward(x, weight, bias=None, act=None, residual=None, with_slope=Fal
     if with_slope and acode:
         slope = y if acode == 1 and residual is None else torch.empty_like(y)  # (16 bits: whole numbers)
     if rows:
-        nbytes = _linear_workspace_bytes(code, 0, rows, k, n, acode)
+        xp, wp = x.data_ptr(), weight.data_ptr()
+        nbytes = _linear_workspace_bytes(code, 0, (xp | wp) % 16 == 0, rows, k, n, acode)
         ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _b.call_on(x.get_device(), "bevk_linear_forward", code, x.data_ptr(), weight.data_ptr(), _b.ptr(bias), bcode,
+        _b.call_on(x.get_device(), "bevk_linear_forward", code, xp, wp, _b.ptr(bias), bcode,
                    _b.ptr(residual), rows, k, n, acode, _b.ptr(ws), nbytes, y.data_ptr(),
                    None if slope is y else _b.ptr(slope))
     return y, slope, sizes
@@ -1570,7 +1574,7 @@ def linear_backward(grad_y, x, weight, bias, slope, sizes, wanted=(True, True, T
     grad_w = new(weight) if wanted[1] else None
     grad_b = new(bias) if wanted[2] and bias is not None else None
     if rows:
-        nbytes = _linear_workspace_bytes(code, 1, rows, k, n, acode)
+        nbytes = _linear_workspace_bytes(code, 1, 0, rows, k, n, acode)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         ptr = _b.ptr
         _b.call_on(x.get_device(), "bevk_linear_backward", code, grad_y.data_ptr(), x.data_ptr(), weight.data_ptr(),

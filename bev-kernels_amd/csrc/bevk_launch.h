@@ -278,7 +278,8 @@ struct LinearArgs {
   int64_t rows;
   int K, N, act;
 };
-int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a);
+int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a, bool aligned);  // x, weight: on 16 bytes
+bool linear_aligned(const LinearArgs &a);
 hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *slope,
                                  void *workspace, hipStream_t stream);
 // slope: the forward's (not read where act is none); outputs are skipped where null.

@@ -1617,10 +1617,12 @@ static bevk::LinearArgs linear_args(const void *x, const void *weight, const voi
   return a;
 }
 
-int64_t bevk_linear_workspace_bytes(int dtype, int backward, int64_t rows, int in_features, int out_features, int act) {
+int64_t bevk_linear_workspace_bytes(int dtype, int backward, int aligned, int64_t rows, int in_features, int out_features,
+                                    int act) {
   if (check_linear("linear", dtype, dtype, rows, in_features, out_features, act)) return -1;
   const bevk::LinearArgs a = linear_args(nullptr, nullptr, nullptr, dtype, rows, in_features, out_features, act);
-  return backward ? bevk::linear_backward_workspace_bytes(dtype, a) : bevk::linear_forward_workspace_bytes(dtype, a);
+  return backward ? bevk::linear_backward_workspace_bytes(dtype, a)
+                  : bevk::linear_forward_workspace_bytes(dtype, a, aligned != 0);
 }
 
 int bevk_linear_forward(int dtype, const void *x, const void *weight, const void *bias, int bias_dtype,
@@ -1631,7 +1633,8 @@ int bevk_linear_forward(int dtype, const void *x, const void *weight, const void
   if (int rc = check_linear(fn, dtype, bias_dtype, rows, in_features, out_features, act)) return rc;
   if (!x || !weight || !y) return fail(BEVK_ERR_INVALID, "%s: null tensor pointer", fn);
   const bevk::LinearArgs a = linear_args(x, weight, bias, bias_dtype, rows, in_features, out_features, act);
-  if (int rc = check_workspace(fn, workspace, workspace_bytes, bevk::linear_forward_workspace_bytes(dtype, a))) return rc;
+  const int64_t need = bevk::linear_forward_workspace_bytes(dtype, a, bevk::linear_aligned(a));
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, need)) return rc;
   return hip_status(bevk::launch_linear_forward(dtype, a, residual, y, slope, workspace, (hipStream_t)stream), fn);
 }
 

@@ -55,8 +55,8 @@ template <typename T> __device__ __forceinline__ void normal(float z, float &cdf
 // act(z), and its derivative.
 template <typename T> __device__ __forceinline__ float activate(float z, int act, float &slope) {
   if (act == kActRelu) {
-    slope = z > 0.f ? 1.f : 0.f;
-    return z > 0.f || z != z ? z : 0.f;
+    slope = z <= 0.f ? 0.f : 1.f;  // (a NaN goes through, both ways)
+    return z <= 0.f ? 0.f : z;
   }
   if (act == kActSilu) {
     const float s = 1.f / (1.f + __expf(-z));
@@ -826,7 +826,8 @@ hipError_t launch_rows(const T *a, const T *b, int64_t M, int64_t K, const Epilo
 // fp32 products of more than a few rows: the split product of dcn_f32.hip (three bf16 pieces an operand).
 // It adds a residual or applies ReLU itself; other epilogues are a pass behind it.
 bool split_takes(const void *a, const void *b, int64_t N, int64_t K, bool transposed) {
-  return (transposed ? K % 32 == 0 && N % 16 == 0 : K % 32 == 0) && K <= 1 << 20 && on_16({a, b});
+  return K % 32 == 0 && K <= 1 << 20 && (!transposed || (N % 16 == 0 && N <= 1 << 20)) &&
+         f32_split_weight_bytes(N, K) < 1LL << 31 && on_16({a, b});  // (32-bit offsets, a grid's second size)
 }
 // The split product loses to the kernel for few rows up to this many (measured at K, N of 256 to 2,048).
 bool split_pays(int64_t M, int64_t N, int64_t K) {
@@ -1049,8 +1050,8 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
                                                           T *__restrict__ gz, int act, int64_t rows, int n, int per,
                                                           float *__restrict__ part) {
   __shared__ float s[kThreads][V + 1];
-  const int lanes = kThreads / per, col = (blockIdx.y * per + threadIdx.x % per) * V, row = threadIdx.x / per;
-  const int64_t r0 = rows * blockIdx.x / gridDim.x, r1 = rows * (blockIdx.x + 1) / gridDim.x;
+  const int lanes = kThreads / per, col = (blockIdx.x * per + threadIdx.x % per) * V, row = threadIdx.x / per;
+  const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   float a[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) a[e] = 0.f;
@@ -1059,17 +1060,21 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
     for (int64_t r = r0 + row; r < r1; r += lanes) {
       const int64_t at = r * n + col;
       Vec<T, V> g = load_vec<T, V>(gy + at);
+      float z[V];  // (the sums are those of gz before its rounding)
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[e] = (float)g.v[e];
       if (act != kActNone) {
         const Vec<T, V> x = load_vec<T, V>(slope + at);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          if (act == kActRelu) g.v[e] = (float)x.v[e] > 0.f ? g.v[e] : static_cast<T>(0.f);  // (slope, or y)
-          else g.v[e] = static_cast<T>((float)g.v[e] * kept_slope(x.v[e]));
+          if (act == kActRelu) z[e] = (float)x.v[e] <= 0.f ? 0.f : z[e];  // (slope, or y)
+          else z[e] *= kept_slope(x.v[e]);
+          g.v[e] = static_cast<T>(z[e]);
         }
         store_vec<T, V>(gz + at, g);
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) a[e] += (float)g.v[e];
+      for (int e = 0; e < V; ++e) a[e] += z[e];
     }
   }
   if (part == nullptr) return;
@@ -1081,7 +1086,7 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
 #pragma unroll
     for (int e = 0; e < V; ++e) a[e] += s[threadIdx.x + l * per][e];
 #pragma unroll
-  for (int e = 0; e < V; ++e) part[(int64_t)blockIdx.x * n + col + e] = a[e];
+  for (int e = 0; e < V; ++e) part[(int64_t)blockIdx.y * n + col + e] = a[e];
 }
 
 // The first `sums` workgroups: 16 columns each, 64 threads add up every 64th part, then in order. The others:
@@ -1095,11 +1100,12 @@ struct TurnArgs {
   int rows, cols;
 };
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p) {
+__global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p, int64_t first) {
   __shared__ float s[64][17];
   __shared__ T tile[64][65];
-  if ((int)blockIdx.x < p.sums) {
-    const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
+  const int64_t block = first + blockIdx.x;
+  if (block < p.sums) {
+    const int c = (int)block * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
     float v = 0.f;
     if (c < p.n)
 #pragma unroll 8
@@ -1116,8 +1122,8 @@ __global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p) {
     }
     return;
   }
-  const int across = (p.cols + 63) / 64, tile_at = (int)blockIdx.x - p.sums;
-  const int r0 = tile_at / across * 64, c0 = tile_at % across * 64, lane = threadIdx.x % 64;
+  const int across = (p.cols + 63) / 64;
+  const int r0 = (int)((block - p.sums) / across) * 64, c0 = (int)((block - p.sums) % across) * 64, lane = threadIdx.x % 64;
   const T *w = static_cast<const T *>(p.weight);
   T *t = static_cast<T *>(p.turned);
 #pragma unroll
@@ -1129,12 +1135,15 @@ __global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p) {
     if (c0 + i < p.cols && r0 + lane < p.rows) t[(int64_t)(c0 + i) * p.rows + r0 + lane] = tile[lane][i];
 }
 
-int sum_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(kSumBlocks, rows / 16)); }
+// (a launch of many columns has workgroups enough: its grid and the parts' memory stay small)
+int sum_blocks(int64_t rows, int n) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kSumBlocks, rows / 16, (1 << 22) / n}));
+}
 
 template <typename T, int V>
 hipError_t launch_grad_z_v(const T *gy, const T *slope, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   const int vecs = (n + V - 1) / V, per = std::min(vecs, kThreads);
-  hipLaunchKernelGGL((grad_z_kernel<T, V>), dim3(sum_blocks(rows), (vecs + per - 1) / per), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((grad_z_kernel<T, V>), dim3((vecs + per - 1) / per, sum_blocks(rows, n)), dim3(kThreads), 0, stream,
                      gy, slope, gz, act, rows, n, per, part);
   return hipGetLastError();
 }
@@ -1144,16 +1153,16 @@ hipError_t launch_grad_z(const T *gy, const T *slope, T *gz, int act, int64_t ro
   return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<T, V>(gy, slope, gz, act, rows, n, part, stream)
                                               : launch_grad_z_v<T, 1>(gy, slope, gz, act, rows, n, part, stream);
 }
-// weight null: sums alone; grad_bias null: the weight alone.
+// The bias' gradient (or null for none) and, with `turn`, the weight turned.
 template <typename T>
 hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wide, const LinearArgs &a, bool turn,
                        void *turned, hipStream_t stream) {
-  const TurnArgs p{part, sum_blocks(rows), a.N, grad_bias != nullptr ? (a.N + 15) / 16 : 0, grad_bias, a.weight, turned, a.N, a.K};
-  const int64_t tiles = turn ? ((a.N + 63) / 64) * (int64_t)((a.K + 63) / 64) : 0, blocks = p.sums + tiles;
-  if (blocks == 0) return hipSuccess;
-  if (wide) hipLaunchKernelGGL((turn_kernel<T, true>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
-  else hipLaunchKernelGGL((turn_kernel<T, false>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
-  return hipGetLastError();
+  const TurnArgs p{part, sum_blocks(rows, a.N), a.N, grad_bias != nullptr ? (a.N + 15) / 16 : 0, grad_bias, a.weight, turned, a.N, a.K};
+  const int64_t tiles = turn ? ((a.N + 63) / 64) * (int64_t)((a.K + 63) / 64) : 0;
+  return launch_in_parts(p.sums + tiles, 1024, [&](int64_t first, unsigned n) {
+    if (wide) hipLaunchKernelGGL((turn_kernel<T, true>), dim3(n), dim3(1024), 0, stream, p, first);
+    else hipLaunchKernelGGL((turn_kernel<T, false>), dim3(n), dim3(1024), 0, stream, p, first);
+  });
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1161,17 +1170,20 @@ hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wi
 // ---------------------------------------------------------------------------------------
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// What a product of rows x [M][K] by weight [N][K] (transposed: [K][N]) needs for either alignment.
-int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t K) {
-  int64_t most = any_bytes(M, N, K);
-  if (dtype == 0) most = std::max(most, f32_split_weight_bytes(N, K));
-  if (transposed) most = std::max(most, up(N * K * (dtype == 0 ? 4 : 2)));
-  return most;
-}
 enum Route { kAny, kSplit, kRows };
 template <typename T> Route route(const T *x, const T *weight, bool transposed, int64_t M, int N, int K) {
   if (sizeof(T) == 4 && split_takes(x, weight, N, K, transposed) && split_pays(M, N, K)) return kSplit;
   return rows_take(x, transposed ? nullptr : weight, K, sizeof(T)) ? kRows : kAny;
+}
+// What a product of rows x [M][K] by weight [N][K] (transposed: [K][N]) needs, its operands on 16-byte boundaries or not.
+int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t K, bool aligned) {
+  if (!aligned) return any_bytes(M, N, K);
+  switch (dtype == 0 ? route<float>(nullptr, nullptr, transposed, M, N, K)
+                     : route<f16>(nullptr, nullptr, transposed, M, N, K)) {
+    case kSplit: return f32_split_weight_bytes(N, K);
+    case kRows: return transposed ? up(N * K * (dtype == 0 ? 4 : 2)) : 0;
+    default: return any_bytes(M, N, K);
+  }
 }
 // transposed: of kRows the workspace holds the weight's transpose already (it is small next to the rows)
 template <typename T>
@@ -1194,7 +1206,9 @@ hipError_t forward(const LinearArgs &a, const void *residual, void *y, void *slo
 
 bool weight_grad_takes(int dtype, const LinearArgs &a) {
   const int64_t size = dtype == 0 ? 4 : 2, vec = 16 / size;
-  return a.K % vec == 0 && a.N % vec == 0 && a.rows < 1LL << 30 && std::max(a.K, a.N) * size * 64 <= 1LL << 28;
+  const int64_t runs = a.N * (int64_t)((a.K + 63) / 64);  // workgroups that add up the parts
+  return a.K % vec == 0 && a.N % vec == 0 && a.rows < 1LL << 30 && std::max(a.K, a.N) * size * 64 <= 1LL << 28 &&
+         runs < 1 << 23;
 }
 
 // Workspace of the backward: gz, the bias' parts, then what the products take.
@@ -1205,10 +1219,11 @@ BackWs back_ws(int dtype, const LinearArgs &a) {
   const int64_t size = dtype == 0 ? 4 : 2;
   BackWs w;
   w.part = a.act != kActNone ? up(a.rows * a.N * size) : 0;
-  w.product = w.part + up((int64_t)kSumBlocks * a.N * 4);
+  w.product = w.part + up((int64_t)sum_blocks(a.rows, a.N) * a.N * 4);
   int64_t grad_w = any_bytes(a.N, a.K, a.rows);
   if (weight_grad_takes(dtype, a)) grad_w = std::max(grad_w, weight_grad_workspace_bytes(dtype, a.rows, a.K, 1, a.N));
-  w.total = w.product + up(std::max(product_bytes(dtype, true, a.rows, a.K, a.N), grad_w));
+  for (bool aligned : {false, true}) grad_w = std::max(grad_w, product_bytes(dtype, true, a.rows, a.K, a.N, aligned));
+  w.total = w.product + up(grad_w);
   return w;
 }
 
@@ -1239,9 +1254,10 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
 
 }  // namespace
 
-int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a) {
-  return product_bytes(dtype, false, a.rows, a.N, a.K);
+int64_t linear_forward_workspace_bytes(int dtype, const LinearArgs &a, bool aligned) {
+  return product_bytes(dtype, false, a.rows, a.N, a.K, aligned);
 }
+bool linear_aligned(const LinearArgs &a) { return on_16({a.x, a.weight}); }
 
 hipError_t launch_linear_forward(int dtype, const LinearArgs &a, const void *residual, void *y, void *slope, void *workspace,
                                  hipStream_t stream) {

@@ -617,14 +617,15 @@ int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_
  *                ReLU dtype, as it is, else whole numbers u of 16 bits, act'(z) = u / 32768 - 0.25
  *                (65535: NaN). Not written for act 0
  * Sums, bias, activation and residual in fp32, rounded once. The backward takes slope (for ReLU anything
- * that is positive where z is, such as y where there is no residual; not read for act 0), and
+ * that is not positive where z is not, such as y where there is no residual; not read for act 0), and
  * writes grad_x, grad_weight (dtype) and grad_bias (bias_dtype), each NULL where it is not wanted;
- * gz = grad_y slope is rounded to dtype, ReLU's derivative at 0 is 0. The residual's gradient is grad_y. The same results on every
- * run. dtype F32, F16, BF16; features at most 2^24, rows less than 2^31 - 256, no size may be 0 and
- * no tensor have more than 2^40 values. The workspace (16-byte aligned) holds what
- * bevk_linear_workspace_bytes says (-1 for sizes not taken). */
-int64_t bevk_linear_workspace_bytes(int dtype, int backward, int64_t rows, int in_features,
-                                    int out_features, int act);
+ * gz = grad_y slope is rounded to dtype, ReLU's derivative at 0 is 0. The residual's gradient is
+ * grad_y. The same results on every run. dtype F32, F16, BF16; features at most 2^24, rows less than
+ * 2^31 - 256, no size may be 0 and no tensor have more than 2^40 values; outputs overlap nothing else.
+ * The workspace (16-byte aligned) holds what bevk_linear_workspace_bytes says (-1 for sizes not
+ * taken); aligned (forward): whether x and weight both begin on 16-byte boundaries. */
+int64_t bevk_linear_workspace_bytes(int dtype, int backward, int aligned, int64_t rows,
+                                    int in_features, int out_features, int act);
 int bevk_linear_forward(int dtype, const void *x, const void *weight, const void *bias,
                         int bias_dtype, const void *residual, int64_t rows, int in_features,
                         int out_features, int act, void *workspace, int64_t workspace_bytes, void *y,

@@ -56,6 +56,70 @@ def test_linear_fp32():
         assert ((y[at].double() - z).abs() <= err).all()
 
 
+def test_linear_fp32_large_weight():
+    """A weight whose three bf16 pieces would pass 32-bit offsets."""
+    from msda_opt2 import linear_act
+    rows, k, n = 70, 2 ** 15, 2 ** 15 - 16
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(rows, k, device=DEV, generator=gen).requires_grad_()
+    w = (torch.randn(n, k, device=DEV, generator=gen) / k ** 0.5).requires_grad_()
+    gy = torch.randn(rows, n, device=DEV, generator=gen)
+    y = linear_act(x, w, None, "relu")
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    with torch.no_grad():
+        at = torch.cat([torch.arange(0, n, n // 60), torch.arange(n - 20, n)]).to(DEV)
+        wd, xd = w[at].double(), x.double()
+        z = xd @ wd.t()
+        err = (k / 4 + 28) * 2.0 ** -24 * (xd.abs() @ wd.abs().t())
+        assert ((y[:, at].double() - z.clamp(min=0)).abs() <= err).all()
+        gz = gy.double() * (y > 0)
+        back = torch.cat([torch.arange(0, k, k // 60), torch.arange(k - 20, k)]).to(DEV)
+        wd = w[:, back].double()
+        err = (n / 4 + 28) * 2.0 ** -24 * (gz.abs() @ wd.abs())
+        assert ((gx[:, back].double() - gz @ wd).abs() <= err).all()
+        err = (rows + 28) * 2.0 ** -24 * (gz[:, at].abs().t() @ xd.abs())
+        assert ((gw[at].double() - gz[:, at].t() @ xd).abs() <= err).all()
+
+
+def test_linear_weight_turned_in_parts():
+    """A weight with more 64 x 64 pieces than one launch takes, turned for the gradient of x."""
+    from msda_opt2 import linear_act
+    rows, k, n = 5, 2 ** 15 + 2 ** 14, 2 ** 18  # 26 GB
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    w = torch.empty(n, k, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    gy = torch.randn(rows, n, device=DEV, generator=gen).bfloat16()
+    gx, = torch.autograd.grad(linear_act(x, w), x, gy)
+    want = torch.zeros(rows, k, dtype=torch.float64, device=DEV)
+    mag = want.clone()
+    for a in range(0, n, 2 ** 14):
+        part, g = w[a:a + 2 ** 14].double(), gy[:, a:a + 2 ** 14].double()
+        want += g @ part
+        mag += g.abs() @ part.abs_()
+    err = (n / 16 + 64) * 2.0 ** -24 * mag
+    assert ((gx.double() - want).abs() <= err + 2.0 ** -8 * (want.abs() + err)).all()
+
+
+def test_linear_most_features():
+    """As many features as there may be, of an odd number: gz, and its sums by columns, exact here."""
+    from msda_opt2 import linear_act
+    rows, k, n = 37, 16, 2 ** 24 - 1
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV)
+    x[:, 0] = torch.randint(-4, 5, (rows,), device=DEV, generator=gen).bfloat16()
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device=DEV)
+    w[:, 0] = torch.randint(-4, 5, (n,), device=DEV, generator=gen).bfloat16()
+    b = torch.randint(-3, 4, (n,), device=DEV, generator=gen).float().requires_grad_()
+    gy = torch.randint(-8, 9, (rows, n), device=DEV, generator=gen, dtype=torch.int8).bfloat16()
+    y = linear_act(x, w, b, "relu")
+    gb, = torch.autograd.grad(y, b, gy)
+    for a in range(0, n, 2 ** 21):
+        s = slice(a, a + 2 ** 21)
+        z = x[:, :1].float() * w[s, 0].float() + b.detach()[s]
+        assert torch.equal(y[:, s].float(), z.clamp(min=0))
+        assert torch.equal(gb[s], (gy[:, s].float() * (z > 0)).sum(0))
+
+
 def test_residual_norm():
     """Each repetition of a small input gives the small result; the parameters' gradients are TIMES as
     large, up to the fp32 sums' (TIMES * 1024 / 16 + 72) u of magnitudes below 4 in the mean."""

@@ -212,6 +212,24 @@ def test_non_finite_values_stay_in_their_rows(rows, dtype):
         assert gw[keep.to(DEV)].isfinite().all() and not gw[5].isfinite().any()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,features,residual", [(4, 264, False), (4, 264, True), (500, 264, False), (500, 264, True),
+                                                    (4000, 256, False), (4000, 256, True), (500, 261, True)])
+def test_relu_of_nan(rows, features, residual, dtype):
+    """A NaN is what ReLU makes of it, and its gradient goes on as it came (as torch's does)."""
+    from msda_opt2 import linear_act
+    t, gy = _inputs(rows, 256, features, TYPES[dtype], 16)
+    r = t["residual"].to(DEV) if residual else None
+    x = t["x"].to(DEV)
+    x[2, 100] = float("nan")
+    leaf, w, b = x.requires_grad_(), t["weight"].to(DEV), t["bias"].to(DEV)
+    y = linear_act(leaf, w, b, "relu", r)
+    assert y[2].isnan().all()
+    gx, = torch.autograd.grad(y, leaf, gy.to(DEV))
+    plain, = torch.autograd.grad(linear_act(leaf, w, b, None, r), leaf, gy.to(DEV))
+    assert torch.equal(gx[2], plain[2]) and not torch.equal(gx, plain)
+
+
 def test_empty():
     from msda_opt2 import linear_act
     x = torch.zeros(0, 5, 32, device=DEV, requires_grad=True)

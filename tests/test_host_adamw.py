@@ -33,6 +33,25 @@ def test_needs_a_device():
         mdc.adamw_state(p, seed=-1)
 
 
+def _on_device(step):
+    """The parts of a call that are checked before the device's own."""
+    class Fake:
+        def __init__(self, t): self.t = t
+        def __getattr__(self, n): return getattr(self.t, n)
+        def get_device(self): return 0
+        is_cuda = True
+    return Fake(step)
+
+
+@pytest.mark.parametrize("seed", [-1, 2 ** 64, 1.0, "1"])
+def test_refuses_a_loaded_seed(seed, monkeypatch):
+    import _modulated_deform_conv_ext as ext
+    monkeypatch.setattr(ext, "_grad_arrays", lambda fn, tensors, device: (None, None, True))
+    p = _on_device(torch.zeros(4))
+    with pytest.raises(RuntimeError, match="seed"):
+        ext.adamw_step([p], [p], {"seed": seed}, 0.1, 0.9, 0.99, 1e-8, 0.0)
+
+
 def test_state_layout():
     p = [torch.zeros(4), torch.zeros(128), torch.zeros(0), torch.zeros(3, 50)]
     state = mdc.adamw_state(p, 8, seed=7)

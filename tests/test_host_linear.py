@@ -47,8 +47,10 @@ def test_refusals(kw, code, match):
 def test_workspace():
     lib = _bevk.lib()
     size = lib.bevk_linear_workspace_bytes
-    assert size(0, 0, 4, 8, 8, 0) >= 0 and size(3, 0, 4, 8, 8, 0) == -1 and size(0, 1, 0, 8, 8, 0) == -1
-    need = size(1, 1, 4000, 256, 256, 3)
+    assert size(0, 0, 0, 4, 8, 8, 0) >= 0 and size(3, 0, 0, 4, 8, 8, 0) == -1 and size(0, 1, 0, 0, 8, 8, 0) == -1
+    # operands on 16-byte boundaries: none for rows that are loaded as they are, some off them for a split sum
+    assert size(1, 0, 1, 4, 2048, 64, 0) == 0 < size(1, 0, 0, 4, 2048, 64, 0)
+    need = size(1, 1, 0, 4000, 256, 256, 3)
     assert need >= 4000 * 256 * 2
 
     def backward(z=P, ws=P, wb=1 << 50):
