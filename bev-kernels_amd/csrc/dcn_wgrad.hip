@@ -490,6 +490,9 @@ hipError_t launch_weight_grad(int dtype, const void *cols, const void *dout, int
   const int64_t wgs = (int64_t)p.ntn * p.ntk * p.parts;
   if (wgs > (1 << 28)) return hipErrorInvalidValue;
   p.per_xcd = (int)((wgs + 7) / 8);
+  // one part of an fp32 gradient without taps to turn is the gradient
+  const bool direct = pl.parts == 1 && T == 1 && out_dtype == 0;
+  if (direct) p.part = static_cast<float *>(grad_w);
   switch (dtype) {
     case 0: launch_tn<float>(p, pl.tn, stream); break;
     case 1: launch_tn<f16>(p, pl.tn, stream); break;
@@ -497,7 +500,7 @@ hipError_t launch_weight_grad(int dtype, const void *cols, const void *dout, int
     default: return hipErrorInvalidValue;
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || direct) return e;
   return launch_reduce(p, C, T, out_dtype, grad_w, stream);
 }
 

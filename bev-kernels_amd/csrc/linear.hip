@@ -30,6 +30,19 @@ __device__ __forceinline__ floatx4 mfma16(int4v a, int4v b, floatx4 c, bf16) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// 16 bytes of a row of each operand: 8 terms of 16 bits in one product, 4 of fp32 in four (each takes one
+// of every lane's, the same of both operands: the terms' order does not matter).
+template <typename T> __device__ __forceinline__ floatx4 multiply16(int4v a, int4v b, floatx4 c) {
+  if constexpr (sizeof(T) == 2) {
+    return mfma16(a, b, c, T());
+  } else {
+    const floatx4 af = __builtin_bit_cast(floatx4, a), bf = __builtin_bit_cast(floatx4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(af[e], bf[e], c, 0, 0, 0);
+    return c;
+  }
+}
+
 // ---------------------------------------------------------------------------------------
 // Activations
 // ---------------------------------------------------------------------------------------
@@ -155,6 +168,13 @@ __global__ void __launch_bounds__(kThreads) any_kernel(const Product<T> p, int64
     const bool along = by_k == 1;
     const int r = along ? tid / 4 : tid % 64, c = (along ? tid % 4 : tid / 64) * 8;
     const T *q = src + (row0 + r) * by_row;
+    if (along && row0 + r < rows && k + c + 8 <= k1) {  // (loads of 16 bytes from any address)
+      struct __attribute__((packed, aligned(sizeof(T)))) Any { T v[8]; };
+      const Any v = *reinterpret_cast<const Any *>(q + k + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[r][c + e] = v.v[e];
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int64_t kk = k + c + e;
@@ -249,8 +269,7 @@ hipError_t launch_any(const T *a, int64_t a_m, int64_t a_k, const T *b, int64_t 
 // writes where its number says. Rows past the end are the last row's again and are not stored; terms
 // past K are zeros in both operands.
 // ---------------------------------------------------------------------------------------
-constexpr int kBK = 64;
-constexpr int kRowBytes = kBK * 2;
+constexpr int kRowBytes = 128;  // of a row a step
 
 // 16 bytes from `off` + `k` of the buffer for each lane, to `to` + 16 lane (`to` and k: the wave's).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, char *to, uint32_t off, uint32_t k) {
@@ -267,51 +286,51 @@ struct TileArgs {
   int64_t tm;
   int tn;
   int64_t per_xcd;
-  bool eights;  // N a multiple of 8, tensors on 16-byte boundaries
+  bool wide;  // N * size a multiple of 16, tensors on 16-byte boundaries
 };
 
-// Eight neighbouring values of a row.
-template <typename T, int ACT>
-__device__ __forceinline__ void finish8(const Epilogue &e, int64_t m, int n, float (&v)[8]) {
+// 16 bytes of a row.
+template <typename T, int ACT, int V>
+__device__ __forceinline__ void finish16(const Epilogue &e, int64_t m, int n, float (&v)[V]) {
   const int64_t at = m * e.N + n;
-  Vec<T, 8> r;
-  if (e.residual != nullptr) r = load_vec<T, 8>(static_cast<const T *>(e.residual) + at);
+  Vec<T, V> r;
+  if (e.residual != nullptr) r = load_vec<T, V>(static_cast<const T *>(e.residual) + at);
   if (e.bias != nullptr) {
     if (e.bias_wide) {
 #pragma unroll
-      for (int h = 0; h < 8; h += 4) {
+      for (int h = 0; h < V; h += 4) {
         const Vec<float, 4> b = load_vec<float, 4>(static_cast<const float *>(e.bias) + n + h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[h + k] += b.v[k];
       }
     } else {
-      const Vec<T, 8> b = load_vec<T, 8>(static_cast<const T *>(e.bias) + n);
+      const Vec<T, V> b = load_vec<T, V>(static_cast<const T *>(e.bias) + n);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += (float)b.v[k];
+      for (int k = 0; k < V; ++k) v[k] += (float)b.v[k];
     }
   }
-  Vec<T, 8> y;
+  Vec<T, V> y;
   if (ACT != kActNone && e.slope != nullptr) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < V; ++k) {
       float s;
       v[k] = activate<T>(v[k], ACT, s);
       y.v[k] = keep_slope<T, ACT>(s);
     }
-    store_vec<T, 8>(static_cast<T *>(e.slope) + at, y);
+    store_vec<T, V>(static_cast<T *>(e.slope) + at, y);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < V; ++k) {
       float s;
       v[k] = activate<T>(v[k], ACT, s);
     }
   }
   if (e.residual != nullptr)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += (float)r.v[k];
+    for (int k = 0; k < V; ++k) v[k] += (float)r.v[k];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) y.v[k] = static_cast<T>(v[k]);
-  store_vec<T, 8>(static_cast<T *>(e.y) + at, y);
+  for (int k = 0; k < V; ++k) y.v[k] = static_cast<T>(v[k]);
+  store_vec<T, V>(static_cast<T *>(e.y) + at, y);
 }
 
 // Tile number L of all: groups of 8 rows of tiles, in a group one column of tiles after another, so that
@@ -325,7 +344,7 @@ __device__ __forceinline__ void tile_at(int64_t L, int64_t tm, int tn, int64_t &
 
 template <typename T, int ACT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, int64_t first) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, kBK = kRowBytes / (int)sizeof(T);
   constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // 8-row pieces that a wave loads a step
   static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && TM * 32 * WM == BM && TN * 32 * WN == BN, "tile");
   __shared__ __attribute__((aligned(1024))) char lds[2][(BM + BN) * kRowBytes];
@@ -340,7 +359,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   // a tile's rows are below 2^31 bytes apart (K at most 2^21)
   const int ma = (int)min((int64_t)BM, p.M - m0), nb = min(BN, N - n0);
-  const uint32_t ld = (uint32_t)K * 2;
+  const uint32_t ld = (uint32_t)K * sizeof(T);
   const __amdgpu_buffer_rsrc_t ra = make_rsrc(static_cast<const char *>(p.a) + m0 * ld, ma * ld);
   const __amdgpu_buffer_rsrc_t rb = make_rsrc(static_cast<const char *>(p.b) + (int64_t)n0 * ld, nb * ld);
   const int piece[2] = {(lane % 8 ^ lane / 16) * 16, (lane % 8 ^ lane / 16 ^ 4) * 16};  // of even and odd groups of 8 rows
@@ -387,7 +406,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
 #pragma unroll
       for (int i = 0; i < TM * 2; ++i)
 #pragma unroll
-        for (int j = 0; j < TN * 2; ++j) acc[i][j] = mfma16(b[k][j], a[k][i], acc[i][j], T());
+        for (int j = 0; j < TN * 2; ++j) acc[i][j] = multiply16<T>(b[k][j], a[k][i], acc[i][j]);
       __builtin_amdgcn_s_setprio(0);
     }
   };
@@ -427,7 +446,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
 
   // A lane holds one row and four times four neighbouring columns of each 32 x 32. Each wave turns 32 rows of
   // its own at a time in LDS, so that eight lanes store 128 neighbouring bytes of a row.
-  constexpr int P = TN * 32 + 4, C = TN * 4;  // floats of a row, and its pieces of 8
+  constexpr int V = 16 / sizeof(T), P = TN * 32 + 4, C = TN * 32 / V;  // floats of a row, and its pieces of V
   float *turn = reinterpret_cast<float *>(lds[0]) + wave * 32 * P;
   static_assert(WAVES * 32 * P * 4 <= (int)sizeof(lds), "turn");
   const int wn0 = n0 + wn * TN * 32;
@@ -439,19 +458,19 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
       for (int j = 0; j < TN * 2; ++j)
         *reinterpret_cast<floatx4 *>(turn + (ii * 16 + row) * P + j * 16 + half * 4) = acc[i * 2 + ii][j];
     const int64_t mi = m0 + wm * TM * 32 + i * 32;
-    if (p.eights) {
+    if (p.wide) {
 #pragma unroll 2
       for (int c = lane; c < 32 * C; c += 64) {
         const int64_t m = mi + c / C;
-        const int n = wn0 + c % C * 8;
-        float v[8];
+        const int n = wn0 + c % C * V;
+        float v[V];
 #pragma unroll
-        for (int h = 0; h < 8; h += 4) {
-          const Vec<float, 4> x = load_vec<float, 4>(turn + c / C * P + c % C * 8 + h);
+        for (int h = 0; h < V; h += 4) {
+          const Vec<float, 4> x = load_vec<float, 4>(turn + c / C * P + c % C * V + h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[h + e] = x.v[e];
         }
-        if (m < p.M && n < N) finish8<T, ACT>(p.e, m, n, v);
+        if (m < p.M && n < N) finish16<T, ACT>(p.e, m, n, v);
       }
     } else {
 #pragma unroll 1
@@ -679,16 +698,6 @@ __global__ void __launch_bounds__(64 * WAVES) few_kernel(const FewArgs p, int64_
 #pragma unroll
   for (int j = 0; j < NT; ++j) ob[j] = min(j * 16 + r16, nt - 1) * ld;
   floatx4 acc[MT][NT] = {};
-  auto multiply = [&](int4v w, int4v x, floatx4 c) __attribute__((always_inline)) {
-    if constexpr (sizeof(T) == 2) {
-      return mfma16(w, x, c, T());
-    } else {
-      const floatx4 wf = __builtin_bit_cast(floatx4, w), xf = __builtin_bit_cast(floatx4, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[e], xf[e], c, 0, 0, 0);
-      return c;
-    }
-  };
   for (uint32_t k = wave * 64; k < ld; k += U * WAVES * 64) {  // bytes of a row; past its end a load gives zeros
     int4v w[U][NT], x[U][MT];
 #pragma unroll
@@ -706,7 +715,7 @@ __global__ void __launch_bounds__(64 * WAVES) few_kernel(const FewArgs p, int64_
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = multiply(w[u][j], x[u][i], acc[i][j]);
+        for (int j = 0; j < NT; ++j) acc[i][j] = multiply16<T>(w[u][j], x[u][i], acc[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -768,15 +777,21 @@ constexpr Shape kShapes[kTile256 + 1] = {
     {16, 16, 0, 2.5, 0, 0},      {16, 16, 0, 2.6, 0, 0},      {32, 32, 0, 3.0, 0, 0},      {64, 32, 0, 3.5, 0, 0},
     {64, 64, 5, 3, 0.21, 0.49}, {64, 128, 3, 3.4, 0.32, 0.56}, {128, 128, 2, 5.9, 0.46, 0.62}, {256, 256, 1, 8, 1.51, 1.51}};
 
-Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
+constexpr Shape kTile64F32 = {64, 64, 5, 2.3, 0.52, 0.35};
+
+Kind plan(int size, int64_t M, int64_t N, int64_t K, bool wide, double *estimate = nullptr) {
   const int64_t cus = std::max(8, device_cus());
-  if (size == 2 && eights && (K == 256 || K == 512) &&
-      (M + 15) / 16 * ((N + 65536 / K - 1) / (65536 / K)) >= cus * (K == 256 ? 12 : 24))
-    return kStream;
+  // streamed rows: enough of them that the weight's way into LDS does not count, and not more parts of the
+  // columns than workgroups on an XCD, whose L2 they read the rows from (10,000 x 256 x 8,192: 54 us streamed, 76 by
+  // tiles; x 12,288: 128 and 109. 40,000 x 512 x 256: 20 and 26; 10,000 x 512 x 256: 11.0 and 10.4)
+  if (size == 2 && wide && (K == 256 || K == 512)) {
+    const int64_t parts = (N + 65536 / K - 1) / (65536 / K);
+    if (parts * 8 <= cus && (M + 15) / 16 * parts >= cus * (K == 256 ? 12 : 24)) return kStream;
+  }
   Kind best = kFew4;
   double best_t = 0;
-  for (int k = kFew4; k <= (size == 2 ? kTile256 : kFew42); ++k) {
-    const Shape &s = kShapes[k];
+  for (int k = kFew4; k <= (size == 2 ? kTile256 : kTile64); ++k) {
+    const Shape &s = size == 4 && k == kTile64 ? kTile64F32 : kShapes[k];
     const int64_t n = (((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn) + cus - 1) / cus;  // workgroups of a CU
     double t;
     if (k <= kFew42) {
@@ -784,7 +799,7 @@ Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
       t = s.first + (double)n * (s.bm + s.bn) * steps * 64 / 33e3 + (k == kFew4 ? 0.0125 : 0.007) * steps;
     } else {
       const int64_t full = n / s.on_cu, rest = n % s.on_cu;
-      const double steps = (double)((K + 63) / 64);
+      const double steps = (double)((K * size + kRowBytes - 1) / kRowBytes);
       t = full * (steps * std::max(s.latency, s.on_cu * s.step) + s.first) +
           (rest > 0 ? steps * std::max(s.latency, rest * s.step) + s.first : 0);
     }
@@ -793,13 +808,14 @@ Kind plan(int size, int64_t M, int64_t N, int64_t K, bool eights) {
       best_t = t;
     }
   }
+  if (estimate != nullptr) *estimate = best_t;
   return best;
 }
 
 template <typename T>
 hipError_t launch_rows(const T *a, const T *b, int64_t M, int64_t K, const Epilogue &e, hipStream_t stream) {
-  const bool eights = e.N % 8 == 0 && on_16({e.residual, e.y, e.slope, e.bias});
-  const Kind kind = plan(sizeof(T), M, e.N, K, eights);
+  const bool wide = e.N * sizeof(T) % 16 == 0 && on_16({e.residual, e.y, e.slope, e.bias});
+  const Kind kind = plan(sizeof(T), M, e.N, K, wide);
   const FewArgs few{a, b, M, (int)K, e, 0};
   switch (kind) {
     case kFew4: return launch_few_of<T, 1, 1, 4, 8>(few, stream);
@@ -808,11 +824,11 @@ hipError_t launch_rows(const T *a, const T *b, int64_t M, int64_t K, const Epilo
     case kFew42: return launch_few_of<T, 4, 2, 8, 4>(few, stream);
     default: break;
   }
+  const TileArgs tile{a, b, M, (int)K, e, 0, 0, 0, wide};
+  if (kind == kTile64) return launch_tile_of<T, 64, 64, 2, 2>(tile, stream);
   if constexpr (sizeof(T) == 2) {
-    const TileArgs tile{a, b, M, (int)K, e, 0, 0, 0, eights};
     const StreamArgs rows{a, b, M, 0, e, 0, 0};
     switch (kind) {
-      case kTile64: return launch_tile_of<T, 64, 64, 2, 2>(tile, stream);
       case kTile64x128: return launch_tile_of<T, 64, 128, 1, 4>(tile, stream);
       case kTile128: return launch_tile_of<T, 128, 128, 2, 2>(tile, stream);
       case kTile256: return launch_tile_of<T, 256, 256, 2, 4>(tile, stream);
@@ -829,11 +845,13 @@ bool split_takes(const void *a, const void *b, int64_t N, int64_t K, bool transp
   return K % 32 == 0 && K <= 1 << 20 && (!transposed || (N % 16 == 0 && N <= 1 << 20)) &&
          f32_split_weight_bytes(N, K) < 1LL << 31 && on_16({a, b});  // (32-bit offsets, a grid's second size)
 }
-// The split product loses to the kernel for few rows up to this many (measured at K, N of 256 to 2,048).
+// Against the kernels that run on the fp32 matrix cores, by estimates of both (us) fitted to 166 shapes from 32 x 256 x 64
+// to 10,000 x 2,048 x 256: the faster in nearly all, 1.3% off it in the mean. Cutting the weight is what few rows
+// do not pay for: 2 x 2,048 x 8,192 18 us without and 62 with, 600 x 2,048 x 8,192 182 and 161.
 bool split_pays(int64_t M, int64_t N, int64_t K) {
-  const int64_t cus = std::max(8, device_cus());
-  const double few = 3.5 + (double)((((M + 63) / 64) * ((N + 31) / 32) + cus - 1) / cus) * 96 * K * 4 / 33e3;
-  return few > 12.0;
+  double rows = 0;
+  plan(4, M, N, K, false, &rows);
+  return rows > 9.5 + 1.4e-6 * N * K + 4e-3 * K + 12.3e-9 * M * N * K;
 }
 
 // y = act(y) + residual, and slope (or null).
@@ -1013,8 +1031,10 @@ hipError_t launch_split(const float *x, const float *weight, bool transposed, in
                               : launch_f32_split_weight(weight, N, K, 1, false, workspace, stream);
   if (err != hipSuccess) return err;
   // (K 512 without anything behind it: 89 us in the tiled kernel at 40,000 x 512 x 256, 94 streamed; with a residual
-  // 111 and 99)
-  if ((K == 256 || (K == 512 && (e.residual != nullptr || e.act != kActNone))) && N % 4 == 0 &&
+  // 111 and 99. More parts of columns than workgroups on an XCD read the rows too often: 10,000 x 256 x 2,048 68 us
+  // streamed and 86 tiled, x 4,096 207 and 154)
+  const bool few_parts = (N + 16384 / K - 1) / (16384 / K) * 8 <= std::max(8, device_cus());
+  if ((K == 256 || (K == 512 && (e.residual != nullptr || e.act != kActNone))) && few_parts && N % 4 == 0 &&
       on_16({e.residual, e.y, e.slope})) {
     const SplitStreamArgs p{x, workspace, M, 0, e, 0, 0};
     return K == 256 ? launch_split_stream<256>(p, stream) : launch_split_stream<512>(p, stream);

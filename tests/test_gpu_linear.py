@@ -152,6 +152,17 @@ def test_ordinary_sizes(size, dtype):
     _check(t, gy, "gelu")
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("size", [(700, 1001, 77), (700, 1003, 1005), (500, 4, 1000), (1001, 516, 255), (600, 2048, 512),
+                                  (2, 2048, 4096), (2000, 256, 4096), (5000, 256, 2048), (1000, 256, 12288),
+                                  (3000, 512, 4104), (4000, 1024, 520)], ids=str)
+def test_where_another_kernel_takes_over(size, dtype):
+    """Odd rows; fp32 by tiles or cut into pieces; more columns than are streamed past."""
+    t, gy = _inputs(*size, TYPES[dtype], 17, device=DEV)
+    for act in (None, "silu"):
+        _check(t, gy, act)
+
+
 def test_shapes_of_x():
     from msda_opt2 import linear_act
     t, _ = _inputs(60, 64, 40, torch.float32, 9)
