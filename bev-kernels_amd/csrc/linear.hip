@@ -72,7 +72,7 @@ template <typename T> __device__ __forceinline__ float activate(float z, int act
     return z <= 0.f ? 0.f : z;
   }
   if (act == kActSilu) {
-    const float s = 1.f / (1.f + __expf(-z));
+    const float d = 1.f + __expf(-z), s = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(d) : 1.f / d;  // (16 bits: off by an ulp of fp32)
     slope = s * __builtin_fmaf(z, 1.f - s, 1.f);
     return z * s;
   }
@@ -289,26 +289,12 @@ struct TileArgs {
   bool wide;  // N * size a multiple of 16, tensors on 16-byte boundaries
 };
 
-// 16 bytes of a row.
+// 16 bytes of a row, whose sums have the bias.
 template <typename T, int ACT, int V>
 __device__ __forceinline__ void finish16(const Epilogue &e, int64_t m, int n, float (&v)[V]) {
   const int64_t at = m * e.N + n;
   Vec<T, V> r;
   if (e.residual != nullptr) r = load_vec<T, V>(static_cast<const T *>(e.residual) + at);
-  if (e.bias != nullptr) {
-    if (e.bias_wide) {
-#pragma unroll
-      for (int h = 0; h < V; h += 4) {
-        const Vec<float, 4> b = load_vec<float, 4>(static_cast<const float *>(e.bias) + n + h);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[h + k] += b.v[k];
-      }
-    } else {
-      const Vec<T, V> b = load_vec<T, V>(static_cast<const T *>(e.bias) + n);
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] += (float)b.v[k];
-    }
-  }
   Vec<T, V> y;
   if (ACT != kActNone && e.slope != nullptr) {
 #pragma unroll
@@ -450,6 +436,10 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
   float *turn = reinterpret_cast<float *>(lds[0]) + wave * 32 * P;
   static_assert(WAVES * 32 * P * 4 <= (int)sizeof(lds), "turn");
   const int wn0 = n0 + wn * TN * 32;
+  static_assert(64 % C == 0, "a lane's columns are the same in every row");
+  float bias[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) bias[e] = p.wide && wn0 + lane % C * V < N ? bias_at<T>(p.e, wn0 + lane % C * V + e) : 0.f;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -468,7 +458,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
         for (int h = 0; h < V; h += 4) {
           const Vec<float, 4> x = load_vec<float, 4>(turn + c / C * P + c % C * V + h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[h + e] = x.v[e];
+          for (int e = 0; e < 4; ++e) v[h + e] = x.v[e] + bias[h + e];
         }
         if (m < p.M && n < N) finish16<T, ACT>(p.e, m, n, v);
       }
