@@ -30,7 +30,6 @@ constexpr int kThreads = 256;
 constexpr int kTensors = 64;   // 47 bytes each: 3.0 KB of the 4 KB of arguments
 constexpr int kBlock = kAdamwBlock;
 constexpr int kChunks = 4096;  // about that many for a large model
-constexpr int64_t kCached = 192 << 20;  // bytes, about, that stay in the last-level cache until the next step
 
 struct Table {
   void *p[kTensors], *copy[kTensors];
@@ -100,13 +99,13 @@ __device__ __forceinline__ int find_tensor(const Table &t, int chunk) {
 }
 
 // V values at p, or the first `left` of them (the others 0).
-template <typename T, int V, bool STREAM>
+template <typename T, int V>
 __device__ __forceinline__ void load_values(const T *p, int64_t left, bool whole, float (&x)[V]) {
   if (whole && left >= V) {
     constexpr int W = sizeof(T) * V > 16 ? 16 / sizeof(T) : V;
 #pragma unroll
     for (int k = 0; k < V; k += W) {
-      const Vec<T, W> y = STREAM ? load_vec_nt<T, W>(p + k) : load_vec<T, W>(p + k);
+      const Vec<T, W> y = load_vec<T, W>(p + k);
 #pragma unroll
       for (int e = 0; e < W; ++e) x[k + e] = (float)y.v[e];
     }
@@ -115,7 +114,7 @@ __device__ __forceinline__ void load_values(const T *p, int64_t left, bool whole
     for (int e = 0; e < V; ++e) x[e] = e < left ? (float)p[e] : 0.f;
   }
 }
-template <typename T, int V, bool STREAM>
+template <typename T, int V>
 __device__ __forceinline__ void store_values(T *p, int64_t left, bool whole, const float (&x)[V]) {
   if (whole && left >= V) {
     constexpr int W = sizeof(T) * V > 16 ? 16 / sizeof(T) : V;
@@ -124,7 +123,7 @@ __device__ __forceinline__ void store_values(T *p, int64_t left, bool whole, con
       Vec<T, W> y;
 #pragma unroll
       for (int e = 0; e < W; ++e) y.v[e] = static_cast<T>(x[k + e]);
-      if constexpr (STREAM) store_vec_nt<T, W>(p + k, y); else store_vec<T, W>(p + k, y);
+      store_vec<T, W>(p + k, y);
     }
   } else {
 #pragma unroll
@@ -132,20 +131,20 @@ __device__ __forceinline__ void store_values(T *p, int64_t left, bool whole, con
       if (e < left) p[e] = static_cast<T>(x[e]);
   }
 }
-template <bool STREAM, int V>
+template <int V>
 __device__ __forceinline__ void load_as(const void *p, int type, int64_t i, int64_t left, bool whole, float (&x)[V]) {
   switch (type) {
-    case 0: load_values<float, V, STREAM>(static_cast<const float *>(p) + i, left, whole, x); break;
-    case 1: load_values<f16, V, STREAM>(static_cast<const f16 *>(p) + i, left, whole, x); break;
-    default: load_values<bf16, V, STREAM>(static_cast<const bf16 *>(p) + i, left, whole, x); break;
+    case 0: load_values<float, V>(static_cast<const float *>(p) + i, left, whole, x); break;
+    case 1: load_values<f16, V>(static_cast<const f16 *>(p) + i, left, whole, x); break;
+    default: load_values<bf16, V>(static_cast<const bf16 *>(p) + i, left, whole, x); break;
   }
 }
-template <bool STREAM, int V>
+template <int V>
 __device__ __forceinline__ void store_as(void *p, int type, int64_t i, int64_t left, bool whole, const float (&x)[V]) {
   switch (type) {
-    case 0: store_values<float, V, STREAM>(static_cast<float *>(p) + i, left, whole, x); break;
-    case 1: store_values<f16, V, STREAM>(static_cast<f16 *>(p) + i, left, whole, x); break;
-    default: store_values<bf16, V, STREAM>(static_cast<bf16 *>(p) + i, left, whole, x); break;
+    case 0: store_values<float, V>(static_cast<float *>(p) + i, left, whole, x); break;
+    case 1: store_values<f16, V>(static_cast<f16 *>(p) + i, left, whole, x); break;
+    default: store_values<bf16, V>(static_cast<bf16 *>(p) + i, left, whole, x); break;
   }
 }
 
@@ -174,7 +173,7 @@ template <int TOP> __device__ __forceinline__ uint32_t encode(uint32_t bits, uin
   return q < 8 ? 0 : q;
 }
 
-template <int BITS, bool STREAM>
+template <int BITS>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t per, const Moments mo,
                                                          const Factors *__restrict__ fs) {
   constexpr int V = BITS == 8 ? 8 : 4;  // 8: a row of 16 lanes holds a block
@@ -189,13 +188,13 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
     float p[V], g[V], m[V], v[V];
     uint32_t ms = 0, vs = 0;
     Vec<unsigned char, 8> mc, vc;
-    load_as<STREAM>(t.p[k], t.p_type[k], i, there ? left : 0, p_whole, p);
-    load_as<STREAM>(t.g[k], t.g_type[k], i, there ? left : 0, g_whole, g);
+    load_as(t.p[k], t.p_type[k], i, there ? left : 0, p_whole, p);
+    load_as(t.g[k], t.g_type[k], i, there ? left : 0, g_whole, g);
     if constexpr (BITS == 8) {
       if (there) {
         const unsigned char *pm = static_cast<const unsigned char *>(mo.m) + at, *pv = static_cast<const unsigned char *>(mo.v) + at;
-        mc = STREAM ? load_vec_nt<unsigned char, 8>(pm) : load_vec<unsigned char, 8>(pm);
-        vc = STREAM ? load_vec_nt<unsigned char, 8>(pv) : load_vec<unsigned char, 8>(pv);
+        mc = load_vec<unsigned char, 8>(pm);
+        vc = load_vec<unsigned char, 8>(pv);
         ms = mo.m_scale[at / kBlock];
         vs = mo.v_scale[at / kBlock];
       }
@@ -207,8 +206,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
         v[e] = decode<31>(there && e < left ? vc.v[e] : 0, vs);
       }
     } else {
-      load_values<float, V, STREAM>(static_cast<const float *>(mo.m) + at, there ? left : 0, true, m);
-      load_values<float, V, STREAM>(static_cast<const float *>(mo.v) + at, there ? left : 0, true, v);
+      load_values<float, V>(static_cast<const float *>(mo.m) + at, there ? left : 0, true, m);
+      load_values<float, V>(static_cast<const float *>(mo.v) + at, there ? left : 0, true, v);
     }
     {
 #pragma clang fp contract(off)
@@ -224,8 +223,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
       }
     }
     if (there) {
-      store_as<STREAM>(t.p[k], t.p_type[k], i, left, p_whole, p);
-      if (t.copy[k] != nullptr) store_as<STREAM>(t.copy[k], t.c_type[k], i, left, c_whole, p);
+      store_as(t.p[k], t.p_type[k], i, left, p_whole, p);
+      if (t.copy[k] != nullptr) store_as(t.copy[k], t.c_type[k], i, left, c_whole, p);
     }
     if constexpr (BITS == 8) {
       uint32_t mb[V], vb[V], ml = 0, vl = 0;
@@ -247,21 +246,16 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
       }
       if (there) {
         unsigned char *pm = static_cast<unsigned char *>(mo.m) + at, *pv = static_cast<unsigned char *>(mo.v) + at;
-        if constexpr (STREAM) {
-          store_vec_nt<unsigned char, 8>(pm, mc);
-          store_vec_nt<unsigned char, 8>(pv, vc);
-        } else {
-          store_vec<unsigned char, 8>(pm, mc);
-          store_vec<unsigned char, 8>(pv, vc);
-        }
+        store_vec<unsigned char, 8>(pm, mc);
+        store_vec<unsigned char, 8>(pv, vc);
         if (threadIdx.x % 16 == 0) {
           mo.m_scale[at / kBlock] = (unsigned char)ms;
           mo.v_scale[at / kBlock] = (unsigned char)vs;
         }
       }
     } else if (there) {
-      store_values<float, V, STREAM>(static_cast<float *>(mo.m) + at, left, true, m);
-      store_values<float, V, STREAM>(static_cast<float *>(mo.v) + at, left, true, v);
+      store_values<float, V>(static_cast<float *>(mo.m) + at, left, true, m);
+      store_values<float, V>(static_cast<float *>(mo.v) + at, left, true, v);
     }
   }
 }
@@ -281,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const unsigned char *
     const float size = decode<TOP>(c.v[e], s);
     x[e] = TOP == 15 && c.v[e] >= 128 ? -size : size;
   }
-  store_values<O, 8, true>(out + i, 8, true, x);
+  store_values<O, 8>(out + i, 8, true, x);
 }
 
 template <typename O>
@@ -308,7 +302,6 @@ hipError_t launch_adamw(const AdamwTensors &a, const AdamwMoments &mo, const Ada
   for (int k = 0; k < a.count; ++k) total += a.n[k];
   // whole rounds of a workgroup, and no more chunks than 2^31 / kThreads a launch
   const int64_t per = std::max<int64_t>(2048, (total / kChunks + 2047) / 2048 * 2048);
-  const bool past = total * (mo.bits == 8 ? 14 : 28) > kCached;
   const Moments m{mo.m, mo.v, mo.m_scale, mo.v_scale};
   int64_t at = 0;
   for (int k = 0; k < a.count;) {
@@ -332,9 +325,7 @@ hipError_t launch_adamw(const AdamwTensors &a, const AdamwMoments &mo, const Ada
     }
     if (t.count == 0) break;
     const dim3 grid(t.first[t.count]);
-    const auto kernel = mo.bits == 8 ? (past ? adamw_kernel<8, true> : adamw_kernel<8, false>)
-                                     : (past ? adamw_kernel<32, true> : adamw_kernel<32, false>);
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, t, per, m, f);
+    hipLaunchKernelGGL((mo.bits == 8 ? adamw_kernel<8> : adamw_kernel<32>), grid, dim3(kThreads), 0, stream, t, per, m, f);
     if (hipError_t e = hipGetLastError()) return e;
   }
   return hipSuccess;
