@@ -19,6 +19,11 @@
 // quarter of v. 20 random bits are added below the kept ones: 16 from a mixing of place, step and
 // seed, and a half (fewer would bias 1,000 steps' sum: 2^-16 of a step each is 0.1% of v). Same
 // seed, step and inputs: same results.
+//
+// Bound by memory: 15 M values with 32-bit moments 420 MB in 89 us from memory (4.7 TB/s, a copy's rate at that
+// size 5.2), 69 us where the state is still in the last-level cache; 109 M with 8-bit moments, bf16 gradients and
+// copies 1.75 GB in 390 us (4.5 TB/s); the codes' values as bf16 330 MB in 65 us. Non-temporal loads and stores:
+// 92 for 96 us a call from memory, 89 for 69 from the cache, not kept.
 #include <algorithm>
 
 #include "bevk_launch.h"

@@ -141,8 +141,9 @@ template <typename T> __device__ __forceinline__ void finish(const Epilogue &e, 
 // ---------------------------------------------------------------------------------------
 // Any sizes, strides and alignments: out[m][n] = sum_k a(m, k) b(n, k). A workgroup of four waves takes
 // 64 x 64 values, 32 terms at a time through LDS (rows padded by 16 bytes: no two of 8 neighbouring
-// rows' reads meet in a bank), elements loaded one by one. Few tiles of a long sum: the sum in parts,
-// added up in order by finish_kernel.
+// rows' reads meet in a bank). Eight neighbouring terms are loaded at once, from whatever address (114,075 x
+// 1,001 x 64 fp16: 89 us, 2.7 TB/s; 393 one by one). Few tiles of a long sum: the sum in parts, added up
+// in order by finish_kernel. Bound by the latency of its loads, which nothing else is under way beside.
 // ---------------------------------------------------------------------------------------
 template <typename T> struct Product {
   const T *a, *b;
@@ -261,9 +262,13 @@ hipError_t launch_any(const T *a, int64_t a_m, int64_t a_k, const T *b, int64_t 
 }
 
 // ---------------------------------------------------------------------------------------
-// 16-bit products of tiles: both operands' rows dense, K a multiple of 8, 16-byte aligned. A workgroup
-// of WM x WN waves takes BM x BN values, 64 terms at a time: rows of 128 bytes go straight from memory
-// into LDS (8 rows an instruction), the next step's while this one multiplies. A row's eight 16-byte
+// Products of tiles: both operands' rows dense, of a multiple of 16 bytes and on such boundaries. A workgroup
+// of WM x WN waves takes BM x BN values, 128 bytes of a row (64 terms of 16 bits) at a time: they go straight from
+// memory into LDS (8 rows an instruction), the next step's while this one multiplies, in products of 16 x 16
+// (of 32 x 32: 245 us where these take 235) that go before the other waves' instructions. Tiles whose
+// fragments of a whole step fit read them all before the first product (2,048 x 4,096 x 4,096: 65 us, 73 without).
+// 8,192 x 2,048 x 8,192 bf16: 235 us, 1,170 TF; silu, 242. Bound there by what the loads into LDS cost beside the
+// products (a quarter of them: 188 us); small ones by the latency of a step, 0.5 us. A row's eight 16-byte
 // pieces lie in the order piece ^ (row / 2 % 8), so that 16 neighbouring rows' reads of one piece
 // meet none of the 64 banks twice; the order is made by the address that a lane loads from, since it always
 // writes where its number says. Rows past the end are the last row's again and are not stored; terms
@@ -475,7 +480,8 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
 
 // ---------------------------------------------------------------------------------------
 // 16-bit products of many rows by a weight of few terms (K 256 or 512): bound by memory, where a tile of
-// few steps waits for its first loads and its stores. A workgroup of eight waves a CU keeps NT
+// few steps waits for its first loads and its stores: 184,950 x 256 x 256 fp16 45 us, 4.2 TB/s (a copy of as
+// much 6.0); 40,000 x 256 x 512 bf16 gelu with its slope 37 us (20 without either). A workgroup of eight waves a CU keeps NT
 // columns of the weight in LDS (128 KB) for the whole launch; each wave takes R x 16 rows at a time, whose
 // fragments it loads straight into registers, a whole 256 terms ahead, across the rows' ends.
 // Rows of the weight lie in LDS so that a lane ends up with eight neighbouring columns: row 16 j + 4 g + e
@@ -660,9 +666,10 @@ hipError_t launch_stream_of(StreamArgs p, hipStream_t stream) {
 
 // ---------------------------------------------------------------------------------------
 // Few rows (single tokens, a decoder's queries): the weight's bytes or the latency of a launch are the
-// bound. A workgroup of four waves takes 16 columns of up to MT x 16 rows; the waves take every
-// fourth 64 bytes of the rows, which they load straight into the fragments, eight loads of the weight in
-// flight; their sums meet in LDS. fp32 runs on the fp32 matrix cores.
+// bound. A workgroup of WAVES waves takes NT x 16 columns of MT x 16 rows; the waves take 64 bytes of the rows in
+// turn, which they load straight into the fragments, U loads ahead; their sums meet in LDS. fp32 runs on the
+// fp32 matrix cores. 300 x 256 x 256 fp16 4.3 us, of which a launch that does nothing has about 2.5; 4 x 2,048 x
+// 8,192 bf16 9.2 us (34 MB at 3.7 TB/s: 16 rows of 64 bytes a load are half the cache lines' width).
 // ---------------------------------------------------------------------------------------
 struct FewArgs {
   const void *a, *b;
@@ -752,12 +759,13 @@ hipError_t launch_tile_of(TileArgs p, hipStream_t stream) {
 }
 // Which kernel a product of dense rows takes. 16 bits, K 256 or 512 and enough rows for a few strips a
 // wave: the streaming kernel (measured at 40,000 x 256 x 512, 184,950 x 256 x 256, 20,000 x 256 x 4,096
-// and 184,950 x 512 x 256: 20.4, 43, 49 and 72 us, the fastest tile 24.5, 54, 76 and 80; below it
-// loses: 20,000 x 256 x 768 20.0 and 19.6, 40,000 x 512 x 256 22.2 and 20.3). Else the least of these
-// estimates in us, fitted to some 200 shapes from 1 x 256 x 256 to 40,000 x 4,096 x 1,024:
-//   tiles   rounds over the CUs, each of K / 64 steps that take the longer of a step's latency and what the
+// and 184,950 x 512 x 256: 20.4, 43, 49 and 72 us, the fastest tile 24.5, 54, 76 and 80). Else the least of these
+// estimates in us, fitted to some 200 shapes from 1 x 256 x 256 to 40,000 x 4,096 x 1,024, of whose
+// measured times the choice is 0.2% off the fastest in the mean:
+//   tiles   rounds over the CUs, each of steps of 128 bytes that take the longer of a step's latency and what the
 //           tiles on a CU take at its full rate, and what a round's first loads and stores take
 //   few     a CU's loads at 33 bytes a ns (each touches 16 rows' 64 bytes)
+// fp32: 64 x 64 tiles alone (larger ones were the faster by 5% at the most, below where the split product wins).
 enum Kind { kFew4, kFew8, kFew22, kFew42, kTile64, kTile64x128, kTile128, kTile256, kStream };
 struct Shape {
   int bm, bn, on_cu;          // rows and columns, workgroups on a CU
@@ -874,7 +882,8 @@ __global__ void __launch_bounds__(kThreads) act_kernel(T *__restrict__ y, const 
 // The streaming kernel for fp32: K 256 or 512, N a multiple of 4. NB x 16 columns of the split weight (its three planes
 // in the order of the fragments, 96 KB) stay in LDS, a wave takes 16 rows at a time, eight steps of 32 terms ahead,
 // and cuts its fragments as they come. A strip that meets a value that is not finite (or rounds to Inf as a bf16) is
-// computed again in plain fp32.
+// computed again in plain fp32. 40,000 x 256 x 256 36 us and 44 with a residual (82 and 123 MB, six products of bf16
+// for each of fp32: 31 GF at 880 TF): bound by the products and their operands' cutting.
 struct SplitStreamArgs {
   const float *a;
   const void *w;  // split weight, then its flags
@@ -1049,7 +1058,8 @@ hipError_t launch_split(const float *x, const float *weight, bool transposed, in
 }
 
 // ---------------------------------------------------------------------------------------
-// gz = gy slope and its column sums: a workgroup takes a range of rows of up to 256 vectors of columns;
+// gz = gy slope and its column sums, bound by memory (40,000 x 512 bf16: 123 MB in 25 us, 4.9 TB/s): a workgroup
+// takes a range of rows of up to 256 vectors of columns;
 // each thread keeps its columns' sums, the workgroup adds up its rows side by side and turn_kernel the
 // workgroups, in order; in the same launch it turns the weight for the gradient of x.
 // ---------------------------------------------------------------------------------------

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bevk_launch.h"
 

@@ -12,6 +12,10 @@
 // part of the parameters' sums in registers; at its end (for the gate: at the end of a set) they are
 // added over its rows in LDS and written to the workspace, and join_kernel adds up the workgroups' parts
 // in order: no atomics, the same results on every run.
+//
+// Bound by memory and by what a thread can have in flight beside its sums (a row ahead, two or three waves a
+// SIMD): 16,384 x 2,048 bf16 with both norms 336 MB in 80 us (4.2 TB/s; a workgroup a row and no prefetch
+// 147 us), 34,800 x 512 fp16 178 MB in 38 us (4.7), and 5 to 6 us for the parts' sums.
 #include "residual_norm.h"
 
 namespace bevk {
