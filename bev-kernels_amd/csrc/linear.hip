@@ -894,7 +894,7 @@ struct SplitStreamArgs {
 
 template <int ACT, bool RES, int K>
 __global__ void __launch_bounds__(512) split_stream_kernel(const SplitStreamArgs p) {
-  constexpr int S = K / 32, NB = 32 / S, WAVES = 8, BLOCK = S * 3072;  // S steps; bytes of 16 columns
+  constexpr int S = K / 32, NB = 32 / S, WAVES = 8, PIECE = 3 * 1024, BLOCK = S * PIECE;  // S steps; bytes of 16 columns
   __shared__ __attribute__((aligned(1024))) char w[NB * BLOCK];
   __shared__ __attribute__((aligned(16))) float bias[NB * 16];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -935,7 +935,7 @@ __global__ void __launch_bounds__(512) split_stream_kernel(const SplitStreamArgs
     const int j = unit % NB, k = unit / NB % S;
 #pragma unroll
     for (int q = 0; q < 3; ++q)
-      b[to][q] = *reinterpret_cast<const int4v *>(w + j * BLOCK + k * 3072 + q * 1024 + lane * 16);
+      b[to][q] = *reinterpret_cast<const int4v *>(w + j * BLOCK + k * PIECE + q * 1024 + lane * 16);
   };
   read(0, 0);
   for (; strip < p.strips; strip += step) {
@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(512) split_stream_kernel(const SplitStreamArgs
         floatx4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int k = 0; k < K; ++k) {
-          const char *blk = w + j * BLOCK + k / 32 * 3072 + k % 32 / 8 * 256 + k % 8 * 2 + g * 64;  // column 4 g
+          const char *blk = w + j * BLOCK + k / 32 * PIECE + k % 32 / 8 * 256 + k % 8 * 2 + g * 64;  // column 4 g
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float wv = 0.f;

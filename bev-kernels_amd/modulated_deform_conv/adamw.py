@@ -70,6 +70,9 @@ def adamw_step_(params, grads, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_d
         raise RuntimeError(f"adamw_step_: {len(grads)} gradients for {len(params)} parameters")
     if not params:
         raise RuntimeError("adamw_step_: no parameters")
+    for k, g in enumerate(grads):
+        if g is None:
+            raise RuntimeError(f"adamw_step_: parameter {k} has no gradient; give zeros, or leave it out of the state")
     if norm is not None and max_norm is None:
         raise RuntimeError("adamw_step_: norm without max_norm")
     if max_norm is not None and norm is None:

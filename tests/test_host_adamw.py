@@ -25,6 +25,8 @@ def test_needs_a_device():
         mdc.adamw_step_([], [], state, lr=0.1)
     with pytest.raises(RuntimeError, match="2 gradients for 1"):
         mdc.adamw_step_(p, g * 2, state, lr=0.1)
+    with pytest.raises(RuntimeError, match="parameter 0 has no gradient"):
+        mdc.adamw_step_(p, [None], state, lr=0.1, max_norm=1.0)
     with pytest.raises(RuntimeError, match="8 or 32"):
         mdc.adamw_state(p, bits=16)
     with pytest.raises(RuntimeError, match="no parameters"):
