@@ -7,7 +7,7 @@
 // Products of 16-bit types on the matrix cores with fp32 sums; bias, activation and residual in fp32 on the
 // sums in registers, one rounding at the end. The forward keeps the slope, as wide as the input, where the
 // backward needs it, which then has no exp to take (gz of 40,000 x 512 gelu bf16: 46 us from z, 24 from
-// the slope). gz is rounded to the input's type, which is what the matrix cores read.
+// the slope). gz of more than a few rows is rounded to the input's type, which is what the matrix cores read.
 #include <algorithm>
 #include <type_traits>
 
@@ -145,16 +145,19 @@ template <typename T> __device__ __forceinline__ void finish(const Epilogue &e, 
 // 1,001 x 64 fp16: 89 us, 2.7 TB/s; 393 one by one). Few tiles of a long sum: the sum in parts, added up
 // in order by finish_kernel. Bound by the latency of its loads, which nothing else is under way beside.
 // ---------------------------------------------------------------------------------------
-template <typename T> struct Product {
-  const T *a, *b;
+template <typename A, typename B> struct Product {
+  const A *a;
+  const B *b;
   int64_t a_m, a_k, b_n, b_k;
   int64_t M, K, per;  // per: terms of a part, a multiple of 32
   float *part;        // [parts][M][N], or null for one part
   Epilogue e;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) any_kernel(const Product<T> p, int64_t first) {
+// Operands of two types (few rows' gz in fp32 by 16-bit values) meet in fp32. O: the output's type.
+template <typename A, typename B, typename O>
+__global__ void __launch_bounds__(kThreads) any_kernel(const Product<A, B> p, int64_t first) {
+  using T = std::conditional_t<std::is_same_v<A, B>, A, float>;
   constexpr int P = 32 + 16 / (int)sizeof(T);
   __shared__ __attribute__((aligned(16))) T sa[64][P], sb[64][P];
   const int N = p.e.N;
@@ -164,22 +167,23 @@ __global__ void __launch_bounds__(kThreads) any_kernel(const Product<T> p, int64
   const int64_t k0 = z * p.per, k1 = min(p.K, k0 + p.per);
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   // a thread's 8 elements of each tile: along k where that is dense, else of one row after another
-  auto stage = [&](const T *src, int64_t by_row, int64_t by_k, int64_t row0, int64_t rows, int64_t k,
+  auto stage = [&](const auto *src, int64_t by_row, int64_t by_k, int64_t row0, int64_t rows, int64_t k,
                    T (&s)[64][P]) __attribute__((always_inline)) {
+    using S = std::remove_cv_t<std::remove_pointer_t<decltype(src)>>;
     const bool along = by_k == 1;
     const int r = along ? tid / 4 : tid % 64, c = (along ? tid % 4 : tid / 64) * 8;
-    const T *q = src + (row0 + r) * by_row;
+    const S *q = src + (row0 + r) * by_row;
     if (along && row0 + r < rows && k + c + 8 <= k1) {  // (loads of 16 bytes from any address)
-      struct __attribute__((packed, aligned(sizeof(T)))) Any { T v[8]; };
+      struct __attribute__((packed, aligned(sizeof(S)))) Any { S v[8]; };
       const Any v = *reinterpret_cast<const Any *>(q + k + c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[r][c + e] = v.v[e];
+      for (int e = 0; e < 8; ++e) s[r][c + e] = static_cast<T>(v.v[e]);
       return;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int64_t kk = k + c + e;
-      s[r][c + e] = row0 + r < rows && kk < k1 ? q[kk * by_k] : static_cast<T>(0.f);
+      s[r][c + e] = row0 + r < rows && kk < k1 ? static_cast<T>(q[kk * by_k]) : static_cast<T>(0.f);
     }
   };
   floatx4 acc[2][2] = {};
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) any_kernel(const Product<T> p, int64
         const int n = n0 + wave % 2 * 32 + j * 16 + lane / 16 * 4 + e;
         if (m >= p.M || n >= N) continue;
         if (p.part != nullptr) p.part[(z * p.M + m) * N + n] = acc[i][j][e];
-        else finish<T>(p.e, m, n, acc[i][j][e]);
+        else finish<O>(p.e, m, n, acc[i][j][e]);
       }
 }
 
@@ -234,8 +238,11 @@ struct AnyPlan {
   int64_t per;
 };
 AnyPlan any_plan(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64), want = 4 * std::max(1, device_cus());
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want / tiles, K / 256, 64}));
+  const int64_t tiles = ((M + 63) / 64) * ((N + 63) / 64), cus = std::max(1, device_cus());
+  // four workgroups a CU in parts of 256 terms or more, or one in shorter ones (300 x 1,001 x 64: 11 us, 18 in parts
+  // of 256; 5,000 x 1,001 x 64: 24 us in 12 parts, 19 in 3)
+  const int64_t long_parts = std::min(4 * cus / tiles, K / 256), short_parts = std::min(cus / tiles, K / 64);
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::max(long_parts, short_parts), 64));
   AnyPlan pl;
   pl.per = ((K + parts - 1) / parts + 31) / 32 * 32;
   pl.parts = (int)((K + pl.per - 1) / pl.per);
@@ -245,19 +252,19 @@ int64_t any_bytes(int64_t M, int64_t N, int64_t K) {
   const AnyPlan pl = any_plan(M, N, K);
   return pl.parts > 1 ? pl.parts * M * N * 4 : 0;
 }
-template <typename T>
-hipError_t launch_any(const T *a, int64_t a_m, int64_t a_k, const T *b, int64_t b_n, int64_t b_k, int64_t M, int64_t K,
+template <typename O, typename A, typename B>
+hipError_t launch_any(const A *a, int64_t a_m, int64_t a_k, const B *b, int64_t b_n, int64_t b_k, int64_t M, int64_t K,
                       const Epilogue &e, void *workspace, hipStream_t stream) {
   const AnyPlan pl = any_plan(M, e.N, K);
-  Product<T> p{a, b, a_m, a_k, b_n, b_k, M, K, pl.per, pl.parts > 1 ? static_cast<float *>(workspace) : nullptr, e};
+  Product<A, B> p{a, b, a_m, a_k, b_n, b_k, M, K, pl.per, pl.parts > 1 ? static_cast<float *>(workspace) : nullptr, e};
   const int64_t tiles = ((M + 63) / 64) * (((int64_t)e.N + 63) / 64) * pl.parts;
   hipError_t err = launch_in_parts(tiles, kThreads, [&](int64_t first, unsigned n) {
-    hipLaunchKernelGGL((any_kernel<T>), dim3(n), dim3(kThreads), 0, stream, p, first);
+    hipLaunchKernelGGL((any_kernel<A, B, O>), dim3(n), dim3(kThreads), 0, stream, p, first);
   });
   if (err != hipSuccess || pl.parts == 1) return err;
   const int64_t total = M * e.N;
   return launch_in_parts((total + kThreads - 1) / kThreads, kThreads, [&](int64_t first, unsigned n) {
-    hipLaunchKernelGGL((finish_kernel<T>), dim3(n), dim3(kThreads), 0, stream, e, p.part, pl.parts, total, first);
+    hipLaunchKernelGGL((finish_kernel<O>), dim3(n), dim3(kThreads), 0, stream, e, p.part, pl.parts, total, first);
   });
 }
 
@@ -1065,9 +1072,9 @@ hipError_t launch_split(const float *x, const float *weight, bool transposed, in
 // ---------------------------------------------------------------------------------------
 constexpr int kSumBlocks = 1024;
 
-template <typename T, int V>
+template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ gy, const T *__restrict__ slope,
-                                                          T *__restrict__ gz, int act, int64_t rows, int n, int per,
+                                                          O *__restrict__ gz, int act, int64_t rows, int n, int per,
                                                           float *__restrict__ part) {
   __shared__ float s[kThreads][V + 1];
   const int lanes = kThreads / per, col = (blockIdx.x * per + threadIdx.x % per) * V, row = threadIdx.x / per;
@@ -1079,19 +1086,20 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
 #pragma unroll 4
     for (int64_t r = r0 + row; r < r1; r += lanes) {
       const int64_t at = r * n + col;
-      Vec<T, V> g = load_vec<T, V>(gy + at);
+      const Vec<T, V> g = load_vec<T, V>(gy + at);
       float z[V];  // (the sums are those of gz before its rounding)
 #pragma unroll
       for (int e = 0; e < V; ++e) z[e] = (float)g.v[e];
       if (act != kActNone) {
         const Vec<T, V> x = load_vec<T, V>(slope + at);
+        Vec<O, V> out;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (act == kActRelu) z[e] = (float)x.v[e] <= 0.f ? 0.f : z[e];  // (slope, or y)
           else z[e] *= kept_slope(x.v[e]);
-          g.v[e] = static_cast<T>(z[e]);
+          out.v[e] = static_cast<O>(z[e]);
         }
-        store_vec<T, V>(gz + at, g);
+        store_vec<O, V>(gz + at, out);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) a[e] += z[e];
@@ -1160,18 +1168,18 @@ int sum_blocks(int64_t rows, int n) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({kSumBlocks, rows / 16, (1 << 22) / n}));
 }
 
-template <typename T, int V>
-hipError_t launch_grad_z_v(const T *gy, const T *slope, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
+template <int V, typename T, typename O>
+hipError_t launch_grad_z_v(const T *gy, const T *slope, O *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   const int vecs = (n + V - 1) / V, per = std::min(vecs, kThreads);
-  hipLaunchKernelGGL((grad_z_kernel<T, V>), dim3((vecs + per - 1) / per, sum_blocks(rows, n)), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((grad_z_kernel<T, O, V>), dim3((vecs + per - 1) / per, sum_blocks(rows, n)), dim3(kThreads), 0, stream,
                      gy, slope, gz, act, rows, n, per, part);
   return hipGetLastError();
 }
-template <typename T>
-hipError_t launch_grad_z(const T *gy, const T *slope, T *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
+template <typename T, typename O>
+hipError_t launch_grad_z(const T *gy, const T *slope, O *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<T, V>(gy, slope, gz, act, rows, n, part, stream)
-                                              : launch_grad_z_v<T, 1>(gy, slope, gz, act, rows, n, part, stream);
+  return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<V>(gy, slope, gz, act, rows, n, part, stream)
+                                              : launch_grad_z_v<1>(gy, slope, gz, act, rows, n, part, stream);
 }
 // The bias' gradient (or null for none) and, with `turn`, the weight turned.
 template <typename T>
@@ -1231,6 +1239,13 @@ bool weight_grad_takes(int dtype, const LinearArgs &a) {
          runs < 1 << 23;
 }
 
+// Few rows of 16 bits keep gz in fp32, and their products meet in fp32 (any_kernel): gradients with one rounding
+// (relative error 0.0017 in bf16, with gz rounded 0.0024 and for one row up to 0.0028), without the weight's
+// turning. The whole backward of 4 x 2,048 x 8,192 takes 101 us, by the kernels for more rows 177; 4 x 256 x 512 22
+// and 16, 64 x 256 x 512 31 and 19, which is why more rows than one product of 16 take the others.
+constexpr int64_t kWideRows = 16;
+bool keeps_wide(int dtype, const LinearArgs &a) { return dtype != 0 && a.act != kActNone && a.rows <= kWideRows; }
+
 // Workspace of the backward: gz, the bias' parts, then what the products take.
 struct BackWs {
   int64_t part, product, total;
@@ -1238,7 +1253,7 @@ struct BackWs {
 BackWs back_ws(int dtype, const LinearArgs &a) {
   const int64_t size = dtype == 0 ? 4 : 2;
   BackWs w;
-  w.part = a.act != kActNone ? up(a.rows * a.N * size) : 0;
+  w.part = a.act != kActNone ? up(a.rows * a.N * (keeps_wide(dtype, a) ? 4 : size)) : 0;
   w.product = w.part + up((int64_t)sum_blocks(a.rows, a.N) * a.N * 4);
   int64_t grad_w = any_bytes(a.N, a.K, a.rows);
   if (weight_grad_takes(dtype, a)) grad_w = std::max(grad_w, weight_grad_workspace_bytes(dtype, a.rows, a.K, 1, a.N));
@@ -1255,9 +1270,20 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
   const T *gy = static_cast<const T *>(grad_y), *gz = gy, *x = static_cast<const T *>(a.x);
   const T *weight = static_cast<const T *>(a.weight);
   float *part = grad_b != nullptr ? reinterpret_cast<float *>(base + ws.part) : nullptr;
+  if (keeps_wide(dtype, a)) {
+    float *wide = reinterpret_cast<float *>(base);
+    if (hipError_t e = launch_grad_z(gy, static_cast<const T *>(slope), wide, a.act, a.rows, a.N, part, stream)) return e;
+    if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, false, nullptr, stream)) return e;
+    Epilogue e{nullptr, nullptr, grad_x, nullptr, false, kActNone, a.K};
+    if (grad_x != nullptr)
+      if (hipError_t err = launch_any<T>(wide, a.N, 1, weight, 1, a.K, a.rows, a.N, e, base + ws.product, stream)) return err;
+    e.y = grad_w;
+    if (grad_w == nullptr) return hipSuccess;
+    return launch_any<T>(wide, 1, a.N, x, 1, a.K, a.N, a.rows, e, base + ws.product, stream);
+  }
   if (a.act != kActNone) gz = reinterpret_cast<T *>(base);
   if (a.act != kActNone || grad_b != nullptr)
-    if (hipError_t e = launch_grad_z<T>(gy, static_cast<const T *>(slope), const_cast<T *>(gz), a.act, a.rows, a.N, part, stream))
+    if (hipError_t e = launch_grad_z(gy, static_cast<const T *>(slope), const_cast<T *>(gz), a.act, a.rows, a.N, part, stream))
       return e;
   const bool turn = grad_x != nullptr && route(gz, weight, true, a.rows, a.K, a.N) == kRows;
   if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, turn, base + ws.product, stream)) return e;

@@ -241,6 +241,33 @@ def test_relu_of_nan(rows, features, residual, dtype):
     assert torch.equal(gx[2], plain[2]) and not torch.equal(gx, plain)
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("size", [(1, 1, 1), (1, 100, 300), (1, 256, 256), (3, 33, 1), (2, 1, 40), (7, 2048, 512), (15, 257, 1001),
+                                  (16, 64, 64), (16, 1024, 1024)], ids=str)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_gradients_of_few_rows(size, dtype, act):
+    """Up to 16 rows of 16 bits: gz is not rounded, so the gradients have one rounding. The slope is off by its
+    half step 2^-16, exp's and the formula's roundings (below 32 u of 1.13) and what z's error does to it (its
+    derivative is below 0.8); each product adds its own and its sum's."""
+    rows, k, n = size
+    t, gy = _inputs(rows, k, n, TYPES[dtype], sum(size) + 1, False)
+    _, grads = _check(t, gy, act)
+    if act == "relu":  # (next to 0 the sign of z is not certain)
+        return
+    u, d = 2.0 ** -24, {m: v.double() for m, v in t.items() if v is not None}
+    z = (d["x"] @ d["weight"].t() + d["bias"]).requires_grad_()
+    gz, = torch.autograd.grad(getattr(torch.nn.functional, act)(z), z, gy.double())
+    z_err = (k / 4 + 28) * u * (d["x"].abs() @ d["weight"].abs().t() + d["bias"].abs())
+    gz_err = gy.double().abs() * (2.0 ** -16 + 32 * 1.13 * u + 0.8 * z_err) + u * gz.abs()
+    for name, ref, err, mag, terms in (
+            ("x", gz @ d["weight"], gz_err @ d["weight"].abs(), gz.abs() @ d["weight"].abs(), n),
+            ("weight", gz.t() @ d["x"], gz_err.t() @ d["x"].abs(), gz.abs().t() @ d["x"].abs(), rows)):
+        err = err + (terms + 28) * u * (mag + err)
+        half = _half_step(TYPES[dtype])
+        bound = err + half * (ref.abs() + err) + torch.finfo(TYPES[dtype]).smallest_normal * half
+        assert ((grads[name].cpu().double() - ref).abs() <= bound).all(), name
+
+
 def test_empty():
     from msda_opt2 import linear_act
     x = torch.zeros(0, 5, 32, device=DEV, requires_grad=True)
