@@ -165,11 +165,12 @@ hipError_t launch_f32_tconv(const DcnGeom &g, const float *y32, const void *w_sp
 
 // Weight gradient [Cout][C][T] (out_dtype) = sum over the M pixels of dout [M][Cout] times cols
 // [M][T*C] (both dtype). Cout and C multiples of 16 bytes' worth of elements, T <= 25; the
-// workspace holds weight_grad_workspace_bytes.
-int64_t weight_grad_workspace_bytes(int dtype, int64_t M, int C, int T, int cout);
+// workspace holds weight_grad_workspace_bytes. halves 2 (16 bits): dout is [M][2][Cout], its
+// value the sum of a row's two.
+int64_t weight_grad_workspace_bytes(int dtype, int64_t M, int C, int T, int cout, int halves = 1);
 hipError_t launch_weight_grad(int dtype, const void *cols, const void *dout, int64_t M, int C, int T,
                               int cout, void *workspace, int out_dtype, void *grad_w,
-                              hipStream_t stream);
+                              hipStream_t stream, int halves = 1);
 
 // The offset conv's weight gradient [n3][C][T] (out_dtype) from its input x [B, H, W, C] and fp32
 // output gradient y32 [M][32] (n3 <= 32 columns used; C % 4 == 0).

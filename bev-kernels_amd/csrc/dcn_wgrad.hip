@@ -94,11 +94,15 @@ __device__ __forceinline__ int frag_at(int col, int oct) {
   return (oct >> 2) * (COLS * 64) + blk * 1024 + (oct & 3) * 256 + (((col & 15) + blk) & 15) * 16;
 }
 
-template <typename T, typename X, int TN, bool CONV>
+// HALVES 2 (16 bits): dO is the sum of two, the second N values behind the first in each row. Both meet the
+// same fragments of the columns (40,000 x 256 x 512 bf16 39 us, with one 31).
+template <typename T, typename X, int TN, bool CONV, int HALVES = 1>
 __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams p) {
   using KD = Kind<T, X>;
   using MT = typename KD::M;
-  constexpr int PA = KD::PA, PB = KD::PB, V = KD::V, ST = KD::kStep;
+  constexpr bool RAW = KD::PA == 1;  // the operands go to the matrix cores as they are
+  static_assert(RAW || HALVES == 1, "halves of 16 bits");
+  constexpr int PA = RAW ? HALVES : KD::PA, PB = KD::PB, V = KD::V, ST = KD::kStep;
   constexpr int kA = TN * ST * 2, kB = kTK * ST * 2;  // bytes of one plane of each operand
   constexpr int RA = TN / 32, RB = 4;                 // 16-blocks per wave: dO, columns
   __shared__ __attribute__((aligned(16))) char lds[PA * kA + PB * kB];
@@ -149,8 +153,15 @@ __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams 
       if (++ch == p.Ho) { ch = 0; ++cb; }
     }
   };
-  uint4v v[8];
+  uint4v v[8], second[HALVES == 2 ? 8 : 1];
   auto load = [&](int s) __attribute__((always_inline)) {
+    if constexpr (HALVES == 2)
+      if (is_a) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          second[r] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(
+              ra, voff + (uint32_t)p.N * (uint32_t)sizeof(T) + (uint32_t)(s * ST) * ld + r * ld, 0, 0));
+      }
     if (is_a || !CONV) {
       const uint32_t so = (uint32_t)(s * ST) * ld;
 #pragma unroll
@@ -218,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams 
       for (int q = 0; q < NP; ++q) *reinterpret_cast<int4v *>(d + q * plane) = o[q];
     }
   };
-  auto store_raw = [&](char *base, auto cols_tag) __attribute__((always_inline)) {
+  auto store_raw = [&](char *base, auto cols_tag, const auto &v) __attribute__((always_inline)) {
     constexpr int COLS = decltype(cols_tag)::value;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -235,10 +246,11 @@ __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams 
     using CB = std::integral_constant<int, kTK>;
     if (!live) return;
     if (is_a) {
-      if constexpr (PA == 1) store_raw(lds, CA{});
+      if constexpr (RAW) store_raw(lds, CA{}, v);
       else store_cut(lds, kA, CA{}, float{});
+      if constexpr (HALVES == 2) store_raw(lds + kA, CA{}, second);
     } else {
-      if constexpr (PA == 1) store_raw(lds + PA * kA, CB{});
+      if constexpr (RAW) store_raw(lds + PA * kA, CB{}, v);
       else store_cut(lds + PA * kA, kB, CB{}, X{});
     }
   };
@@ -272,9 +284,11 @@ __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams 
         int4v b[PB];
 #pragma unroll
         for (int q = 0; q < PB; ++q) b[q] = frag(lb, wb + j, q * kB);
-        if constexpr (PA == 1) {
+        if constexpr (RAW) {
 #pragma unroll
-          for (int i = 0; i < RA; ++i) acc[i][j] = mfma<MT>(a[i][0], b[0], acc[i][j]);
+          for (int q = PA - 1; q >= 0; --q)
+#pragma unroll
+            for (int i = 0; i < RA; ++i) acc[i][j] = mfma<MT>(a[i][q], b[0], acc[i][j]);
         } else {
           // small products (piece qa of dO, qb of the columns, qa + qb <= 2), then the large one
           floatx4 lo[RA];
@@ -299,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) weight_grad_kernel(const WParams 
 
   // Lane: column k = 16 j + (lane & 15), channels n = 16 i + 4 (lane >> 4) + e.
   float *out = p.part + (int64_t)part * p.N * p.K;
-  if constexpr (PA == 3) {
+  if constexpr (!RAW) {
     if (__syncthreads_or(!(nf == nf))) {
       // plain fp32: column tid % 128, every second channel
       const float *dp = static_cast<const float *>(p.dout) + (int64_t)m0 * p.ldn;
@@ -371,14 +385,14 @@ __global__ void __launch_bounds__(kThreads) weight_grad_reduce(const float *__re
 struct Plan {
   int tn, parts, rows;
 };
-Plan plan(int dtype, int64_t M, int64_t N, int64_t K, bool conv = false) {
+Plan plan(int dtype, int64_t M, int64_t N, int64_t K, bool conv = false, int halves = 1) {
   const int es = dtype == 0 ? 4 : 2, st = dtype == 0 ? 32 : 64;
   Plan pl;
   pl.tn = conv ? 32 : N > 64 ? 128 : 64;
   const double step_us = conv ? 0.7 : dtype == 0 ? (N > 64 ? 1.83 : 1.0) : (N > 64 ? 0.7 : 0.45);
   const int64_t tiles = ((N + pl.tn - 1) / pl.tn) * ((K + kTK - 1) / kTK);
   const int64_t steps = (M + st - 1) / st, cus = std::max(1, device_cus());
-  const int64_t cap = (((int64_t)1 << 31) - 4096) / (std::max(N, K) * es * st);
+  const int64_t cap = (((int64_t)1 << 31) - 4096) / (std::max(N * halves, K) * es * st);
   int64_t best = 0;
   double best_t = 0;
   for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 64) || best == 0; ++parts) {
@@ -400,6 +414,12 @@ Plan plan(int dtype, int64_t M, int64_t N, int64_t K, bool conv = false) {
 template <typename T>
 void launch_tn(const WParams &p, int tn, hipStream_t stream) {
   const dim3 g(8 * p.per_xcd), b(kThreads);
+  if constexpr (sizeof(T) == 2)
+    if (p.ldn != p.N) {
+      if (tn == 128) hipLaunchKernelGGL((weight_grad_kernel<T, T, 128, false, 2>), g, b, 0, stream, p);
+      else hipLaunchKernelGGL((weight_grad_kernel<T, T, 64, false, 2>), g, b, 0, stream, p);
+      return;
+    }
   if (tn == 128) hipLaunchKernelGGL((weight_grad_kernel<T, T, 128, false>), g, b, 0, stream, p);
   else hipLaunchKernelGGL((weight_grad_kernel<T, T, 64, false>), g, b, 0, stream, p);
 }
@@ -471,19 +491,19 @@ __global__ void __launch_bounds__(64) column_sums_total(const float *__restrict_
 
 }  // namespace
 
-int64_t weight_grad_workspace_bytes(int dtype, int64_t M, int C, int T, int cout) {
+int64_t weight_grad_workspace_bytes(int dtype, int64_t M, int C, int T, int cout, int halves) {
   const int64_t K = (int64_t)C * T;
-  return plan(dtype, M, cout, K).parts * (int64_t)cout * K * 4;
+  return plan(dtype, M, cout, K, false, halves).parts * (int64_t)cout * K * 4;
 }
 
 hipError_t launch_weight_grad(int dtype, const void *cols, const void *dout, int64_t M, int C, int T,
                               int cout, void *workspace, int out_dtype, void *grad_w,
-                              hipStream_t stream) {
+                              hipStream_t stream, int halves) {
   const int K = C * T;
-  const Plan pl = plan(dtype, M, cout, K);
+  const Plan pl = plan(dtype, M, cout, K, false, halves);
   WParams p{};
   p.dout = dout; p.cols = cols; p.part = static_cast<float *>(workspace);
-  p.M = (int)M; p.N = cout; p.K = K; p.ldn = cout;
+  p.M = (int)M; p.N = cout; p.K = K; p.ldn = cout * halves;
   p.rows = pl.rows; p.parts = pl.parts;
   p.ntn = (cout + pl.tn - 1) / pl.tn;
   p.ntk = (K + kTK - 1) / kTK;

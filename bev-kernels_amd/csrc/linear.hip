@@ -7,7 +7,8 @@
 // Products of 16-bit types on the matrix cores with fp32 sums; bias, activation and residual in fp32 on the
 // sums in registers, one rounding at the end. The forward keeps the slope, as wide as the input, where the
 // backward needs it, which then has no exp to take (gz of 40,000 x 512 gelu bf16: 46 us from z, 24 from
-// the slope). gz of more than a few rows is rounded to the input's type, which is what the matrix cores read.
+// the slope). gz of 16-bit types is kept as two values of the type, what the first leaves in the second: the
+// matrix cores read 16 bits, and one value's rounding would be as large an error of gx and gW as their own.
 #include <algorithm>
 #include <type_traits>
 
@@ -152,6 +153,8 @@ template <typename A, typename B> struct Product {
   int64_t M, K, per;  // per: terms of a part, a multiple of 32
   float *part;        // [parts][M][N], or null for one part
   Epilogue e;
+  int halves;         // 2: a is the sum of two, the second a_half behind
+  int64_t a_half;
 };
 
 // Operands of two types (few rows' gz in fp32 by 16-bit values) meet in fp32. O: the output's type.
@@ -188,25 +191,26 @@ __global__ void __launch_bounds__(kThreads) any_kernel(const Product<A, B> p, in
   };
   floatx4 acc[2][2] = {};
   const int ra = wave / 2 * 32 + lane % 16, rb = wave % 2 * 32 + lane % 16, c = lane / 16 * 8;
-  for (int64_t k = k0; k < k1; k += 32) {
-    stage(p.a, p.a_m, p.a_k, m0, p.M, k, sa);
-    stage(p.b, p.b_n, p.b_k, n0, N, k, sb);
-    __syncthreads();
+  for (int half = 0; half < p.halves; ++half)
+    for (int64_t k = k0; k < k1; k += 32) {
+      stage(p.a + half * p.a_half, p.a_m, p.a_k, m0, p.M, k, sa);
+      stage(p.b, p.b_n, p.b_k, n0, N, k, sb);
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const T *qa = &sa[ra + i * 16][c], *qb = &sb[rb + j * 16][c];
-        if constexpr (sizeof(T) == 2) {
-          acc[i][j] = mfma16(*reinterpret_cast<const int4v *>(qb), *reinterpret_cast<const int4v *>(qa), acc[i][j], T());
-        } else {
+        for (int j = 0; j < 2; ++j) {
+          const T *qa = &sa[ra + i * 16][c], *qb = &sb[rb + j * 16][c];
+          if constexpr (sizeof(T) == 2) {
+            acc[i][j] = mfma16(*reinterpret_cast<const int4v *>(qb), *reinterpret_cast<const int4v *>(qa), acc[i][j], T());
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qb[e], qa[e], acc[i][j], 0, 0, 0);
+            for (int e = 0; e < 8; ++e)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(qb[e], qa[e], acc[i][j], 0, 0, 0);
+          }
         }
-      }
-    __syncthreads();
-  }
+      __syncthreads();
+    }
   // a lane holds one m and four neighbouring n
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -254,9 +258,10 @@ int64_t any_bytes(int64_t M, int64_t N, int64_t K) {
 }
 template <typename O, typename A, typename B>
 hipError_t launch_any(const A *a, int64_t a_m, int64_t a_k, const B *b, int64_t b_n, int64_t b_k, int64_t M, int64_t K,
-                      const Epilogue &e, void *workspace, hipStream_t stream) {
+                      const Epilogue &e, void *workspace, hipStream_t stream, int halves = 1, int64_t a_half = 0) {
   const AnyPlan pl = any_plan(M, e.N, K);
-  Product<A, B> p{a, b, a_m, a_k, b_n, b_k, M, K, pl.per, pl.parts > 1 ? static_cast<float *>(workspace) : nullptr, e};
+  Product<A, B> p{a, b, a_m, a_k, b_n, b_k, M, K, pl.per, pl.parts > 1 ? static_cast<float *>(workspace) : nullptr, e,
+                  halves, a_half};
   const int64_t tiles = ((M + 63) / 64) * (((int64_t)e.N + 63) / 64) * pl.parts;
   hipError_t err = launch_in_parts(tiles, kThreads, [&](int64_t first, unsigned n) {
     hipLaunchKernelGGL((any_kernel<A, B, O>), dim3(n), dim3(kThreads), 0, stream, p, first);
@@ -1065,14 +1070,25 @@ hipError_t launch_split(const float *x, const float *weight, bool transposed, in
 }
 
 // ---------------------------------------------------------------------------------------
-// gz = gy slope and its column sums, bound by memory (40,000 x 512 bf16: 123 MB in 25 us, 4.9 TB/s): a workgroup
+// gz = gy slope and its column sums, bound by memory (40,000 x 512 bf16, gz in two values: 164 MB in 31 us, 5.2 TB/s): a workgroup
 // takes a range of rows of up to 256 vectors of columns;
 // each thread keeps its columns' sums, the workgroup adds up its rows side by side and turn_kernel the
 // workgroups, in order; in the same launch it turns the weight for the gradient of x.
 // ---------------------------------------------------------------------------------------
 constexpr int kSumBlocks = 1024;
 
-template <typename T, typename O, int V>
+// v = first + second: the nearest value of T, kept finite where v is (a slope is up to 1.13, so gz may leave T's
+// range), and the nearest to what it leaves (|second| at most half a step of first, its own error 2^-8 of that
+// in bf16). NaN and Inf are the first's alone.
+template <typename T> __device__ __forceinline__ void in_two(float v, T &first, T &second) {
+  constexpr float kMost = std::is_same_v<T, f16> ? 65504.f : 3.38953139e38f;
+  const bool finite = __builtin_fabsf(v) <= 3.402823466e38f;
+  first = static_cast<T>(finite ? __builtin_amdgcn_fmed3f(v, -kMost, kMost) : v);
+  second = static_cast<T>(finite ? v - (float)first : 0.f);
+}
+
+// PAIR: gz in two values, a row's first ones and then its second ones.
+template <typename T, typename O, int V, bool PAIR>
 __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ gy, const T *__restrict__ slope,
                                                           O *__restrict__ gz, int act, int64_t rows, int n, int per,
                                                           float *__restrict__ part) {
@@ -1092,14 +1108,17 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
       for (int e = 0; e < V; ++e) z[e] = (float)g.v[e];
       if (act != kActNone) {
         const Vec<T, V> x = load_vec<T, V>(slope + at);
-        Vec<O, V> out;
+        Vec<O, V> out, rest;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (act == kActRelu) z[e] = (float)x.v[e] <= 0.f ? 0.f : z[e];  // (slope, or y)
           else z[e] *= kept_slope(x.v[e]);
-          out.v[e] = static_cast<O>(z[e]);
+          if constexpr (PAIR) in_two(z[e], out.v[e], rest.v[e]);
+          else out.v[e] = static_cast<O>(z[e]);
         }
-        store_vec<O, V>(gz + at, out);
+        O *to = gz + (PAIR ? at + r * n : at);
+        store_vec<O, V>(to, out);
+        if constexpr (PAIR) store_vec<O, V>(to + n, rest);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) a[e] += z[e];
@@ -1118,14 +1137,14 @@ __global__ void __launch_bounds__(kThreads) grad_z_kernel(const T *__restrict__ 
 }
 
 // The first `sums` workgroups: 16 columns each, 64 threads add up every 64th part, then in order. The others:
-// 64 x 64 values of weight [rows][cols] into turned [cols][rows].
+// 64 x 64 values of weight [rows][cols] into turned [cols][halves][rows].
 struct TurnArgs {
   const float *part;
   int parts, n, sums;
   void *out;
   const void *weight;
   void *turned;
-  int rows, cols;
+  int rows, cols, halves;
 };
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p, int64_t first) {
@@ -1160,7 +1179,8 @@ __global__ void __launch_bounds__(1024) turn_kernel(const TurnArgs p, int64_t fi
   __syncthreads();
 #pragma unroll
   for (int i = threadIdx.x / 64; i < 64; i += 16)
-    if (c0 + i < p.cols && r0 + lane < p.rows) t[(int64_t)(c0 + i) * p.rows + r0 + lane] = tile[lane][i];
+    if (c0 + i < p.cols && r0 + lane < p.rows)
+      for (int h = 0; h < p.halves; ++h) t[((int64_t)(c0 + i) * p.halves + h) * p.rows + r0 + lane] = tile[lane][i];
 }
 
 // (a launch of many columns has workgroups enough: its grid and the parts' memory stay small)
@@ -1168,25 +1188,25 @@ int sum_blocks(int64_t rows, int n) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({kSumBlocks, rows / 16, (1 << 22) / n}));
 }
 
-template <int V, typename T, typename O>
+template <int V, bool PAIR, typename T, typename O>
 hipError_t launch_grad_z_v(const T *gy, const T *slope, O *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   const int vecs = (n + V - 1) / V, per = std::min(vecs, kThreads);
-  hipLaunchKernelGGL((grad_z_kernel<T, O, V>), dim3((vecs + per - 1) / per, sum_blocks(rows, n)), dim3(kThreads), 0, stream,
+  hipLaunchKernelGGL((grad_z_kernel<T, O, V, PAIR>), dim3((vecs + per - 1) / per, sum_blocks(rows, n)), dim3(kThreads), 0, stream,
                      gy, slope, gz, act, rows, n, per, part);
   return hipGetLastError();
 }
-template <typename T, typename O>
+template <bool PAIR, typename T, typename O>
 hipError_t launch_grad_z(const T *gy, const T *slope, O *gz, int act, int64_t rows, int n, float *part, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<V>(gy, slope, gz, act, rows, n, part, stream)
-                                              : launch_grad_z_v<1>(gy, slope, gz, act, rows, n, part, stream);
+  return n % V == 0 && on_16({gy, slope, gz}) ? launch_grad_z_v<V, PAIR>(gy, slope, gz, act, rows, n, part, stream)
+                                              : launch_grad_z_v<1, PAIR>(gy, slope, gz, act, rows, n, part, stream);
 }
-// The bias' gradient (or null for none) and, with `turn`, the weight turned.
+// The bias' gradient (or null for none) and, where `halves` is not 0, the weight turned, that many times side by side.
 template <typename T>
-hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wide, const LinearArgs &a, bool turn,
+hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wide, const LinearArgs &a, int halves,
                        void *turned, hipStream_t stream) {
-  const TurnArgs p{part, sum_blocks(rows, a.N), a.N, grad_bias != nullptr ? (a.N + 15) / 16 : 0, grad_bias, a.weight, turned, a.N, a.K};
-  const int64_t tiles = turn ? ((a.N + 63) / 64) * (int64_t)((a.K + 63) / 64) : 0;
+  const TurnArgs p{part, sum_blocks(rows, a.N), a.N, grad_bias != nullptr ? (a.N + 15) / 16 : 0, grad_bias, a.weight, turned, a.N, a.K, halves};
+  const int64_t tiles = halves > 0 ? ((a.N + 63) / 64) * (int64_t)((a.K + 63) / 64) : 0;
   return launch_in_parts(p.sums + tiles, 1024, [&](int64_t first, unsigned n) {
     if (wide) hipLaunchKernelGGL((turn_kernel<T, true>), dim3(n), dim3(1024), 0, stream, p, first);
     else hipLaunchKernelGGL((turn_kernel<T, false>), dim3(n), dim3(1024), 0, stream, p, first);
@@ -1199,27 +1219,30 @@ hipError_t launch_turn(const float *part, int64_t rows, void *grad_bias, bool wi
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 enum Route { kAny, kSplit, kRows };
-template <typename T> Route route(const T *x, const T *weight, bool transposed, int64_t M, int N, int K) {
+template <typename T> Route route(const T *x, const T *weight, bool transposed, int64_t M, int64_t N, int64_t K) {
   if (sizeof(T) == 4 && split_takes(x, weight, N, K, transposed) && split_pays(M, N, K)) return kSplit;
   return rows_take(x, transposed ? nullptr : weight, K, sizeof(T)) ? kRows : kAny;
 }
-// What a product of rows x [M][K] by weight [N][K] (transposed: [K][N]) needs, its operands on 16-byte boundaries or not.
-int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t K, bool aligned) {
+// What a product of rows x [M][halves][K] by weight [N][K] (transposed: [K][N]) needs, its operands on 16-byte boundaries
+// or not.
+int64_t product_bytes(int dtype, bool transposed, int64_t M, int64_t N, int64_t K, bool aligned, int halves = 1) {
   if (!aligned) return any_bytes(M, N, K);
   switch (dtype == 0 ? route<float>(nullptr, nullptr, transposed, M, N, K)
-                     : route<f16>(nullptr, nullptr, transposed, M, N, K)) {
+                     : route<f16>(nullptr, nullptr, transposed, M, N, K * halves)) {
     case kSplit: return f32_split_weight_bytes(N, K);
-    case kRows: return transposed ? up(N * K * (dtype == 0 ? 4 : 2)) : 0;
+    case kRows: return transposed ? up(N * K * halves * (dtype == 0 ? 4 : 2)) : 0;
     default: return any_bytes(M, N, K);
   }
 }
-// transposed: of kRows the workspace holds the weight's transpose already (it is small next to the rows)
+// transposed: of kRows the workspace holds the weight's transpose already (it is small next to the rows), for each
+// of x's halves, whose sum is then one product of twice the terms
 template <typename T>
 hipError_t product(const T *x, const T *weight, bool transposed, int64_t M, int K, const Epilogue &e, void *workspace,
-                   hipStream_t stream) {
-  switch (route(x, weight, transposed, M, e.N, K)) {
-    case kAny: return launch_any<T>(x, K, 1, weight, transposed ? 1 : K, transposed ? e.N : 1, M, K, e, workspace, stream);
-    case kRows: return launch_rows(x, transposed ? static_cast<const T *>(workspace) : weight, M, K, e, stream);
+                   hipStream_t stream, int halves = 1) {
+  switch (route(x, weight, transposed, M, e.N, K * halves)) {
+    case kAny: return launch_any<T>(x, (int64_t)K * halves, 1, weight, transposed ? 1 : K, transposed ? e.N : 1, M, K, e, workspace,
+                                    stream, halves, K);
+    case kRows: return launch_rows(x, transposed ? static_cast<const T *>(workspace) : weight, M, K * halves, e, stream);
     default: break;
   }
   if constexpr (sizeof(T) == 4) return launch_split(x, weight, transposed, M, e.N, K, e, workspace, stream);
@@ -1239,12 +1262,18 @@ bool weight_grad_takes(int dtype, const LinearArgs &a) {
          runs < 1 << 23;
 }
 
-// Few rows of 16 bits keep gz in fp32, and their products meet in fp32 (any_kernel): gradients with one rounding
-// (relative error 0.0017 in bf16, with gz rounded 0.0024 and for one row up to 0.0028), without the weight's
-// turning. The whole backward of 4 x 2,048 x 8,192 takes 101 us, by the kernels for more rows 177; 4 x 256 x 512 22
-// and 16, 64 x 256 x 512 31 and 19, which is why more rows than one product of 16 take the others.
+// Few rows of 16 bits keep gz in fp32, and their products meet in fp32 (any_kernel), without the weight's turning.
+// The whole backward of 4 x 2,048 x 8,192 takes 105 us, of 17 rows by the kernels for more 217; of 4 x 256 x 512 26
+// and 23, which is why more rows than one product of 16 take the others.
 constexpr int64_t kWideRows = 16;
 bool keeps_wide(int dtype, const LinearArgs &a) { return dtype != 0 && a.act != kActNone && a.rows <= kWideRows; }
+// More rows of 16 bits keep gz in two values where a slope has made it longer than gy (SiLU, GELU): rounded to one,
+// gx and gW were off by two roundings (bf16 0.00235 relative, 0.00166 with two values, as from 64 bits).
+// The backward of 40,000 x 256 x 512 takes 114 us where the rounded one took 89, of 8,192 x 2,048 x 8,192 1,313
+// and 831 (the products have twice the terms); ReLU's gz has gy's bits and stays one value.
+int halves_of(int dtype, const LinearArgs &a) {
+  return dtype != 0 && (a.act == kActSilu || a.act == kActGelu) && !keeps_wide(dtype, a) ? 2 : 1;
+}
 
 // Workspace of the backward: gz, the bias' parts, then what the products take.
 struct BackWs {
@@ -1253,11 +1282,12 @@ struct BackWs {
 BackWs back_ws(int dtype, const LinearArgs &a) {
   const int64_t size = dtype == 0 ? 4 : 2;
   BackWs w;
-  w.part = a.act != kActNone ? up(a.rows * a.N * (keeps_wide(dtype, a) ? 4 : size)) : 0;
+  const int halves = halves_of(dtype, a);
+  w.part = a.act != kActNone ? up(a.rows * a.N * (keeps_wide(dtype, a) ? 4 : size * halves)) : 0;
   w.product = w.part + up((int64_t)sum_blocks(a.rows, a.N) * a.N * 4);
   int64_t grad_w = any_bytes(a.N, a.K, a.rows);
-  if (weight_grad_takes(dtype, a)) grad_w = std::max(grad_w, weight_grad_workspace_bytes(dtype, a.rows, a.K, 1, a.N));
-  for (bool aligned : {false, true}) grad_w = std::max(grad_w, product_bytes(dtype, true, a.rows, a.K, a.N, aligned));
+  if (weight_grad_takes(dtype, a)) grad_w = std::max(grad_w, weight_grad_workspace_bytes(dtype, a.rows, a.K, 1, a.N, halves));
+  for (bool aligned : {false, true}) grad_w = std::max(grad_w, product_bytes(dtype, true, a.rows, a.K, a.N, aligned, halves));
   w.total = w.product + up(grad_w);
   return w;
 }
@@ -1272,8 +1302,8 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
   float *part = grad_b != nullptr ? reinterpret_cast<float *>(base + ws.part) : nullptr;
   if (keeps_wide(dtype, a)) {
     float *wide = reinterpret_cast<float *>(base);
-    if (hipError_t e = launch_grad_z(gy, static_cast<const T *>(slope), wide, a.act, a.rows, a.N, part, stream)) return e;
-    if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, false, nullptr, stream)) return e;
+    if (hipError_t e = launch_grad_z<false>(gy, static_cast<const T *>(slope), wide, a.act, a.rows, a.N, part, stream)) return e;
+    if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, 0, nullptr, stream)) return e;
     Epilogue e{nullptr, nullptr, grad_x, nullptr, false, kActNone, a.K};
     if (grad_x != nullptr)
       if (hipError_t err = launch_any<T>(wide, a.N, 1, weight, 1, a.K, a.rows, a.N, e, base + ws.product, stream)) return err;
@@ -1281,21 +1311,27 @@ hipError_t backward(int dtype, const LinearArgs &a, const void *grad_y, const vo
     if (grad_w == nullptr) return hipSuccess;
     return launch_any<T>(wide, 1, a.N, x, 1, a.K, a.N, a.rows, e, base + ws.product, stream);
   }
+  const int halves = halves_of(dtype, a);
   if (a.act != kActNone) gz = reinterpret_cast<T *>(base);
-  if (a.act != kActNone || grad_b != nullptr)
-    if (hipError_t e = launch_grad_z(gy, static_cast<const T *>(slope), const_cast<T *>(gz), a.act, a.rows, a.N, part, stream))
-      return e;
-  const bool turn = grad_x != nullptr && route(gz, weight, true, a.rows, a.K, a.N) == kRows;
-  if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, turn, base + ws.product, stream)) return e;
+  if (a.act != kActNone || grad_b != nullptr) {
+    const T *s = static_cast<const T *>(slope);
+    hipError_t e = hipErrorInvalidValue;
+    if constexpr (sizeof(T) == 2)
+      if (halves == 2) e = launch_grad_z<true>(gy, s, const_cast<T *>(gz), a.act, a.rows, a.N, part, stream);
+    if (halves == 1) e = launch_grad_z<false>(gy, s, const_cast<T *>(gz), a.act, a.rows, a.N, part, stream);
+    if (e != hipSuccess) return e;
+  }
+  const bool turn = grad_x != nullptr && route(gz, weight, true, a.rows, a.K, (int64_t)a.N * halves) == kRows;
+  if (hipError_t e = launch_turn<T>(part, a.rows, grad_b, a.bias_wide, a, turn ? halves : 0, base + ws.product, stream)) return e;
   if (grad_x != nullptr) {
     const Epilogue e{nullptr, nullptr, grad_x, nullptr, false, kActNone, a.K};
-    if (hipError_t err = product<T>(gz, weight, true, a.rows, a.N, e, base + ws.product, stream)) return err;
+    if (hipError_t err = product<T>(gz, weight, true, a.rows, a.N, e, base + ws.product, stream, halves)) return err;
   }
   if (grad_w == nullptr) return hipSuccess;
   if (weight_grad_takes(dtype, a) && on_16({gz, x}))
-    return launch_weight_grad(dtype, x, gz, a.rows, a.K, 1, a.N, base + ws.product, dtype, grad_w, stream);
+    return launch_weight_grad(dtype, x, gz, a.rows, a.K, 1, a.N, base + ws.product, dtype, grad_w, stream, halves);
   const Epilogue e{nullptr, nullptr, grad_w, nullptr, false, kActNone, a.K};
-  return launch_any<T>(gz, 1, a.N, x, 1, a.K, a.N, a.rows, e, base + ws.product, stream);
+  return launch_any<T>(gz, 1, (int64_t)a.N * halves, x, 1, a.K, a.N, a.rows, e, base + ws.product, stream, halves, a.N);
 }
 
 }  // namespace

@@ -619,8 +619,8 @@ int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_
  * Sums, bias, activation and residual in fp32, rounded once. The backward takes slope (for ReLU anything
  * that is not positive where z is not, such as y where there is no residual; not read for act 0), and
  * writes grad_x, grad_weight (dtype) and grad_bias (bias_dtype), each NULL where it is not wanted;
- * gz = grad_y slope of more than 16 rows is rounded to dtype, ReLU's derivative at 0 is 0. The residual's gradient is
- * grad_y. The same results on every run. dtype F32, F16, BF16; features at most 2^24, rows less than
+ * gz = grad_y slope is kept in fp32 or, of more than 16 rows, in two values of dtype (16 bits or more of it); ReLU's
+ * derivative at 0 is 0. The residual's gradient is grad_y. The same results on every run. dtype F32, F16, BF16; features at most 2^24, rows less than
  * 2^31 - 256, no size may be 0 and no tensor have more than 2^40 values; outputs overlap nothing else.
  * The workspace (16-byte aligned) holds what bevk_linear_workspace_bytes says (-1 for sizes not
  * taken); aligned (forward): whether x and weight both begin on 16-byte boundaries. */
