@@ -1548,13 +1548,16 @@ def _linear_workspace_bytes(code, backward, aligned, rows, k, n, act):
 def linear_forward(x, weight, bias=None, act=None, residual=None, with_slope=False):
     """(y, slope, sizes): y = act(x @ weight.T + bias) + residual for x [..., K], weight [N, K]; slope, with
     with_slope, what linear_backward takes for it (None where that needs none, y itself where its sign
-    is enough)."""
+    is enough, int16 for SiLU and GELU in 16 bits)."""
     sizes = _linear_check("linear_forward", x, weight, bias, act, residual)
     code, rows, k, n, acode, bcode = sizes
     y = x.new_empty((*x.shape[:-1], n))
     slope = None
     if with_slope and acode:
-        slope = y if acode == 1 and residual is None else torch.empty_like(y)  # (16 bits: whole numbers)
+        # the slopes of SiLU and GELU in 16 bits are whole numbers, and a tensor of those: what packs saved tensors
+        # by converting floating types would take them for values, NaN among them
+        whole = acode != 1 and y.dtype != torch.float32
+        slope = y if acode == 1 and residual is None else torch.empty_like(y, dtype=torch.int16 if whole else None)
     if rows:
         xp, wp = x.data_ptr(), weight.data_ptr()
         nbytes = _linear_workspace_bytes(code, 0, (xp | wp) % 16 == 0, rows, k, n, acode)

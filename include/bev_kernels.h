@@ -615,7 +615,7 @@ int bevk_residual_norm_backward(int dtype, const void *grad_y, const void *grad_
  *                distribution below z)
  *   slope        [rows, out_features] act'(z) for the backward, or NULL; as wide as dtype: F32, and for
  *                ReLU dtype, as it is, else whole numbers u of 16 bits, act'(z) = u / 32768 - 0.25
- *                (65535: NaN). Not written for act 0
+ *                (65535: NaN), a tensor of whole numbers rather than of dtype. Not written for act 0
  * Sums, bias, activation and residual in fp32, rounded once. The backward takes slope (for ReLU anything
  * that is not positive where z is not, such as y where there is no residual; not read for act 0), and
  * writes grad_x, grad_weight (dtype) and grad_bias (bias_dtype), each NULL where it is not wanted;
