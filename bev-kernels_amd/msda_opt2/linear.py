@@ -27,17 +27,19 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        y, slope, ctx.sizes = _ext().linear_forward(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(x, weight, bias, slope)
+        wanted = any(ctx.needs_input_grad[:3])  # (the residual's gradient is grad_y: nothing is kept for it)
+        y, slope, ctx.sizes = _ext().linear_forward(x, weight, bias, act, residual, wanted)
+        if wanted:
+            ctx.save_for_backward(x, weight, bias, slope)
         return y
 
     @staticmethod
     @_b.once_differentiable
     def backward(ctx, grad_y):
-        x, weight, bias, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         grads = (None, None, None)
         if any(need[:3]):
+            x, weight, bias, slope = ctx.saved_tensors
             grads = _ext().linear_backward(_dense(grad_y), x, weight, bias, slope, ctx.sizes, need[:3])
         return (*grads, None, grad_y if need[4] else None)
 
