@@ -52,13 +52,21 @@ template <typename T> __device__ __forceinline__ floatx4 multiply16(int4v a, int
 // p |z|), which is nowhere 0 and flat where z is large; Q of degree 6 and p by linear programming over 3,001
 // places for the least largest error, of 7e-8 in all or 3e-5 of the value, whichever is less. Q itself is off by 6e-8 at most
 // and by 2.5e-5 of the value, however small (half a step of fp16 is 4.9e-4 of it), in 16 instructions where
-// erfcf takes 40 of a kernel that is bound by memory.
+// erfcf takes 40 of a kernel that is bound by memory. fp32: z^2 and z / sqrt(2) are taken in two pieces, since their
+// rounding alone is z^2 / 2 and z^2 half steps of the result, and exp is the exact one.
 template <typename T> __device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
-  const float e = __expf(-0.5f * z * z);
-  pdf = 0.3989422804f * e;
   if constexpr (sizeof(T) == 4) {
-    cdf = 0.5f * erfcf(-0.7071067812f * z);
+    const float q = z * z, e = expf(-0.5f * q);
+    const float rest = __builtin_fmaf(z, z, -q);  // (NaN where q is Inf, and e 0)
+    pdf = e > 0.f ? 0.3989422804f * __builtin_fmaf(-0.5f * rest, e, e) : 0.3989422804f * e;
+    // erfc(y + d) = erfc(y) - 2 / sqrt(pi) exp(-y^2) d
+    constexpr float kHigh = 0.707106769f, kLow = 1.21016175e-8f;  // 1 / sqrt(2)
+    const float y = -kHigh * z, d = -__builtin_fmaf(kLow, z, __builtin_fmaf(kHigh, z, y));
+    cdf = 0.5f * erfcf(y);
+    if (e > 0.f) cdf = __builtin_fmaf(-0.5641895835f * e, d, cdf);
   } else {
+    const float e = __expf(-0.5f * z * z);
+    pdf = 0.3989422804f * e;
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.361881793f, __builtin_fabsf(z), 1.f));
     float q = __builtin_fmaf(t, 0.0427341759f, -0.160822466f);
     q = __builtin_fmaf(t, q, 0.148689866f);
@@ -77,7 +85,13 @@ template <typename T> __device__ __forceinline__ float activate(float z, int act
     return z <= 0.f ? 0.f : z;
   }
   if (act == kActSilu) {
-    const float d = 1.f + __expf(-z), s = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(d) : 1.f / d;  // (16 bits: off by an ulp of fp32)
+    if constexpr (sizeof(T) == 4) {  // s and 1 - s, each to its own last places
+      const float e = expf(-__builtin_fabsf(z)), high = 1.f / (1.f + e), low = e * high;
+      const float s = z < 0.f ? low : high;
+      slope = s * __builtin_fmaf(z, z < 0.f ? high : low, 1.f);
+      return z * s;
+    }
+    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));  // (16 bits: off by |z| ulps of fp32)
     slope = s * __builtin_fmaf(z, 1.f - s, 1.f);
     return z * s;
   }

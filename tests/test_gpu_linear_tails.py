@@ -36,3 +36,26 @@ def test_16_bits(rows, dtype, act):
     off = (y - want).abs()
     at = (off / bound).argmax()
     assert (off <= bound).all(), f"z {z[at].item()}: {y[at].item()} for {want[at].item()}"
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows", [5, 400, 4000])
+def test_fp32(rows, act):
+    from msda_opt2 import linear_act
+    last = 12.9 if act == "gelu" else 86
+    z = torch.linspace(-last, last, 40001, dtype=torch.float64).float().to(DEV).requires_grad_()
+    w = torch.ones(1, 1, device=DEV)
+    y = torch.cat([linear_act(part[:, None], w, None, act)[:, 0] for part in z.split(rows)])
+    slope, = torch.autograd.grad(y.sum(), z)
+    with torch.no_grad():
+        d = z.double()
+        if act == "gelu":
+            terms = 0.5 * torch.erfc(-d * 0.5 ** 0.5), d * torch.exp(-0.5 * d * d) * (2 * torch.pi) ** -0.5
+        else:
+            terms = torch.sigmoid(d), d * torch.sigmoid(d) * torch.sigmoid(-d)
+        least = (1 + d.abs()) * 2.0 ** -126
+        for got, want, size, what in ((y, _exact(z, act), _exact(z, act).abs(), "y"),
+                                      (slope, sum(terms), sum(t.abs() for t in terms), "slope")):
+            off, bound = (got.double() - want).abs(), 16 * U * size + least
+            at = (off / bound).argmax()
+            assert (off <= bound).all(), f"{what} at z {d[at].item()}: {got[at].item()} for {want[at].item()}"
