@@ -222,9 +222,12 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
         m[e] = __builtin_fmaf(x, f.rest1, m[e] * f.b1);
         v[e] = __builtin_fmaf(x * x, f.rest2, v[e] * f.b2);
         // the hardware's square root and reciprocal, each right to a unit in the last place of a step that
-        // is small next to p; v from the smallest normal on (its square root, 1e-19, is lost in eps)
-        const float root = __builtin_amdgcn_sqrtf(fmaxf(v[e], 1.17549435e-38f));
-        p[e] = __builtin_fmaf(-f.size, m[e] * __builtin_amdgcn_rcpf(__builtin_fmaf(root, f.root, f.eps)), p[e] * f.decay);
+        // is small next to p; a small v 2^64 times as large, as that root takes no subnormals. Where root and eps are
+        // both 0 (v has underflown) there is no step
+        const bool small = v[e] < 0x1p-96f;
+        const float root = __builtin_amdgcn_sqrtf(small ? v[e] * 0x1p64f : v[e]) * (small ? 0x1p-32f : 1.f);
+        const float den = __builtin_fmaf(root, f.root, f.eps);
+        p[e] = __builtin_fmaf(-f.size, den == 0.f ? 0.f : m[e] * __builtin_amdgcn_rcpf(den), p[e] * f.decay);
       }
     }
     if (there) {

@@ -61,6 +61,7 @@ def adamw_step_(params, grads, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_d
     max_norm: gradients are clipped by the norm of all of them on the way, without being written:
     norm, a float32 on the device from grad_norm, or None, and it is computed here.
     copies: tensors that receive the new parameters in their own type.
+    eps may be 0: where v is 0 too (never used, or a gradient below 1e-21) a value only decays.
     Nothing waits for the device; a captured step counts on at every replay. A gradient of Inf or NaN
     goes through as in torch.optim.AdamW (with 8-bit moments into the 128 values around it): test
     the norm before the step. The same results on every run."""

@@ -539,7 +539,7 @@ int bevk_clip_gradients(int count, const void *const *grads, const int *dtypes,
  *   g = min(1, max_norm / (norm + 1e-6)) * grad       (the factor where norm is not NULL)
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
- * in fp32, each result rounded once.
+ * in fp32, each result rounded once (where sqrt(v) and eps are both 0, the quotient is 0).
  *   params, grads, copies   HOST arrays of `count` device pointers, with types (F32, F16, BF16) and
  *                           sizes; copies (NULL for none) receive the new parameters in their type
  *   exp_avg, exp_avg_sq     m and v of all tensors, `values` in all: tensor k's begin at the sum of the
