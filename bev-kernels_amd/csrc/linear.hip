@@ -466,7 +466,13 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
   __syncthreads();
 
   // A lane holds one row and four times four neighbouring columns of each 32 x 32. Each wave turns 32 rows of
-  // its own at a time in LDS, so that eight lanes store 128 neighbouring bytes of a row.
+  // its own at a time in LDS, so that eight lanes store 128 neighbouring bytes of a row. LDS serves a wave's
+  // instructions in order: what keeps the compiler from moving them past each other is turned() alone.
+  auto turned = [] __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  };
   constexpr int V = 16 / sizeof(T), P = TN * 32 + 4, C = TN * 32 / V;  // floats of a row, and its pieces of V
   float *turn = reinterpret_cast<float *>(lds[0]) + wave * 32 * P;
   static_assert(WAVES * 32 * P * 4 <= (int)sizeof(lds), "turn");
@@ -482,6 +488,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
 #pragma unroll
       for (int j = 0; j < TN * 2; ++j)
         *reinterpret_cast<floatx4 *>(turn + (ii * 16 + row) * P + j * 16 + half * 4) = acc[i * 2 + ii][j];
+    turned();
     const int64_t mi = m0 + wm * TM * 32 + i * 32;
     if (p.wide) {
 #pragma unroll 2
@@ -505,6 +512,7 @@ __global__ void __launch_bounds__(64 * WM * WN) tile_kernel(const TileArgs p, in
         if (m < p.M && n < N) finish<T>(p.e, m, n, turn[c / (TN * 32) * P + c % (TN * 32)]);
       }
     }
+    turned();
   }
 }
 
