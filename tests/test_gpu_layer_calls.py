@@ -7,10 +7,6 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
-def _rand(g, *s):
-    return torch.randn(*s, generator=g, device=DEV)
-
-
 def test_linear_refuses_forward_mode():
     import torch.autograd.forward_ad as fwd
 
@@ -38,38 +34,45 @@ def _orders(t):
     yield base[1:].view(t.shape)
 
 
-@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 def test_norm_gradients_in_any_order(dtype):
-    """Both gradients in each order against dense ones: the same values (off 16 bytes the sums have another order:
-    a rounding of each)."""
+    """Both gradients in each order of strides: the same bits as dense ones, and off 16 bytes (another order of sums)
+    within the bounds of test_gpu_residual_norm.py."""
+    import test_gpu_residual_norm as norm
+    t, grads = norm._inputs((6, 10, 64), norm.TYPES[dtype], 4, "channels", True)
+    leaves = {n: v.to(DEV).requires_grad_() for n, v in t.items()}
     from msda_opt2 import residual_norm
-    g = torch.Generator(device=DEV).manual_seed(4)
-    x, r, gy, gs = (_rand(g, 6, 10, 64).to(dtype) for _ in range(4))
-    leaves = [t.requires_grad_() for t in (x, r, _rand(g, 64), _rand(g, 64))]
-    out = residual_norm(*leaves)
-    want = torch.autograd.grad(out, leaves, (gy, gs), retain_graph=True)
+    out = residual_norm(leaves["x"], leaves["residual"], leaves["weight"], leaves["bias"], leaves["gate"], 0.5,
+                        (leaves["block_weight"], leaves["block_bias"]))
+    gy, gs = (g.to(DEV) for g in grads)
+    want = torch.autograd.grad(out, list(leaves.values()), (gy, gs), retain_graph=True)
+    r = norm.Reference(t, *grads, 0.5, True, "layer", 1e-5)
     for a in _orders(gy):
         for b in _orders(gs):
-            got = torch.autograd.grad(out, leaves, (a, b), retain_graph=True)
-            for p, q in zip(got, want):
+            got = torch.autograd.grad(out, list(leaves.values()), (a, b), retain_graph=True)
+            for n, p, q in zip(leaves, got, want):
                 if a.data_ptr() % 16 or b.data_ptr() % 16:
-                    assert (p.float() - q.float()).abs().max() <= 2 * torch.finfo(dtype).eps * q.float().abs().max()
+                    norm._near(p, *r.grads[n], n)
                 else:
-                    assert torch.equal(p, q)
+                    assert torch.equal(p, q), n
 
 
 @pytest.mark.parametrize("act", [None, "relu", "gelu"])
-@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 def test_linear_gradients_in_any_order(dtype, act):
+    """As above, with the bounds of test_gpu_linear.py."""
+    import test_gpu_linear as lin
     from msda_opt2 import linear_act
-    g = torch.Generator(device=DEV).manual_seed(5)
-    leaves = [t.to(dtype).requires_grad_() for t in (_rand(g, 8, 9, 64), _rand(g, 72, 64) / 8, _rand(g, 72))]
-    gy = _rand(g, 8, 9, 72).to(dtype)
+    t, gy = lin._inputs(72, 64, 72, lin.TYPES[dtype], 5, False)
+    leaves = [v.to(DEV).requires_grad_() for v in t.values() if v is not None]
+    gy = gy.to(DEV)
     y = linear_act(*leaves, act)
     want = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+    r = lin.Reference(t, gy.cpu(), act)
+    bounds = ((r.gx, r.gx_err), (r.gw, r.gw_err), (r.gb, r.gb_err))
     for a in _orders(gy):
-        for p, q in zip(torch.autograd.grad(y, leaves, a, retain_graph=True), want):
+        for p, q, bound in zip(torch.autograd.grad(y, leaves, a, retain_graph=True), want, bounds):
             if a.data_ptr() % 16:
-                assert (p.float() - q.float()).abs().max() <= 2 * torch.finfo(dtype).eps * q.float().abs().max()
+                lin._near(p, *bound, "off 16 bytes")
             else:
                 assert torch.equal(p, q)
