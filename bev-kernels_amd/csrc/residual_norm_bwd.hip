@@ -13,6 +13,9 @@
 // added over its rows in LDS and written to the workspace, and join_kernel adds up the workgroups' parts
 // in order: no atomics, the same results on every run.
 //
+// Rows of more than 512 vectors of 16 bits or 1,024 of fp32 (4,096 channels) take two passes, rows_kernel and sums_kernel:
+// 10 tensors read or written for 6, and no scratch memory. 4,096 x 8,192 bf16 with both norms 200 us (479 in one
+// pass), 2,048 x 16,384 198 (796), without the block's norm 155 (211 and 488); 2,048 x 8,192 fp32 161 (371).
 // Bound by memory and by what a thread can have in flight beside its sums (a row ahead, two or three waves a
 // SIMD): 16,384 x 2,048 bf16 with both norms 336 MB in 80 us (4.2 TB/s; a workgroup a row and no prefetch
 // 147 us), 34,800 x 512 fp16 178 MB in 38 us (4.7), and 5 to 6 us for the parts' sums.
@@ -22,8 +25,13 @@ namespace bevk {
 namespace {
 using namespace rnorm;
 
-// Workgroups on the chip at a time: what a thread keeps leaves room for two or three waves a SIMD.
-constexpr int parts_at_most(int tpr) { return tpr <= 64 ? 768 : 512 * 256 / threads_of(tpr); }
+// Rows that take two passes: 1,024 threads have 128 registers each, and one with 8 values or more of every sum, parameter
+// and tensor has no room for them (up to 524 of them went through scratch memory).
+constexpr bool in_two_passes(int tpr, int values) { return tpr == 1024 && values >= 8; }
+
+// Workgroups on the chip at a time: what a thread keeps leaves room for two or three waves a SIMD (four of 1,024 threads:
+// 4,096 x 4,096 fp32 with both norms 96 us on all CUs, 114 on half of them).
+constexpr int parts_at_most(int tpr) { return tpr <= 64 ? 768 : std::max(256, 512 * 256 / threads_of(tpr)); }
 
 template <typename T, int V>
 __device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t r, uint32_t off, const Vec<T, V> &y) {
@@ -52,6 +60,7 @@ Split split_of(const ResidualNormArgs &a, int rows_a_block, int64_t most_blocks)
 // are wanted), then the gate's [sets][per][channels].
 struct Parts {
   float *sum[4], *gate;
+  float *means;  // two passes: [rows][2] mean(t) (rms: 0) and mean(t hh); or null where no sums are wanted
 };
 
 template <typename T, int V, int TPR, int L, bool BLOCK>
@@ -254,6 +263,201 @@ __global__ void __launch_bounds__(threads_of(TPR)) backward_kernel(const Residua
     if (parts.sum[n - 1] != nullptr) write(sum[n], parts.sum[n - 1] + (int64_t)blockIdx.x * a.channels);
 }
 
+// The first pass over long rows: the rows' own gradients. A workgroup takes a row at a time, whose four tensors stay in
+// registers as they were loaded; what is computed from them is computed again behind each sum, with the parameters
+// from the L2.
+template <typename T, int V, int L, bool BLOCK>
+__global__ void __launch_bounds__(1024) rows_kernel(const ResidualNormArgs a, const ResidualNormGrads g, float *means) {
+  __shared__ float s[2 * 1024 / 64 * 2];
+  int turn = 0;
+  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+  const float inv = 1.f / (float)a.channels;
+  const uint32_t bytes = (uint32_t)a.channels * sizeof(T);
+  uint32_t off[L];
+#pragma unroll
+  for (int l = 0; l < L; ++l) off[l] = (uint32_t)(l * 1024 + threadIdx.x) * V * sizeof(T);  // (past a row's end: nothing)
+  typedef int int4v __attribute__((ext_vector_type(4)));
+  int4v now[4][L], next[4][L];  // 16 bytes of the gradient of y, x, the gradient of the stream, the residual
+  auto value = [&](int n, int l, int e) __attribute__((always_inline)) {
+    return (float)__builtin_bit_cast(Vec<T, V>, now[n][l]).v[e];
+  };
+  auto load = [&](int64_t r) __attribute__((always_inline)) {
+    const void *from[4] = {g.grad_y, a.x, g.grad_h, a.residual};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const __amdgpu_buffer_rsrc_t b = make_rsrc(static_cast<const T *>(from[n]) + r * a.channels, from[n] != nullptr ? bytes : 0);
+#pragma unroll
+      for (int l = 0; l < L; ++l) next[n][l] = __builtin_bit_cast(int4v, buffer_load_vec<T, V>(b, off[l]));
+    }
+  };
+  constexpr bool AHEAD = L == 1;
+  if constexpr (AHEAD) load(r0);
+  for (int64_t r = r0; r < r1; ++r) {
+    if constexpr (!AHEAD) load(r);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int l = 0; l < L; ++l) now[n][l] = next[n][l];
+    if constexpr (AHEAD) load(min(r + 1, r1 - 1));
+    const Vec<float, BLOCK ? 4 : 2> st = load_vec<float, BLOCK ? 4 : 2>(g.stats + r * (BLOCK ? 4 : 2));
+    const int64_t gate_at = a.set_rows > 0 ? r / a.set_rows * a.channels : 0;
+    // f(value, t = gy w, hh, ph, scale * gate, bw) for each value of vector l that there is
+    auto each = [&](int l, auto f) __attribute__((always_inline)) {
+      // (to the compiler new values, and parameters that may have changed: what it computes from them twice it would
+      // keep, and that does not fit)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) asm volatile("" : "+v"(now[n][l]));
+      asm volatile("" ::: "memory");
+      const int c = (l * 1024 + (int)threadIdx.x) * V;
+      if (c >= a.channels) return;
+      float w[V], gate[V], bw[V], bb[V];
+      load_param<T, V>(a.weight, a.wide, c, 1.f, w);
+      load_param<T, V>(a.gate, a.gate_wide, gate_at + c, 1.f, gate);
+      if constexpr (BLOCK) {
+        load_param<T, V>(a.block_weight, a.wide, c, 1.f, bw);
+        load_param<T, V>(a.block_bias, a.wide, c, 0.f, bb);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float p = value(1, l, e), ph = 0.f;
+        if constexpr (BLOCK) {
+          ph = (p - st.v[2]) * st.v[3];
+          p = __builtin_fmaf(ph, bw[e], bb[e]);
+        }
+        const float hh = (stream_value(p, a.scale, gate[e], value(3, l, e)) - st.v[0]) * st.v[1];
+        f(e, value(0, l, e) * w[e], hh, ph, gate[e], BLOCK ? bw[e] : 1.f);
+      }
+    };
+    auto store = [&](void *to, int l, const float (&v)[V]) __attribute__((always_inline)) {
+      Vec<T, V> y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) y.v[e] = static_cast<T>(v[e]);
+      buffer_store(make_rsrc(static_cast<T *>(to) + r * a.channels, to != nullptr ? bytes : 0), off[l], y);
+    };
+    float t[2] = {0.f, 0.f};
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+      each(l, [&](int, float u, float hh, float, float, float) __attribute__((always_inline)) {
+        t[0] += u;
+        t[1] = __builtin_fmaf(u, hh, t[1]);
+      });
+    row_sums<1024, 1024, 2>(t, s, turn);
+    const float c1 = a.rms ? 0.f : t[0] * inv, c2 = t[1] * inv;
+    if (threadIdx.x == 0 && means != nullptr) {
+      means[r * 2] = c1;
+      means[r * 2 + 1] = c2;
+    }
+    auto grad_stream = [&](int l, int e, float u, float hh) __attribute__((always_inline)) {
+      return __builtin_fmaf(st.v[1], u - c1 - hh * c2, value(2, l, e));
+    };
+    t[0] = t[1] = 0.f;
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      float gr[V], gx[V];
+      each(l, [&](int e, float u, float hh, float ph, float gate, float bw) __attribute__((always_inline)) {
+        gr[e] = grad_stream(l, e, u, hh);
+        gx[e] = gate * (a.scale * gr[e]);
+        if constexpr (BLOCK) {
+          const float v = gx[e] * bw;
+          t[0] += v;
+          t[1] = __builtin_fmaf(v, ph, t[1]);
+        }
+      });
+      store(g.grad_residual, l, gr);
+      if constexpr (!BLOCK) store(g.grad_x, l, gx);
+    }
+    if constexpr (BLOCK) {
+      row_sums<1024, 1024, 2>(t, s, turn);
+      const float d1 = a.rms ? 0.f : t[0] * inv, d2 = t[1] * inv;
+#pragma unroll
+      for (int l = 0; l < L; ++l) {
+        float gx[V];
+        each(l, [&](int e, float u, float hh, float ph, float gate, float bw) __attribute__((always_inline)) {
+          gx[e] = st.v[3] * (gate * (a.scale * grad_stream(l, e, u, hh)) * bw - d1 - ph * d2);
+        });
+        store(g.grad_x, l, gx);
+      }
+    }
+  }
+}
+
+// The parameters' sums of long rows, in a second pass: a thread has V channels of a part's rows, one after another, with
+// the means over each row that the first pass found. No sum over a row, so no wait between two of them.
+template <typename T, int V, bool BLOCK>
+__global__ void __launch_bounds__(256) sums_kernel(const ResidualNormArgs a, const ResidualNormGrads g, const Split sp,
+                                                   const Parts parts) {
+  const int c = (int)(blockIdx.y * 256 + threadIdx.x) * V;
+  if (c >= a.channels) return;
+  const int64_t set0 = sp.per > 1 ? blockIdx.x / sp.per : sp.sets * blockIdx.x / sp.blocks;
+  const int64_t set1 = sp.per > 1 ? set0 + 1 : sp.sets * (blockIdx.x + 1) / sp.blocks;
+  const int part = sp.per > 1 ? blockIdx.x % sp.per : 0;
+  const T *from[4] = {static_cast<const T *>(g.grad_y) + c, static_cast<const T *>(a.x) + c,
+                      g.grad_h != nullptr ? static_cast<const T *>(g.grad_h) + c : nullptr,
+                      a.residual != nullptr ? static_cast<const T *>(a.residual) + c : nullptr};
+  constexpr int N = BLOCK ? 5 : 3, S = BLOCK ? 4 : 2;
+  float sum[N][V], w[V], gate[V], bw[V], bb[V];  // gate, weight, bias, block weight, block bias
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[n][e] = 0.f;
+  load_param<T, V>(a.weight, a.wide, c, 1.f, w);
+  if constexpr (BLOCK) {
+    load_param<T, V>(a.block_weight, a.wide, c, 1.f, bw);
+    load_param<T, V>(a.block_bias, a.wide, c, 0.f, bb);
+  }
+  auto write = [&](const float (&v)[V], float *to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) to[c + e] = v[e];
+  };
+  for (int64_t set = set0; set < set1; ++set) {
+    const int64_t r0 = set * sp.set_rows + sp.set_rows * part / sp.per;
+    const int64_t r1 = set * sp.set_rows + sp.set_rows * (part + 1) / sp.per;
+    load_param<T, V>(a.gate, a.gate_wide, (a.set_rows > 0 ? set * a.channels : 0) + c, 1.f, gate);
+    Vec<T, V> next[4];
+    auto load = [&](int64_t r) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        next[n] = from[n] != nullptr ? load_vec<T, V>(from[n] + r * a.channels) : Vec<T, V>{};
+    };
+    load(r0);
+    for (int64_t r = r0; r < r1; ++r) {
+      const Vec<float, S> st = load_vec<float, S>(g.stats + r * S);
+      const Vec<float, 2> means = load_vec<float, 2>(parts.means + r * 2);
+      Vec<T, V> now[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) now[n] = next[n];
+      load(min(r + 1, r1 - 1));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float gy = (float)now[0].v[e];
+        float p = (float)now[1].v[e], ph = 0.f;
+        if constexpr (BLOCK) {
+          ph = (p - st.v[2]) * st.v[3];
+          p = __builtin_fmaf(ph, bw[e], bb[e]);
+        }
+        const float hh = (stream_value(p, a.scale, gate[e], (float)now[3].v[e]) - st.v[0]) * st.v[1];
+        const float gh = a.scale * __builtin_fmaf(st.v[1], gy * w[e] - means.v[0] - hh * means.v[1], (float)now[2].v[e]);
+        sum[0][e] = __builtin_fmaf(gh, p, sum[0][e]);
+        sum[1][e] = __builtin_fmaf(gy, hh, sum[1][e]);
+        sum[2][e] += gy;
+        if constexpr (BLOCK) {
+          const float gp = gate[e] * gh;
+          sum[3][e] = __builtin_fmaf(gp, ph, sum[3][e]);
+          sum[4][e] += gp;
+        }
+      }
+    }
+    if (parts.gate != nullptr) {
+      write(sum[0], parts.gate + (set * sp.per + part) * a.channels);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int n = 1; n < N; ++n)
+    if (parts.sum[n - 1] != nullptr) write(sum[n], parts.sum[n - 1] + (int64_t)blockIdx.x * a.channels);
+}
+
 // Any row length: a workgroup a row at a time, each sum a pass over it; a thread adds its channels' parts
 // up in the workspace.
 template <typename T, bool BLOCK>
@@ -385,16 +589,23 @@ __global__ void __launch_bounds__(1024) join_kernel(const Joins all, int64_t fir
   }
 }
 
-// The split for rows of vectors of v values.
-Split split_for(const ResidualNormArgs &a, int v) {
+// The split of the sums for rows of vectors of v values, and whether they are a second pass.
+struct Plan {
+  Split split;
+  bool two;
+};
+Plan plan(const ResidualNormArgs &a, int v) {
   int rows = 1;
   int64_t blocks = 1024;
-  for_row((a.channels + v - 1) / v, [&](auto tpr, auto) {
-    constexpr int TPR = decltype(tpr)::value;
-    rows = threads_of(TPR) / TPR;
-    blocks = parts_at_most(TPR);
+  bool two = false;
+  const int64_t vecs = (a.channels + v - 1) / v;
+  for_row(vecs, [&](auto tpr, auto l) {
+    constexpr int TPR = decltype(tpr)::value, L = decltype(l)::value;
+    two = in_two_passes(TPR, v * L);
+    rows = two ? 1 : threads_of(TPR) / TPR;
+    blocks = two ? 512 / ((vecs + 255) / 256) : parts_at_most(TPR);  // (two workgroups of sums_kernel a CU)
   });
-  return split_of(a, rows, blocks);
+  return {split_of(a, rows, blocks), two};
 }
 
 template <typename T, int V, bool BLOCK>
@@ -402,8 +613,17 @@ hipError_t launch_v(const ResidualNormArgs &a, const ResidualNormGrads &g, const
                     hipStream_t stream) {
   const bool fits = for_row((a.channels + V - 1) / V, [&](auto tpr, auto l) {
     constexpr int TPR = decltype(tpr)::value, L = decltype(l)::value;
-    hipLaunchKernelGGL((backward_kernel<T, V, TPR, L, BLOCK>), dim3(sp.blocks), dim3(threads_of(TPR)), 0, stream, a,
-                       g, sp, parts);
+    if constexpr (in_two_passes(TPR, V * L)) {
+      const int cus = std::max(1, device_cus());  // (a workgroup fills a CU)
+      hipLaunchKernelGGL((rows_kernel<T, V, L, BLOCK>), dim3((unsigned)std::min<int64_t>(a.rows, cus)), dim3(1024), 0, stream,
+                         a, g, parts.means);
+      if (parts.means != nullptr)
+        hipLaunchKernelGGL((sums_kernel<T, V, BLOCK>), dim3(sp.blocks, (unsigned)((a.channels / V + 255) / 256)), dim3(256), 0,
+                           stream, a, g, sp, parts);
+    } else {
+      hipLaunchKernelGGL((backward_kernel<T, V, TPR, L, BLOCK>), dim3(sp.blocks), dim3(threads_of(TPR)), 0, stream, a,
+                         g, sp, parts);
+    }
   });
   if (!fits)
     hipLaunchKernelGGL((any_backward_kernel<T, BLOCK>), dim3(sp.blocks), dim3(256), 0, stream, a, g, sp, parts);
@@ -414,7 +634,8 @@ template <typename T>
 hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool whole, void *workspace,
                     hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  const Split sp = split_for(a, whole ? V : 1);
+  const Plan pl = plan(a, whole ? V : 1);
+  const Split &sp = pl.split;
   float *ws = static_cast<float *>(workspace);
   Parts parts{};
   Joins joins{};
@@ -431,7 +652,9 @@ hipError_t launch_t(const ResidualNormArgs &a, const ResidualNormGrads &g, bool 
     parts.gate = ws;
     joins.of[joins.count++] = Join{ws, g.grad_gate, sp.per, sp.sets, a.gate_wide};
     rows += sp.sets;
+    ws += sp.sets * sp.per * a.channels;
   }
+  if (pl.two && joins.count > 0) parts.means = ws;
   hipError_t e;
   if (whole) e = a.block ? launch_v<T, V, true>(a, g, sp, parts, stream) : launch_v<T, V, false>(a, g, sp, parts, stream);
   else e = a.block ? launch_v<T, 1, true>(a, g, sp, parts, stream) : launch_v<T, 1, false>(a, g, sp, parts, stream);
@@ -451,8 +674,8 @@ bool whole_rows(int dtype, const ResidualNormArgs &a, const ResidualNormGrads &g
 int64_t residual_norm_backward_workspace_bytes(int dtype, const ResidualNormArgs &a) {
   int64_t most = 0;  // for either alignment
   for (int v : {dtype == 0 ? 4 : 8, 1}) {
-    const Split sp = split_for(a, v);
-    most = std::max(most, (4 * (int64_t)sp.blocks + sp.sets * sp.per) * a.channels * 4);
+    const Plan pl = plan(a, v);
+    most = std::max(most, (4 * (int64_t)pl.split.blocks + pl.split.sets * pl.split.per) * a.channels * 4 + (pl.two ? a.rows * 8 : 0));
   }
   return most;
 }
