@@ -1347,7 +1347,7 @@ def adamw_moments(state, dtype=torch.float32):
     """(exp_avg, exp_avg_sq) of a state as values, flat: its own tensors where they have that type,
     else new ones. 8-bit moments: float32 or bfloat16, both exact."""
     fn = "adamw_moments"
-    m, v, ms, vs, _ = _adamw_moments_of(fn, state, state["exp_avg"].get_device())
+    m, v, ms, vs, _ = _adamw_moments_of(fn, state, state["exp_avg"].get_device() if "exp_avg" in state else -1)
     if ms is None:
         return m.to(dtype), v.to(dtype)
     if dtype not in (torch.float32, torch.bfloat16):
