@@ -223,11 +223,11 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const Table t, int64_t 
         v[e] = __builtin_fmaf(x * x, f.rest2, v[e] * f.b2);
         // the hardware's square root and reciprocal, each right to a unit in the last place of a step that
         // is small next to p; a small v 2^64 times as large, as that root takes no subnormals. Where root and eps are
-        // both 0 (v has underflown) there is no step
+        // both 0 (v has underflown; or eps is a subnormal, of which the reciprocal is Inf) there is no step
         const bool small = v[e] < 0x1p-96f;
         const float root = __builtin_amdgcn_sqrtf(small ? v[e] * 0x1p64f : v[e]) * (small ? 0x1p-32f : 1.f);
         const float den = __builtin_fmaf(root, f.root, f.eps);
-        p[e] = __builtin_fmaf(-f.size, den == 0.f ? 0.f : m[e] * __builtin_amdgcn_rcpf(den), p[e] * f.decay);
+        p[e] = __builtin_fmaf(-f.size, den < 0x1p-126f ? 0.f : m[e] * __builtin_amdgcn_rcpf(den), p[e] * f.decay);
       }
     }
     if (there) {

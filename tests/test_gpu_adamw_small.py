@@ -38,16 +38,17 @@ def test_first_step(g, eps):
         assert not p.any()
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-39, 1e-38])
 @pytest.mark.parametrize("bits", [32, 8])
-def test_no_eps_and_no_gradient(bits):
-    """Moments of 0: a value decays and stays a number."""
+def test_no_eps_and_no_gradient(bits, eps):
+    """Moments of 0: a value decays and stays a number, also where eps is a subnormal."""
     import modulated_deform_conv as mdc
     p = torch.full((200,), 2.0, device=DEV)
     g = torch.zeros(200, device=DEV)
     g[7] = 0.5
     state = mdc.adamw_state(p, bits)
     for _ in range(2):
-        mdc.adamw_step_(p, g, state, lr=0.125, eps=0.0, weight_decay=0.5)
+        mdc.adamw_step_(p, g, state, lr=0.125, eps=eps, weight_decay=0.5)
     want = torch.full((200,), 2.0 * (1 - 0.0625) ** 2, dtype=torch.float64, device=DEV)
     rest = torch.arange(200, device=DEV) != 7
     assert ((p.double() - want).abs() <= 4 * U * want)[rest].all()
