@@ -6,8 +6,8 @@
 //
 // Products of 16-bit types on the matrix cores with fp32 sums; bias, activation and residual in fp32 on the
 // sums in registers, one rounding at the end. The forward keeps the slope, as wide as the input, where the
-// backward needs it, which then has no exp to take (gz of 40,000 x 512 gelu bf16: 46 us from z, 24 from
-// the slope). gz of 16-bit types is kept as two values of the type, what the first leaves in the second: the
+// backward needs it, which then has no exp to take (gz of 40,000 x 512 gelu bf16 in one value: 46 us from z,
+// 24 from the slope). gz of 16-bit types is kept as two values of the type, what the first leaves in the second: the
 // matrix cores read 16 bits, and one value's rounding would be as large an error of gx and gW as their own.
 #include <algorithm>
 #include <type_traits>
